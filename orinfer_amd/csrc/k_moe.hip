@@ -908,6 +908,7 @@ int few_tokens_launch(const orx_function& f, int rows, const Geometry& g, hipStr
 #undef ORX_FEW_TOKENS
     return hip_check(hipGetLastError(), "launch router_topk with metadata");
 }
+constexpr const char* kScoreKeys[] = {"scoring", "bias", "groups", "top_groups", "group_best", "scale"};
 int make_router(const Variant& v, orx_function* f) {
     if (!geometry_fields(v, f, true)) return ORX_ERR_BAD_VARIANT;
     bool bad = false;
@@ -917,6 +918,9 @@ int make_router(const Variant& v, orx_function* f) {
         set_error("router_topk: invalid MoE router dimensions (need top_k <= min(E,64), E <= 1024)");
         return ORX_ERR_BAD_VARIANT;
     }
+    // by scores, with a bias or groups: a kernel of its own, routes only (the keys below are unknown to it)
+    for (const char* key : kScoreKeys)
+        if (v.has(key)) return make_router_scores(v, f->flags != 0, f);
     // quantize_hidden=H: the launch also writes the A8 codes Q (M, H) and scales S (M) of the fp16 rows X (M, H)
     f->H = (int)v.integer("quantize_hidden", 0, &bad);
     if (bad || f->H < 0 || f->H % 8) {
@@ -974,6 +978,11 @@ int make_router(const Variant& v, orx_function* f) {
 // logit, ties to the lower id, +-0 equal) and probabilities renormalised over the selected routes.
 int make_router_warp(const Variant& v, orx_function* f) {
     bool bad = false;
+    for (const char* key : kScoreKeys)
+        if (v.fields.count(key)) {
+            set_error("router_topk_warp: %s is router_topk's", key);
+            return ORX_ERR_BAD_VARIANT;
+        }
     const long long experts = v.integer("E", 0, &bad), top_k = v.integer("top_k", 0, &bad), warps = v.integer("warps", 4, &bad);
     if (bad || !v.has("E") || !v.has("top_k") || experts % 32 || top_k > 32 || (warps != 1 && warps != 2 && warps != 4) ||
         v.has("renormalize")) {
@@ -1451,8 +1460,9 @@ int make_combine(const Variant& v, orx_function* f) {
 
 const Registration* moe_registrations(int* count) {
     static const Registration rows[] = {
-    {"router_topk", make_router, "M, E=512, top_k=10, renormalize=true, dynamic_rows=false, quantize_hidden=0, row_max=false, metadata=false, block_m=32",
-     "[Counts,]IDs,Logits,Prob[,Q][,RelativeSlot,RowMax,RowOffsets][,S][,SlotMap,SlotToken,TileCount,TileExpert,TileOffsets,TileRow,TileUnits][,X][,m]"},
+    {"router_topk", make_router, "M, E=512, top_k=10, renormalize=true, dynamic_rows=false, quantize_hidden=0, row_max=false, metadata=false, block_m=32; "
+     "or scoring=softmax|sigmoid, bias=false, groups=1, top_groups=groups, group_best=2, scale=1 (M, E, top_k, renormalize, dynamic_rows)",
+     "[Bias,][Counts,]IDs,Logits,Prob[,Q][,RelativeSlot,RowMax,RowOffsets][,S][,SlotMap,SlotToken,TileCount,TileExpert,TileOffsets,TileRow,TileUnits][,X][,m]"},
     {"router_projection", make_router_projection, "M, H, E, dynamic_rows=false, block_m=16, block_n=32, block_k=128, stages=2",
      "Logits,SharedGate,W,X[,m]"},
     {"router_topk_warp", make_router_warp, "M, E, top_k, dynamic_rows=false, warps=4", "IDs,Logits,Prob[,m]"},

@@ -239,6 +239,20 @@ bool Variant::boolean(const char* key, bool fallback, bool* bad) const {
     return it->second.number != 0;
 }
 
+double Variant::real(const char* key, double fallback, bool* bad) const {
+    (*read)[key] = true;
+    auto it = fields.find(key);
+    if (it == fields.end() || it->second.kind == Value::Null) return fallback;
+    char* end = nullptr;
+    const double value = it->second.kind == Value::String ? strtod(it->second.text.c_str(), &end) : it->second.number;
+    if (it->second.kind == Value::Bool || (end != nullptr && (end == it->second.text.c_str() || *end != 0))) {
+        *bad = true;
+        set_error("variant field %s must be a number", key);
+        return fallback;
+    }
+    return value;
+}
+
 std::string Variant::string(const char* key, const char* fallback, bool* bad) const {
     (*read)[key] = true;
     auto it = fields.find(key);
@@ -270,13 +284,14 @@ struct Table {
     const Registration* rows;
     int count;
 };
-constexpr int kTables = 5;
+constexpr int kTables = 6;
 void tables(Table out[kTables]) {
     out[0].rows = quant_registrations(&out[0].count);
     out[1].rows = gemv_registrations(&out[1].count);
     out[2].rows = gemm_registrations(&out[2].count);
     out[3].rows = moe_registrations(&out[3].count);
     out[4].rows = plane_registrations(&out[4].count);
+    out[5].rows = mx_registrations(&out[5].count);
 }
 const Registration* find(const char* symbol) {
     Table t[kTables];

@@ -36,10 +36,14 @@ struct Variant {
     // Integer field with a default; sets `bad` if the field exists but is not an integer.
     long long integer(const char* key, long long fallback, bool* bad) const;
     bool boolean(const char* key, bool fallback, bool* bad) const;
+    // Number field (also as text, which is what a symbol's own variant holds).
+    double real(const char* key, double fallback, bool* bad) const;
     std::string string(const char* key, const char* fallback, bool* bad) const;
 };
 
 bool parse_variant(const char* json, Variant* out, std::string* error);
+// A value type by name as the microscaled kernels number it (mx_device.h); sets `bad` and the error for any other.
+int mx_type(const Variant& v, const char* key, const char* fallback, bool* bad);
 // false (with the error set) unless the variant's `coefficients` are absent or (4, 1)
 bool two_stage_coefficients_ok(const Variant& v, const char* symbol);
 
@@ -72,6 +76,7 @@ struct orx_function {
     int M = 0, N = 0, K = 0, E = 0, top_k = 0, H = 0, stride = 0, group = 0, tiles = 0, slots = 0;
     int block_m = 0, block_n = 0, packed_k = 0, algorithm = 0, flags = 0, flags2 = 0;
     int tile_hint = 0;  // projections: row tile preferred while the live rows fit one such tile (0 = none)
+    float weight_scale = 1.f;  // router by scores
     bool out_f32 = false;
     bool input_f16 = false;  // single-row projection that quantises its fp16 activations itself
     bool publish_codes = false; // ... and writes their int8 codes (takes a Q buffer)
@@ -134,6 +139,8 @@ const Registration* gemv_registrations(int* count);
 const Registration* gemm_registrations(int* count);
 const Registration* moe_registrations(int* count);
 const Registration* plane_registrations(int* count);
+const Registration* mx_registrations(int* count);
+int make_router_scores(const Variant& v, bool renormalize, orx_function* f);
 
 template <typename T>
 static inline T* pointer_arg(void** args, int index) {

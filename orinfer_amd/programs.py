@@ -12,7 +12,7 @@ import math
 import numpy as np
 import torch
 
-from . import codebook
+from . import codebook, mxfp4
 from .lib import ORX_ERR_BAD_VARIANT, Kernel, OrxError, current_stream
 
 
@@ -699,3 +699,170 @@ class MoeTokenLayer:
         self.k_combine(stream=s, Expert=self.down_out, Output=self.out, Prob=self.prob, Shared=None, SharedGate=None,
                        SlotMap=self.slot_map)
         return self.out
+
+
+def _check_rows(x, rows, columns, dtype, device, what):
+    if x.dim() != 2 or x.shape[1] != columns or x.dtype != dtype or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor (rows, {columns}) on {device}, not {tuple(x.shape)} {x.dtype} on {x.device}")
+    if isinstance(rows, int) and x.shape[0] != rows:
+        raise ValueError(f"{what} has {x.shape[0]} rows, not {rows}")
+
+
+class _OnDevice:
+    """Launches on the device of the weights, whichever is current; its current stream unless the caller names one."""
+
+    def _call(self, body, *args, stream=None, **named):
+        if torch._C._cuda_getDevice() == self.device.index:
+            return body(*args, stream=current_stream() if stream is None else stream, **named)
+        with torch.cuda.device(self.device):
+            return body(*args, stream=current_stream() if stream is None else stream, **named)
+
+
+class Mxfp4Linear(_OnDevice):
+    """Rows of 16-bit values, quantised to MXFP4, times MXFP4 weights: codes (N, K / 2) and exponents (N, K / 32), both uint8 (the format: mxfp4.py), up to `capacity`
+    rows at a time.  epilogue="swiglu": the upper half of the channels are the up channels of the gate channels in the lower half, and silu(gate) * up comes out.
+    `run` returns a view of the object's own output buffer, which the next call overwrites; one object serves one stream at a time."""
+
+    def __init__(self, codes, exponents, capacity, *, dtype=torch.float16, epilogue="none", scale="floor"):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+        if codes.ndim != 2:
+            raise ValueError("codes must be (N, K / 2)")
+        if not 0 < capacity <= 1 << 24:
+            raise ValueError("capacity must be 1 to 2^24 rows")
+        self.capacity, self.dtype = capacity, dtype
+        channels, self.k = codes.shape[0], 2 * codes.shape[1]
+        self.weight, self.powers = (t.cuda() for t in mxfp4.tiles(codes, exponents, paired=epilogue == "swiglu"))
+        self.device = self.weight.device
+        name = mxfp4.dtype_name(dtype)
+        with torch.cuda.device(self.device):
+            self.projection = Kernel("mxfp4_projection", M=capacity, N=channels, K=self.k, dynamic_rows=True, epilogue=epilogue, output_dtype=name)
+            self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, scale=scale, pad=mxfp4.STEP)
+        self.n = channels // 2 if epilogue == "swiglu" else channels
+        wide = mxfp4.padded(self.k)
+        self.a_q = torch.empty((capacity, wide // 2), dtype=torch.uint8, device=self.device)
+        self.a_s = torch.empty((capacity, wide // mxfp4.BLOCK), dtype=torch.uint8, device=self.device)
+        self.out = torch.empty((capacity, self.n), dtype=dtype, device=self.device)
+
+    def run(self, x, stream=None):
+        _check_rows(x, None, self.k, self.dtype, self.device, "x")
+        rows = x.shape[0]
+        if rows > self.capacity:
+            raise ValueError(f"{rows} rows are more than the capacity of {self.capacity}")
+        if rows:
+            self._call(self._run, x, rows, stream=stream)
+        return self.out.as_strided((rows, self.n), (self.n, 1))
+
+    def _run(self, x, rows, stream):
+        self.quantizer(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=rows)
+        self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, WS=self.powers, m=rows)
+
+
+class Mxfp4MoeLayer(_OnDevice):
+    """Routed experts with MXFP4 weights for `tokens` fp16 rows: router, places of the routes, gate | up with SwiGLU, down, weighted sum.
+
+    gate_up (E, 2 I, H / 2) and gate_up_exponents (E, 2 I, H / 32): gate channels, then up channels; down (E, H, I / 2), down_exponents (E, H, I / 32); uint8.
+    scoring, bias (E fp32 values added for the choice only), groups, top_groups, group_best, renormalize and scale: the router's (k_router_scores.hip); as they stand here, the softmax router.
+    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own.  They work on the object's buffers: one stream at a time."""
+
+    def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, gate_up_exponents, down, down_exponents, *, scoring="softmax", bias=None, groups=1,
+                 top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None):
+        self.tokens, self.experts, self.top_k, self.hidden, self.inter = tokens, experts, top_k, hidden, intermediate
+        if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden // 2) or tuple(down.shape) != (experts, hidden, intermediate // 2):
+            raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden // 2}) and down ({experts}, {hidden}, {intermediate // 2}), "
+                             f"not {tuple(gate_up.shape)} and {tuple(down.shape)}")
+        self.w1, self.p1 = (t.cuda() for t in mxfp4.tiles(gate_up, gate_up_exponents, paired=True))
+        self.w2, self.p2 = (t.cuda() for t in mxfp4.tiles(down, down_exponents))
+        self.device = self.w1.device
+        self.bias = None
+        if bias is not None:
+            self.bias = torch.as_tensor(bias, dtype=torch.float32).to(self.device).contiguous()
+            if self.bias.shape != (experts,):
+                raise ValueError(f"bias must have {experts} values")
+        routes = self.assignments = tokens * top_k
+        if block_m is None:
+            block_m = 16 if routes <= 24 * experts else 32 if routes <= 48 * experts else 64
+        self.block_m = block_m
+        capacity = -(-routes // block_m) + min(experts, routes)
+        common = dict(M=tokens, E=experts, top_k=top_k)
+        scores = dict(scoring=scoring, bias=bias is not None, groups=groups, top_groups=groups if top_groups is None else top_groups, group_best=group_best, scale=scale)
+        plain = scoring == "softmax" and bias is None and groups == 1 and top_groups in (None, 1) and scale == 1.0
+        with torch.cuda.device(self.device):
+            self.k_router = Kernel("router_topk", renormalize=renormalize, **common, **({} if plain else scores))
+            self.k_metadata = Kernel("route_metadata", block_m=block_m, slot_maps=True, workspace=True, tile_units=True, **common)
+            grouped = dict(rows=routes, E=experts, tiles=capacity, block_m=block_m)
+            self.k_quantise_tokens = Kernel("mxfp4_quantization", K=hidden, pad=mxfp4.STEP)
+            self.k_up = Kernel("mxfp4_grouped", N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", **grouped)
+            self.k_quantise_act = Kernel("mxfp4_quantization", K=intermediate, pad=mxfp4.STEP)
+            self.k_down = Kernel("mxfp4_grouped", N=hidden, K=intermediate, **grouped)
+            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, **common)
+            self.segments = self.k_metadata.workspace()
+        i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)
+        f16 = dict(dtype=torch.float16, device=self.device)
+        self.ids = torch.empty((tokens, top_k), **i32)
+        self.prob = torch.empty((tokens, top_k), dtype=torch.float32, device=self.device)
+        self.counts, self.row_offsets, self.tile_offsets = (torch.empty(experts, **i32) for _ in range(3))
+        self.relative, self.slot_map = torch.empty((tokens, top_k), **i32), torch.empty((tokens, top_k), **i32)
+        self.slot_token = torch.empty(routes, **i32)
+        self.tile_count = torch.empty(1, **i32)
+        self.tile_expert, self.tile_row, self.tile_units = torch.empty(capacity, **i32), torch.empty(capacity, **i32), torch.empty((capacity, 4), **i32)
+        wide, inner = mxfp4.padded(hidden), mxfp4.padded(intermediate)
+        self.a_q, self.a_s = torch.empty((tokens, wide // 2), **u8), torch.empty((tokens, wide // 32), **u8)
+        self.h_q, self.h_s = torch.empty((routes, inner // 2), **u8), torch.empty((routes, inner // 32), **u8)
+        self.act = torch.empty((routes, intermediate), **f16)
+        self.down_out = torch.empty((routes, hidden), **f16)
+        self.out = torch.empty((tokens, hidden), **f16)
+
+    def route(self, logits, stream=None):
+        """fp32 logits (tokens, experts) -> the routes' experts (tokens, top_k) int32 and weights fp32."""
+        _check_rows(logits, self.tokens, self.experts, torch.float32, self.device, "logits")
+        self._call(self._route, logits, stream=stream)
+        return self.ids, self.prob
+
+    def _route(self, logits, stream):
+        bias = {} if self.bias is None else {"Bias": self.bias}
+        self.k_router(stream=stream, IDs=self.ids, Logits=logits, Prob=self.prob, **bias)
+
+    def place(self, ids, stream=None):
+        """Experts of every token's routes, int32 in [0, experts) -> the order of the slots: by expert, then by token (`slot_map`, `slot_token`)."""
+        _check_rows(ids, self.tokens, self.top_k, torch.int32, self.device, "ids")
+        self._call(self._place, ids, stream=stream)
+        return self.slot_map
+
+    def _place(self, ids, stream):
+        self.k_metadata(stream=stream, Counts=self.counts, IDs=ids, RelativeSlot=self.relative, RowMax=None, RowOffsets=self.row_offsets, SlotMap=self.slot_map,
+                        SlotToken=self.slot_token, TileCount=self.tile_count, TileExpert=self.tile_expert, TileOffsets=self.tile_offsets, TileRow=self.tile_row,
+                        TileUnits=self.tile_units, Workspace=self.segments)
+
+    def up(self, x, stream=None):
+        """fp16 rows (tokens, hidden) -> silu(gate) * up of every route, fp16 (tokens * top_k, intermediate) in the order of the slots."""
+        _check_rows(x, self.tokens, self.hidden, torch.float16, self.device, "x")
+        self._call(self._up, x, stream=stream)
+        return self.act
+
+    def _up(self, x, stream):
+        self.k_quantise_tokens(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=self.tokens)
+        self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
+
+    def down(self, act, prob, shared=None, shared_gate=None, stream=None):
+        """fp16 rows in the order of the slots and fp32 weights (tokens, top_k) -> fp16 (tokens, hidden): the weighted sum of the routes' second products (rounded to fp16
+        each, as moe_combine takes them) and, where they are given, of sigmoid(shared_gate) (tokens) times shared (tokens, hidden), fp16 both."""
+        _check_rows(act, self.assignments, self.inter, torch.float16, self.device, "act")
+        _check_rows(prob, self.tokens, self.top_k, torch.float32, self.device, "prob")
+        if (shared is None) != (shared_gate is None):
+            raise ValueError("shared and shared_gate go together")
+        if shared is not None:
+            _check_rows(shared, self.tokens, self.hidden, torch.float16, self.device, "shared")
+            _check_rows(shared_gate.view(-1, 1), self.tokens, 1, torch.float16, self.device, "shared_gate")
+        self._call(self._down, act, prob, shared, shared_gate, stream=stream)
+        return self.out
+
+    def _down(self, act, prob, shared, shared_gate, stream):
+        self.k_quantise_act(stream=stream, Q=self.h_q, S=self.h_s, X=act, rows=self.assignments)
+        self.k_down(stream=stream, A=self.h_q, AS=self.h_s, Out=self.down_out, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w2, WS=self.p2)
+        self.k_combine(stream=stream, Expert=self.down_out, Output=self.out, Prob=prob, Shared=shared, SharedGate=shared_gate, SlotMap=self.slot_map)
+
+    def run(self, x, logits, shared=None, shared_gate=None, stream=None):
+        self.route(logits, stream=stream)
+        self.place(self.ids, stream=stream)
+        return self.down(self.up(x, stream=stream), self.prob, shared, shared_gate, stream=stream)
