@@ -9,7 +9,7 @@ def quantise(x, ceil=False, pad=32):
     """x (..., K) -> codes (..., KP / 2) and exponents (..., KP / 32), uint8."""
     x = np.asarray(x, np.float64)
     k = x.shape[-1]
-    wide = np.zeros((*x.shape[:-1], -(-k // pad) * pad))
+    wide = np.zeros((*x.shape[:-1], -(-k // 32) * 32 if pad == 32 else (-(-k // 256) | 1) * 256))  # (for the products an odd multiple of 256)
     wide[..., :k] = x
     blocks = wide.reshape(*x.shape[:-1], -1, 32)
     largest = np.abs(blocks).max(-1)

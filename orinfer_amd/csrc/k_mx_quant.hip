@@ -19,7 +19,6 @@ struct QuantParams {
     int64_t pieces_total;
     uint32_t pieces;  // of a row
     int k, ceil;
-    int whole;  // 16-byte loads: the rows start at multiples of 16 bytes
 };
 
 // largest over the four lanes of a quad
@@ -47,8 +46,8 @@ __global__ __launch_bounds__(kThreads) void mx_quantise_kernel(QuantParams p) {
 #pragma unroll
         for (int j = 0; j < WORDS; ++j) words[i][j] = 0;
         const int64_t offset = row[i] * p.k + first;
-        if (count >= 8 && p.whole) {
-            const mx::v4u* const from = reinterpret_cast<const mx::v4u*>(reinterpret_cast<const uint8_t*>(p.x) + offset * (TYPE == mx::F32 ? 4 : 2));
+        if (count >= 8) {
+            const mx::words4* const from = reinterpret_cast<const mx::words4*>(reinterpret_cast<const uint8_t*>(p.x) + offset * (TYPE == mx::F32 ? 4 : 2));
 #pragma unroll
             for (int j = 0; j < WORDS / 4; ++j) {
                 const mx::v4u four = from[j];
@@ -92,7 +91,6 @@ struct DequantParams {
     int64_t pieces_total;
     uint32_t pieces;
     int k, type;
-    int whole;
 };
 
 __global__ __launch_bounds__(kThreads) void mx_dequantise_kernel(DequantParams p) {
@@ -110,22 +108,20 @@ __global__ __launch_bounds__(kThreads) void mx_dequantise_kernel(DequantParams p
         const uint32_t codes = reinterpret_cast<const uint32_t*>(p.q)[from];
         const uint32_t byte = p.s[from >> 2];
         const float power = __uint_as_float(byte << 23);
-        mx::v4f low, high;
         auto two = [&](auto pair, float& a, float& b) { a = byte == 255u ? __uint_as_float(0x7FC00000u) : pair[0], b = byte == 255u ? __uint_as_float(0x7FC00000u) : pair[1]; };
         float v[8];
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 0), v[0], v[1]);
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 1), v[2], v[3]);
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 2), v[4], v[5]);
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 3), v[6], v[7]);
-        low = mx::v4f{v[0], v[1], v[2], v[3]}, high = mx::v4f{v[4], v[5], v[6], v[7]};
-        if (p.whole && first + 8 <= p.k && p.type != mx::F32) {
-            const mx::v4u eight = {mx::two_values(v[0], v[1], p.type), mx::two_values(v[2], v[3], p.type), mx::two_values(v[4], v[5], p.type),
-                                   mx::two_values(v[6], v[7], p.type)};
-            *reinterpret_cast<mx::v4u*>(reinterpret_cast<unsigned short*>(p.y) + row * p.k + first) = eight;
+        const mx::v4f low = {v[0], v[1], v[2], v[3]}, high = {v[4], v[5], v[6], v[7]};
+        if (p.type != mx::F32) {
+            mx::store_eight_halves(p.y, row * p.k, first, p.k, mx::v4u{mx::two_values(v[0], v[1], p.type), mx::two_values(v[2], v[3], p.type),
+                                                                      mx::two_values(v[4], v[5], p.type), mx::two_values(v[6], v[7], p.type)});
             continue;
         }
-        mx::store_four(p.y, p.type, row * p.k, first, p.k, low, p.whole);
-        mx::store_four(p.y, p.type, row * p.k, first + 4, p.k, high, p.whole);
+        mx::store_four(p.y, p.type, row * p.k, first, p.k, low);
+        mx::store_four(p.y, p.type, row * p.k, first + 4, p.k, high);
     }
 }
 
@@ -142,7 +138,6 @@ int quantise_launch(const orx_function& f, int rows, const Geometry& g, hipStrea
     p.q = pointer_arg<uint8_t>(args, 0), p.s = pointer_arg<uint8_t>(args, 1), p.x = pointer_arg<const void>(args, 2);
     p.pieces = (uint32_t)f.stride / 8, p.pieces_total = (int64_t)rows * p.pieces;
     p.k = f.K, p.ceil = f.flags;
-    p.whole = f.K % (f.algorithm == mx::F32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
     const dim3 grid(g.grid[0]), block(kThreads);
     if (f.algorithm == mx::F16) ORX_LAUNCH(mx_quantise_kernel<mx::F16>, grid, block, 0, s, p);
     else if (f.algorithm == mx::BF16) ORX_LAUNCH(mx_quantise_kernel<mx::BF16>, grid, block, 0, s, p);
@@ -155,7 +150,6 @@ int dequantise_launch(const orx_function& f, int rows, const Geometry& g, hipStr
     p.q = pointer_arg<const uint8_t>(args, 0), p.s = pointer_arg<const uint8_t>(args, 1), p.y = pointer_arg<void>(args, 2);
     p.pieces = (uint32_t)f.stride / 8, p.pieces_total = (int64_t)rows * p.pieces;
     p.k = f.K, p.type = f.algorithm;
-    p.whole = f.K % (f.algorithm == mx::F32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
     ORX_LAUNCH(mx_dequantise_kernel, dim3(g.grid[0]), dim3(kThreads), 0, s, p);
     return hip_check(hipGetLastError(), "launch mxfp4_dequantization");
 }
@@ -172,7 +166,7 @@ int shape(const Variant& v, orx_function* f, const char* type_key) {
         set_error("%s: need 0 < K <= %d and pad 32 or 256", f->symbol.c_str(), kMaxK);
         return ORX_ERR_BAD_VARIANT;
     }
-    f->stride = (f->K + pad - 1) / pad * pad;
+    f->stride = pad == mx::kBlock ? (f->K + 31) / 32 * 32 : ((f->K + 255) / 256 | 1) * 256;  // (for the products an odd multiple)
     f->dynamic_rows = true;
     // (a launch's threads are counted in 32 bits)
     const int most = (int)std::min<int64_t>(1 << 24, ((1ll << 32) / kThreads - 1) * (kThreads * kPieces) / (f->stride / 8));
@@ -233,7 +227,7 @@ const Registration* mx_registrations(int* count) {
         {"mxfp4_projection", make_mx_projection, "M, N, K, dynamic_rows=false, epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
          "A,AS,Out,W,WS[,m]"},
         {"mxfp4_grouped", make_mx_grouped,
-         "rows, E, N, K, tiles, block_m=16|32|64, gather=false, epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
+         "rows, E, N, K, tiles, block_m=16|32|64|128|256, gather=false, epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
          "A,AS,Out[,SlotToken],TileCount,TileUnits,W,WS"},
     };
     *count = (int)(sizeof(rows) / sizeof(rows[0]));

@@ -3,7 +3,10 @@
 //   out[m, n] = sum_k A[m, k] W[n, k], fp32 sums of exact products, rounded once; SwiGLU: columns are pairs of a gate and an up channel.
 // Bound by the weights' bytes, 17/32 each: a wave streams whole tiles (2 KiB of codes, 128 bytes of powers, no LDS in front of the multiplier) and the K steps are dealt to
 // the waves of a workgroup, whose sums meet in LDS.  The weights are the first operand, so a lane ends with four neighbouring channels of one row.
+#include <algorithm>
+
 #include "mx_device.h"
+#include "mx_tiles.h"
 #include "orx_internal.h"
 
 namespace orx {
@@ -78,7 +81,6 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) sums[wave][i * TILES + t][lane] = sum[i][t];
     __syncthreads();
-    const bool whole = p.cols % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (p.type == F32 ? 16 : 8) == 0;
     constexpr int KINDS = SWIGLU ? 2 : 1;
     for (int q = threadIdx.x; q < ROWS * TILES / KINDS * 64; q += WAVES * 64) {
         const int l = q & 63, i = (q >> 6) / (TILES / KINDS), t = (q >> 6) % (TILES / KINDS);
@@ -95,7 +97,7 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
         }
         const int row = 16 * i + (l & 15);
         if (row < rows)
-            store_four(p.out, p.type, (int64_t)(first_row + row) * p.cols, ((group * TILES) / KINDS + t) * 16 + 4 * (l >> 4), p.cols, total[0], whole);
+            store_four(p.out, p.type, (int64_t)(first_row + row) * p.cols, ((group * TILES) / KINDS + t) * 16 + 4 * (l >> 4), p.cols, total[0]);
     }
 }
 
@@ -104,23 +106,56 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
 enum { kSwiglu = 1, kGather = 2 };
 constexpr int kWaves = 4;
 
-int rows_to_a_unit(const orx_function& f, int rows) { return f.E > 0 ? f.block_m : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS (0: the kernel above, 32 of them)
+struct Plan {
+    int rows, channels;
+};
+// us that tiles of one kind take: a start, then what the busiest CU has to do, step by step, or all of them at the rate that they sustain (the clock falls with the power that
+// the multipliers draw).  Measured alone, 256 CUs, M x N x K, us with 64 x 128 / 128 x 128 / 256 x 256: 512 x 4096 x 4096 10.1 / 12.1 / 25.6; 2048 x 4096 x 4096 29.2 / 26.8 / 32.2;
+// 8192 x 4096 x 4096 105 / 91 / 76; 333 x 7168 x 5120 16.3 / 15.6 / 31.9; 1500 x 7168 x 5120 49.4 / 44.7 / 38.1; 512 x 17408 x 5120 40.0 / 43.4 / 35.8; 1024 x 17408 x 5120 74 / 69 / 76.
+double tiles_us(int64_t tiles, int steps, int rows, int channels, double step_us, double petaflops) {
+    const int cus = device_compute_units();
+    const double busiest = (double)((tiles + cus - 1) / cus) * steps * step_us;
+    const double all = (double)tiles * steps * (2e-9 * kStepK * rows * channels) / petaflops * (256.0 / cus);
+    return 2.5 + std::max(busiest, all);
+}
+Plan plan(const orx_function& f, int rows) {
+#ifdef MX_SWEEP
+    const char* force = getenv("MX_FORCE");
+    if (force && rows >= 100) { int r, c; sscanf(force, "%d,%d", &r, &c); if (f.E == 0 || f.block_m == r) return {r, c}; }
+#endif
+    if (f.E > 0) return {f.block_m, f.block_m >= 64 ? (f.block_m == 256 ? 256 : 128) : 0};
+    if (rows <= 64) return {rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 0};
+    const int steps = (f.K + kStepK - 1) / kStepK;
+    const int64_t across = ceil_div(f.slots, 8);
+    const double small = tiles_us(ceil_div(rows, 64) * across, steps, 64, 128, 0.40, 2.6), medium = tiles_us(ceil_div(rows, 128) * across, steps, 128, 128, 0.62, 3.05);
+    const double large = tiles_us((int64_t)ceil_div(rows, 256) * ceil_div(f.slots, 16), steps, 256, 256, 1.75, 3.65);
+    if (large <= medium && large <= small) return {256, 256};
+    return medium <= small ? Plan{128, 128} : Plan{64, 128};
+}
 
 int geometry(const orx_function& f, int rows, Geometry* g) {
-    const int unit = rows_to_a_unit(f, rows);
-    const int64_t units = f.E > 0 ? f.tiles : ceil_div(rows, unit);
-    const int64_t blocks = units * ((f.slots + 1) / 2);
-    if (blocks >= (1ll << 32) / (64 * kWaves)) {
+    const Plan plan = orx::plan(f, rows);
+    const int64_t units = f.E > 0 ? f.tiles : ceil_div(rows, plan.rows);
+    int64_t blocks = units * ceil_div(f.slots, plan.channels ? plan.channels / 16 : 2);
+    if (blocks >= (1ll << 32) / 256) {
         set_error("%s: %d rows of %d channels are more than one launch takes", f.symbol.c_str(), rows, f.N);
         return ORX_ERR_ROWS;
     }
+    if (plan.channels) {
+        blocks = std::min<int64_t>(blocks, (int64_t)device_compute_units() * mx_tiles_to_a_cu(plan.rows));
+        g->block[0] = mx_tiles_threads(plan.rows);
+        g->shared = mx_tiles_lds(plan.rows, plan.channels);
+    } else {
+        g->block[0] = 64 * kWaves;
+    }
     g->grid[0] = (uint32_t)blocks;
-    g->block[0] = 64 * kWaves;
     return ORX_OK;
 }
 
-int launch_rows(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
-    const int unit = rows_to_a_unit(f, rows);
+int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
+    const Plan plan = orx::plan(f, rows);
+    if (plan.channels) return launch_mx_tiles(p, plan.rows, plan.channels, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
     const dim3 grid(g.grid[0]), block(64 * kWaves);
 #define ORX_MX(ROWS)                                                                                                          \
     do {                                                                                                                      \
@@ -132,8 +167,8 @@ int launch_rows(const orx_function& f, int rows, const Geometry& g, hipStream_t 
             else ORX_LAUNCH((mx_rows_kernel<ROWS, 2, kWaves, false, false>), grid, block, 0, s, p);                            \
         }                                                                                                                     \
     } while (0)
-    if (unit == 16) ORX_MX(1);
-    else if (unit == 32) ORX_MX(2);
+    if (plan.rows == 16) ORX_MX(1);
+    else if (plan.rows == 32) ORX_MX(2);
     else ORX_MX(4);
 #undef ORX_MX
     return hip_check(hipGetLastError(), "launch mxfp4 product");
@@ -141,7 +176,7 @@ int launch_rows(const orx_function& f, int rows, const Geometry& g, hipStream_t 
 
 Product product_of(const orx_function& f, int rows) {
     Product p = {};
-    p.m = rows, p.cols = f.H, p.steps = (f.K + kStepK - 1) / kStepK, p.pitch = p.steps * (kStepK / 2), p.tiles = f.slots, p.type = f.algorithm;
+    p.m = rows, p.cols = f.H, p.steps = (f.K + kStepK - 1) / kStepK, p.pitch = (p.steps | 1) * (kStepK / 2), p.tiles = f.slots, p.type = f.algorithm;
     return p;
 }
 
@@ -150,7 +185,7 @@ int projection_launch(const orx_function& f, int rows, const Geometry& g, hipStr
     Product p = product_of(f, rows);
     p.a = pointer_arg<const uint8_t>(args, 0), p.as = pointer_arg<const uint8_t>(args, 1), p.out = pointer_arg<void>(args, 2);
     p.w = pointer_arg<const uint8_t>(args, 3), p.ws = pointer_arg<const uint8_t>(args, 4);
-    return launch_rows(f, rows, g, s, p);
+    return launch_product(f, rows, g, s, p);
 }
 // A, AS, Out[, SlotToken], TileCount, TileUnits, W, WS
 int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
@@ -160,7 +195,7 @@ int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream
     p.slot_token = gather ? pointer_arg<const int>(args, 3) : nullptr;
     p.unit_count = pointer_arg<const int>(args, 3 + gather), p.units = pointer_arg<const int4>(args, 4 + gather);
     p.w = pointer_arg<const uint8_t>(args, 5 + gather), p.ws = pointer_arg<const uint8_t>(args, 6 + gather);
-    return launch_rows(f, rows, g, s, p);
+    return launch_product(f, rows, g, s, p);
 }
 
 int shape(const Variant& v, orx_function* f) {
@@ -213,8 +248,8 @@ int make_mx_grouped(const Variant& v, orx_function* f) {
     if (bad) return ORX_ERR_BAD_VARIANT;
     const int code = shape(v, f);
     if (code != ORX_OK) return code;
-    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 32 && f->block_m != 64)) {
-        set_error("mxfp4_grouped: need rows, E and tiles above 0 and block_m 16, 32 or 64");
+    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 32 && f->block_m != 64 && f->block_m != 128 && f->block_m != 256)) {
+        set_error("mxfp4_grouped: need rows, E and tiles above 0 and block_m 16, 32, 64, 128 or 256");
         return ORX_ERR_BAD_VARIANT;
     }
     f->flags |= gather ? kGather : 0;

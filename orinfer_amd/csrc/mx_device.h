@@ -3,7 +3,8 @@
 // A row is cut into blocks of 32 along K.  A block has one power of two, kept as a byte e for 2^(e - 127) (255: the block is NaN), and 32 codes of a sign, two
 // exponent and one mantissa bits, 0 0.5 1 1.5 2 3 4 6, two to a byte with the even element in the low half.
 //
-// Rows (activations): codes (rows, KP / 2), bytes (rows, KP / 32), KP = K rounded up to whole blocks, or to 256 for the products; what is behind K is zero.
+// Rows (activations): codes (rows, KP / 2), bytes (rows, KP / 32), KP = K rounded up to whole blocks, or for the products
+// to an odd multiple of 256; what is behind K is zero.  (Odd: rows that lie a multiple of 4 KiB apart meet in few channels of the L2.)
 // Tiles (weights, laid out once): 16 channels x 256 K are 2048 bytes of codes, [block 0..7][channel][16 bytes], and 128 bytes of powers,
 // [channel][block & 1][block >> 1]; tiles of one 16 channels lie along K behind one another.  One 16-byte piece is what a lane holds of an operand of v_mfma_scale_f32_*_f8f6f4
 // with 4-bit codes: 32 elements of one row, whose one power comes from a byte of the lane's scale register.  So a wave's load of an operand is whole kilobytes,
@@ -116,29 +117,41 @@ __device__ __forceinline__ uint32_t two_values(float a, float b, int type) {
     return __builtin_bit_cast(uint32_t, bf2v{(__bf16)a, (__bf16)b});
 }
 
-// Four neighbouring results of a row from column `col` on, of `cols` columns; whole: the address of every such four is a multiple of their size.
-__device__ __forceinline__ void store_four(void* out, int type, int64_t row_start, int col, int cols, v4f v, bool whole) {
-    if (col >= cols) return;
+// Neighbouring results of a row from column `col` on, of `cols` columns: a store for all of them at any address of the type's own alignment (this target's memory
+// instructions take it), those of a last, short piece one after another.
+typedef unsigned int words2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned int words4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float floats4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void store_eight_halves(void* out, int64_t row_start, int col, int cols, v4u v) {
+    unsigned short* to = reinterpret_cast<unsigned short*>(out) + row_start + col;
+    if (col + 8 <= cols) {
+        *reinterpret_cast<words4*>(to) = v;
+    } else {
+#pragma unroll 1
+        for (; col < cols; ++col) {
+            *to++ = (unsigned short)v[0];
+            v = v4u{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+        }
+    }
+}
+__device__ __forceinline__ void store_four(void* out, int type, int64_t row_start, int col, int cols, v4f v) {
     if (type == F32) {
-        float* const to = reinterpret_cast<float*>(out) + row_start + col;
-        if (whole && col + 4 <= cols) {
-            *reinterpret_cast<v4f*>(to) = v;
+        float* to = reinterpret_cast<float*>(out) + row_start + col;
+        if (col + 4 <= cols) {
+            *reinterpret_cast<floats4*>(to) = v;
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < cols) to[i] = v[i];
+#pragma unroll 1
+            for (; col < cols; ++col) *to++ = v[0], v = v4f{v[1], v[2], v[3], 0.f};
         }
         return;
     }
-    unsigned short* const to = reinterpret_cast<unsigned short*>(out) + row_start + col;
-    const uint32_t low = two_values(v[0], v[1], type), high = two_values(v[2], v[3], type);
-    if (whole && col + 4 <= cols) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(low, high);
+    unsigned short* to = reinterpret_cast<unsigned short*>(out) + row_start + col;
+    uint32_t low = two_values(v[0], v[1], type), high = two_values(v[2], v[3], type);
+    if (col + 4 <= cols) {
+        *reinterpret_cast<words2*>(to) = words2{low, high};
     } else {
-        to[0] = (unsigned short)low;
-        if (col + 1 < cols) to[1] = (unsigned short)(low >> 16);
-        if (col + 2 < cols) to[2] = (unsigned short)high;
-        if (col + 3 < cols) to[3] = (unsigned short)(high >> 16);
+#pragma unroll 1
+        for (; col < cols; ++col) *to++ = (unsigned short)low, low = __builtin_amdgcn_alignbit(high, low, 16), high >>= 16;
     }
 }
 

@@ -11,7 +11,7 @@ import torch
 from .lib import Kernel
 
 BLOCK = 32   # elements to a power
-STEP = 256   # K of a tile: the products take rows padded to this
+STEP = 256   # K of a tile; the products take rows padded to an odd multiple of it
 DTYPES = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}
 
 
@@ -22,7 +22,10 @@ def dtype_name(dtype):
 
 
 def padded(k, pad=STEP):
-    return -(-k // pad) * pad
+    """K as rows are stored: whole blocks (pad 32), or an odd multiple of 256 (pad 256: for the products; at even distances rows meet in few channels of the L2)."""
+    if pad not in (BLOCK, STEP):
+        raise ValueError("pad must be 32 or 256")
+    return -(-k // BLOCK) * BLOCK if pad == BLOCK else (-(-k // STEP) | 1) * STEP
 
 
 @functools.lru_cache(maxsize=256)
@@ -31,7 +34,7 @@ def _kernel(symbol, **variant):
 
 
 def quantize(x, scale="floor", pad=BLOCK):
-    """x (..., K) of fp16, bf16 or fp32 values on the GPU -> codes (..., KP / 2), exponents (..., KP / 32), KP = K rounded up to `pad` (32 or 256; zeros behind K).
+    """x (..., K) of fp16, bf16 or fp32 values on the GPU -> codes (..., KP / 2), exponents (..., KP / 32), KP = padded(K, pad), zeros behind K.
     scale: "floor" takes the power of two of a block's largest magnitude (what is above 6 of its units saturates), "ceil" the smallest that nothing saturates with.
     Blocks with an infinity or NaN become NaN."""
     if not x.is_cuda:
@@ -86,7 +89,7 @@ def tiles(codes, exponents, paired=False):
         t = t.unflatten(-2, (-1, 16))
         return t.transpose(-4, -3).flatten(-4, -3) if paired else t  # (..., tiles, 16, columns)
 
-    steps = padded(k) // STEP
+    steps = -(-k // STEP)
     codes = torch.nn.functional.pad(rows(codes), (0, 128 * steps - half_k)).unflatten(-1, (steps, 8, 16))          # (..., tiles, 16, steps, 8, 16)
     exponents = torch.nn.functional.pad(rows(exponents), (0, 8 * steps - k // BLOCK)).unflatten(-1, (steps, 4, 2))  # (..., tiles, 16, steps, 4, 2)
     codes = codes.movedim(-4, -2).contiguous()                               # (..., tiles, steps, 8, 16, 16)

@@ -143,7 +143,8 @@ def test_linear_with_swiglu(rows, n, k, dtype):
     check(linear.run(x), want, bound, dtype)
 
 
-@pytest.mark.parametrize("rows,n,k", [(1, 9728, 2560), (4, 17408, 5120), (40, 5120, 17408), (1000, 640, 4096), (2049, 520, 768), (513, 4096, 512)])
+@pytest.mark.parametrize("rows,n,k", [(1, 9728, 2560), (4, 17408, 5120), (40, 5120, 17408), (1000, 640, 4096), (2049, 520, 768), (513, 4096, 512), (2300, 2200, 544),
+                                      (2049, 4097, 288)])
 def test_linear_of_large_shapes(rows, n, k):
     linear, x, want, bound = linear_case(rows, n, k, torch.bfloat16)
     check(linear.run(x), want, bound, torch.bfloat16)
@@ -232,7 +233,7 @@ SHAPES = [(1, 8, 2, 64, 32), (3, 16, 4, 256, 96), (5, 128, 8, 512, 64), (40, 8, 
 
 
 @pytest.mark.parametrize("tokens,experts,top_k,hidden,inner", SHAPES)
-@pytest.mark.parametrize("block_m", [None, 16, 32, 64])
+@pytest.mark.parametrize("block_m", [None, 16, 32, 64, 128, 256])
 def test_experts(tokens, experts, top_k, hidden, inner, block_m):
     layer, gate_up, down, x, logits, rng = moe_case(tokens, experts, top_k, hidden, inner, skew=1.1, block_m=block_m)
     layer.act.fill_(-7)

@@ -122,9 +122,18 @@ def test_rows_outside_the_capacity_and_bad_pointers_are_refused_before_anything_
 def test_records_name_the_kernel_that_runs():
     for kernel in (lib.Kernel("mxfp4_projection", M=200, N=96, K=320, dynamic_rows=True), lib.Kernel("mxfp4_grouped", **GROUPED),
                    lib.Kernel("mxfp4_quantization", K=64, M=300), lib.Kernel("router_topk", **ROUTER, scoring="sigmoid")):
-        rows = (1, 17, 64, 200) if kernel.symbol == "mxfp4_projection" else (0,)
+        rows = (1, 17, 64, 65, 200) if kernel.symbol == "mxfp4_projection" else (0,)
         for r in rows:
             assert reported(kernel, r) in started(kernel, r)
+
+
+def test_a_projection_takes_larger_tiles_where_there_are_more():
+    """Threads and LDS of the kernel by rows (without a device 256 CUs are taken)."""
+    linear = lib.Kernel("mxfp4_projection", M=8192, N=4096, K=4096, dynamic_rows=True)
+    assert [started(linear, rows)[0][1:] for rows in (64, 65, 512, 2048, 8192)] == [(256, 0), (256, 52224), (256, 52224), (256, 69632), (512, 139264)]
+    assert all(len(started(linear, rows)) == 1 for rows in (1, 64, 65, 8192))
+    for block_m, lds in ((16, 0), (32, 0), (64, 52224), (128, 69632), (256, 139264)):
+        assert started(lib.Kernel("mxfp4_grouped", **GROUPED, block_m=block_m))[0][2] == lds
 
 
 def test_oracle_routes_by_hand():
