@@ -1,8 +1,10 @@
 // Products of few rows with MXFP4 weights (dense and routed experts), and the symbols of both.
 //
 //   out[m, n] = sum_k A[m, k] W[n, k], fp32 sums of exact products, rounded once; SwiGLU: columns are pairs of a gate and an up channel.
-// Bound by the weights' bytes, 17/32 each: a wave streams whole tiles (2 KiB of codes, 128 bytes of powers, no LDS in front of the multiplier) and the K steps are dealt to
-// the waves of a workgroup, whose sums meet in LDS.  The weights are the first operand, so a lane ends with four neighbouring channels of one row.
+// Bound by the weights' bytes, 17/32 each: a wave streams whole tiles (2 KiB of codes, 128 bytes of powers) into registers; the K steps are dealt to the waves of a workgroup,
+// whose sums meet in LDS.  The weights are the first operand, so a lane ends with four neighbouring channels of one row.  Dense rows come as tiles too: as rows of 128 bytes a step they
+// took as long as the weights (weights out of cache, 17408 x 5120: 32 rows 16.7 us, as tiles 12.6, 64 rows 25.0 / 16.6).
+// Rows of 16-bit values (QUANTISE, up to 16): a workgroup makes their codes itself, into LDS, while its first weights are on their way.
 #include <algorithm>
 
 #include "mx_device.h"
@@ -14,11 +16,23 @@ namespace {
 
 using namespace mx;
 
-// ROWS blocks of 16 rows, TILES tiles of 16 channels (SwiGLU: gate and up in turn) to a workgroup of WAVES waves
-template <int ROWS, int TILES, int WAVES, bool GROUPED, bool SWIGLU>
+// 16 or 4 bytes of a lane from a buffer of `bytes`; what lies behind its end reads as 0 and is not fetched.
+struct Buffer {
+    __amdgpu_buffer_rsrc_t from;
+    __device__ __forceinline__ Buffer(const uint8_t* base, int bytes) : from(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, bytes, 0x00027000)) {}
+    __device__ __forceinline__ v4i load_16(int offset) const { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0)); }
+    __device__ __forceinline__ int load_4(int offset) const { return (int)__builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0); }
+};
+
+enum Source { Codes = 0, Halves = 1, Brains = 2 };  // of the rows: codes, fp16, bf16
+
+// ROWS blocks of 16 rows, two tiles of 16 channels (SwiGLU: gate and up) to a workgroup of WAVES waves
+template <int ROWS, int WAVES, int SOURCE, bool GROUPED, bool SWIGLU>
 __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
-    static_assert(!SWIGLU || TILES % 2 == 0, "pairs");
-    __shared__ v4f sums[WAVES][ROWS * TILES][64];
+    constexpr int TILES = 2;
+    static_assert(SOURCE == Codes || ROWS == 1, "few rows are quantised here");
+    extern __shared__ __align__(16) uint8_t lds[];  // sums; in front of them the rows' codes and powers where they are made here
+    v4f(*const sums)[ROWS * TILES][64] = reinterpret_cast<v4f(*)[ROWS * TILES][64]>(lds);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int groups = (p.tiles + TILES - 1) / TILES;
@@ -28,54 +42,119 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
     if (GROUPED) {
         if (unit >= *p.unit_count) return;
         const int4 u = p.units[unit];
-        first_row = u.y, rows = u.z;
-        w += (int64_t)u.x * p.tiles * p.steps * kTileBytes, ws += (int64_t)u.x * p.tiles * p.steps * kTilePowers;
+        first_row = __builtin_amdgcn_readfirstlane(u.y), rows = __builtin_amdgcn_readfirstlane(u.z);
+        const int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane(u.x) * p.tiles * p.steps;
+        w += tile * kTileBytes, ws += tile * kTilePowers;
     }
-    const int r = lane & 15, low = (lane >> 4) & 1, half = lane >> 5;  // lane's channel or row; its blocks 4 half + low and + 2 of every step
-    const uint8_t *a[ROWS], *as[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        int64_t row = first_row + min(16 * i + r, rows - 1);  // (rows that are not there repeat the last: their sums go nowhere)
+    auto row_at = [&](int local) {
+        int64_t row = first_row + min(local, rows - 1);  // (rows that are not there repeat the last: their sums go nowhere)
         if (GROUPED && p.slot_token != nullptr) row = p.slot_token[row];
-        a[i] = p.a + row * p.pitch + (4 * half + low) * 16;
-        as[i] = p.as + row * (p.pitch / 16) + 4 * half;
-    }
-    const uint8_t *wt[TILES], *wst[TILES];
+        return row;
+    };
+    const int r = lane & 15, block = lane >> 4;  // lane's channel or row; its blocks of a step, and 4 behind
+
+    // ---- weights on their way ----
+    const int w_lane = lane * 16, ws_lane = r * 8 + (block & 1) * 4, ws_shift = (block >> 1) * 8;
+    const uint32_t in_row = 0x0400u + 0x0101u * block;  // a row's eight powers: this lane's two, for v_perm
+    struct Step {
+        v4i w[TILES][2], a[ROWS][2];
+        int wp[TILES];
+        uint2 ap[ROWS];
+    };
+    const uint8_t *a[ROWS], *as[ROWS];
+    if constexpr (SOURCE == Codes) {
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const int64_t tile = min(group * TILES + t, p.tiles - 1);
-        wt[t] = w + tile * p.steps * kTileBytes + (4 * half + low) * 256 + r * 16;
-        wst[t] = ws + tile * p.steps * kTilePowers + r * 8 + low * 4 + half * 2;
+        for (int i = 0; i < ROWS; ++i) {
+            if constexpr (GROUPED) {
+                const int64_t row = row_at(16 * i + r);
+                a[i] = p.a + row * p.pitch + block * 16;
+                as[i] = p.as + row * (p.pitch / 16);
+            } else {
+                const int64_t tile = min(first_row / 16 + i, (p.m - 1) / 16);
+                a[i] = p.a + tile * p.steps * kTileBytes + lane * 16;
+                as[i] = p.as + tile * p.steps * kTilePowers + ws_lane;
+            }
+        }
     }
+    auto load = [&](Step& s, int step) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int64_t tile = min(group * TILES + t, p.tiles - 1);
+            const Buffer codes(w + tile * p.steps * kTileBytes, p.steps * kTileBytes), powers(ws + tile * p.steps * kTilePowers, p.steps * kTilePowers);
+            s.w[t][0] = codes.load_16(w_lane + step * kTileBytes);
+            s.w[t][1] = codes.load_16(w_lane + step * kTileBytes + 1024);
+            s.wp[t] = powers.load_4(ws_lane + step * kTilePowers);
+        }
+        if constexpr (SOURCE == Codes) {
+            const int there = min(step, p.steps - 1);  // (behind the last step the weights are 0)
+            constexpr int STEP = GROUPED ? 128 : kTileBytes, SECOND = GROUPED ? 64 : 1024;
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                s.a[i][0] = *reinterpret_cast<const v4i*>(a[i] + there * STEP);
+                s.a[i][1] = *reinterpret_cast<const v4i*>(a[i] + there * STEP + SECOND);
+                if constexpr (GROUPED) s.ap[i] = *reinterpret_cast<const uint2*>(as[i] + there * 8);
+                else s.ap[i].x = *reinterpret_cast<const uint32_t*>(as[i] + there * kTilePowers);
+            }
+        }
+    };
+    Step held;
+    load(held, wave);
+
+    // ---- the rows' codes ----
+    const int live = min(rows, 16);
+    uint8_t* const codes = lds;
+    uint8_t* const powers = lds + p.steps * 128 * live;
+    if constexpr (SOURCE != Codes) {
+        constexpr int TYPE = SOURCE == Halves ? F16 : BF16;
+        const int pieces = p.steps * 32;  // of eight values, of a row
+        for (int at = threadIdx.x; at < live * pieces; at += WAVES * 64) {
+            const int row = at / pieces, piece = at - row * pieces;
+            v4u words = {0, 0, 0, 0};
+            if (piece * 8 < p.k) words = *reinterpret_cast<const words4*>(reinterpret_cast<const uint16_t*>(p.a) + row_at(row) * p.k + piece * 8);
+            uint32_t two = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) two = pair_max(two, words[j]);
+            const uint32_t byte = power_byte<TYPE>(quad_max(max(two & 0xFFFFu, two >> 16)), false);
+            const uint32_t four[4] = {words[0], words[1], words[2], words[3]};
+            *reinterpret_cast<uint32_t*>(codes + ((piece >> 2) * live + row) * 16 + (piece & 3) * 4) = eight_codes<TYPE>(four, byte);
+            if ((piece & 3) == 0) powers[((piece >> 5) * live + row) * 8 + ((piece >> 2) & 7)] = (uint8_t)byte;
+        }
+        __syncthreads();
+    }
+
     v4f sum[ROWS][TILES];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
 #pragma unroll
         for (int t = 0; t < TILES; ++t) sum[i][t] = v4f{0, 0, 0, 0};
-    for (int step = wave; step < p.steps; step += WAVES) {
-        v4i wc[TILES][2], ac[ROWS][2];
-        int wp[TILES], ap[ROWS];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const uint8_t* const from = wt[t] + (int64_t)step * kTileBytes;
-            wc[t][0] = *reinterpret_cast<const v4i*>(from);
-            wc[t][1] = *reinterpret_cast<const v4i*>(from + 512);
-            wp[t] = *reinterpret_cast<const unsigned short*>(wst[t] + (int64_t)step * kTilePowers);
+    auto multiply = [&](Step& s, int step) {
+        if constexpr (SOURCE != Codes) {
+            const int there = min(step, p.steps - 1), row = min(r, live - 1);
+            const uint8_t* const from = codes + ((there * 8 + block) * live + row) * 16;
+            s.a[0][0] = *reinterpret_cast<const v4i*>(from);
+            s.a[0][1] = *reinterpret_cast<const v4i*>(from + 4 * live * 16);
+            s.ap[0] = *reinterpret_cast<const uint2*>(powers + (there * live + row) * 8);
         }
+        int wp[TILES];  // bytes 0 and 2, or 0 and 1, are this lane's
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) wp[t] = (int)((uint32_t)s.wp[t] >> ws_shift);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            ac[i][0] = *reinterpret_cast<const v4i*>(a[i] + step * 128);
-            ac[i][1] = *reinterpret_cast<const v4i*>(a[i] + step * 128 + 32);
-            ap[i] = *reinterpret_cast<const int*>(as[i] + step * 8) >> (8 * low);
-        }
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i)
+            constexpr bool TILED = SOURCE == Codes && !GROUPED;
+            const int ap = TILED ? (int)(s.ap[i].x >> ws_shift) : (int)__builtin_amdgcn_perm(s.ap[i].y, s.ap[i].x, in_row);
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                sum[i][t] = multiply_16<0, 0>(wc[t][0], ac[i][0], sum[i][t], wp[t], ap[i]);
-                sum[i][t] = multiply_16<1, 2>(wc[t][1], ac[i][1], sum[i][t], wp[t], ap[i]);
+                sum[i][t] = multiply_16<0, 0>(s.w[t][0], s.a[i][0], sum[i][t], wp[t], ap);
+                sum[i][t] = multiply_16<2, TILED ? 2 : 1>(s.w[t][1], s.a[i][1], sum[i][t], wp[t], ap);
             }
+        }
+    };
+#pragma unroll 1
+    for (int step = wave; step < p.steps; step += WAVES) {
+        multiply(held, step);
+        load(held, step + WAVES);
     }
+    if constexpr (SOURCE != Codes) __syncthreads();  // (the sums take the codes' place)
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
 #pragma unroll
@@ -103,13 +182,17 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
 // slots used: M (rows; experts: slots), N, K, E, tiles (units), block_m, flags (kSwiglu, kGather), algorithm (output type), H (output columns), slots (16-channel tiles)
+// packed_k (source of the rows)
+constexpr int kMostLds = 80 * 1024;  // of the few-rows kernel
 enum { kSwiglu = 1, kGather = 2 };
-constexpr int kWaves = 4;
 
-// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS (0: the kernel above, 32 of them)
+// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS (0: the kernel above, 32 of them) or its waves
 struct Plan {
-    int rows, channels;
+    int rows, channels, waves;
 };
+// Eight waves where every CU has a workgroup or less, else four (weights out of cache, us with four / eight: 7168 x 5120, 224 workgroups, 16 rows 5.0 / 5.3, 32 rows 7.1 / 6.7, 64 rows
+// 8.8 / 7.4; 5120 x 17408, 160, 13.9 / 12.4, 25 / 19, 36 / 18; 9728 x 2560, 304, 4.6 / 5.2, 5.6 / 5.9, 7.3 / 7.0; 17408 x 5120, 544, 11.9 / 12.1, 12.6 / 13.6, 16.6 / 17.8).
+Plan few_rows(int unit_rows, int64_t workgroups) { return {unit_rows, 0, workgroups > device_compute_units() ? 4 : 8}; }
 // us that tiles of one kind take: a start, then what the busiest CU has to do, step by step, or all of them at the rate that they sustain (the clock falls with the power that
 // the multipliers draw).  Measured alone, 256 CUs, M x N x K, us with 64 x 128 / 128 x 128 / 256 x 256: 512 x 4096 x 4096 10.1 / 12.1 / 25.6; 2048 x 4096 x 4096 29.2 / 26.8 / 32.2;
 // 8192 x 4096 x 4096 105 / 91 / 76; 333 x 7168 x 5120 16.3 / 15.6 / 31.9; 1500 x 7168 x 5120 49.4 / 44.7 / 38.1; 512 x 17408 x 5120 40.0 / 43.4 / 35.8; 1024 x 17408 x 5120 74 / 69 / 76.
@@ -120,18 +203,27 @@ double tiles_us(int64_t tiles, int steps, int rows, int channels, double step_us
     return 2.5 + std::max(busiest, all);
 }
 Plan plan(const orx_function& f, int rows) {
+    const int pairs = (f.slots + 1) / 2;
 #ifdef MX_SWEEP
     const char* force = getenv("MX_FORCE");
-    if (force && rows >= 100) { int r, c; sscanf(force, "%d,%d", &r, &c); if (f.E == 0 || f.block_m == r) return {r, c}; }
+    if (force && f.E == 0 && f.packed_k == Codes && rows > 16) { int r, c; sscanf(force, "%d,%d", &r, &c); if (c) return {r, c, 0}; return few_rows(r, (int64_t)pairs * ceil_div(rows, r)); }
 #endif
-    if (f.E > 0) return {f.block_m, f.block_m >= 64 ? (f.block_m == 256 ? 256 : 128) : 0};
-    if (rows <= 64) return {rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 0};
+    if (f.E > 0) {
+        if (f.block_m < 64) return few_rows(f.block_m, (int64_t)pairs * std::min(f.tiles, f.E));
+        return {f.block_m, f.block_m == 256 ? 256 : 128, 0};
+    }
+    if (rows <= 64) return few_rows(rows <= 16 ? 16 : rows <= 32 ? 32 : 64, pairs);
     const int steps = (f.K + kStepK - 1) / kStepK;
     const int64_t across = ceil_div(f.slots, 8);
     const double small = tiles_us(ceil_div(rows, 64) * across, steps, 64, 128, 0.40, 2.6), medium = tiles_us(ceil_div(rows, 128) * across, steps, 128, 128, 0.62, 3.05);
     const double large = tiles_us((int64_t)ceil_div(rows, 256) * ceil_div(f.slots, 16), steps, 256, 256, 1.75, 3.65);
-    if (large <= medium && large <= small) return {256, 256};
-    return medium <= small ? Plan{128, 128} : Plan{64, 128};
+    if (large <= medium && large <= small) return {256, 256, 0};
+    return medium <= small ? Plan{128, 128, 0} : Plan{64, 128, 0};
+}
+uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
+    const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * 2 * 1024;
+    const uint32_t codes = f.packed_k == Codes ? 0 : (uint32_t)((f.K + kStepK - 1) / kStepK) * 136 * std::min(f.E > 0 ? 16 : rows, 16);
+    return std::max(sums, codes);
 }
 
 int geometry(const orx_function& f, int rows, Geometry* g) {
@@ -147,55 +239,71 @@ int geometry(const orx_function& f, int rows, Geometry* g) {
         g->block[0] = mx_tiles_threads(plan.rows);
         g->shared = mx_tiles_lds(plan.rows, plan.channels);
     } else {
-        g->block[0] = 64 * kWaves;
+        g->block[0] = 64 * plan.waves;
+        g->shared = few_rows_lds(f, rows, plan);
     }
     g->grid[0] = (uint32_t)blocks;
     return ORX_OK;
 }
 
+template <int ROWS, int WAVES, int SOURCE, bool GROUPED, bool SWIGLU>
+int launch_one(const Product& p, const Geometry& g, hipStream_t s) {
+    constexpr auto kernel = &mx_rows_kernel<ROWS, WAVES, SOURCE, GROUPED, SWIGLU>;
+    static DeviceOnce ready;
+    const int code = ready.run([] { return hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds), "hipFuncSetAttribute"); });
+    if (code != ORX_OK) return code;
+    ORX_LAUNCH(kernel, dim3(g.grid[0]), dim3(64 * WAVES), g.shared, s, p);
+    return hip_check(hipGetLastError(), "launch mxfp4 product");
+}
+template <int ROWS, int WAVES, int SOURCE>
+int launch_of(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
+    const bool swiglu = f.flags & kSwiglu;
+    if constexpr (SOURCE != Brains)
+        if (f.E > 0) return swiglu ? launch_one<ROWS, WAVES, SOURCE, true, true>(p, g, s) : launch_one<ROWS, WAVES, SOURCE, true, false>(p, g, s);
+    return swiglu ? launch_one<ROWS, WAVES, SOURCE, false, true>(p, g, s) : launch_one<ROWS, WAVES, SOURCE, false, false>(p, g, s);
+}
+template <int WAVES>
+int launch_rows(const orx_function& f, const Plan& plan, const Product& p, const Geometry& g, hipStream_t s) {
+    if (f.packed_k == Halves) return launch_of<1, WAVES, Halves>(f, p, g, s);
+    if (f.packed_k == Brains) return launch_of<1, WAVES, Brains>(f, p, g, s);
+    if (plan.rows == 16) return launch_of<1, WAVES, Codes>(f, p, g, s);
+    return plan.rows == 32 ? launch_of<2, WAVES, Codes>(f, p, g, s) : launch_of<4, WAVES, Codes>(f, p, g, s);
+}
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
     if (plan.channels) return launch_mx_tiles(p, plan.rows, plan.channels, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
-    const dim3 grid(g.grid[0]), block(64 * kWaves);
-#define ORX_MX(ROWS)                                                                                                          \
-    do {                                                                                                                      \
-        if (f.E > 0) {                                                                                                        \
-            if (f.flags & kSwiglu) ORX_LAUNCH((mx_rows_kernel<ROWS, 2, kWaves, true, true>), grid, block, 0, s, p);            \
-            else ORX_LAUNCH((mx_rows_kernel<ROWS, 2, kWaves, true, false>), grid, block, 0, s, p);                             \
-        } else {                                                                                                              \
-            if (f.flags & kSwiglu) ORX_LAUNCH((mx_rows_kernel<ROWS, 2, kWaves, false, true>), grid, block, 0, s, p);           \
-            else ORX_LAUNCH((mx_rows_kernel<ROWS, 2, kWaves, false, false>), grid, block, 0, s, p);                            \
-        }                                                                                                                     \
-    } while (0)
-    if (plan.rows == 16) ORX_MX(1);
-    else if (plan.rows == 32) ORX_MX(2);
-    else ORX_MX(4);
-#undef ORX_MX
-    return hip_check(hipGetLastError(), "launch mxfp4 product");
+    return plan.waves == 4 ? launch_rows<4>(f, plan, p, g, s) : launch_rows<8>(f, plan, p, g, s);
 }
 
 Product product_of(const orx_function& f, int rows) {
     Product p = {};
-    p.m = rows, p.cols = f.H, p.steps = (f.K + kStepK - 1) / kStepK, p.pitch = (p.steps | 1) * (kStepK / 2), p.tiles = f.slots, p.type = f.algorithm;
+    p.m = rows, p.cols = f.H, p.k = f.K, p.steps = (f.K + kStepK - 1) / kStepK, p.pitch = (p.steps | 1) * (kStepK / 2), p.tiles = f.slots, p.type = f.algorithm;
     return p;
 }
 
-// A, AS, Out, W, WS[, m]
+// A[, AS], Out, W, WS[, m]
 int projection_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
     Product p = product_of(f, rows);
-    p.a = pointer_arg<const uint8_t>(args, 0), p.as = pointer_arg<const uint8_t>(args, 1), p.out = pointer_arg<void>(args, 2);
-    p.w = pointer_arg<const uint8_t>(args, 3), p.ws = pointer_arg<const uint8_t>(args, 4);
+    const int codes = f.packed_k == Codes ? 1 : 0;
+    p.a = pointer_arg<const uint8_t>(args, 0), p.as = codes ? pointer_arg<const uint8_t>(args, 1) : nullptr, p.out = pointer_arg<void>(args, 1 + codes);
+    p.w = pointer_arg<const uint8_t>(args, 2 + codes), p.ws = pointer_arg<const uint8_t>(args, 3 + codes);
     return launch_product(f, rows, g, s, p);
 }
-// A, AS, Out[, SlotToken], TileCount, TileUnits, W, WS
+// A[, AS], Out[, SlotToken], TileCount, TileUnits, W, WS
 int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
     Product p = product_of(f, rows);
-    const int gather = f.flags & kGather ? 1 : 0;
-    p.a = pointer_arg<const uint8_t>(args, 0), p.as = pointer_arg<const uint8_t>(args, 1), p.out = pointer_arg<void>(args, 2);
-    p.slot_token = gather ? pointer_arg<const int>(args, 3) : nullptr;
-    p.unit_count = pointer_arg<const int>(args, 3 + gather), p.units = pointer_arg<const int4>(args, 4 + gather);
-    p.w = pointer_arg<const uint8_t>(args, 5 + gather), p.ws = pointer_arg<const uint8_t>(args, 6 + gather);
+    const int codes = f.packed_k == Codes ? 1 : 0, gather = f.flags & kGather ? 1 : 0;
+    p.a = pointer_arg<const uint8_t>(args, 0), p.as = codes ? pointer_arg<const uint8_t>(args, 1) : nullptr, p.out = pointer_arg<void>(args, 1 + codes);
+    p.slot_token = gather ? pointer_arg<const int>(args, 2 + codes) : nullptr;
+    const int at = 2 + codes + gather;
+    p.unit_count = pointer_arg<const int>(args, at), p.units = pointer_arg<const int4>(args, at + 1);
+    p.w = pointer_arg<const uint8_t>(args, at + 2), p.ws = pointer_arg<const uint8_t>(args, at + 3);
     return launch_product(f, rows, g, s, p);
+}
+void row_arguments(orx_function* f) {
+    f->args = {{"A", ArgPointer, f->packed_k == Codes ? 16u : 2u}};
+    if (f->packed_k == Codes) f->args.push_back({"AS", ArgPointer, 8});
+    f->args.push_back({"Out", ArgPointer, f->algorithm == F32 ? 4u : 2u});
 }
 
 int shape(const Variant& v, orx_function* f) {
@@ -203,7 +311,14 @@ int shape(const Variant& v, orx_function* f) {
     f->N = (int)v.integer("N", 0, &bad), f->K = (int)v.integer("K", 0, &bad);
     const std::string epilogue = v.string("epilogue", "none", &bad);
     f->algorithm = mx_type(v, "output_dtype", "float16", &bad);
+    // 16-bit rows are quantised on their way (few rows)
+    const std::string input = v.string("input_dtype", "mxfp4", &bad);
     if (bad) return ORX_ERR_BAD_VARIANT;
+    if (input != "mxfp4" && input != "float16" && (input != "bfloat16" || f->E > 0)) {
+        set_error("%s: input_dtype must be mxfp4 or float16%s", f->symbol.c_str(), f->E > 0 ? "" : " or bfloat16");
+        return ORX_ERR_BAD_VARIANT;
+    }
+    f->packed_k = input == "mxfp4" ? Codes : input == "float16" ? Halves : Brains;
     if (epilogue != "none" && epilogue != "swiglu") {
         set_error("%s: epilogue must be none or swiglu", f->symbol.c_str());
         return ORX_ERR_BAD_VARIANT;
@@ -234,7 +349,12 @@ int make_mx_projection(const Variant& v, orx_function* f) {
         return ORX_ERR_BAD_VARIANT;
     }
     f->capacity = f->M;
-    f->args = {{"A", ArgPointer, 16}, {"AS", ArgPointer, 8}, {"Out", ArgPointer, f->algorithm == F32 ? 4u : 2u}, {"W", ArgPointer, 16}, {"WS", ArgPointer, 8}};
+    if (f->packed_k != Codes && (f->M > 16 || few_rows_lds(*f, f->M, {16, 0, 8}) > (uint32_t)kMostLds)) {
+        set_error("mxfp4_projection: 16-bit rows go with M up to 16 and codes of all rows up to %d bytes", kMostLds);
+        return ORX_ERR_BAD_VARIANT;
+    }
+    row_arguments(f);
+    f->args.push_back({"W", ArgPointer, 16}), f->args.push_back({"WS", ArgPointer, 8});
     if (f->dynamic_rows) f->args.push_back({"m", ArgI32, 4});
     f->launch = projection_launch;
     return ORX_OK;
@@ -254,7 +374,11 @@ int make_mx_grouped(const Variant& v, orx_function* f) {
     }
     f->flags |= gather ? kGather : 0;
     f->capacity = f->M;
-    f->args = {{"A", ArgPointer, 16}, {"AS", ArgPointer, 8}, {"Out", ArgPointer, f->algorithm == F32 ? 4u : 2u}};
+    if (f->packed_k != Codes && (f->block_m != 16 || few_rows_lds(*f, f->M, {16, 0, 8}) > (uint32_t)kMostLds)) {
+        set_error("mxfp4_grouped: 16-bit rows go with block_m 16 and codes of 16 rows up to %d bytes", kMostLds);
+        return ORX_ERR_BAD_VARIANT;
+    }
+    row_arguments(f);
     if (gather) f->args.push_back({"SlotToken", ArgPointer, 4});
     for (const ArgSpec& a : std::initializer_list<ArgSpec>{{"TileCount", ArgPointer, 4}, {"TileUnits", ArgPointer, 16}, {"W", ArgPointer, 16}, {"WS", ArgPointer, 8}}) f->args.push_back(a);
     f->launch = grouped_launch;

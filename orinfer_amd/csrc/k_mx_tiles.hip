@@ -1,8 +1,8 @@
 // Products of many rows with MXFP4 weights, dense and routed experts: tiles of the output from LDS.
 //
 // DOWN x ACROSS waves share a tile, each 32 ROWS x 32 CHANNELS of it in blocks of 32 x 32; K goes in steps of 256.  Codes and powers come from memory to LDS without passing a
-// register (16 or 4 bytes a lane), two stages.  Weights arrive as they are laid out, a kilobyte to a request; a row's 128 bytes of a step keep their 16-byte piece p at
-// p ^ ((row >> 1) & 7), so that the sixteen rows of a read meet different banks.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their
+// register (16 or 4 bytes a lane), two stages.  Weights and dense rows arrive as they are laid out, a kilobyte to a request; of an expert's rows, which lie anywhere, the 128 bytes of a
+// step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the sixteen rows of a read meet different banks.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their
 // way while the last ones are multiplied, and results drain under the next multiplies.
 //
 // v_mfma_scale_f32_32x32x64 takes 32 cycles, 16 x 16 x 128 18, so the former: 6.2 PFLOP/s on random codes straight from registers, 5.4 the latter.  The multipliers do not run out of
@@ -54,7 +54,8 @@ __device__ __forceinline__ void everybody_arrived() {
 template <int ROWS, int CHANNELS, int DOWN, int ACROSS, bool WIDE, bool GROUPED, bool SWIGLU>
 __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product p) {
     constexpr int BM = 32 * ROWS * DOWN, BN = 32 * CHANNELS * ACROSS, WAVES = DOWN * ACROSS;
-    constexpr int A_REQUESTS = BM / 8 / WAVES, W_REQUESTS = BN / 16 / WAVES, POWERS = BM / 32 + BN / 32;  // of a wave and step (eight rows, a tile); of all waves
+    constexpr int A_REQUESTS = BM / (GROUPED ? 8 : 16) / WAVES, W_REQUESTS = BN / 16 / WAVES;  // of a wave and step: eight rows or a tile, a tile
+    constexpr int POWERS = BM / 32 + BN / 32;                                                   // of all waves
     constexpr int kW = BM * 128, kAS = kW + BN * 128, kWS = kAS + BM * 8, kStage = kWS + BN * 8;
     constexpr int kSmall = (POWERS + WAVES - 1) / WAVES;
     extern __shared__ __align__(128) uint8_t lds[];
@@ -90,18 +91,22 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
 
     // ---- requests ----
     const uint32_t lds_base = lds_asm::lds_address_of(lds);
-    const uint8_t* a_from[A_REQUESTS];  // this lane's piece of eight rows each
+    const uint8_t* a_from[A_REQUESTS];  // a tile, or this lane's piece of eight rows
     const uint8_t* w_from[W_REQUESTS];
-    // powers: request j < BM / 32 is 32 rows of 8 bytes, the others two tiles of 128 each
+    // powers: request j < BM / 32 is 32 rows of 8 bytes or two tiles of 128, the others two tiles
     const uint8_t* power_from[kSmall];
     int power_step[kSmall], power_to[kSmall];
     auto aim = [&](const Tile& t) {
 #pragma unroll
         for (int b = 0; b < A_REQUESTS; ++b) {
-            const int local = (wave * A_REQUESTS + b) * 8 + (lane >> 3);
-            int64_t row = t.first_row + min(local, t.rows - 1);
-            if (GROUPED && p.slot_token != nullptr) row = p.slot_token[row];
-            a_from[b] = p.a + row * p.pitch + ((lane & 7) ^ ((local >> 1) & 7)) * 16;
+            if constexpr (GROUPED) {
+                const int local = (wave * A_REQUESTS + b) * 8 + (lane >> 3);
+                int64_t row = t.first_row + min(local, t.rows - 1);
+                if (p.slot_token != nullptr) row = p.slot_token[row];
+                a_from[b] = p.a + row * p.pitch + ((lane & 7) ^ ((local >> 1) & 7)) * 16;
+            } else {
+                a_from[b] = uniform_pointer(p.a + (int64_t)min(t.first_row / 16 + wave * A_REQUESTS + b, (p.m - 1) / 16) * p.steps * kTileBytes);
+            }
         }
         const int64_t expert = (int64_t)t.expert * p.tiles;
 #pragma unroll
@@ -110,10 +115,16 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
         for (int i = 0; i < kSmall; ++i) {
             const int j = wave + WAVES * i;
             if (j < BM / 32) {
-                int64_t row = t.first_row + min(j * 32 + (lane >> 1), t.rows - 1);
-                if (GROUPED && p.slot_token != nullptr) row = p.slot_token[row];
-                power_from[i] = p.as + row * (p.pitch / 16) + (lane & 1) * 4;
-                power_step[i] = 8, power_to[i] = kAS + j * 256;
+                power_to[i] = kAS + j * 256;
+                if constexpr (GROUPED) {
+                    int64_t row = t.first_row + min(j * 32 + (lane >> 1), t.rows - 1);
+                    if (p.slot_token != nullptr) row = p.slot_token[row];
+                    power_from[i] = p.as + row * (p.pitch / 16) + (lane & 1) * 4;
+                    power_step[i] = 8;
+                } else {
+                    power_from[i] = p.as + (int64_t)min(t.first_row / 16 + j * 2 + (lane >> 5), (p.m - 1) / 16) * p.steps * kTilePowers + (lane & 31) * 4;
+                    power_step[i] = kTilePowers;
+                }
             } else {
                 const int64_t tile = expert + min(t.group * (BN / 16) + (j - BM / 32) * 2 + (lane >> 5), p.tiles - 1);
                 power_from[i] = p.ws + tile * p.steps * kTilePowers + (lane & 31) * 4;
@@ -131,8 +142,9 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
     auto request = [&](int id, uint32_t stage, int wanted) {  // the next step's; in order
         const uint32_t to = lds_base + stage;
         if (id < A_REQUESTS) {
-            request_16_from(a_from[id], to + (wave * A_REQUESTS + id) * 1024, wanted);
-            a_from[id] += 128;
+            if constexpr (GROUPED) request_16_from(a_from[id], to + (wave * A_REQUESTS + id) * 1024, wanted);
+            else request_tile(lane * 16, a_from[id], to + (wave * A_REQUESTS + id) * 2048, wanted);
+            a_from[id] += GROUPED ? 128 : kTileBytes;
         } else if (id < A_REQUESTS + W_REQUESTS) {
             const int b = id - A_REQUESTS;
             request_tile(lane * 16, w_from[b], to + kW + (wave * W_REQUESTS + b) * 2048, wanted);
@@ -146,9 +158,9 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
 
     // ---- operands ----
     const int r = lane & 31, low = lane >> 5;  // row or channel of a block; blocks 2 t + low of a step's eight
-    const uint32_t a_at = (wave_m * 32 * ROWS + r) * 128 + ((low ^ ((r >> 1) & 7)) * 16);
+    const uint32_t a_at = GROUPED ? (wave_m * 32 * ROWS + r) * 128 + ((low ^ ((r >> 1) & 7)) * 16) : (wave_m * 2 * ROWS + (r >> 4)) * 2048 + low * 256 + (r & 15) * 16;
     const uint32_t w_at = kW + (wave_n * 2 * CHANNELS + (r >> 4)) * 2048 + low * 256 + (r & 15) * 16;
-    const uint32_t as_at = kAS + (wave_m * 32 * ROWS + r) * 8;
+    const uint32_t as_at = GROUPED ? kAS + (wave_m * 32 * ROWS + r) * 8 : kAS + (wave_m * 2 * ROWS + (r >> 4)) * 128 + (r & 15) * 8 + low * 4;
     const uint32_t ws_at = kWS + (wave_n * 2 * CHANNELS + (r >> 4)) * 128 + (r & 15) * 8 + low * 4;
     v4i fa[2][ROWS], fw[2][CHANNELS];
     uint2 read_a[ROWS];  // of the next step
@@ -159,20 +171,22 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
     auto read_operand = [&](auto t, auto at, uint32_t stage) {
         constexpr int T = decltype(t)::value, AT = decltype(at)::value;
         if constexpr (AT < ROWS)
-            fa[T & 1][AT] = *reinterpret_cast<const v4i*>(lds + ((a_at ^ (T * 32)) + stage) + AT * 4096);
+            fa[T & 1][AT] = *reinterpret_cast<const v4i*>(lds + ((GROUPED ? a_at ^ (T * 32) : a_at) + stage) + (AT * 4096 + (GROUPED ? 0 : T * 512)));
         else
             fw[T & 1][AT - ROWS] = *reinterpret_cast<const v4i*>(lds + (w_at + stage) + ((AT - ROWS) * 4096 + T * 512));
     };
     auto read_power = [&](auto at, uint32_t stage) {
         constexpr int AT = decltype(at)::value;
-        if constexpr (AT < ROWS)
+        if constexpr (AT < ROWS && GROUPED)
             read_a[AT] = *reinterpret_cast<const uint2*>(lds + (as_at + stage) + AT * 256);
+        else if constexpr (AT < ROWS)
+            read_a[AT].x = *reinterpret_cast<const uint32_t*>(lds + (as_at + stage) + AT * 256);
         else
             read_w[AT - ROWS] = *reinterpret_cast<const int*>(lds + (ws_at + stage) + (AT - ROWS) * 256);
     };
     auto take_powers = [&]() {
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) powers_a[i] = (int)__builtin_amdgcn_perm(read_a[i].y, read_a[i].x, select);
+        for (int i = 0; i < ROWS; ++i) powers_a[i] = GROUPED ? (int)__builtin_amdgcn_perm(read_a[i].y, read_a[i].x, select) : (int)read_a[i].x;
 #pragma unroll
         for (int j = 0; j < CHANNELS; ++j) powers_w[j] = read_w[j];
         __builtin_amdgcn_sched_barrier(0);

@@ -67,6 +67,12 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t so_far, uint32_t word) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, so_far), __builtin_bit_cast(pair, word & 0x7FFF7FFFu)));
 }
 
+// largest over the four lanes of a quad
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+}
+
 // Eight codes of one block, rounded to nearest, ties to the even code, saturating: the conversion instruction divides by the power of the scale's exponent
 // field, also by 2^-127 where that is zero (it agrees with the rule for every fp16 and bf16 value and powers of 2^-127 to 2^127).
 template <int TYPE>
@@ -162,7 +168,7 @@ struct Product {
     const uint8_t* w;   // tiles
     const uint8_t* ws;
     void* out;
-    int m, cols, steps;    // rows, output columns, K / 256
+    int m, cols, k, steps;  // rows, output columns, K, K / 256
     int pitch;             // bytes of a row's codes
     int tiles;             // 16-channel tiles of the weights (of one expert)
     int type;              // of the output

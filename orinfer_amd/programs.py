@@ -718,12 +718,15 @@ class _OnDevice:
             return body(*args, stream=current_stream() if stream is None else stream, **named)
 
 
+MX_FEW_ROWS = 4  # rows that an MXFP4 projection quantises itself
+
+
 class Mxfp4Linear(_OnDevice):
     """Rows of 16-bit values, quantised to MXFP4, times MXFP4 weights: codes (N, K / 2) and exponents (N, K / 32), both uint8 (the format: mxfp4.py), up to `capacity`
     rows at a time.  epilogue="swiglu": the upper half of the channels are the up channels of the gate channels in the lower half, and silu(gate) * up comes out.
     `run` returns a view of the object's own output buffer, which the next call overwrites; one object serves one stream at a time."""
 
-    def __init__(self, codes, exponents, capacity, *, dtype=torch.float16, epilogue="none", scale="floor"):
+    def __init__(self, codes, exponents, capacity, *, dtype=torch.float16, epilogue="none"):
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("dtype must be torch.float16 or torch.bfloat16")
         if codes.ndim != 2:
@@ -735,13 +738,23 @@ class Mxfp4Linear(_OnDevice):
         self.weight, self.powers = (t.cuda() for t in mxfp4.tiles(codes, exponents, paired=epilogue == "swiglu"))
         self.device = self.weight.device
         name = mxfp4.dtype_name(dtype)
+        shape = dict(N=channels, K=self.k, dynamic_rows=True, epilogue=epilogue, output_dtype=name)
         with torch.cuda.device(self.device):
-            self.projection = Kernel("mxfp4_projection", M=capacity, N=channels, K=self.k, dynamic_rows=True, epilogue=epilogue, output_dtype=name)
-            self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, scale=scale, pad=mxfp4.STEP)
+            self.projection = Kernel("mxfp4_projection", M=capacity, **shape)
+            self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, layout="tiles")
+            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (weights out of cache, us of the projection alone without / with it,
+            # and a quantiser is 2.8: 17408 x 5120 1 row 10.6 / 11.1, 4 rows 11.5 / 13.5, 8 rows 12 / 17; 9728 x 2560 4.4 / 4.6, 4.5 / 5.9, 4.6 / 7.4).  Not where their codes do not fit LDS.
+            self.few = None
+            try:
+                self.few = Kernel("mxfp4_projection", M=min(capacity, MX_FEW_ROWS), input_dtype=name, **shape)
+            except OrxError as error:
+                if error.code != ORX_ERR_BAD_VARIANT:
+                    raise
         self.n = channels // 2 if epilogue == "swiglu" else channels
-        wide = mxfp4.padded(self.k)
-        self.a_q = torch.empty((capacity, wide // 2), dtype=torch.uint8, device=self.device)
-        self.a_s = torch.empty((capacity, wide // mxfp4.BLOCK), dtype=torch.uint8, device=self.device)
+        # the quantised rows, by tiles of 16
+        tiles = -(-capacity // 16) * -(-self.k // mxfp4.STEP)
+        self.a_q = torch.empty((tiles, 2048), dtype=torch.uint8, device=self.device)
+        self.a_s = torch.empty((tiles, 128), dtype=torch.uint8, device=self.device)
         self.out = torch.empty((capacity, self.n), dtype=dtype, device=self.device)
 
     def run(self, x, stream=None):
@@ -754,6 +767,9 @@ class Mxfp4Linear(_OnDevice):
         return self.out.as_strided((rows, self.n), (self.n, 1))
 
     def _run(self, x, rows, stream):
+        if rows <= MX_FEW_ROWS and self.few is not None:
+            self.few(stream=stream, A=x, Out=self.out, W=self.weight, WS=self.powers, m=rows)
+            return
         self.quantizer(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=rows)
         self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, WS=self.powers, m=rows)
 

@@ -65,6 +65,19 @@ def test_quantisation_is_the_oracles(name, rows, k, pad, scale):
         assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 7), (5, 300), (16, 256), (17, 2560), (100, 1000), (33, 4096)])
+def test_quantisation_by_tiles(name, rows, k):
+    x = rows_of(np.random.default_rng(rows * k), rows, k, TYPES[name])
+    codes, exponents = orc.quantise(np.pad(x.double().numpy(), ((0, -rows % 16), (0, -k % 256))))
+    want = mxfp4.tiles(torch.from_numpy(codes), torch.from_numpy(exponents))
+    tiles, steps = -(-rows // 16), -(-k // 256)
+    q, s = torch.full((tiles * steps * 2048 + 16,), 171, dtype=torch.uint8, device=DEV), torch.full((tiles * steps * 128 + 16,), 171, dtype=torch.uint8, device=DEV)
+    kernel("mxfp4_quantization", K=k, input_dtype=name, layout="tiles")(Q=q, S=s, X=x.to(DEV), rows=rows)
+    assert torch.equal(q[:-16].cpu(), want[0].flatten()) and torch.equal(s[:-16].cpu(), want[1].flatten())
+    assert (q[-16:] == 171).all() and (s[-16:] == 171).all()
+
+
 @pytest.mark.parametrize("name", ["float16", "bfloat16"])
 @pytest.mark.parametrize("offset", [1, 4])
 def test_quantisation_of_rows_that_are_not_16_byte_aligned(name, offset):
@@ -155,13 +168,30 @@ def test_linear_with_fp32_output_at_an_odd_address(rows, n):
     rng = np.random.default_rng(n)
     codes, exponents = weights(rng, n, 320)
     x = rows_of(rng, rows, 320, torch.float32)
-    q, s = mxfp4.quantize(x.to(DEV), pad=256)
+    q, s = torch.empty(-(-rows // 16) * 2 * 2048, dtype=torch.uint8, device=DEV), torch.empty(-(-rows // 16) * 2 * 128, dtype=torch.uint8, device=DEV)
+    kernel("mxfp4_quantization", K=320, input_dtype="float32", layout="tiles")(Q=q, S=s, X=x.to(DEV), rows=rows)
     w, ws = mxfp4.tiles(dev(codes), dev(exponents))
     out = torch.full((rows * n + 9,), -7.0, device=DEV)
     kernel("mxfp4_projection", M=rows, N=n, K=320, output_dtype="float32")(A=q, AS=s, Out=out[1:], W=w, WS=ws)
     want, bound = product(orc.values(*orc.quantise(x.double().numpy())), orc.values(codes, exponents))
     check(out[1:1 + rows * n].view(rows, n), want, bound, torch.float32)
     assert out[0] == -7 and (out[1 + rows * n:] == -7).all()
+
+
+@pytest.mark.parametrize("epilogue", ["none", "swiglu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 2, 7, 16])
+@pytest.mark.parametrize("n,k", [(32, 32), (94, 608), (700, 2304), (9000, 512)])
+def test_rows_that_the_projection_quantises(rows, n, k, dtype, epilogue):
+    """16-bit rows at an address of their own alignment give what the quantiser and the projection give."""
+    linear, x, want, bound = linear_case(rows, n, k, dtype, epilogue)
+    moved = torch.empty(rows * k + 1, dtype=dtype, device=DEV)[1:].view(rows, k).copy_(x)
+    out = torch.full((rows * want.shape[1] + 3,), -7, dtype=dtype, device=DEV)
+    kernel("mxfp4_projection", M=16, N=n, K=k, dynamic_rows=True, input_dtype=mxfp4.dtype_name(dtype), output_dtype=mxfp4.dtype_name(dtype), epilogue=epilogue)(
+        A=moved, Out=out[1:], W=linear.weight, WS=linear.powers, m=rows)
+    got = out[1:1 + want.size].view(want.shape)
+    check(got, want, bound, dtype)
+    assert out[0] == -7 and (out[1 + want.size:] == -7).all()
 
 
 @pytest.mark.parametrize("rows", [1, 20, 300])

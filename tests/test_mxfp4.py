@@ -65,9 +65,11 @@ def test_arguments_in_launch_order():
     shape = dict(N=96, K=320)
     assert lib.Kernel("mxfp4_projection", M=3, **shape).arg_names == ["A", "AS", "Out", "W", "WS"]
     assert lib.Kernel("mxfp4_projection", M=3, dynamic_rows=True, **shape).arg_names == ["A", "AS", "Out", "W", "WS", "m"]
+    assert lib.Kernel("mxfp4_projection", M=3, input_dtype="bfloat16", **shape).arg_names == ["A", "Out", "W", "WS"]
     grouped = dict(rows=12, E=4, tiles=8, **shape)
     assert lib.Kernel("mxfp4_grouped", **grouped).arg_names == ["A", "AS", "Out", "TileCount", "TileUnits", "W", "WS"]
     assert lib.Kernel("mxfp4_grouped", gather=True, **grouped).arg_names == ["A", "AS", "Out", "SlotToken", "TileCount", "TileUnits", "W", "WS"]
+    assert lib.Kernel("mxfp4_grouped", gather=True, input_dtype="float16", **grouped).arg_names == ["A", "Out", "SlotToken", "TileCount", "TileUnits", "W", "WS"]
     router = dict(M=3, E=64, top_k=4)
     assert lib.Kernel("router_topk", scoring="sigmoid", **router).arg_names == ["IDs", "Logits", "Prob"]
     assert lib.Kernel("router_topk", bias=True, dynamic_rows=True, **router).arg_names == ["Bias", "IDs", "Logits", "Prob", "m"]
@@ -81,7 +83,10 @@ ROUTER = dict(M=3, E=64, top_k=4)
 @pytest.mark.parametrize("symbol,variant", [
     ("mxfp4_quantization", dict(K=0)), ("mxfp4_quantization", dict(K=64, pad=64)), ("mxfp4_quantization", dict(K=64, scale="round")),
     ("mxfp4_quantization", dict(K=64, input_dtype="int8")), ("mxfp4_quantization", dict(K=64, M=0)), ("mxfp4_quantization", dict(K=1 << 25)),
-    ("mxfp4_dequantization", dict(K=64, output_dtype="e4m3")), ("mxfp4_dequantization", dict(K=64, scale="ceil")),
+    ("mxfp4_quantization", dict(K=64, layout="columns")), ("mxfp4_quantization", dict(K=64, layout="tiles", pad=256)),
+    ("mxfp4_projection", dict(M=17, N=96, K=320, input_dtype="float16")), ("mxfp4_projection", dict(M=16, N=96, K=1 << 16, input_dtype="float16")),
+    ("mxfp4_projection", dict(M=1, N=96, K=320, input_dtype="float32")), ("mxfp4_grouped", dict(GROUPED, block_m=32, input_dtype="float16")),
+    ("mxfp4_grouped", dict(GROUPED, input_dtype="bfloat16")), ("mxfp4_dequantization", dict(K=64, output_dtype="e4m3")), ("mxfp4_dequantization", dict(K=64, scale="ceil")),
     ("mxfp4_projection", dict(M=1, N=96, K=100)), ("mxfp4_projection", dict(M=0, N=96, K=320)), ("mxfp4_projection", dict(M=1, N=0, K=320)),
     ("mxfp4_projection", dict(M=1, N=97, K=320, epilogue="swiglu")), ("mxfp4_projection", dict(M=1, N=96, K=320, epilogue="gelu")),
     ("mxfp4_projection", dict(M=1, N=96, K=320, output_dtype="int8")), ("mxfp4_projection", dict(M=1, N=96, K=320, packed_k=128)),
@@ -130,9 +135,9 @@ def test_records_name_the_kernel_that_runs():
 def test_a_projection_takes_larger_tiles_where_there_are_more():
     """Threads and LDS of the kernel by rows (without a device 256 CUs are taken)."""
     linear = lib.Kernel("mxfp4_projection", M=8192, N=4096, K=4096, dynamic_rows=True)
-    assert [started(linear, rows)[0][1:] for rows in (64, 65, 512, 2048, 8192)] == [(256, 0), (256, 52224), (256, 52224), (256, 69632), (512, 139264)]
+    assert [started(linear, rows)[0][1:] for rows in (64, 65, 512, 2048, 8192)] == [(512, 65536), (256, 52224), (256, 52224), (256, 69632), (512, 139264)]
     assert all(len(started(linear, rows)) == 1 for rows in (1, 64, 65, 8192))
-    for block_m, lds in ((16, 0), (32, 0), (64, 52224), (128, 69632), (256, 139264)):
+    for block_m, lds in ((16, 16384), (32, 32768), (64, 52224), (128, 69632), (256, 139264)):
         assert started(lib.Kernel("mxfp4_grouped", **GROUPED, block_m=block_m))[0][2] == lds
 
 
