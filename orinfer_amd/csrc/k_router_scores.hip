@@ -19,33 +19,76 @@ struct ScoreParams {
     int* ids;
     float* prob;
     int m, e, top_k, groups, top_groups, group_best, sigmoid, renormalize;
+    int lanes;         // to a group, a power of two
+    uint32_t inverse;  // ceil(2^21 / experts of a group): ids below 1024 divided by it
     float scale;
 };
 
-// Larger key, larger value; 0 is left for what is never chosen, 1 for what is chosen last.
-__device__ __forceinline__ uint64_t key_of(double v) {
-    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-    return bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
+// Larger key, larger value, in two words; 0 is left for what is never chosen, 1 for what is chosen last.
+struct Key {
+    uint32_t high, low;
+};
+__device__ __forceinline__ Key key_of(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v), key = bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
+    return {(uint32_t)(key >> 32), (uint32_t)key};
 }
-constexpr uint64_t kLast = 1;
 
-__device__ __forceinline__ double wave_sum_double(double v) {
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+// Moves of 64-bit values between lanes, as wave_sum makes them of 32-bit ones.
+__device__ __forceinline__ double join(uint32_t low, uint32_t high) { return __builtin_bit_cast(double, ((uint64_t)high << 32) | low); }
+template <int CONTROL>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    return join(__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CONTROL, 0xF, 0xF, true), __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), CONTROL, 0xF, 0xF, true));
 }
-// The largest key of the wave and the lowest id that has it.
-__device__ __forceinline__ void wave_best(uint64_t& key, int& id) {
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint64_t other = __shfl_xor(key, d);
-        const int other_id = __shfl_xor(id, d);
-        if (other > key || (other == key && other_id < id)) key = other, id = other_id;
+// a lane's value and its partner's, 16 or 32 lanes away, in the same order for both
+template <int LANES>
+__device__ __forceinline__ void both(double v, double& one, double& other) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    if constexpr (LANES == 16) {
+        auto low = __builtin_amdgcn_permlane16_swap((uint32_t)bits, (uint32_t)bits, false, false), high = __builtin_amdgcn_permlane16_swap((uint32_t)(bits >> 32), (uint32_t)(bits >> 32), false, false);
+        one = join(low[0], high[0]), other = join(low[1], high[1]);
+    } else {
+        auto low = __builtin_amdgcn_permlane32_swap((uint32_t)bits, (uint32_t)bits, false, false), high = __builtin_amdgcn_permlane32_swap((uint32_t)(bits >> 32), (uint32_t)(bits >> 32), false, false);
+        one = join(low[0], high[0]), other = join(low[1], high[1]);
     }
 }
-
+__device__ __forceinline__ double wave_sum_double(double v) {
+    double one, other;
+    both<32>(v, one, other), v = one + other;
+    both<16>(v, one, other), v = one + other;
+    v += moved<0x128>(v);  // row_ror:8
+    v += moved<0x124>(v);  // row_ror:4
+    v += moved<0x4E>(v);   // quad_perm [2,3,0,1]
+    v += moved<0xB1>(v);   // quad_perm [1,0,3,2]
+    return v;
+}
+// the two largest of two pairs
+__device__ __forceinline__ void two_of(double& first, double& second, double a, double b) {
+    second = fmax(fmin(first, a), fmax(second, b));
+    first = fmax(first, a);
+}
+// The two largest of LANES neighbouring lanes, known to all of them (mirrors: lane i's partner is 7 - i, 15 - i of its group).
+__device__ __forceinline__ void two_of_lanes(double& first, double& second, int lanes) {
+    if (lanes > 1) two_of(first, second, moved<0xB1>(first), moved<0xB1>(second));
+    if (lanes > 2) two_of(first, second, moved<0x4E>(first), moved<0x4E>(second));
+    if (lanes > 4) two_of(first, second, moved<0x141>(first), moved<0x141>(second));
+    if (lanes > 8) two_of(first, second, moved<0x140>(first), moved<0x140>(second));
+    double a, b, c, d;
+    if (lanes > 16) {
+        both<16>(first, a, b), both<16>(second, c, d);
+        first = a, second = c, two_of(first, second, b, d);
+    }
+    if (lanes > 32) {
+        both<32>(first, a, b), both<32>(second, c, d);
+        first = a, second = c, two_of(first, second, b, d);
+    }
+}
 // A wave's LDS accesses run in their order; this keeps the compiler to it where lanes read what others wrote.
 __device__ __forceinline__ void lane_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // A wave to a token, LOCAL scores to a lane (expert j * 64 + lane).
+// With many tokens bound by instructions, with few by one chain: 64-bit exponentials, then ranks.  A rank is one maximum of the keys' high words and one ballot for every held key; only
+// where several lanes have it do the low words decide.  8192 tokens of 256 experts, 8 groups, top 8: 32.6 us with 64-bit shuffles, 16.2 now; 5 tokens of 128: 7.0, 3.6 now.
 template <int LOCAL>
 __global__ __launch_bounds__(256) void router_scores_kernel(ScoreParams p) {
     __shared__ double held[4][LOCAL * 64];
@@ -55,84 +98,105 @@ __global__ __launch_bounds__(256) void router_scores_kernel(ScoreParams p) {
     if (row >= p.m) return;
     double* const mine = held[wave];
     double score[LOCAL];
+    float bias[LOCAL];
     bool known[LOCAL];  // the expert is there and its logit is a number
     float largest = -FLT_MAX;
 #pragma unroll
     for (int j = 0; j < LOCAL; ++j) {
         const int id = j * 64 + lane;
-        const float l = id < p.e ? p.logits[row * p.e + id] : 0.f;
+        const float l = p.logits[row * p.e + min(id, p.e - 1)];
+        bias[j] = p.bias != nullptr ? p.bias[min(id, p.e - 1)] : 0.f;
         known[j] = id < p.e && l == l;
-        score[j] = fminf(fmaxf(l, -FLT_MAX), FLT_MAX);
-        if (known[j]) largest = fmaxf(largest, (float)score[j]);
+        const float finite = fminf(fmaxf(l, -FLT_MAX), FLT_MAX);
+        score[j] = finite;
+        largest = known[j] ? fmaxf(largest, finite) : largest;
     }
     if (p.sigmoid) {
 #pragma unroll
         for (int j = 0; j < LOCAL; ++j) score[j] = 1.0 / (1.0 + exp(-score[j]));
     } else {
-        for (int d = 32; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+        const double top = key_value(wave_max_u32(ordered_key(largest)));
         double sum = 0;
 #pragma unroll
         for (int j = 0; j < LOCAL; ++j) {
-            score[j] = exp(score[j] - (double)largest);
+            score[j] = exp(score[j] - top);
             sum += known[j] ? score[j] : 0.0;
         }
-        sum = wave_sum_double(sum);
+        const double inverse = 1.0 / wave_sum_double(sum);
 #pragma unroll
-        for (int j = 0; j < LOCAL; ++j) score[j] /= sum;
+        for (int j = 0; j < LOCAL; ++j) score[j] *= inverse;
     }
-    uint64_t key[LOCAL];
+    Key key[LOCAL];
 #pragma unroll
     for (int j = 0; j < LOCAL; ++j) {
         const int id = j * 64 + lane;
-        const double choice = score[j] + (p.bias != nullptr && id < p.e ? (double)p.bias[id] : 0.0);
+        const double choice = score[j] + (double)bias[j];
         const bool open = known[j] && choice > -__builtin_inf();  // (false for NaN too)
-        key[j] = id >= p.e ? 0 : open ? key_of(choice) : kLast;
+        key[j] = key_of(choice);
+        if (!open) key[j] = Key{0, id < p.e ? 1u : 0u};
         mine[id] = open ? choice : -__builtin_inf();
     }
     lane_order();
     if (p.top_groups < p.groups) {
-        // a lane to a group: its two largest
-        const int size = p.e / p.groups;
+        // LANES lanes to a group; then a group stays if fewer than top_groups are in front of it
+        const int size = p.e / p.groups, lanes = p.lanes, group = lane / lanes;
         double first = -__builtin_inf(), second = -__builtin_inf();
-        if (lane < p.groups)
-            for (int i = 0; i < size; ++i) {
-                const double c = mine[lane * size + i];
-                second = fmax(second, fmin(first, c)), first = fmax(first, c);
-            }
-        const double total = p.group_best > 1 && second > -__builtin_inf() ? first + second : first;
-        uint64_t group_key = lane < p.groups ? key_of(total) : 0;
-        uint64_t kept = 0;
-        for (int i = 0; i < p.top_groups; ++i) {
-            uint64_t best = group_key;
-            int at = lane;
-            wave_best(best, at);
-            kept |= 1ull << at;
-            if (lane == at) group_key = 0;
+        if (group < p.groups)
+            for (int i = lane & (lanes - 1); i < size; i += lanes) two_of(first, second, mine[group * size + i], -__builtin_inf());
+        two_of_lanes(first, second, lanes);
+        const Key own = key_of(p.group_best > 1 && second > -__builtin_inf() ? first + second : first);
+        const uint64_t own_key = (uint64_t)own.high << 32 | own.low;
+        int in_front = 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)own.high, g * lanes) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)own.low, g * lanes);
+            in_front += other > own_key || (other == own_key && g < group) ? 1 : 0;
         }
+        const uint64_t kept = __ballot(group < p.groups && in_front < p.top_groups);
 #pragma unroll
-        for (int j = 0; j < LOCAL; ++j)
-            if (j * 64 + lane < p.e && !(kept >> ((j * 64 + lane) / size) & 1)) key[j] = 0;
+        for (int j = 0; j < LOCAL; ++j) {
+            const int of = (int)((uint32_t)(j * 64 + lane) * p.inverse >> 21);  // id / size
+            if (!(kept >> (min(of, p.groups - 1) * lanes) & 1)) key[j] = Key{0, 0};
+        }
+        lane_order();
     }
-    lane_order();
 #pragma unroll
     for (int j = 0; j < LOCAL; ++j) mine[j * 64 + lane] = score[j];
     lane_order();
     int my_id = 0;
-    uint64_t my_key = 0;
+    bool my_last = false;  // chosen for want of another
     for (int rank = 0; rank < p.top_k; ++rank) {
-        uint64_t best = 0;
-        int at = 0x7FFFFFFF;
+        uint32_t best = key[0].high;
+#pragma unroll
+        for (int j = 1; j < LOCAL; ++j) best = max(best, key[j].high);
+        best = wave_max_u32(best);
+        uint64_t having[LOCAL];
+        int count = 0;
+#pragma unroll
+        for (int j = 0; j < LOCAL; ++j) having[j] = __ballot(key[j].high == best), count += __popcll(having[j]);
+        uint32_t low = 2;
+        if (count > 1) {
+            low = 0;
+#pragma unroll
+            for (int j = 0; j < LOCAL; ++j) low = max(low, key[j].high == best ? key[j].low : 0u);
+            low = wave_max_u32(low);
+#pragma unroll
+            for (int j = 0; j < LOCAL; ++j) having[j] &= __ballot(key[j].low == low);
+        }
+        int chosen = 0;
+        uint64_t lowest = 0;
+#pragma unroll
+        for (int j = LOCAL - 1; j >= 0; --j)
+            if (having[j] != 0) chosen = j, lowest = having[j];
+        lowest &= 0 - lowest;
+        const int id = chosen * 64 + __builtin_ctzll(lowest);
+        const bool last = best == 0 && low == 1;
 #pragma unroll
         for (int j = 0; j < LOCAL; ++j)
-            if (key[j] > best) best = key[j], at = j * 64 + lane;
-        wave_best(best, at);
-#pragma unroll
-        for (int j = 0; j < LOCAL; ++j)
-            if (j * 64 + lane == at) key[j] = 0;
-        if (lane == rank) my_id = at, my_key = best;
+            if (j == chosen && (lowest >> lane & 1)) key[j] = Key{0, 0};
+        if (lane == rank) my_id = id, my_last = last;
     }
     const bool route = lane < p.top_k;
-    const double s = route && my_key != kLast ? mine[my_id] : 0.0;
+    const double s = route && !my_last ? mine[my_id] : 0.0;
     const double sum = p.renormalize ? wave_sum_double(s) : 1.0;
     if (route) {
         p.ids[row * p.top_k + lane] = my_id;
@@ -153,6 +217,9 @@ int launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, vo
     p.bias = bias ? pointer_arg<const float>(args, 0) : nullptr;
     p.ids = pointer_arg<int>(args, bias), p.logits = pointer_arg<const float>(args, bias + 1), p.prob = pointer_arg<float>(args, bias + 2);
     p.m = rows, p.e = f.E, p.top_k = f.top_k, p.groups = f.group, p.top_groups = f.slots, p.group_best = f.tiles;
+    p.lanes = 1;
+    while (2 * p.lanes * f.group <= 64) p.lanes *= 2;
+    p.inverse = ceil_div(1u << 21, (uint32_t)(f.E / f.group));
     p.sigmoid = f.flags & kSigmoid, p.renormalize = f.flags & kRenormalize, p.scale = f.weight_scale;
     const dim3 grid(g.grid[0]), block(256);
     if (f.E <= 64) ORX_LAUNCH(router_scores_kernel<1>, grid, block, 0, s, p);
