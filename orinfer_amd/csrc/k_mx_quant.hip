@@ -2,7 +2,8 @@
 //
 //   a = max |x| of a block, e = max(exponent(a) - 2, 0), code = E2M1(x / 2^(e - 127)), nearest, ties to even, saturating.
 // Bound by memory: 2 bytes in and 17/32 out an element.  A lane takes eight values (16 bytes of 16-bit ones), four lanes a block: the largest magnitude is two
-// exchanges within a quad, a lane's eight codes are one word, so both sides are whole lines, and nothing is kept across lanes otherwise.
+// exchanges within a quad, a lane's eight codes are one word, so both sides are whole lines, and nothing is kept across lanes otherwise.  Read past the caches: 8192 x 5120 bf16
+// 25.0 -> 17.4 us (6.1 TB/s), by tiles 8192 x 4096 fp16 22.8 -> 17.5; two or eight pieces to a thread instead of four 24.0, 18.5.
 #include <algorithm>
 
 #include "mx_device.h"
@@ -13,12 +14,26 @@ namespace {
 
 constexpr int kThreads = 256, kPieces = 4;  // eight-value pieces to a thread
 
+// Rows of `pieces` eight-value pieces, one behind the other in one sequence of fewer than 2^32.
+struct Rows {
+    uint32_t total, pieces, inverse;  // inverse = floor(2^32 / pieces)
+    uint32_t pitch;                   // pieces from one stored row to the next
+    int k;
+    // Row and piece of number `at`: the quotient by the inverse is at most one too small.
+    __device__ __forceinline__ void split(uint32_t at, uint32_t& row, uint32_t& piece) const {
+        row = __umulhi(at, inverse), piece = at - row * pieces;
+        if (piece >= pieces) ++row, piece -= pieces;
+    }
+};
+Rows rows_of(int rows, int pieces, int pitch, int k) {
+    return {(uint32_t)rows * (uint32_t)pieces, (uint32_t)pieces, (uint32_t)std::min<uint64_t>((1ull << 32) / pieces, 0xFFFFFFFFull), (uint32_t)pitch, k};
+}
+
 struct QuantParams {
     const void* x;
     uint8_t *q, *s;
-    int64_t pieces_total;
-    uint32_t pieces;  // of a row
-    int k, ceil;
+    Rows rows;
+    int ceil;
 };
 
 // bits of the largest magnitude of a lane's eight values
@@ -30,51 +45,59 @@ __device__ __forceinline__ uint32_t largest_of(const uint32_t (&words)[WORDS]) {
     return TYPE == mx::F32 ? found : max(found & 0xFFFFu, found >> 16);
 }
 
-template <int TYPE>
+// `count` of eight values from an address of their own alignment; what is not there is 0
+template <int TYPE, int WORDS>
+__device__ __forceinline__ void read_eight(uint32_t (&words)[WORDS], const void* x, int64_t offset, int count) {
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) words[j] = 0;
+    if (count >= 8) {
+        const mx::words4* const from = reinterpret_cast<const mx::words4*>(reinterpret_cast<const uint8_t*>(x) + offset * (TYPE == mx::F32 ? 4 : 2));
+#pragma unroll
+        for (int j = 0; j < WORDS / 4; ++j) {
+            const mx::v4u four = __builtin_nontemporal_load(from + j);
+            words[4 * j] = four[0], words[4 * j + 1] = four[1], words[4 * j + 2] = four[2], words[4 * j + 3] = four[3];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) {
+                if constexpr (TYPE == mx::F32)
+                    words[j] = reinterpret_cast<const uint32_t*>(x)[offset + j];
+                else
+                    words[j / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(x)[offset + j] << (16 * (j & 1));
+            }
+    }
+}
+
+// WHOLE: rows of whole blocks without a gap on either side, so that a piece's number is its place and no row is looked for.
+template <int TYPE, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void mx_quantise_kernel(QuantParams p) {
     constexpr int WORDS = TYPE == mx::F32 ? 8 : 4;
-    const int64_t base = (int64_t)blockIdx.x * (kThreads * kPieces);
-    const int64_t first_row = base / p.pieces;  // uniform: once a workgroup
-    const uint32_t first_piece = (uint32_t)(base - first_row * p.pieces);
-    uint32_t words[kPieces][WORDS];
-    int64_t row[kPieces];
-    uint32_t piece[kPieces];
+    const uint32_t base = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
+    uint32_t words[kPieces][WORDS], to[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-        const uint32_t at = first_piece + i * kThreads + threadIdx.x;
-        const uint32_t down = at / p.pieces;
-        row[i] = first_row + down, piece[i] = at - down * p.pieces;
-        const bool live = base + i * kThreads + threadIdx.x < p.pieces_total;
-        const int first = (int)piece[i] * 8, count = live ? p.k - first : 0;
-#pragma unroll
-        for (int j = 0; j < WORDS; ++j) words[i][j] = 0;
-        const int64_t offset = row[i] * p.k + first;
-        if (count >= 8) {
-            const mx::words4* const from = reinterpret_cast<const mx::words4*>(reinterpret_cast<const uint8_t*>(p.x) + offset * (TYPE == mx::F32 ? 4 : 2));
-#pragma unroll
-            for (int j = 0; j < WORDS / 4; ++j) {
-                const mx::v4u four = from[j];
-                words[i][4 * j] = four[0], words[i][4 * j + 1] = four[1], words[i][4 * j + 2] = four[2], words[i][4 * j + 3] = four[3];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j < count) {
-                    if constexpr (TYPE == mx::F32)
-                        words[i][j] = reinterpret_cast<const uint32_t*>(p.x)[offset + j];
-                    else
-                        words[i][j / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p.x)[offset + j] << (16 * (j & 1));
-                }
+        const uint32_t at = base + i * kThreads;
+        const bool live = at < p.rows.total;
+        int count = live ? 8 : 0;
+        int64_t offset = (int64_t)at * 8;
+        to[i] = at;
+        if constexpr (!WHOLE) {
+            uint32_t row, piece;
+            p.rows.split(at, row, piece);
+            count = live ? p.rows.k - (int)piece * 8 : 0;
+            offset = (int64_t)row * p.rows.k + piece * 8;
+            to[i] = row * p.rows.pitch + piece;
         }
+        read_eight<TYPE>(words[i], p.x, offset, count);
     }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
         // (a row is whole blocks, so the lanes of a quad are pieces of one block, or all behind the end)
         const uint32_t byte = mx::power_byte<TYPE>(mx::quad_max(largest_of<TYPE>(words[i])), p.ceil != 0);
-        if (base + i * kThreads + threadIdx.x >= p.pieces_total) continue;
-        const int64_t at = row[i] * p.pieces + piece[i];
-        reinterpret_cast<uint32_t*>(p.q)[at] = mx::eight_codes<TYPE>(words[i], byte);
-        if ((threadIdx.x & 3) == 0) p.s[at >> 2] = (uint8_t)byte;
+        if (base + i * kThreads >= p.rows.total) continue;
+        reinterpret_cast<uint32_t*>(p.q)[to[i]] = mx::eight_codes<TYPE>(words[i], byte);
+        if ((threadIdx.x & 3) == 0) p.s[to[i] >> 2] = (uint8_t)byte;
     }
 }
 
@@ -92,27 +115,7 @@ __global__ __launch_bounds__(kThreads) void mx_quantise_tiles_kernel(QuantParams
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = (int64_t)tile * 16 + 4 * i + (lane >> 4);
-        const int count = row < rows ? p.k - column : 0;
-        const int64_t offset = row * p.k + column;
-#pragma unroll
-        for (int j = 0; j < WORDS; ++j) words[i][j] = 0;
-        if (count >= 8) {
-            const mx::words4* const from = reinterpret_cast<const mx::words4*>(reinterpret_cast<const uint8_t*>(p.x) + offset * (TYPE == mx::F32 ? 4 : 2));
-#pragma unroll
-            for (int j = 0; j < WORDS / 4; ++j) {
-                const mx::v4u four = from[j];
-                words[i][4 * j] = four[0], words[i][4 * j + 1] = four[1], words[i][4 * j + 2] = four[2], words[i][4 * j + 3] = four[3];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j < count) {
-                    if constexpr (TYPE == mx::F32)
-                        words[i][j] = reinterpret_cast<const uint32_t*>(p.x)[offset + j];
-                    else
-                        words[i][j / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p.x)[offset + j] << (16 * (j & 1));
-                }
-        }
+        read_eight<TYPE>(words[i], p.x, row * p.rows.k + column, row < rows ? p.rows.k - column : 0);
     }
     const int64_t at = (int64_t)tile * steps + (window >> 1);
     const int block = (window & 1) * 4 + ((lane & 15) >> 2);
@@ -128,81 +131,78 @@ __global__ __launch_bounds__(kThreads) void mx_quantise_tiles_kernel(QuantParams
 struct DequantParams {
     const uint8_t *q, *s;
     void* y;
-    int64_t pieces_total;
-    uint32_t pieces;
-    int k, type;
+    Rows rows;
+    int type;
 };
 
+template <bool WHOLE>
 __global__ __launch_bounds__(kThreads) void mx_dequantise_kernel(DequantParams p) {
-    const int64_t base = (int64_t)blockIdx.x * (kThreads * kPieces);
-    const int64_t first_row = base / p.pieces;
-    const uint32_t first_piece = (uint32_t)(base - first_row * p.pieces);
+    const uint32_t base = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-        if (base + i * kThreads + threadIdx.x >= p.pieces_total) return;
-        const uint32_t at = first_piece + i * kThreads + threadIdx.x;
-        const uint32_t down = at / p.pieces, piece = at - down * p.pieces;
-        const int64_t row = first_row + down, from = row * p.pieces + piece;
-        const int first = (int)piece * 8;
-        if (first >= p.k) continue;
+        const uint32_t at = base + i * kThreads;
+        if (at >= p.rows.total) return;
+        uint32_t from = at;
+        int64_t row_start = 0;
+        int first = 0, k = 8;
+        if constexpr (WHOLE) {
+            row_start = (int64_t)at * 8;
+        } else {
+            uint32_t row, piece;
+            p.rows.split(at, row, piece);
+            from = row * p.rows.pitch + piece, row_start = (int64_t)row * p.rows.k, first = (int)piece * 8, k = p.rows.k;
+            if (first >= k) continue;
+        }
         const uint32_t codes = reinterpret_cast<const uint32_t*>(p.q)[from];
         const uint32_t byte = p.s[from >> 2];
         const float power = __uint_as_float(byte << 23);
-        auto two = [&](auto pair, float& a, float& b) { a = byte == 255u ? __uint_as_float(0x7FC00000u) : pair[0], b = byte == 255u ? __uint_as_float(0x7FC00000u) : pair[1]; };
         float v[8];
+        auto two = [&](auto pair, float& a, float& b) { a = byte == 255u ? __uint_as_float(0x7FC00000u) : pair[0], b = byte == 255u ? __uint_as_float(0x7FC00000u) : pair[1]; };
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 0), v[0], v[1]);
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 1), v[2], v[3]);
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 2), v[4], v[5]);
         two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, power, 3), v[6], v[7]);
-        const mx::v4f low = {v[0], v[1], v[2], v[3]}, high = {v[4], v[5], v[6], v[7]};
         if (p.type != mx::F32) {
-            mx::store_eight_halves(p.y, row * p.k, first, p.k, mx::v4u{mx::two_values(v[0], v[1], p.type), mx::two_values(v[2], v[3], p.type),
-                                                                      mx::two_values(v[4], v[5], p.type), mx::two_values(v[6], v[7], p.type)});
+            mx::store_eight_halves(p.y, row_start, first, k, mx::v4u{mx::two_values(v[0], v[1], p.type), mx::two_values(v[2], v[3], p.type), mx::two_values(v[4], v[5], p.type),
+                                                                     mx::two_values(v[6], v[7], p.type)});
             continue;
         }
-        mx::store_four(p.y, p.type, row * p.k, first, p.k, low);
-        mx::store_four(p.y, p.type, row * p.k, first + 4, p.k, high);
+        mx::store_four(p.y, p.type, row_start, first, k, mx::v4f{v[0], v[1], v[2], v[3]});
+        mx::store_four(p.y, p.type, row_start, first + 4, k, mx::v4f{v[4], v[5], v[6], v[7]});
     }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
-// slots used: K, stride (K as stored), algorithm (type), flags (ceil), flags2 (tiles)
+// slots used: K, group (K in whole blocks, or in steps of 256 for the products), stride (from one stored row to the next), algorithm (type), flags (ceil), flags2 (tiles)
 int geometry(const orx_function& f, int rows, Geometry* g) {
-    if (f.flags2) {
-        g->grid[0] = ceil_div(rows, 16) * ceil_div(2 * (f.stride / mx::kStepK), kThreads / 64);
-        g->block[0] = kThreads;
-        return ORX_OK;
-    }
-    g->grid[0] = (uint32_t)(((int64_t)rows * (f.stride / 8) + kThreads * kPieces - 1) / (kThreads * kPieces));
+    g->grid[0] = f.flags2 ? ceil_div(rows, 16) * ceil_div(f.group / 128, kThreads / 64) : (uint32_t)(((int64_t)rows * (f.group / 8) + kThreads * kPieces - 1) / (kThreads * kPieces));
     g->block[0] = kThreads;
     return ORX_OK;
+}
+template <int TYPE>
+void quantise(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const QuantParams& p) {
+    const dim3 grid(g.grid[0]), block(kThreads);
+    if (f.flags2) ORX_LAUNCH(mx_quantise_tiles_kernel<TYPE>, grid, block, 0, s, p, rows, f.group / mx::kStepK, (int)ceil_div(f.group / 128, kThreads / 64));
+    else if (f.K == f.stride) ORX_LAUNCH((mx_quantise_kernel<TYPE, true>), grid, block, 0, s, p);
+    else ORX_LAUNCH((mx_quantise_kernel<TYPE, false>), grid, block, 0, s, p);
 }
 // Q, S, X, rows
 int quantise_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
     QuantParams p;
     p.q = pointer_arg<uint8_t>(args, 0), p.s = pointer_arg<uint8_t>(args, 1), p.x = pointer_arg<const void>(args, 2);
-    p.pieces = (uint32_t)f.stride / 8, p.pieces_total = (int64_t)rows * p.pieces;
-    p.k = f.K, p.ceil = f.flags;
-    const dim3 grid(g.grid[0]), block(kThreads);
-    if (f.flags2) {  // tiles
-        const int steps = f.stride / mx::kStepK, groups = (2 * steps + kThreads / 64 - 1) / (kThreads / 64);
-        if (f.algorithm == mx::F16) ORX_LAUNCH(mx_quantise_tiles_kernel<mx::F16>, grid, block, 0, s, p, rows, steps, groups);
-        else if (f.algorithm == mx::BF16) ORX_LAUNCH(mx_quantise_tiles_kernel<mx::BF16>, grid, block, 0, s, p, rows, steps, groups);
-        else ORX_LAUNCH(mx_quantise_tiles_kernel<mx::F32>, grid, block, 0, s, p, rows, steps, groups);
-        return hip_check(hipGetLastError(), "launch mxfp4_quantization");
-    }
-    if (f.algorithm == mx::F16) ORX_LAUNCH(mx_quantise_kernel<mx::F16>, grid, block, 0, s, p);
-    else if (f.algorithm == mx::BF16) ORX_LAUNCH(mx_quantise_kernel<mx::BF16>, grid, block, 0, s, p);
-    else ORX_LAUNCH(mx_quantise_kernel<mx::F32>, grid, block, 0, s, p);
+    p.rows = rows_of(rows, f.group / 8, f.stride / 8, f.K), p.ceil = f.flags;
+    if (f.algorithm == mx::F16) quantise<mx::F16>(f, rows, g, s, p);
+    else if (f.algorithm == mx::BF16) quantise<mx::BF16>(f, rows, g, s, p);
+    else quantise<mx::F32>(f, rows, g, s, p);
     return hip_check(hipGetLastError(), "launch mxfp4_quantization");
 }
 // Q, S, Y, rows
 int dequantise_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
     DequantParams p;
     p.q = pointer_arg<const uint8_t>(args, 0), p.s = pointer_arg<const uint8_t>(args, 1), p.y = pointer_arg<void>(args, 2);
-    p.pieces = (uint32_t)f.stride / 8, p.pieces_total = (int64_t)rows * p.pieces;
-    p.k = f.K, p.type = f.algorithm;
-    ORX_LAUNCH(mx_dequantise_kernel, dim3(g.grid[0]), dim3(kThreads), 0, s, p);
+    p.rows = rows_of(rows, f.group / 8, f.stride / 8, f.K), p.type = f.algorithm;
+    if (f.K == f.stride) ORX_LAUNCH(mx_dequantise_kernel<true>, dim3(g.grid[0]), dim3(kThreads), 0, s, p);
+    else ORX_LAUNCH(mx_dequantise_kernel<false>, dim3(g.grid[0]), dim3(kThreads), 0, s, p);
     return hip_check(hipGetLastError(), "launch mxfp4_dequantization");
 }
 
@@ -218,10 +218,11 @@ int shape(const Variant& v, orx_function* f, const char* type_key) {
         set_error("%s: need 0 < K <= %d and pad 32 or 256", f->symbol.c_str(), kMaxK);
         return ORX_ERR_BAD_VARIANT;
     }
-    f->stride = pad == mx::kBlock ? (f->K + 31) / 32 * 32 : ((f->K + 255) / 256 | 1) * 256;  // (for the products an odd multiple)
+    f->group = pad == mx::kBlock ? (f->K + 31) / 32 * 32 : (f->K + 255) / 256 * 256;
+    f->stride = pad == mx::kBlock ? f->group : (f->group / 256 | 1) * 256;  // (for the products an odd multiple; what is behind `group` is not written)
     f->dynamic_rows = true;
-    // (a launch's threads are counted in 32 bits)
-    const int most = (int)std::min<int64_t>(1 << 24, ((1ll << 32) / kThreads - 1) * (kThreads * kPieces) / (f->stride / 8 + 64)) - 16;  // (or the tiles that these rows touch)
+    // (pieces are counted in 32 bits, and so are a launch's threads: a quarter of them)
+    const int most = (int)std::min<int64_t>(1 << 24, ((1ll << 32) - 65536) / (f->stride / 8));
     f->capacity = (int)v.integer("M", most, &bad);
     if (bad || f->capacity < 1 || f->capacity > most) {
         if (!bad) set_error("%s: M must be 1 to %d for this K", f->symbol.c_str(), most);
@@ -242,7 +243,7 @@ int make_quantise(const Variant& v, orx_function* f) {
         set_error("mxfp4_quantization: layout must be rows or tiles, and pad goes with rows");
         return ORX_ERR_BAD_VARIANT;
     }
-    if (layout == "tiles") f->flags2 = 1, f->stride = (f->K + mx::kStepK - 1) / mx::kStepK * mx::kStepK;
+    if (layout == "tiles") f->flags2 = 1, f->group = (f->K + mx::kStepK - 1) / mx::kStepK * mx::kStepK;
     if (scale != "floor" && scale != "ceil") {
         set_error("mxfp4_quantization: scale must be floor or ceil");
         return ORX_ERR_BAD_VARIANT;
@@ -250,12 +251,13 @@ int make_quantise(const Variant& v, orx_function* f) {
     f->flags = scale == "ceil";
     f->args = {{"Q", ArgPointer, 4}, {"S", ArgPointer, 1}, {"X", ArgPointer, f->algorithm == mx::F32 ? 4u : 2u}, {"rows", ArgI32, 4}};
     f->launch = quantise_launch;
-    f->device_function = f->flags2 ? (f->algorithm == mx::F16    ? reinterpret_cast<const void*>(&mx_quantise_tiles_kernel<mx::F16>)
-                                      : f->algorithm == mx::BF16 ? reinterpret_cast<const void*>(&mx_quantise_tiles_kernel<mx::BF16>)
-                                                                 : reinterpret_cast<const void*>(&mx_quantise_tiles_kernel<mx::F32>))
-                         : f->algorithm == mx::F16    ? reinterpret_cast<const void*>(&mx_quantise_kernel<mx::F16>)
-                         : f->algorithm == mx::BF16 ? reinterpret_cast<const void*>(&mx_quantise_kernel<mx::BF16>)
-                                                    : reinterpret_cast<const void*>(&mx_quantise_kernel<mx::F32>);
+    const bool whole = f->K == f->stride;
+#define ORX_QUANTISE(TYPE)                                                                            \
+    (f->flags2 ? reinterpret_cast<const void*>(&mx_quantise_tiles_kernel<TYPE>)                       \
+     : whole   ? reinterpret_cast<const void*>(&mx_quantise_kernel<TYPE, true>)                       \
+               : reinterpret_cast<const void*>(&mx_quantise_kernel<TYPE, false>))
+    f->device_function = f->algorithm == mx::F16 ? ORX_QUANTISE(mx::F16) : f->algorithm == mx::BF16 ? ORX_QUANTISE(mx::BF16) : ORX_QUANTISE(mx::F32);
+#undef ORX_QUANTISE
     return ORX_OK;
 }
 int make_dequantise(const Variant& v, orx_function* f) {
@@ -263,7 +265,7 @@ int make_dequantise(const Variant& v, orx_function* f) {
     if (code != ORX_OK) return code;
     f->args = {{"Q", ArgPointer, 4}, {"S", ArgPointer, 1}, {"Y", ArgPointer, f->algorithm == mx::F32 ? 4u : 2u}, {"rows", ArgI32, 4}};
     f->launch = dequantise_launch;
-    f->device_function = reinterpret_cast<const void*>(&mx_dequantise_kernel);
+    f->device_function = f->K == f->stride ? reinterpret_cast<const void*>(&mx_dequantise_kernel<true>) : reinterpret_cast<const void*>(&mx_dequantise_kernel<false>);
     return ORX_OK;
 }
 
@@ -289,7 +291,7 @@ const Registration* mx_registrations(int* count) {
         {"mxfp4_projection", make_mx_projection, "M, N, K, dynamic_rows=false, input_dtype=mxfp4|float16|bfloat16 (up to 16 rows), epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
          "A[,AS],Out,W,WS[,m]"},
         {"mxfp4_grouped", make_mx_grouped,
-         "rows, E, N, K, tiles, block_m=16|32|64|128|256, gather=false, input_dtype=mxfp4|float16 (block_m=16), epilogue=none|swiglu, "
+         "rows, E, N, K, tiles, block_m=16|64|128|256, gather=false, input_dtype=mxfp4|float16 (block_m=16), epilogue=none|swiglu, "
          "output_dtype=float16|bfloat16|float32",
          "A[,AS],Out[,SlotToken],TileCount,TileUnits,W,WS"},
     };

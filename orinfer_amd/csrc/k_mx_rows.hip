@@ -192,7 +192,8 @@ struct Plan {
 };
 // Eight waves where every CU has a workgroup or less, else four (weights out of cache, us with four / eight: 7168 x 5120, 224 workgroups, 16 rows 5.0 / 5.3, 32 rows 7.1 / 6.7, 64 rows
 // 8.8 / 7.4; 5120 x 17408, 160, 13.9 / 12.4, 25 / 19, 36 / 18; 9728 x 2560, 304, 4.6 / 5.2, 5.6 / 5.9, 7.3 / 7.0; 17408 x 5120, 544, 11.9 / 12.1, 12.6 / 13.6, 16.6 / 17.8).
-Plan few_rows(int unit_rows, int64_t workgroups) { return {unit_rows, 0, workgroups > device_compute_units() ? 4 : 8}; }
+// Rows that the workgroups quantise want eight (17408 x 5120, 4 rows 14.8 / 13.5, 1 row 11.4 / 11.1).
+Plan few_rows(const orx_function& f, int unit_rows, int64_t workgroups) { return {unit_rows, 0, f.packed_k == Codes && workgroups > device_compute_units() ? 4 : 8}; }
 // us that tiles of one kind take: a start, then what the busiest CU has to do, step by step, or all of them at the rate that they sustain (the clock falls with the power that
 // the multipliers draw).  Measured alone, 256 CUs, M x N x K, us with 64 x 128 / 128 x 128 / 256 x 256: 512 x 4096 x 4096 10.1 / 12.1 / 25.6; 2048 x 4096 x 4096 29.2 / 26.8 / 32.2;
 // 8192 x 4096 x 4096 105 / 91 / 76; 333 x 7168 x 5120 16.3 / 15.6 / 31.9; 1500 x 7168 x 5120 49.4 / 44.7 / 38.1; 512 x 17408 x 5120 40.0 / 43.4 / 35.8; 1024 x 17408 x 5120 74 / 69 / 76.
@@ -206,13 +207,13 @@ Plan plan(const orx_function& f, int rows) {
     const int pairs = (f.slots + 1) / 2;
 #ifdef MX_SWEEP
     const char* force = getenv("MX_FORCE");
-    if (force && f.E == 0 && f.packed_k == Codes && rows > 16) { int r, c; sscanf(force, "%d,%d", &r, &c); if (c) return {r, c, 0}; return few_rows(r, (int64_t)pairs * ceil_div(rows, r)); }
+    if (force && f.E == 0 && f.packed_k == Codes && rows > 16) { int r, c; sscanf(force, "%d,%d", &r, &c); if (c) return {r, c, 0}; return few_rows(f, r, (int64_t)pairs * ceil_div(rows, r)); }
 #endif
     if (f.E > 0) {
-        if (f.block_m < 64) return few_rows(f.block_m, (int64_t)pairs * std::min(f.tiles, f.E));
+        if (f.block_m == 16) return few_rows(f, 16, (int64_t)pairs * std::min(f.tiles, f.E));
         return {f.block_m, f.block_m == 256 ? 256 : 128, 0};
     }
-    if (rows <= 64) return few_rows(rows <= 16 ? 16 : rows <= 32 ? 32 : 64, pairs);
+    if (rows <= 64) return few_rows(f, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, pairs);
     const int steps = (f.K + kStepK - 1) / kStepK;
     const int64_t across = ceil_div(f.slots, 8);
     const double small = tiles_us(ceil_div(rows, 64) * across, steps, 64, 128, 0.40, 2.6), medium = tiles_us(ceil_div(rows, 128) * across, steps, 128, 128, 0.62, 3.05);
@@ -258,21 +259,21 @@ int launch_one(const Product& p, const Geometry& g, hipStream_t s) {
 template <int ROWS, int WAVES, int SOURCE>
 int launch_of(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
     const bool swiglu = f.flags & kSwiglu;
-    if constexpr (SOURCE != Brains)
+    if constexpr (ROWS == 1 && SOURCE != Brains)
         if (f.E > 0) return swiglu ? launch_one<ROWS, WAVES, SOURCE, true, true>(p, g, s) : launch_one<ROWS, WAVES, SOURCE, true, false>(p, g, s);
     return swiglu ? launch_one<ROWS, WAVES, SOURCE, false, true>(p, g, s) : launch_one<ROWS, WAVES, SOURCE, false, false>(p, g, s);
 }
 template <int WAVES>
-int launch_rows(const orx_function& f, const Plan& plan, const Product& p, const Geometry& g, hipStream_t s) {
-    if (f.packed_k == Halves) return launch_of<1, WAVES, Halves>(f, p, g, s);
-    if (f.packed_k == Brains) return launch_of<1, WAVES, Brains>(f, p, g, s);
+int launch_codes(const orx_function& f, const Plan& plan, const Product& p, const Geometry& g, hipStream_t s) {
     if (plan.rows == 16) return launch_of<1, WAVES, Codes>(f, p, g, s);
     return plan.rows == 32 ? launch_of<2, WAVES, Codes>(f, p, g, s) : launch_of<4, WAVES, Codes>(f, p, g, s);
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
     if (plan.channels) return launch_mx_tiles(p, plan.rows, plan.channels, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
-    return plan.waves == 4 ? launch_rows<4>(f, plan, p, g, s) : launch_rows<8>(f, plan, p, g, s);
+    if (f.packed_k == Halves) return launch_of<1, 8, Halves>(f, p, g, s);
+    if (f.packed_k == Brains) return launch_of<1, 8, Brains>(f, p, g, s);
+    return plan.waves == 4 ? launch_codes<4>(f, plan, p, g, s) : launch_codes<8>(f, plan, p, g, s);
 }
 
 Product product_of(const orx_function& f, int rows) {
@@ -368,8 +369,8 @@ int make_mx_grouped(const Variant& v, orx_function* f) {
     if (bad) return ORX_ERR_BAD_VARIANT;
     const int code = shape(v, f);
     if (code != ORX_OK) return code;
-    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 32 && f->block_m != 64 && f->block_m != 128 && f->block_m != 256)) {
-        set_error("mxfp4_grouped: need rows, E and tiles above 0 and block_m 16, 32, 64, 128 or 256");
+    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 64 && f->block_m != 128 && f->block_m != 256)) {
+        set_error("mxfp4_grouped: need rows, E and tiles above 0 and block_m 16, 64, 128 or 256");
         return ORX_ERR_BAD_VARIANT;
     }
     f->flags |= gather ? kGather : 0;

@@ -34,7 +34,8 @@ def _kernel(symbol, **variant):
 
 
 def quantize(x, scale="floor", pad=BLOCK):
-    """x (..., K) of fp16, bf16 or fp32 values on the GPU -> codes (..., KP / 2), exponents (..., KP / 32), KP = padded(K, pad), zeros behind K.
+    """x (..., K) of fp16, bf16 or fp32 values on the GPU -> codes (..., KP / 2), exponents (..., KP / 32), KP = padded(K, pad), zeros behind K up to a
+    multiple of 32 (pad 256: of 256; what lies behind that is not written and not read).
     scale: "floor" takes the power of two of a block's largest magnitude (what is above 6 of its units saturates), "ceil" the smallest that nothing saturates with.
     Blocks with an infinity or NaN become NaN."""
     if not x.is_cuda:

@@ -797,7 +797,7 @@ class Mxfp4MoeLayer(_OnDevice):
                 raise ValueError(f"bias must have {experts} values")
         routes = self.assignments = tokens * top_k
         if block_m is None:
-            block_m = 16 if routes <= 24 * experts else 32 if routes <= 48 * experts else 64
+            block_m = 16 if routes <= 10 * experts else 64 if routes < 256 * experts else 128 if routes < 512 * experts else 256
         self.block_m = block_m
         capacity = -(-routes // block_m) + min(experts, routes)
         common = dict(M=tokens, E=experts, top_k=top_k)

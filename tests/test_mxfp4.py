@@ -85,7 +85,7 @@ ROUTER = dict(M=3, E=64, top_k=4)
     ("mxfp4_quantization", dict(K=64, input_dtype="int8")), ("mxfp4_quantization", dict(K=64, M=0)), ("mxfp4_quantization", dict(K=1 << 25)),
     ("mxfp4_quantization", dict(K=64, layout="columns")), ("mxfp4_quantization", dict(K=64, layout="tiles", pad=256)),
     ("mxfp4_projection", dict(M=17, N=96, K=320, input_dtype="float16")), ("mxfp4_projection", dict(M=16, N=96, K=1 << 16, input_dtype="float16")),
-    ("mxfp4_projection", dict(M=1, N=96, K=320, input_dtype="float32")), ("mxfp4_grouped", dict(GROUPED, block_m=32, input_dtype="float16")),
+    ("mxfp4_projection", dict(M=1, N=96, K=320, input_dtype="float32")), ("mxfp4_grouped", dict(GROUPED, block_m=64, input_dtype="float16")), ("mxfp4_grouped", dict(GROUPED, block_m=32)),
     ("mxfp4_grouped", dict(GROUPED, input_dtype="bfloat16")), ("mxfp4_dequantization", dict(K=64, output_dtype="e4m3")), ("mxfp4_dequantization", dict(K=64, scale="ceil")),
     ("mxfp4_projection", dict(M=1, N=96, K=100)), ("mxfp4_projection", dict(M=0, N=96, K=320)), ("mxfp4_projection", dict(M=1, N=0, K=320)),
     ("mxfp4_projection", dict(M=1, N=97, K=320, epilogue="swiglu")), ("mxfp4_projection", dict(M=1, N=96, K=320, epilogue="gelu")),
@@ -137,7 +137,7 @@ def test_a_projection_takes_larger_tiles_where_there_are_more():
     linear = lib.Kernel("mxfp4_projection", M=8192, N=4096, K=4096, dynamic_rows=True)
     assert [started(linear, rows)[0][1:] for rows in (64, 65, 512, 2048, 8192)] == [(512, 65536), (256, 52224), (256, 52224), (256, 69632), (512, 139264)]
     assert all(len(started(linear, rows)) == 1 for rows in (1, 64, 65, 8192))
-    for block_m, lds in ((16, 16384), (32, 32768), (64, 52224), (128, 69632), (256, 139264)):
+    for block_m, lds in ((16, 16384), (64, 52224), (128, 69632), (256, 139264)):
         assert started(lib.Kernel("mxfp4_grouped", **GROUPED, block_m=block_m))[0][2] == lds
 
 
