@@ -721,6 +721,16 @@ class _OnDevice:
 MX_FEW_ROWS = 4  # rows that an MXFP4 projection quantises itself
 
 
+def _where_it_fits(symbol, **keys):
+    """The kernel, or None where its codes do not fit LDS."""
+    try:
+        return Kernel(symbol, **keys)
+    except OrxError as error:
+        if error.code != ORX_ERR_BAD_VARIANT:
+            raise
+        return None
+
+
 class Mxfp4Linear(_OnDevice):
     """Rows of 16-bit values, quantised to MXFP4, times MXFP4 weights: codes (N, K / 2) and exponents (N, K / 32), both uint8 (the format: mxfp4.py), up to `capacity`
     rows at a time.  epilogue="swiglu": the upper half of the channels are the up channels of the gate channels in the lower half, and silu(gate) * up comes out.
@@ -744,12 +754,7 @@ class Mxfp4Linear(_OnDevice):
             self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, layout="tiles")
             # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (weights out of cache, us of the projection alone without / with it,
             # and a quantiser is 2.8: 17408 x 5120 1 row 10.6 / 11.1, 4 rows 11.5 / 13.5, 8 rows 12 / 17; 9728 x 2560 4.4 / 4.6, 4.5 / 5.9, 4.6 / 7.4).  Not where their codes do not fit LDS.
-            self.few = None
-            try:
-                self.few = Kernel("mxfp4_projection", M=min(capacity, MX_FEW_ROWS), input_dtype=name, **shape)
-            except OrxError as error:
-                if error.code != ORX_ERR_BAD_VARIANT:
-                    raise
+            self.few = _where_it_fits("mxfp4_projection", M=min(capacity, MX_FEW_ROWS), input_dtype=name, **shape)
         self.n = channels // 2 if epilogue == "swiglu" else channels
         # the quantised rows, by tiles of 16
         tiles = -(-capacity // 16) * -(-self.k // mxfp4.STEP)
@@ -808,9 +813,16 @@ class Mxfp4MoeLayer(_OnDevice):
             self.k_metadata = Kernel("route_metadata", block_m=block_m, slot_maps=True, workspace=True, tile_units=True, **common)
             grouped = dict(rows=routes, E=experts, tiles=capacity, block_m=block_m)
             self.k_quantise_tokens = Kernel("mxfp4_quantization", K=hidden, pad=mxfp4.STEP)
-            self.k_up = Kernel("mxfp4_grouped", N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", **grouped)
+            up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", **grouped)
+            self.k_up = Kernel("mxfp4_grouped", **up)
             self.k_quantise_act = Kernel("mxfp4_quantization", K=intermediate, pad=mxfp4.STEP)
-            self.k_down = Kernel("mxfp4_grouped", N=hidden, K=intermediate, **grouped)
+            down = dict(N=hidden, K=intermediate, **grouped)
+            self.k_down = Kernel("mxfp4_grouped", **down)
+            # A route to an expert or less: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
+            # 9.1 / 6.5 and down 6.3 / 4.6, 16 tokens 12.6 / 11.3 and 10.7 / 10.5, 32 tokens 14.6 / 14.1 and 11.6 / 13.1, 64 tokens 17.6 / 19.3 and 13.9 / 17.4).
+            self.few_up = self.few_down = None
+            if block_m == 16 and routes <= experts:
+                self.few_up, self.few_down = (_where_it_fits("mxfp4_grouped", input_dtype="float16", **keys) for keys in (up, down))
             self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, **common)
             self.segments = self.k_metadata.workspace()
         i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)
@@ -857,6 +869,9 @@ class Mxfp4MoeLayer(_OnDevice):
         return self.act
 
     def _up(self, x, stream):
+        if self.few_up is not None:
+            self.few_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
+            return
         self.k_quantise_tokens(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=self.tokens)
         self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
 
@@ -874,8 +889,11 @@ class Mxfp4MoeLayer(_OnDevice):
         return self.out
 
     def _down(self, act, prob, shared, shared_gate, stream):
-        self.k_quantise_act(stream=stream, Q=self.h_q, S=self.h_s, X=act, rows=self.assignments)
-        self.k_down(stream=stream, A=self.h_q, AS=self.h_s, Out=self.down_out, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w2, WS=self.p2)
+        if self.few_down is not None:
+            self.few_down(stream=stream, A=act, Out=self.down_out, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w2, WS=self.p2)
+        else:
+            self.k_quantise_act(stream=stream, Q=self.h_q, S=self.h_s, X=act, rows=self.assignments)
+            self.k_down(stream=stream, A=self.h_q, AS=self.h_s, Out=self.down_out, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w2, WS=self.p2)
         self.k_combine(stream=stream, Expert=self.down_out, Output=self.out, Prob=prob, Shared=shared, SharedGate=shared_gate, SlotMap=self.slot_map)
 
     def run(self, x, logits, shared=None, shared_gate=None, stream=None):

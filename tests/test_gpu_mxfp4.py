@@ -261,7 +261,7 @@ def slots_of(ids):
 
 
 SHAPES = [(1, 8, 2, 64, 32), (3, 16, 4, 256, 96), (5, 128, 8, 512, 64), (40, 8, 2, 320, 160), (64, 60, 6, 288, 128), (256, 32, 4, 512, 256), (300, 4, 2, 256, 544),
-          (700, 8, 3, 512, 256), (1100, 2, 1, 256, 128)]
+          (700, 8, 3, 512, 256), (1100, 2, 1, 256, 128), (2, 8, 2, 9728, 64), (2, 8, 3, 64, 9728)]
 
 
 @pytest.mark.parametrize("tokens,experts,top_k,hidden,inner", SHAPES)
@@ -298,6 +298,25 @@ def test_experts(tokens, experts, top_k, hidden, inner, block_m):
     want, each = (y[slot] * p).sum(1), (np.abs(y[slot]) * p).sum(1)
     # each product is rounded to fp16, then top_k products and sums in fp32
     check(out, want, (dy[slot] * p).sum(1) + each * (2.0**-11 + 2 * top_k * 2.0**-24) + 2.0**-25, torch.float16)
+
+
+@pytest.mark.parametrize("tokens,experts,top_k,block_m", [(8, 64, 8, None), (1, 3, 3, None), (40, 64, 8, None), (40, 64, 8, 64), (90, 5, 4, 128), (300, 7, 2, 256)])
+def test_every_route_to_one_expert(tokens, experts, top_k, block_m):
+    """A token may name an expert more than once: its slots are in the order of its routes, the others have none."""
+    hidden, inner = 288, 96
+    layer, gate_up, down, x, _, rng = moe_case(tokens, experts, top_k, hidden, inner, block_m=block_m)
+    ids, e = torch.full((tokens, top_k), experts - 1, dtype=torch.int32, device=DEV), experts - 1
+    np.testing.assert_array_equal(host(layer.place(ids)), np.arange(tokens * top_k).reshape(tokens, top_k))
+    a, w = orc.values(*orc.quantise(x.double().numpy())), orc.values(gate_up[0][e], gate_up[1][e])
+    (gate, dg), (up, du) = product(a, w[:inner]), product(a, w[inner:])
+    want = orc.silu(gate) * up
+    bound = 1.1 * dg * (np.abs(up) + du) + np.abs(gate) * du + 8 * 2.0**-24 * np.abs(want)
+    check(layer.up(x.to(DEV)), want.repeat(top_k, 0), bound.repeat(top_k, 0), torch.float16)
+    rows = torch.from_numpy(rng.standard_normal((tokens * top_k, inner)).astype(np.float16))
+    prob = rng.random((tokens, top_k)).astype(np.float32)
+    y, dy = product(orc.values(*orc.quantise(rows.double().numpy())), orc.values(down[0][e], down[1][e]))
+    y, dy, p = y.reshape(tokens, top_k, hidden), dy.reshape(tokens, top_k, hidden), prob.astype(np.float64)[:, :, None]
+    check(layer.down(rows.to(DEV), dev(prob)), (y * p).sum(1), (dy * p).sum(1) + (np.abs(y) * p).sum(1) * (2.0**-11 + 2 * top_k * 2.0**-24) + 2.0**-25, torch.float16)
 
 
 def same(a, b):
