@@ -205,10 +205,6 @@ double tiles_us(int64_t tiles, int steps, int rows, int channels, double step_us
 }
 Plan plan(const orx_function& f, int rows) {
     const int pairs = (f.slots + 1) / 2;
-#ifdef MX_SWEEP
-    const char* force = getenv("MX_FORCE");
-    if (force && f.E == 0 && f.packed_k == Codes && rows > 16) { int r, c; sscanf(force, "%d,%d", &r, &c); if (c) return {r, c, 0}; return few_rows(f, r, (int64_t)pairs * ceil_div(rows, r)); }
-#endif
     if (f.E > 0) {
         if (f.block_m == 16) return few_rows(f, 16, (int64_t)pairs * std::min(f.tiles, f.E));
         return {f.block_m, f.block_m == 256 ? 256 : 128, 0};

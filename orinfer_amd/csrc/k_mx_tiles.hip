@@ -9,7 +9,9 @@
 // work there, the chip runs into its power: 1.5 GHz with random codes, 2.35 with zeros (9.6 PFLOP/s).  With operands from LDS and requests the step of a 256 x 256 tile takes
 // 1.6-1.75 us on all CUs, 4.9-5.2 PFLOP/s; what is left is the start of a launch and the results.  8192 x 4096 x 4096 76 us (3.6 PFLOP/s), 8192 x 17408 x 5120 410 us (3.55).
 // Tried: four waves of 128 x 128 results (a third less from LDS, 1.63 us a step, but sums come out of accumulation registers by moves, 4.4-6.2 us a tile against 2.1: the same in
-// all); results by lines of 128 bytes through LDS (more instructions, and not faster: what a tile's end took was its instructions).
+// all); results by lines of 128 bytes through LDS (more instructions, and not faster: what a tile's end took was its instructions); three to six stages, a CU then holding one workgroup
+// (305 units of 128 expert rows, 1024 x 2048: 64 us with two stages and two workgroups, 80 with four and one); operands read two quarters ahead and requests masked instead of branched
+// around (each within 3%); barriers that do not wait for the last tile's stores (no faster, and 256 x 256 spills).  Without its requests that product takes 46 us, without results 55.
 #include "lds_asm.h"
 #include "mx_device.h"
 #include "mx_tiles.h"
