@@ -293,7 +293,7 @@ int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream
     p.a = pointer_arg<const uint8_t>(args, 0), p.as = codes ? pointer_arg<const uint8_t>(args, 1) : nullptr, p.out = pointer_arg<void>(args, 1 + codes);
     p.slot_token = gather ? pointer_arg<const int>(args, 2 + codes) : nullptr;
     const int at = 2 + codes + gather;
-    p.unit_count = pointer_arg<const int>(args, at), p.units = pointer_arg<const int4>(args, at + 1);
+    p.unit_count = pointer_arg<const int>(args, at), p.units = pointer_arg<const int4>(args, at + 1), p.most_units = f.tiles;
     p.w = pointer_arg<const uint8_t>(args, at + 2), p.ws = pointer_arg<const uint8_t>(args, at + 3);
     return launch_product(f, rows, g, s, p);
 }

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
 
     // ---- which results: tiles blockIdx.x, blockIdx.x + gridDim.x, .. of an order in which every XCD has one run ----
     const int groups = (p.tiles + BN / 16 - 1) / (BN / 16);
-    const int row_tiles = GROUPED ? __builtin_amdgcn_readfirstlane(*p.unit_count) : (p.m + BM - 1) / BM;
+    const int row_tiles = GROUPED ? min(__builtin_amdgcn_readfirstlane(*p.unit_count), p.most_units) : (p.m + BM - 1) / BM;
     const int total = row_tiles * groups;
     const int my_tiles = (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     if (my_tiles <= 0) return;

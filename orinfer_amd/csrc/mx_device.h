@@ -177,6 +177,7 @@ struct Product {
     // experts: unit = expert, first slot, slots (TileUnits), row of a slot's token or of the slot itself
     const int4* units;
     const int* unit_count;
+    int most_units;  // that the list holds
     const int* slot_token;
 };
 

@@ -243,6 +243,47 @@ def test_linear_on_another_stream_and_replayed_from_a_graph(rows):
         torch.cuda.synchronize()
 
 
+def test_two_linears_on_two_streams_at_once():
+    cases = [linear_case(rows, 700, 1184, seed=seed) for seed, rows in enumerate((300, 17, 2, 40))]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (linear, x, _, _), stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                linear.run(x)
+    torch.cuda.synchronize()
+    for linear, x, want, bound in cases:
+        check(linear.out, want, bound, torch.float16)
+
+
+def sampled(rows):
+    return np.unique(np.concatenate([np.arange(3), np.arange(rows // 2, rows // 2 + 3), np.arange(rows - 5, rows)]))
+
+
+def test_quantisation_of_more_than_4_gib():
+    rows, k = 2**20 + 3, 2304
+    x = torch.randn((rows // 8 + 1, k), device=DEV).to(torch.bfloat16).repeat(8, 1)[:rows]
+    at = torch.from_numpy(sampled(rows)).to(DEV)
+    x[-5:] *= 3
+    codes, exponents = mxfp4.quantize(x)
+    want_codes, want_exponents = orc.quantise(x[at].double().cpu().numpy())
+    np.testing.assert_array_equal(host(codes[at]), want_codes)
+    np.testing.assert_array_equal(host(exponents[at]), want_exponents)
+    back = mxfp4.dequantize(codes, exponents, k, torch.bfloat16)
+    np.testing.assert_array_equal(host(back[at].float()), orc.values(want_codes, want_exponents))
+
+
+def test_linear_with_more_than_4_gib_of_results():
+    rows, n, k = 2**20 + 3, 2100, 64
+    rng = np.random.default_rng(4)
+    codes, exponents = weights(rng, n, k)
+    x = torch.randn((rows, k), device=DEV).half()
+    linear = programs.Mxfp4Linear(dev(codes), dev(exponents), rows)
+    at = sampled(rows)
+    want, bound = product(orc.values(*orc.quantise(x[torch.from_numpy(at).to(DEV)].double().cpu().numpy())), orc.values(codes, exponents))
+    check(linear.run(x)[torch.from_numpy(at).to(DEV)], want, bound, torch.float16)
+
+
 # ---- experts -----------------------------------------------------------------------------------------------------------------------------------
 def moe_case(tokens, experts, top_k, hidden, inner, seed=0, skew=0.0, **options):
     rng = np.random.default_rng(seed + tokens * 131 + experts)
@@ -317,6 +358,24 @@ def test_every_route_to_one_expert(tokens, experts, top_k, block_m):
     y, dy = product(orc.values(*orc.quantise(rows.double().numpy())), orc.values(down[0][e], down[1][e]))
     y, dy, p = y.reshape(tokens, top_k, hidden), dy.reshape(tokens, top_k, hidden), prob.astype(np.float64)[:, :, None]
     check(layer.down(rows.to(DEV), dev(prob)), (y * p).sum(1), (dy * p).sum(1) + (np.abs(y) * p).sum(1) * (2.0**-11 + 2 * top_k * 2.0**-24) + 2.0**-25, torch.float16)
+
+
+def test_experts_with_more_than_4_gib_of_rows():
+    tokens, experts, top_k, hidden, inner = 2**18 + 1, 5, 4, 2112, 64
+    rng = np.random.default_rng(11)
+    gate_up, down = weights(rng, experts, 2 * inner, hidden), weights(rng, experts, hidden, inner)
+    layer = programs.Mxfp4MoeLayer(tokens, experts, top_k, hidden, inner, *map(dev, gate_up), *map(dev, down))
+    ids = torch.rand((tokens, experts), device=DEV).argsort(1)[:, :top_k].int().contiguous()
+    slot = layer.place(ids).long()
+    prob = torch.rand((tokens, top_k), device=DEV)
+    act = torch.randn((tokens * top_k, inner), device=DEV).half()
+    out = layer.down(act, prob)
+    at = torch.from_numpy(sampled(tokens)).to(DEV)
+    rows, chosen, p = act[slot[at]].double().cpu().numpy(), host(ids[at]), host(prob[at]).astype(np.float64)[:, :, None]
+    y, dy = np.empty((*chosen.shape, hidden)), np.empty((*chosen.shape, hidden))
+    for i, e in np.ndindex(*chosen.shape):
+        y[i, e], dy[i, e] = (r[0] for r in product(orc.values(*orc.quantise(rows[i, e][None])), orc.values(down[0][chosen[i, e]], down[1][chosen[i, e]])))
+    check(out[at], (y * p).sum(1), (dy * p).sum(1) + (np.abs(y) * p).sum(1) * (2.0**-11 + 2 * top_k * 2.0**-24) + 2.0**-25, torch.float16)
 
 
 def same(a, b):

@@ -116,3 +116,23 @@ def test_fewer_rows_than_the_capacity_leave_the_rest():
     np.testing.assert_array_equal(ids[:5], want)
     np.testing.assert_allclose(prob[:5], weights, rtol=2.0**-23)
     assert (ids[5:] == -7).all() and (prob[5:] == -7).all()
+
+
+def test_captured_and_replayed():
+    logits = torch.randn((37, 160), device="cuda")
+    bias = torch.randn(160, device="cuda") * 0.1
+    ids, prob = torch.empty((37, 6), dtype=torch.int32, device="cuda"), torch.empty((37, 6), device="cuda")
+    router = kernel("router_topk", M=37, E=160, top_k=6, scoring="sigmoid", bias=True, groups=8, top_groups=3, scale=2.5)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        router(stream=stream.cuda_stream, Bias=bias, IDs=ids, Logits=logits, Prob=prob)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want_ids, want = orc.routes(host(logits), 6, scoring="sigmoid", bias=host(bias), groups=8, top_groups=3, scale=2.5)
+        np.testing.assert_array_equal(host(ids), want_ids)
+        np.testing.assert_allclose(host(prob), want, rtol=2.0**-23, atol=2.0**-149)
+        logits.copy_(logits.roll(1, 1))
+        bias.neg_()
+        torch.cuda.synchronize()
