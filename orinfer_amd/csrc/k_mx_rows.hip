@@ -6,6 +6,7 @@
 // took as long as the weights (weights out of cache, 17408 x 5120: 32 rows 16.7 us, as tiles 12.6, 64 rows 25.0 / 16.6).
 // Rows of 16-bit values (QUANTISE, up to 16): a workgroup makes their codes itself, into LDS, while its first weights are on their way.
 #include <algorithm>
+#include <cmath>
 
 #include "mx_device.h"
 #include "mx_tiles.h"
@@ -186,22 +187,35 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
 constexpr int kMostLds = 80 * 1024;  // of the few-rows kernel
 enum { kSwiglu = 1, kGather = 2 };
 
-// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS (0: the kernel above, 32 of them) or its waves
+// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS, whose waves may take K in two halves (0: the kernel above, 32 channels), or its waves
 struct Plan {
-    int rows, channels, waves;
+    int rows, channels, waves, halves = 1;
 };
-// Eight waves where every CU has a workgroup or less, else four (weights out of cache, us with four / eight: 7168 x 5120, 224 workgroups, 16 rows 5.0 / 5.3, 32 rows 7.1 / 6.7, 64 rows
-// 8.8 / 7.4; 5120 x 17408, 160, 13.9 / 12.4, 25 / 19, 36 / 18; 9728 x 2560, 304, 4.6 / 5.2, 5.6 / 5.9, 7.3 / 7.0; 17408 x 5120, 544, 11.9 / 12.1, 12.6 / 13.6, 16.6 / 17.8).
-// Rows that the workgroups quantise want eight (17408 x 5120, 4 rows 14.8 / 13.5, 1 row 11.4 / 11.1).
-Plan few_rows(const orx_function& f, int unit_rows, int64_t workgroups) { return {unit_rows, 0, f.packed_k == Codes && workgroups > device_compute_units() ? 4 : 8}; }
-// us that tiles of one kind take: a start, then what the busiest CU has to do, step by step, or all of them at the rate that they sustain (the clock falls with the power that
-// the multipliers draw).  Measured alone, 256 CUs, M x N x K, us with 64 x 128 / 128 x 128 / 256 x 256: 512 x 4096 x 4096 10.1 / 12.1 / 25.6; 2048 x 4096 x 4096 29.2 / 26.8 / 32.2;
-// 8192 x 4096 x 4096 105 / 91 / 76; 333 x 7168 x 5120 16.3 / 15.6 / 31.9; 1500 x 7168 x 5120 49.4 / 44.7 / 38.1; 512 x 17408 x 5120 40.0 / 43.4 / 35.8; 1024 x 17408 x 5120 74 / 69 / 76.
-double tiles_us(int64_t tiles, int steps, int rows, int channels, double step_us, double petaflops) {
-    const int cus = device_compute_units();
-    const double busiest = (double)((tiles + cus - 1) / cus) * steps * step_us;
-    const double all = (double)tiles * steps * (2e-9 * kStepK * rows * channels) / petaflops * (256.0 / cus);
-    return 2.5 + std::max(busiest, all);
+// Eight waves where every CU has a workgroup or less, or two and K is long enough or the rows many enough for eight, else four.  Us with four / eight, weights out of cache: 32 rows to a
+// unit, 7168 x 5120, 448 workgroups 12.0 / 10.0; 4096 x 4096, 384, 7.4 / 6.8, 1024, 10.7 / 11.2; 17408 x 5120, 1088, 19.4 / 19.9; 9728 x 2560, 304, 5.6 / 5.9, 608, 8.0 / 8.2; 64 rows, 9728 x 2560, 304,
+// 10.0 / 8.9, 608, 10.7 / 12.3; 4096 x 4096, 512, 10.9 / 9.2, 768, 12.5 / 14.4; 5120 x 17408, 160, 44 / 25.  Rows that the workgroups quantise want eight (17408 x 5120, 4 rows 14.8 / 13.5,
+// 1 row 11.4 / 11.1).
+Plan few_rows(const orx_function& f, int unit_rows, int64_t workgroups) {
+    const int64_t cus = device_compute_units();
+    const bool eight = workgroups <= cus || (workgroups <= 2 * cus && (unit_rows == 64 || f.K > 10 * kStepK));
+    return {unit_rows, 0, f.packed_k == Codes && !eight ? 4 : 8};
+}
+// Us that a launch takes, weights out of cache, 256 CUs (within a fifth of what was measured at 40-700 rows of 7168 x 5120, 4096 x 4096, 1024 x 4096, 17408 x 5120, 5120 x 17408, 2048 x 1024,
+// 1056 x 2080, 9728 x 2560).  The kernel above: a chain of steps for each wave, or what all workgroups read through the L2s.  Tiles: a chain of steps, longer where a CU has several
+// workgroups side by side or one after another.  So few rows of few channels go to the former (128 rows of 4096 x 4096: 7.1, tiles 12.4 and 14.1), 32 to a unit first (64 rows: 5.9, as one unit 7.0), tiles where there are
+// enough for all CUs, in halves of K where there are not (333 rows of 7168 x 5120: 20.4, else 23.1; 333 rows of 5120 x 17408 45, else 57).
+double few_rows_us(const orx_function& f, int rows, int unit_rows) {
+    const double steps = (f.K + kStepK - 1) / kStepK, workgroups = (double)ceil_div(rows, unit_rows) * ((f.slots + 1) / 2);
+    const double chain = std::ceil(steps / 8) * (unit_rows == 32 ? 1.7 : 2.4);
+    const double bytes = workgroups * (unit_rows + 32) * steps * 136, rate = unit_rows == 32 ? 13.5e6 : 13e6;
+    return 2.5 + std::max(chain, bytes / rate * (256.0 / device_compute_units()));
+}
+double tiles_us(const orx_function& f, int rows, const Plan& tile) {
+    const int64_t cus = device_compute_units(), tiles = (int64_t)ceil_div(rows, tile.rows) * ceil_div(f.slots, tile.channels / 16);
+    const double steps = (f.K + kStepK - 1) / kStepK, to_a_cu = (double)((tiles + cus - 1) / cus);
+    if (tile.halves == 2) return tiles > cus || steps < 2 ? 1e30 : 2.5 + std::ceil(steps / 2) * (tile.rows == 64 ? 1.35 : 1.65);
+    if (tile.rows == 64) return 2.5 + steps * std::max(0.85, 0.45 * to_a_cu);
+    return 2.5 + steps * (tile.rows == 256 ? 1.8 * to_a_cu : to_a_cu == 1 ? 1.0 : 1.27 * std::ceil(to_a_cu / 2));
 }
 Plan plan(const orx_function& f, int rows) {
     const int pairs = (f.slots + 1) / 2;
@@ -209,13 +223,17 @@ Plan plan(const orx_function& f, int rows) {
         if (f.block_m == 16) return few_rows(f, 16, (int64_t)pairs * std::min(f.tiles, f.E));
         return {f.block_m, f.block_m == 256 ? 256 : 128, 0};
     }
-    if (rows <= 64) return few_rows(f, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, pairs);
-    const int steps = (f.K + kStepK - 1) / kStepK;
-    const int64_t across = ceil_div(f.slots, 8);
-    const double small = tiles_us(ceil_div(rows, 64) * across, steps, 64, 128, 0.40, 2.6), medium = tiles_us(ceil_div(rows, 128) * across, steps, 128, 128, 0.62, 3.05);
-    const double large = tiles_us((int64_t)ceil_div(rows, 256) * ceil_div(f.slots, 16), steps, 256, 256, 1.75, 3.65);
-    if (large <= medium && large <= small) return {256, 256, 0};
-    return medium <= small ? Plan{128, 128, 0} : Plan{64, 128, 0};
+    if (rows <= 16) return few_rows(f, 16, pairs);
+    Plan best = few_rows(f, 32, (int64_t)ceil_div(rows, 32) * pairs);
+    if (rows <= 32) return best;
+    double best_us = few_rows_us(f, rows, 32);
+    auto weigh = [&](const Plan& other, double us) {
+        if (us < best_us) best = other, best_us = us;
+    };
+    weigh(few_rows(f, 64, (int64_t)ceil_div(rows, 64) * pairs), few_rows_us(f, rows, 64));
+    if (rows > 64)
+        for (const Plan& tile : {Plan{64, 128, 0, 1}, Plan{64, 128, 0, 2}, Plan{128, 128, 0, 1}, Plan{128, 128, 0, 2}, Plan{256, 256, 0, 1}}) weigh(tile, tiles_us(f, rows, tile));
+    return best;
 }
 uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
     const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * 2 * 1024;
@@ -232,9 +250,9 @@ int geometry(const orx_function& f, int rows, Geometry* g) {
         return ORX_ERR_ROWS;
     }
     if (plan.channels) {
-        blocks = std::min<int64_t>(blocks, (int64_t)device_compute_units() * mx_tiles_to_a_cu(plan.rows));
-        g->block[0] = mx_tiles_threads(plan.rows);
-        g->shared = mx_tiles_lds(plan.rows, plan.channels);
+        if (plan.halves == 1) blocks = std::min<int64_t>(blocks, (int64_t)device_compute_units() * mx_tiles_to_a_cu(plan.rows));
+        g->block[0] = mx_tiles_threads(plan.rows, plan.halves);
+        g->shared = mx_tiles_lds(plan.rows, plan.channels, plan.halves);
     } else {
         g->block[0] = 64 * plan.waves;
         g->shared = few_rows_lds(f, rows, plan);
@@ -266,7 +284,7 @@ int launch_codes(const orx_function& f, const Plan& plan, const Product& p, cons
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
-    if (plan.channels) return launch_mx_tiles(p, plan.rows, plan.channels, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
+    if (plan.channels) return launch_mx_tiles(p, plan.rows, plan.channels, plan.halves, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
     if (f.packed_k == Halves) return launch_of<1, 8, Halves>(f, p, g, s);
     if (f.packed_k == Brains) return launch_of<1, 8, Brains>(f, p, g, s);
     return plan.waves == 4 ? launch_codes<4>(f, plan, p, g, s) : launch_codes<8>(f, plan, p, g, s);

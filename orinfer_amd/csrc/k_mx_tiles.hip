@@ -2,16 +2,20 @@
 //
 // DOWN x ACROSS waves share a tile, each 32 ROWS x 32 CHANNELS of it in blocks of 32 x 32; K goes in steps of 256.  Codes and powers come from memory to LDS without passing a
 // register (16 or 4 bytes a lane), two stages.  Weights and dense rows arrive as they are laid out, a kilobyte to a request; of an expert's rows, which lie anywhere, the 128 bytes of a
-// step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the sixteen rows of a read meet different banks.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their
-// way while the last ones are multiplied, and results drain under the next multiplies.
+// step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the sixteen rows of a read meet different banks.  A workgroup goes through its tiles as one sequence of steps: the next
+// tile's first steps are on their way while the last ones are multiplied, and results drain under the next multiplies.
+// HALVES 2: as many waves again take the second half of K, for launches whose tiles do not fill the CUs (7168 x 5120, weights out of cache, us with / without: 333 rows in tiles of 128
+// 20.4 / 23.1, 200 rows in tiles of 64 17.0 / 19.6; 5120 x 17408, 333 rows, 64: 45 / 57).
+// LOOK: quarters of a step that operands are read ahead, two where the registers hold them (128 x 128: 333 rows 17.6 / 17.9, experts of 2048 x 512 70.2 / 74.0).
 //
 // v_mfma_scale_f32_32x32x64 takes 32 cycles, 16 x 16 x 128 18, so the former: 6.2 PFLOP/s on random codes straight from registers, 5.4 the latter.  The multipliers do not run out of
 // work there, the chip runs into its power: 1.5 GHz with random codes, 2.35 with zeros (9.6 PFLOP/s).  With operands from LDS and requests the step of a 256 x 256 tile takes
-// 1.6-1.75 us on all CUs, 4.9-5.2 PFLOP/s; what is left is the start of a launch and the results.  8192 x 4096 x 4096 76 us (3.6 PFLOP/s), 8192 x 17408 x 5120 410 us (3.55).
+// 1.6-1.75 us on all CUs, 4.9-5.2 PFLOP/s; what is left is the start of a launch and the results.  8192 x 4096 x 4096 75 us (3.65 PFLOP/s), 8192 x 17408 x 5120 410 us (3.55).
+// A 128 x 128 step alone on a CU takes 0.5-0.65 us, 0.3 without its requests, 0.15 without its multiplies either.
 // Tried: four waves of 128 x 128 results (a third less from LDS, 1.63 us a step, but sums come out of accumulation registers by moves, 4.4-6.2 us a tile against 2.1: the same in
 // all); results by lines of 128 bytes through LDS (more instructions, and not faster: what a tile's end took was its instructions); three to six stages, a CU then holding one workgroup
-// (305 units of 128 expert rows, 1024 x 2048: 64 us with two stages and two workgroups, 80 with four and one); operands read two quarters ahead and requests masked instead of branched
-// around (each within 3%); barriers that do not wait for the last tile's stores (no faster, and 256 x 256 spills).  Without its requests that product takes 46 us, without results 55.
+// (305 units of 128 expert rows, 1024 x 2048: 64 us with two stages and two workgroups, 80 with four and one); requests masked instead of branched around (level); barriers that do not
+// wait for the last tile's stores (no faster, and 256 x 256 spills).  Without its requests that product takes 46 us, without results 55.
 #include "lds_asm.h"
 #include "mx_device.h"
 #include "mx_tiles.h"
@@ -53,16 +57,19 @@ __device__ __forceinline__ void everybody_arrived() {
     asm volatile("" ::: "memory");
 }
 
-template <int ROWS, int CHANNELS, int DOWN, int ACROSS, bool WIDE, bool GROUPED, bool SWIGLU>
-__global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product p) {
+template <int ROWS, int CHANNELS, int DOWN, int ACROSS, int LOOK, int HALVES, bool WIDE, bool GROUPED, bool SWIGLU>
+__global__ __launch_bounds__(64 * DOWN * ACROSS * HALVES, 2) void mx_tiles_kernel(Product p) {
     constexpr int BM = 32 * ROWS * DOWN, BN = 32 * CHANNELS * ACROSS, WAVES = DOWN * ACROSS;
     constexpr int A_REQUESTS = BM / (GROUPED ? 8 : 16) / WAVES, W_REQUESTS = BN / 16 / WAVES;  // of a wave and step: eight rows or a tile, a tile
     constexpr int POWERS = BM / 32 + BN / 32;                                                   // of all waves
     constexpr int kW = BM * 128, kAS = kW + BN * 128, kWS = kAS + BM * 8, kStage = kWS + BN * 8;
     constexpr int kSmall = (POWERS + WAVES - 1) / WAVES;
-    extern __shared__ __align__(128) uint8_t lds[];
+    extern __shared__ __align__(128) uint8_t whole_lds[];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % WAVES, half = HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) / WAVES;
+    uint8_t* const lds = whole_lds + half * (2 * kStage);
+    // of K, two halves of equal steps: of an odd number both have the middle one, and the second half drops it
+    const int steps = HALVES == 1 ? p.steps : (p.steps + 1) / 2, first_step = half ? p.steps - steps : 0;
     const int wave_m = wave % DOWN, wave_n = wave / DOWN;
 
     // ---- which results: tiles blockIdx.x, blockIdx.x + gridDim.x, .. of an order in which every XCD has one run ----
@@ -105,14 +112,14 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
                 const int local = (wave * A_REQUESTS + b) * 8 + (lane >> 3);
                 int64_t row = t.first_row + min(local, t.rows - 1);
                 if (p.slot_token != nullptr) row = p.slot_token[row];
-                a_from[b] = p.a + row * p.pitch + ((lane & 7) ^ ((local >> 1) & 7)) * 16;
+                a_from[b] = p.a + row * p.pitch + first_step * 128 + ((lane & 7) ^ ((local >> 1) & 7)) * 16;
             } else {
-                a_from[b] = uniform_pointer(p.a + (int64_t)min(t.first_row / 16 + wave * A_REQUESTS + b, (p.m - 1) / 16) * p.steps * kTileBytes);
+                a_from[b] = uniform_pointer(p.a + ((int64_t)min(t.first_row / 16 + wave * A_REQUESTS + b, (p.m - 1) / 16) * p.steps + first_step) * kTileBytes);
             }
         }
         const int64_t expert = (int64_t)t.expert * p.tiles;
 #pragma unroll
-        for (int b = 0; b < W_REQUESTS; ++b) w_from[b] = uniform_pointer(p.w + (expert + min(t.group * (BN / 16) + wave * W_REQUESTS + b, p.tiles - 1)) * p.steps * kTileBytes);
+        for (int b = 0; b < W_REQUESTS; ++b) w_from[b] = uniform_pointer(p.w + ((expert + min(t.group * (BN / 16) + wave * W_REQUESTS + b, p.tiles - 1)) * p.steps + first_step) * kTileBytes);
 #pragma unroll
         for (int i = 0; i < kSmall; ++i) {
             const int j = wave + WAVES * i;
@@ -132,11 +139,12 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
                 power_from[i] = p.ws + tile * p.steps * kTilePowers + (lane & 31) * 4;
                 power_step[i] = kTilePowers, power_to[i] = kWS + (j - BM / 32) * 256;
             }
+            power_from[i] += first_step * power_step[i];
         }
     };
     int load_tile = 0, load_step = 0;
     auto advance = [&]() {
-        if (++load_step < p.steps) return;
+        if (++load_step < steps) return;
         load_step = 0;
         if (++load_tile < my_tiles) aim(tile_of(load_tile));
     };
@@ -164,7 +172,8 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
     const uint32_t w_at = kW + (wave_n * 2 * CHANNELS + (r >> 4)) * 2048 + low * 256 + (r & 15) * 16;
     const uint32_t as_at = GROUPED ? kAS + (wave_m * 32 * ROWS + r) * 8 : kAS + (wave_m * 2 * ROWS + (r >> 4)) * 128 + (r & 15) * 8 + low * 4;
     const uint32_t ws_at = kWS + (wave_n * 2 * CHANNELS + (r >> 4)) * 128 + (r & 15) * 8 + low * 4;
-    v4i fa[2][ROWS], fw[2][CHANNELS];
+    constexpr int kHeld = LOOK == 1 ? 2 : 4;  // quarters' operands
+    v4i fa[kHeld][ROWS], fw[kHeld][CHANNELS];
     uint2 read_a[ROWS];  // of the next step
     int read_w[CHANNELS], powers_a[ROWS], powers_w[CHANNELS];
     const uint32_t select = low ? 0x07050301u : 0x06040200u;  // a row's eight powers, those of this lane's four blocks
@@ -173,9 +182,9 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
     auto read_operand = [&](auto t, auto at, uint32_t stage) {
         constexpr int T = decltype(t)::value, AT = decltype(at)::value;
         if constexpr (AT < ROWS)
-            fa[T & 1][AT] = *reinterpret_cast<const v4i*>(lds + ((GROUPED ? a_at ^ (T * 32) : a_at) + stage) + (AT * 4096 + (GROUPED ? 0 : T * 512)));
+            fa[T % kHeld][AT] = *reinterpret_cast<const v4i*>(lds + ((GROUPED ? a_at ^ (T * 32) : a_at) + stage) + (AT * 4096 + (GROUPED ? 0 : T * 512)));
         else
-            fw[T & 1][AT - ROWS] = *reinterpret_cast<const v4i*>(lds + (w_at + stage) + ((AT - ROWS) * 4096 + T * 512));
+            fw[T % kHeld][AT - ROWS] = *reinterpret_cast<const v4i*>(lds + (w_at + stage) + ((AT - ROWS) * 4096 + T * 512));
     };
     auto read_power = [&](auto at, uint32_t stage) {
         constexpr int AT = decltype(at)::value;
@@ -199,9 +208,9 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
         constexpr int T = decltype(t)::value, I = decltype(at)::value / CHANNELS, JJ = decltype(at)::value % CHANNELS;
         constexpr int J = I & 1 ? CHANNELS - 1 - JJ : JJ;  // one operand changes between neighbours
         if constexpr (decltype(fresh)::value)
-            sum[I][J] = multiply_32<T, T>(fw[T & 1][J], fa[T & 1][I], v16f{}, powers_w[J], powers_a[I]);
+            sum[I][J] = multiply_32<T, T>(fw[T % kHeld][J], fa[T % kHeld][I], v16f{}, powers_w[J], powers_a[I]);
         else
-            sum[I][J] = multiply_32<T, T>(fw[T & 1][J], fa[T & 1][I], sum[I][J], powers_w[J], powers_a[I]);
+            sum[I][J] = multiply_32<T, T>(fw[T % kHeld][J], fa[T % kHeld][I], sum[I][J], powers_w[J], powers_a[I]);
     };
     using Fresh = std::true_type;
     using Added = std::false_type;
@@ -211,7 +220,8 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
     using T3 = std::integral_constant<int, 3>;
     // A wave cannot issue anything while an LDS read or a request waits for its slot, and with one wave to a SIMD the multiplier then runs dry: behind every multiply stands at most
     // a read or two.  A step's requests go out in three parts, behind the barrier that frees their stage and in the two quarters of the next step behind it.
-    constexpr int kPart3 = kAll * 8 / 20, kPart0 = (kAll - kPart3 + 1) / 2, kPart1 = kAll - kPart3 - kPart0;
+    constexpr int kPart0 = kAll * 8 / 20, kPart1 = (kAll - kPart0 + 1) / 2;
+    constexpr int kAtOnce = LOOK == 1 ? kPart0 : kPart0 + kPart1;  // in front of the next step
     // Multiplies FIRST.. of quarter t with `other(0)` .. `other(COUNT - 1)` among them.
     auto multiply_among = [&](auto t, auto first, auto fresh, auto count, auto other) {
         constexpr int FIRST = decltype(first)::value, LEFT = ROWS * CHANNELS - FIRST, COUNT = decltype(count)::value;
@@ -225,32 +235,44 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    // Quarter t: the next quarter's operands are read, requests BEGIN.. of the next step go out.
-    auto quarter = [&](auto t, auto next, auto fresh, uint32_t stage, auto begin, auto count, int wanted) {
-        multiply_among(t, T0{}, fresh, std::integral_constant<int, kSet + decltype(count)::value>{}, [&](auto q) {
+    constexpr int FOURS = SWIGLU ? 2 : 4;  // results of a block and lane, by four
+    uint32_t stage = 0;
+    int left = my_tiles * steps;  // steps, with this one
+    // Quarter t, with the reads of quarter t + LOOK's operands, of the next step's powers in the last one, and a part of the requests.  In quarter 4 - LOOK, after one multiply to go on
+    // with, the next stage is whole and nobody reads this one any more.
+    auto quarter = [&](auto t, auto fresh, uint32_t next) {
+        constexpr int T = decltype(t)::value, PART = (T + LOOK) % 4, kFirst = PART == 0 ? 1 : 0, kPowers = T == 3 ? kSet : 0;
+        constexpr int kBegin = PART == 0 ? 0 : PART == 1 ? kPart0 : kPart0 + kPart1, kRequests = PART == 0 ? kPart0 : PART == 1 ? kPart1 : PART == 2 ? kAll - kPart0 - kPart1 : 0;
+        if constexpr (PART == 0) {
+            multiply(t, T0{}, fresh);
+            __builtin_amdgcn_sched_barrier(0);
+            everybody_arrived();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        multiply_among(t, std::integral_constant<int, kFirst>{}, fresh, std::integral_constant<int, kSet + kPowers + kRequests>{}, [&](auto q) {
             constexpr int Q = decltype(q)::value;
-            if constexpr (Q < kSet) read_operand(next, q, stage);
-            else request(decltype(begin)::value + Q - kSet, kStage - stage, wanted);
+            if constexpr (Q < kSet) read_operand(std::integral_constant<int, (T + LOOK) % 4>{}, q, T + LOOK < 4 ? stage : next);
+            else if constexpr (Q < kSet + kPowers) read_power(std::integral_constant<int, Q - kSet>{}, next);
+            else if constexpr (T + LOOK < 4) request(kBegin + Q - kSet - kPowers, next, left - 1);
+            else request(kBegin + Q - kSet - kPowers, stage, left - 2);
         });
     };
-    using Part3 = std::integral_constant<int, kPart3>;
-    using Part0 = std::integral_constant<int, kPart0>;
-    using Part1 = std::integral_constant<int, kPart1>;
-    using Parts30 = std::integral_constant<int, kPart3 + kPart0>;
 
     // ---- results: block (i, j) has channels 8 (e / 4) + 4 low + e % 4 of row r; pairs of fours change halves, and a lane has eight neighbours ----
-    constexpr int FOURS = SWIGLU ? 2 : 4;  // results of a block and lane, by four
     auto results = [&](v16f& s, v4f(&four)[FOURS]) {
 #pragma unroll
         for (int q = 0; q < FOURS; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) four[q][e] = SWIGLU ? swiglu(s[4 * q + e], s[8 + 4 * q + e]) : s[4 * q + e];
     };
+    // Two halves of K: each hands half of its blocks over in LDS, adds what it gets to the others, and stores those.
+    auto kept = [&](int at) { return HALVES == 1 || (at < ROWS * CHANNELS / 2) == (half == 0); };
     auto store = [&](const Tile& t) {
         const int first_col = (t.group * ACROSS + wave_n) * CHANNELS * (8 * FOURS);
         if (first_col + CHANNELS * 8 * FOURS <= p.cols) {
             Each<ROWS * CHANNELS>::run([&](auto at) {
                 constexpr int I = decltype(at)::value / CHANNELS, J = decltype(at)::value % CHANNELS;
+                if (!kept(decltype(at)::value)) return;
                 const int row = (wave_m * ROWS + I) * 32 + r;
                 v16f& s = sum[I][J];
                 v4f four[FOURS];
@@ -290,6 +312,7 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
         // the last channels: one piece of code for all blocks, column by column where they end
 #pragma unroll 1
         for (int at = 0; at < ROWS * CHANNELS; ++at) {
+            if (!kept(at)) continue;
             v16f s;
             Each<ROWS * CHANNELS>::run([&](auto which) {
                 v16f& block = sum[decltype(which)::value / CHANNELS][decltype(which)::value % CHANNELS];
@@ -310,73 +333,97 @@ __global__ __launch_bounds__(64 * DOWN * ACROSS, 2) void mx_tiles_kernel(Product
     };
 
     aim(tile_of(0));
-    const int total_steps = my_tiles * p.steps;
 #pragma unroll
     for (int q = 0; q < kAll; ++q) request(q, 0, 1);
     advance();
     everybody_arrived();
 #pragma unroll
-    for (int q = 0; q < kPart3; ++q) request(q, kStage, total_steps - 1);
+    for (int q = 0; q < kAtOnce; ++q) request(q, kStage, left - 1);
     Each<kSet>::run([&](auto at) { read_operand(T0{}, at, 0); });
+    if constexpr (LOOK > 1) Each<kSet>::run([&](auto at) { read_operand(T1{}, at, 0); });
     Each<kSet>::run([&](auto at) { read_power(at, 0); });
-    uint32_t stage = 0;
-    int left = total_steps;
     // One sequence of steps over all tiles: the next tile's first steps are on their way while this one's last are multiplied.  (The last step of all reads a stage that nobody filled.)
     auto one_step = [&](auto fresh) {
+        const uint32_t next = kStage - stage;
         take_powers();
-        quarter(T0{}, T1{}, fresh, stage, Part3{}, Part0{}, left - 1);
-        quarter(T1{}, T2{}, Added{}, stage, Parts30{}, Part1{}, left - 1);
-        advance();
-        quarter(T2{}, T3{}, Added{}, stage, T0{}, T0{}, 0);
-        // a multiply to go on with; then the next stage is whole and nobody reads this one any more
-        multiply(T3{}, T0{}, Added{});
-        __builtin_amdgcn_sched_barrier(0);
-        everybody_arrived();
-        __builtin_amdgcn_sched_barrier(0);
-        multiply_among(T3{}, T1{}, Added{}, std::integral_constant<int, 2 * kSet + kPart3>{}, [&](auto q) {
-            constexpr int Q = decltype(q)::value;
-            if constexpr (Q < kSet) read_operand(T0{}, q, kStage - stage);
-            else if constexpr (Q < 2 * kSet) read_power(std::integral_constant<int, Q - kSet>{}, kStage - stage);
-            else request(Q - 2 * kSet, stage, left - 2);
-        });
-        stage = kStage - stage;
+        quarter(T0{}, fresh, next);
+        if constexpr (LOOK > 1) advance();
+        quarter(T1{}, Added{}, next);
+        if constexpr (LOOK == 1) advance();
+        quarter(T2{}, Added{}, next);
+        quarter(T3{}, Added{}, next);
+        stage = next;
         --left;
     };
+    if constexpr (HALVES == 1) {
 #pragma unroll 1
-    for (int tile = 0; tile < my_tiles; ++tile) {
+        for (int tile = 0; tile < my_tiles; ++tile) {
+            one_step(Fresh{});
+#pragma unroll 1
+            for (int step = 1; step < steps; ++step) one_step(Added{});
+            store(tile_of(tile));
+        }
+    } else {  // one tile
         one_step(Fresh{});
+        int step = 1;
+        if (half && (p.steps & 1)) one_step(Fresh{}), ++step;
 #pragma unroll 1
-        for (int step = 1; step < p.steps; ++step) one_step(Added{});
-        store(tile_of(tile));
+        for (; step < steps; ++step) one_step(Added{});
+        constexpr int kGiven = ROWS * CHANNELS / 2;
+        v4f(*const given)[WAVES][kGiven * 4][64] = reinterpret_cast<v4f(*)[WAVES][kGiven * 4][64]>(whole_lds);
+        Each<ROWS * CHANNELS>::run([&](auto at) {
+            constexpr int AT = decltype(at)::value;
+            const v16f& s = sum[AT / CHANNELS][AT % CHANNELS];
+            if (!kept(AT)) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) given[half][wave][AT % kGiven * 4 + q][lane] = v4f{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+            }
+        });
+        __syncthreads();
+        Each<ROWS * CHANNELS>::run([&](auto at) {
+            constexpr int AT = decltype(at)::value;
+            v16f& s = sum[AT / CHANNELS][AT % CHANNELS];
+            if (kept(AT)) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const v4f other = given[1 - half][wave][AT % kGiven * 4 + q][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[4 * q + e] += other[e];
+                }
+            }
+        });
+        store(tile_of(0));
     }
 }
 
-template <int ROWS, int CHANNELS, int DOWN, int ACROSS, bool WIDE, bool GROUPED, bool SWIGLU>
+template <int ROWS, int CHANNELS, int DOWN, int ACROSS, int LOOK, int HALVES, bool WIDE, bool GROUPED, bool SWIGLU>
 int launch_one(const Product& p, uint32_t blocks, hipStream_t s) {
-    constexpr uint32_t kLds = 2 * (32 * ROWS * DOWN + 32 * CHANNELS * ACROSS) * 136;
-    constexpr auto kernel = &mx_tiles_kernel<ROWS, CHANNELS, DOWN, ACROSS, WIDE, GROUPED, SWIGLU>;
+    constexpr uint32_t kLds = HALVES * 2 * (32 * ROWS * DOWN + 32 * CHANNELS * ACROSS) * 136;
+    constexpr auto kernel = &mx_tiles_kernel<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, WIDE, GROUPED, SWIGLU>;
     static DeviceOnce ready;
     const int code = ready.run([] { return hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds), "hipFuncSetAttribute"); });
     if (code != ORX_OK) return code;
-    ORX_LAUNCH(kernel, dim3(blocks), dim3(64 * DOWN * ACROSS), kLds, s, p);
+    ORX_LAUNCH(kernel, dim3(blocks), dim3(64 * DOWN * ACROSS * HALVES), kLds, s, p);
     return hip_check(hipGetLastError(), "launch mxfp4 tiles");
 }
-template <int ROWS, int CHANNELS, int DOWN, int ACROSS, bool WIDE>
+template <int ROWS, int CHANNELS, int DOWN, int ACROSS, int LOOK, int HALVES, bool WIDE>
 int launch_of_type(const Product& p, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s) {
-    if (grouped) return swiglu ? launch_one<ROWS, CHANNELS, DOWN, ACROSS, WIDE, true, true>(p, blocks, s) : launch_one<ROWS, CHANNELS, DOWN, ACROSS, WIDE, true, false>(p, blocks, s);
-    return swiglu ? launch_one<ROWS, CHANNELS, DOWN, ACROSS, WIDE, false, true>(p, blocks, s) : launch_one<ROWS, CHANNELS, DOWN, ACROSS, WIDE, false, false>(p, blocks, s);
+    if constexpr (HALVES == 1)
+        if (grouped) return swiglu ? launch_one<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, WIDE, true, true>(p, blocks, s) : launch_one<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, WIDE, true, false>(p, blocks, s);
+    return swiglu ? launch_one<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, WIDE, false, true>(p, blocks, s) : launch_one<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, WIDE, false, false>(p, blocks, s);
 }
-template <int ROWS, int CHANNELS, int DOWN, int ACROSS>
+template <int ROWS, int CHANNELS, int DOWN, int ACROSS, int LOOK, int HALVES>
 int launch(const Product& p, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s) {
-    return p.type == F32 ? launch_of_type<ROWS, CHANNELS, DOWN, ACROSS, true>(p, grouped, swiglu, blocks, s) : launch_of_type<ROWS, CHANNELS, DOWN, ACROSS, false>(p, grouped, swiglu, blocks, s);
+    return p.type == F32 ? launch_of_type<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, true>(p, grouped, swiglu, blocks, s) : launch_of_type<ROWS, CHANNELS, DOWN, ACROSS, LOOK, HALVES, false>(p, grouped, swiglu, blocks, s);
 }
 
 }  // namespace
 
-int launch_mx_tiles(const mx::Product& p, int rows, int channels, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s) {
-    if (rows == 256 && channels == 256) return launch<4, 2, 2, 4>(p, grouped, swiglu, blocks, s);
-    if (rows == 128 && channels == 128) return launch<2, 2, 2, 2>(p, grouped, swiglu, blocks, s);
-    return launch<1, 2, 2, 2>(p, grouped, swiglu, blocks, s);
+int launch_mx_tiles(const mx::Product& p, int rows, int channels, int halves, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s) {
+    if (rows == 256 && channels == 256) return launch<4, 2, 2, 4, 1, 1>(p, grouped, swiglu, blocks, s);
+    if (halves == 2) return rows == 128 ? launch<2, 2, 2, 2, 2, 2>(p, false, swiglu, blocks, s) : launch<1, 2, 2, 2, 1, 2>(p, false, swiglu, blocks, s);
+    if (rows == 128 && channels == 128) return launch<2, 2, 2, 2, 2, 1>(p, grouped, swiglu, blocks, s);
+    return launch<1, 2, 2, 2, 1, 1>(p, grouped, swiglu, blocks, s);
 }
 
 }  // namespace orx

@@ -11,6 +11,7 @@ import torch
 from oracle import mxfp4 as orc
 from orinfer_amd import lib, mxfp4, programs
 from tests.gpu_util import dev, host, kernel
+from tests.test_mxfp4 import TILES
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -178,6 +179,31 @@ def test_linear_with_fp32_output_at_an_odd_address(rows, n):
     want, bound = product(orc.values(*orc.quantise(x.double().numpy())), orc.values(codes, exponents))
     check(out[1:1 + rows * n].view(rows, n), want, bound, torch.float32)
     assert out[0] == -7 and (out[1 + rows * n:] == -7).all()
+
+
+@pytest.mark.parametrize("epilogue", ["none", "swiglu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,n,k", [shape for shape, _, _ in TILES])
+def test_tiles_of_every_kind(rows, n, k, dtype, epilogue):
+    """The last rows and channels of a tile, results at an odd address, nothing behind them."""
+    rng = np.random.default_rng(n)
+    codes, exponents = weights(rng, n, k)
+    x = rows_of(rng, rows, k, torch.float16)
+    q, s = (torch.empty(-(-rows // 16) * -(-k // 256) * size, dtype=torch.uint8, device=DEV) for size in (2048, 128))
+    kernel("mxfp4_quantization", K=k, layout="tiles")(Q=q, S=s, X=x.to(DEV), rows=rows)
+    w, ws = mxfp4.tiles(dev(codes), dev(exponents), paired=epilogue == "swiglu")
+    columns = n // 2 if epilogue == "swiglu" else n
+    out = torch.full((rows * columns + 9,), -7.0, dtype=dtype, device=DEV)
+    kernel("mxfp4_projection", M=rows, N=n, K=k, output_dtype=mxfp4.dtype_name(dtype), epilogue=epilogue)(A=q, AS=s, Out=out[1:], W=w, WS=ws)
+    a, b = orc.values(*orc.quantise(x.double().numpy())), orc.values(codes, exponents)
+    if epilogue == "none":
+        want, bound = product(a, b)
+    else:
+        (gate, dg), (up, du) = product(a, b[:columns]), product(a, b[columns:])
+        want = orc.silu(gate) * up
+        bound = 1.1 * dg * (np.abs(up) + du) + np.abs(gate) * du + 8 * 2.0**-24 * np.abs(want)
+    check(out[1:1 + rows * columns].view(rows, columns), want, bound, dtype)
+    assert out[0] == -7 and (out[1 + rows * columns:] == -7).all()
 
 
 @pytest.mark.parametrize("epilogue", ["none", "swiglu"])
