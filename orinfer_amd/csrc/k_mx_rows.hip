@@ -31,7 +31,6 @@ enum Source { Codes = 0, Halves = 1, Brains = 2 };  // of the rows: codes, fp16,
 template <int ROWS, int WAVES, int SOURCE, bool GROUPED, bool SWIGLU>
 __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
     constexpr int TILES = 2;
-    static_assert(SOURCE == Codes || ROWS == 1, "few rows are quantised here");
     extern __shared__ __align__(16) uint8_t lds[];  // sums; in front of them the rows' codes and powers where they are made here
     v4f(*const sums)[ROWS * TILES][64] = reinterpret_cast<v4f(*)[ROWS * TILES][64]>(lds);
     const int lane = threadIdx.x & 63;
@@ -72,8 +71,8 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
                 as[i] = p.as + row * (p.pitch / 16);
             } else {
                 const int64_t tile = min(first_row / 16 + i, (p.m - 1) / 16);
-                a[i] = p.a + tile * p.steps * kTileBytes + lane * 16;
-                as[i] = p.as + tile * p.steps * kTilePowers + ws_lane;
+                a[i] = p.a + tile * p.steps * kTileBytes;
+                as[i] = p.as + tile * p.steps * kTilePowers;
             }
         }
     }
@@ -86,15 +85,30 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
             s.w[t][1] = codes.load_16(w_lane + step * kTileBytes + 1024);
             s.wp[t] = powers.load_4(ws_lane + step * kTilePowers);
         }
-        if constexpr (SOURCE == Codes) {
-            const int there = min(step, p.steps - 1);  // (behind the last step the weights are 0)
-            constexpr int STEP = GROUPED ? 128 : kTileBytes, SECOND = GROUPED ? 64 : 1024;
+        if constexpr (SOURCE == Codes && GROUPED) {
+            const int there = min(step, p.steps - 1);  // (a wave without a step)
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-                s.a[i][0] = *reinterpret_cast<const v4i*>(a[i] + there * STEP);
-                s.a[i][1] = *reinterpret_cast<const v4i*>(a[i] + there * STEP + SECOND);
-                if constexpr (GROUPED) s.ap[i] = *reinterpret_cast<const uint2*>(as[i] + there * 8);
-                else s.ap[i].x = *reinterpret_cast<const uint32_t*>(as[i] + there * kTilePowers);
+                s.a[i][0] = *reinterpret_cast<const v4i*>(a[i] + there * 128);
+                s.a[i][1] = *reinterpret_cast<const v4i*>(a[i] + there * 128 + 64);
+                s.ap[i] = *reinterpret_cast<const uint2*>(as[i] + there * 8);
+            }
+        } else if constexpr (SOURCE == Codes) {
+            // The compiler makes one plain load of the first step's and the next one's, behind the wait for the weights.  Loads from buffers stay with the weights', and up to 32 rows that is
+            // faster (us with buffers / without, 32 rows: 17408 x 5120 14.9 / 15.5, 9728 x 2560 6.6 / 6.7, 1056 x 2080 3.6 / 4.0), with 64 it is not (200 rows of 5120 x 17408 44.4 / 38.9).
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                if constexpr (ROWS <= 2) {
+                    const Buffer codes(a[i], p.steps * kTileBytes), powers(as[i], p.steps * kTilePowers);
+                    s.a[i][0] = codes.load_16(w_lane + step * kTileBytes);
+                    s.a[i][1] = codes.load_16(w_lane + step * kTileBytes + 1024);
+                    s.ap[i].x = (uint32_t)powers.load_4(ws_lane + step * kTilePowers);
+                } else {
+                    const int there = min(step, p.steps - 1);
+                    s.a[i][0] = *reinterpret_cast<const v4i*>(a[i] + w_lane + there * kTileBytes);
+                    s.a[i][1] = *reinterpret_cast<const v4i*>(a[i] + w_lane + there * kTileBytes + 1024);
+                    s.ap[i].x = *reinterpret_cast<const uint32_t*>(as[i] + ws_lane + there * kTilePowers);
+                }
             }
         }
     };
@@ -153,7 +167,7 @@ __global__ __launch_bounds__(WAVES * 64) void mx_rows_kernel(Product p) {
 #pragma unroll 1
     for (int step = wave; step < p.steps; step += WAVES) {
         multiply(held, step);
-        load(held, step + WAVES);
+        if (step + WAVES < p.steps) load(held, step + WAVES);  // (what lies behind the end would still be waited for: 7168 x 5120, 32 rows 7.5 us, else 9.2)
     }
     if constexpr (SOURCE != Codes) __syncthreads();  // (the sums take the codes' place)
 #pragma unroll
@@ -191,24 +205,17 @@ enum { kSwiglu = 1, kGather = 2 };
 struct Plan {
     int rows, channels, waves, halves = 1;
 };
-// Eight waves where every CU has a workgroup or less, or two and K is long enough or the rows many enough for eight, else four.  Us with four / eight, weights out of cache: 32 rows to a
-// unit, 7168 x 5120, 448 workgroups 12.0 / 10.0; 4096 x 4096, 384, 7.4 / 6.8, 1024, 10.7 / 11.2; 17408 x 5120, 1088, 19.4 / 19.9; 9728 x 2560, 304, 5.6 / 5.9, 608, 8.0 / 8.2; 64 rows, 9728 x 2560, 304,
-// 10.0 / 8.9, 608, 10.7 / 12.3; 4096 x 4096, 512, 10.9 / 9.2, 768, 12.5 / 14.4; 5120 x 17408, 160, 44 / 25.  Rows that the workgroups quantise want eight (17408 x 5120, 4 rows 14.8 / 13.5,
-// 1 row 11.4 / 11.1).
-Plan few_rows(const orx_function& f, int unit_rows, int64_t workgroups) {
-    const int64_t cus = device_compute_units();
-    const bool eight = workgroups <= cus || (workgroups <= 2 * cus && (unit_rows == 64 || f.K > 10 * kStepK));
-    return {unit_rows, 0, f.packed_k == Codes && !eight ? 4 : 8};
-}
-// Us that a launch takes, weights out of cache, 256 CUs (within a fifth of what was measured at 40-700 rows of 7168 x 5120, 4096 x 4096, 1024 x 4096, 17408 x 5120, 5120 x 17408, 2048 x 1024,
+// Eight waves share K, four with 64 rows (us with four / eight, weights out of cache: 16 rows, 7168 x 5120 7.1 / 6.4, 17408 x 5120 13.4 / 13.0, 9728 x 2560 level; 32 rows, 7168 x 5120 7.9 / 7.5,
+// 17408 x 5120 16.0 / 15.4, 2048 x 1024 3.4 / 3.1; 64 rows to a unit, 160 of 7168 x 5120 14.3 / 16.5, 333 of 4096 x 4096 11.4 / 13.7, 64 of 1024 x 4096 level).
+Plan few_rows(int unit_rows) { return {unit_rows, 0, unit_rows == 64 ? 4 : 8}; }
+// Us that a launch takes, weights out of cache, 256 CUs (within a fifth of what was measured at 32-700 rows of 7168 x 5120, 4096 x 4096, 1024 x 4096, 17408 x 5120, 5120 x 17408, 2048 x 1024,
 // 1056 x 2080, 9728 x 2560).  The kernel above: a chain of steps for each wave, or what all workgroups read through the L2s.  Tiles: a chain of steps, longer where a CU has several
-// workgroups side by side or one after another.  So few rows of few channels go to the former (128 rows of 4096 x 4096: 7.1, tiles 12.4 and 14.1), 32 to a unit first (64 rows: 5.9, as one unit 7.0), tiles where there are
-// enough for all CUs, in halves of K where there are not (333 rows of 7168 x 5120: 20.4, else 23.1; 333 rows of 5120 x 17408 45, else 57).
-double few_rows_us(const orx_function& f, int rows, int unit_rows) {
-    const double steps = (f.K + kStepK - 1) / kStepK, workgroups = (double)ceil_div(rows, unit_rows) * ((f.slots + 1) / 2);
-    const double chain = std::ceil(steps / 8) * (unit_rows == 32 ? 1.7 : 2.4);
-    const double bytes = workgroups * (unit_rows + 32) * steps * 136, rate = unit_rows == 32 ? 13.5e6 : 13e6;
-    return 2.5 + std::max(chain, bytes / rate * (256.0 / device_compute_units()));
+// workgroups side by side or one after another.  So few rows of few channels go to the former (128 rows of 4096 x 4096: 6.8, tiles 12.1 and 14.0), 32 to a unit first (64 rows: 5.3, as one
+// unit 6.7), tiles where there are enough for all CUs, in halves of K where there are not (333 rows of 7168 x 5120: 20.1, else 23.1; 333 rows of 5120 x 17408 45, else 57).
+double few_rows_us(const orx_function& f, int rows, const Plan& plan) {
+    const double steps = (f.K + kStepK - 1) / kStepK, workgroups = (double)ceil_div(rows, plan.rows) * ((f.slots + 1) / 2);
+    const double chain = std::ceil(steps / plan.waves) * (plan.rows == 64 ? 1.2 : 1.5);
+    return 2.5 + std::max(chain, workgroups * (plan.rows + 32) * steps * 136 / 15.2e6 * (256.0 / device_compute_units()));
 }
 double tiles_us(const orx_function& f, int rows, const Plan& tile) {
     const int64_t cus = device_compute_units(), tiles = (int64_t)ceil_div(rows, tile.rows) * ceil_div(f.slots, tile.channels / 16);
@@ -218,19 +225,18 @@ double tiles_us(const orx_function& f, int rows, const Plan& tile) {
     return 2.5 + steps * (tile.rows == 256 ? 1.8 * to_a_cu : to_a_cu == 1 ? 1.0 : 1.27 * std::ceil(to_a_cu / 2));
 }
 Plan plan(const orx_function& f, int rows) {
-    const int pairs = (f.slots + 1) / 2;
     if (f.E > 0) {
-        if (f.block_m == 16) return few_rows(f, 16, (int64_t)pairs * std::min(f.tiles, f.E));
+        // (of few steps: 128 experts x 8, 16 tokens, 512 deep, us with four / eight waves 10.4 / 13.5, 2048 deep 12.5 / 12.9)
+        if (f.block_m == 16) return {16, 0, f.packed_k == Codes ? 4 : 8};
         return {f.block_m, f.block_m == 256 ? 256 : 128, 0};
     }
-    if (rows <= 16) return few_rows(f, 16, pairs);
-    Plan best = few_rows(f, 32, (int64_t)ceil_div(rows, 32) * pairs);
-    if (rows <= 32) return best;
-    double best_us = few_rows_us(f, rows, 32);
+    if (rows <= 32) return few_rows(rows <= 16 ? 16 : 32);
+    Plan best = few_rows(32);
+    double best_us = few_rows_us(f, rows, best);
     auto weigh = [&](const Plan& other, double us) {
         if (us < best_us) best = other, best_us = us;
     };
-    weigh(few_rows(f, 64, (int64_t)ceil_div(rows, 64) * pairs), few_rows_us(f, rows, 64));
+    weigh(few_rows(64), few_rows_us(f, rows, few_rows(64)));
     if (rows > 64)
         for (const Plan& tile : {Plan{64, 128, 0, 1}, Plan{64, 128, 0, 2}, Plan{128, 128, 0, 1}, Plan{128, 128, 0, 2}, Plan{256, 256, 0, 1}}) weigh(tile, tiles_us(f, rows, tile));
     return best;
@@ -273,21 +279,18 @@ int launch_one(const Product& p, const Geometry& g, hipStream_t s) {
 template <int ROWS, int WAVES, int SOURCE>
 int launch_of(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
     const bool swiglu = f.flags & kSwiglu;
-    if constexpr (ROWS == 1 && SOURCE != Brains)
+    if constexpr (SOURCE == Halves)
         if (f.E > 0) return swiglu ? launch_one<ROWS, WAVES, SOURCE, true, true>(p, g, s) : launch_one<ROWS, WAVES, SOURCE, true, false>(p, g, s);
     return swiglu ? launch_one<ROWS, WAVES, SOURCE, false, true>(p, g, s) : launch_one<ROWS, WAVES, SOURCE, false, false>(p, g, s);
-}
-template <int WAVES>
-int launch_codes(const orx_function& f, const Plan& plan, const Product& p, const Geometry& g, hipStream_t s) {
-    if (plan.rows == 16) return launch_of<1, WAVES, Codes>(f, p, g, s);
-    return plan.rows == 32 ? launch_of<2, WAVES, Codes>(f, p, g, s) : launch_of<4, WAVES, Codes>(f, p, g, s);
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
     if (plan.channels) return launch_mx_tiles(p, plan.rows, plan.channels, plan.halves, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
     if (f.packed_k == Halves) return launch_of<1, 8, Halves>(f, p, g, s);
     if (f.packed_k == Brains) return launch_of<1, 8, Brains>(f, p, g, s);
-    return plan.waves == 4 ? launch_codes<4>(f, plan, p, g, s) : launch_codes<8>(f, plan, p, g, s);
+    if (f.E > 0) return f.flags & kSwiglu ? launch_one<1, 4, Codes, true, true>(p, g, s) : launch_one<1, 4, Codes, true, false>(p, g, s);
+    if (plan.rows == 16) return launch_of<1, 8, Codes>(f, p, g, s);
+    return plan.rows == 32 ? launch_of<2, 8, Codes>(f, p, g, s) : launch_of<4, 4, Codes>(f, p, g, s);
 }
 
 Product product_of(const orx_function& f, int rows) {

@@ -711,14 +711,11 @@ def _check_rows(x, rows, columns, dtype, device, what):
 class _OnDevice:
     """Launches on the device of the weights, whichever is current; its current stream unless the caller names one."""
 
-    def _call(self, body, *args, stream=None, **named):
+    def _call(self, body, *args, stream=None):
         if torch._C._cuda_getDevice() == self.device.index:
-            return body(*args, stream=current_stream() if stream is None else stream, **named)
+            return body(*args, stream=current_stream() if stream is None else stream)
         with torch.cuda.device(self.device):
-            return body(*args, stream=current_stream() if stream is None else stream, **named)
-
-
-MX_FEW_ROWS = 4  # rows that an MXFP4 projection quantises itself
+            return body(*args, stream=current_stream() if stream is None else stream)
 
 
 def _where_it_fits(symbol, **keys):
@@ -734,7 +731,7 @@ def _where_it_fits(symbol, **keys):
 class Mxfp4Linear(_OnDevice):
     """Rows of 16-bit values, quantised to MXFP4, times MXFP4 weights: codes (N, K / 2) and exponents (N, K / 32), both uint8 (the format: mxfp4.py), up to `capacity`
     rows at a time.  epilogue="swiglu": the upper half of the channels are the up channels of the gate channels in the lower half, and silu(gate) * up comes out.
-    `run` returns a view of the object's own output buffer, which the next call overwrites; one object serves one stream at a time."""
+    `run` returns the object's own output buffer, or a view of its first rows, which the next call overwrites; one object serves one stream at a time."""
 
     def __init__(self, codes, exponents, capacity, *, dtype=torch.float16, epilogue="none"):
         if dtype not in (torch.float16, torch.bfloat16):
@@ -752,9 +749,11 @@ class Mxfp4Linear(_OnDevice):
         with torch.cuda.device(self.device):
             self.projection = Kernel("mxfp4_projection", M=capacity, **shape)
             self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, layout="tiles")
-            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (weights out of cache, us of the projection alone without / with it,
-            # and a quantiser is 2.8: 17408 x 5120 1 row 10.6 / 11.1, 4 rows 11.5 / 13.5, 8 rows 12 / 17; 9728 x 2560 4.4 / 4.6, 4.5 / 5.9, 4.6 / 7.4).  Not where their codes do not fit LDS.
-            self.few = _where_it_fits("mxfp4_projection", M=min(capacity, MX_FEW_ROWS), input_dtype=name, **shape)
+            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (weights out of cache, us of the two launches / of the one:
+            # 17408 x 5120, 1 row 16.3 / 12.4, 4 rows 16.0 / 14.9, 6 rows 16.5 / 16.7, 8 rows 16.4 / 18.5; 9728 x 2560, 1 row 9.4 / 5.9, 8 rows 9.4 / 8.5; 4096 x 4096 7.4 / 4.4, 7.6 / 6.9).
+            # Not where their codes do not fit LDS.
+            self.few_rows = min(capacity, 8 if channels <= 10240 else 6)
+            self.few = _where_it_fits("mxfp4_projection", M=self.few_rows, input_dtype=name, **shape)
         self.n = channels // 2 if epilogue == "swiglu" else channels
         # the quantised rows, by tiles of 16
         tiles = -(-capacity // 16) * -(-self.k // mxfp4.STEP)
@@ -769,10 +768,10 @@ class Mxfp4Linear(_OnDevice):
             raise ValueError(f"{rows} rows are more than the capacity of {self.capacity}")
         if rows:
             self._call(self._run, x, rows, stream=stream)
-        return self.out.as_strided((rows, self.n), (self.n, 1))
+        return self.out if rows == self.capacity else self.out.as_strided((rows, self.n), (self.n, 1))
 
     def _run(self, x, rows, stream):
-        if rows <= MX_FEW_ROWS and self.few is not None:
+        if rows <= self.few_rows and self.few is not None:
             self.few(stream=stream, A=x, Out=self.out, W=self.weight, WS=self.powers, m=rows)
             return
         self.quantizer(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=rows)
@@ -802,7 +801,7 @@ class Mxfp4MoeLayer(_OnDevice):
                 raise ValueError(f"bias must have {experts} values")
         routes = self.assignments = tokens * top_k
         if block_m is None:
-            block_m = 16 if routes <= 10 * experts else 64 if routes < 256 * experts else 128 if routes < 512 * experts else 256
+            block_m = 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
         self.block_m = block_m
         capacity = -(-routes // block_m) + min(experts, routes)
         common = dict(M=tokens, E=experts, top_k=top_k)
@@ -818,11 +817,10 @@ class Mxfp4MoeLayer(_OnDevice):
             self.k_quantise_act = Kernel("mxfp4_quantization", K=intermediate, pad=mxfp4.STEP)
             down = dict(N=hidden, K=intermediate, **grouped)
             self.k_down = Kernel("mxfp4_grouped", **down)
-            # A route to an expert or less: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
-            # 9.1 / 6.5 and down 6.3 / 4.6, 16 tokens 12.6 / 11.3 and 10.7 / 10.5, 32 tokens 14.6 / 14.1 and 11.6 / 13.1, 64 tokens 17.6 / 19.3 and 13.9 / 17.4).
-            self.few_up = self.few_down = None
-            if block_m == 16 and routes <= experts:
-                self.few_up, self.few_down = (_where_it_fits("mxfp4_grouped", input_dtype="float16", **keys) for keys in (up, down))
+            # A route to an expert or less, two for gate and up: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of
+            # 2048 x 512, 3 tokens, up 9.3 / 6.0 and down 5.9 / 4.3, 16 tokens 12.6 / 10.9 and 10.9 / 10.3, 32 tokens 14.5 / 13.3 and 11.5 / 12.5, 64 tokens 17.3 / 17.9 and 13.6 / 16.4).
+            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if block_m == 16 and routes <= 2 * experts else None
+            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if block_m == 16 and routes <= experts else None
             self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, **common)
             self.segments = self.k_metadata.workspace()
         i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)

@@ -133,18 +133,18 @@ def test_records_name_the_kernel_that_runs():
 
 
 # a shape for every kind of tile: 64 x 128 as a whole and in halves of an odd number of steps, 128 x 128 likewise and of an even number, 256 x 256
-TILES = [((160, 17400, 512), 256, 52224), ((400, 4090, 1056), 512, 104448), ((256, 17402, 512), 256, 69632), ((700, 4096, 3232), 512, 139264), ((680, 4002, 1536), 512, 139264),
+TILES = [((160, 17400, 512), 256, 52224), ((440, 4090, 2080), 512, 104448), ((256, 17402, 512), 256, 69632), ((700, 4096, 3232), 512, 139264), ((680, 4002, 1536), 512, 139264),
          ((2049, 4098, 512), 512, 139264)]
 
 
 def test_a_projection_takes_larger_tiles_where_there_are_more():
     """Threads and LDS of the kernel by rows (without a device 256 CUs are taken)."""
     linear = lib.Kernel("mxfp4_projection", M=8192, N=4096, K=4096, dynamic_rows=True)
-    assert [started(linear, rows)[0][1:] for rows in (64, 100, 512, 2048, 8192)] == [(512, 32768), (512, 65536), (512, 104448), (256, 69632), (512, 139264)]
+    assert [started(linear, rows)[0][1:] for rows in (32, 64, 300, 512, 2048, 8192)] == [(512, 32768), (512, 32768), (256, 32768), (512, 104448), (256, 69632), (512, 139264)]
     assert all(len(started(linear, rows)) == 1 for rows in (1, 64, 65, 8192))
     for (rows, n, k), threads, lds in TILES:
         assert started(lib.Kernel("mxfp4_projection", M=rows, N=n, K=k), 0)[0][1:] == (threads, lds), (rows, n, k)
-    for block_m, lds in ((16, 16384), (64, 52224), (128, 69632), (256, 139264)):
+    for block_m, lds in ((16, 8192), (64, 52224), (128, 69632), (256, 139264)):
         assert started(lib.Kernel("mxfp4_grouped", **GROUPED, block_m=block_m))[0][2] == lds
 
 
