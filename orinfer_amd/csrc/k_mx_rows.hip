@@ -211,10 +211,11 @@ Plan few_rows(int unit_rows) { return {unit_rows, 0, unit_rows == 64 ? 4 : 8}; }
 // Us that a launch takes, weights out of cache, 256 CUs (within a fifth of what was measured at 32-700 rows of 7168 x 5120, 4096 x 4096, 1024 x 4096, 17408 x 5120, 5120 x 17408, 2048 x 1024,
 // 1056 x 2080, 9728 x 2560).  The kernel above: a chain of steps for each wave, or what all workgroups read through the L2s.  Tiles: a chain of steps, longer where a CU has several
 // workgroups side by side or one after another.  So few rows of few channels go to the former (128 rows of 4096 x 4096: 6.8, tiles 12.1 and 14.0), 32 to a unit first (64 rows: 5.3, as one
-// unit 6.7), tiles where there are enough for all CUs, in halves of K where there are not (333 rows of 7168 x 5120: 20.1, else 23.1; 333 rows of 5120 x 17408 45, else 57).
+// unit 6.7), tiles where there are enough for all CUs, in halves of K where there are not (333 rows of 7168 x 5120: 20.1, else 23.1; 333 rows of 5120 x 17408 45, else 57).  64 rows x 64
+// channels to a workgroup of the former were within a tenth of the better of the others.
 double few_rows_us(const orx_function& f, int rows, const Plan& plan) {
     const double steps = (f.K + kStepK - 1) / kStepK, workgroups = (double)ceil_div(rows, plan.rows) * ((f.slots + 1) / 2);
-    const double chain = std::ceil(steps / plan.waves) * (plan.rows == 64 ? 1.2 : 1.5);
+    const double chain = std::ceil(steps / plan.waves) * (plan.rows == 64 ? 1.2 : 1.1);
     return 2.5 + std::max(chain, workgroups * (plan.rows + 32) * steps * 136 / 15.2e6 * (256.0 / device_compute_units()));
 }
 double tiles_us(const orx_function& f, int rows, const Plan& tile) {
@@ -251,7 +252,7 @@ int geometry(const orx_function& f, int rows, Geometry* g) {
     const Plan plan = orx::plan(f, rows);
     const int64_t units = f.E > 0 ? f.tiles : ceil_div(rows, plan.rows);
     int64_t blocks = units * ceil_div(f.slots, plan.channels ? plan.channels / 16 : 2);
-    if (blocks >= (1ll << 32) / 256) {
+    if (blocks >= (1ll << 32) / 512) {
         set_error("%s: %d rows of %d channels are more than one launch takes", f.symbol.c_str(), rows, f.N);
         return ORX_ERR_ROWS;
     }
