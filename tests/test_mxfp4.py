@@ -132,9 +132,9 @@ def test_records_name_the_kernel_that_runs():
             assert reported(kernel, r) in started(kernel, r)
 
 
-# a shape for every kind of tile: 64 x 128 as a whole and in halves of an odd number of steps, 128 x 128 likewise and of an even number, 256 x 256
+# a shape for every kind of tile: 64 x 128 as a whole and in halves of an odd number of steps, 128 x 128 likewise and of an even number, 256 x 256, halves of a step each
 TILES = [((160, 17400, 512), 256, 52224), ((440, 4090, 2080), 512, 104448), ((256, 17402, 512), 256, 69632), ((700, 4096, 3232), 512, 139264), ((680, 4002, 1536), 512, 139264),
-         ((2049, 4098, 512), 512, 139264)]
+         ((2049, 4098, 512), 512, 139264), ((200, 8100, 512), 512, 104448)]
 
 
 def test_a_projection_takes_larger_tiles_where_there_are_more():
