@@ -496,10 +496,11 @@ __device__ __forceinline__ void place_experts(PlaceLds& lds, const SegmentOutput
                                               int total_segments) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid < experts) lds.in_front[tid] = before;
-    const int tiles = (count + block_m - 1) / block_m;
+    const int shift = 31 - __builtin_clz(block_m);  // (a power of two)
+    const int tiles = (count + block_m - 1) >> shift;
     // Units: the tiles in the order of their size, so that what starts last is short: above half a tile's rows, above a quarter, the rest
     // (an expert's last tile is the only one that is not full; tiles of the two small sizes are counted in the halves of a word)
-    const int full = count / block_m, rest = count % block_m;
+    const int full = count >> shift, rest = count & (block_m - 1);
     const int size = 2 * rest > block_m ? 0 : 4 * rest > block_m ? 1 : 2;  // of the last tile
     const int large = full + (rest > 0 && size == 0), small = rest > 0 && size > 0 ? 1 << (16 * (size - 1)) : 0;
     const int row_scan = wave_prefix_sum(count), tile_scan = wave_prefix_sum(tiles), large_scan = wave_prefix_sum(large), small_scan = wave_prefix_sum(small);
