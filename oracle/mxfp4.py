@@ -1,4 +1,4 @@
-"""MXFP4 and the router by scores in 64 bits (numpy): the checker of the kernels, test infrastructure only."""
+"""MXFP4 and the router by scores in 64 bits (numpy): the oracle of the kernels, test infrastructure only."""
 import numpy as np
 
 MAGNITUDES = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])

@@ -12,7 +12,11 @@
 namespace orx {
 namespace {
 
-constexpr int kThreads = 256, kPieces = 4;  // eight-value pieces to a thread
+constexpr int kThreads = 256;
+// Eight-value pieces to a thread, all of whose loads are on their way together: four, one where there are few (us with four / one: 3 rows of 2048 3.1 / 2.4, 2048 of 512 5.0 / 3.0,
+// 4096 of 2048 6.8 / 6.5, 32768 of 512 level, 8192 of 5120 19.9 / 21.9).
+constexpr int kPieces = 4;
+constexpr int64_t kFewPieces = 1 << 21;
 
 // Rows of `pieces` eight-value pieces, one behind the other in one sequence of fewer than 2^32.
 struct Rows {
@@ -70,13 +74,13 @@ __device__ __forceinline__ void read_eight(uint32_t (&words)[WORDS], const void*
 }
 
 // WHOLE: rows of whole blocks without a gap on either side, so that a piece's number is its place and no row is looked for.
-template <int TYPE, bool WHOLE>
+template <int TYPE, bool WHOLE, int PIECES>
 __global__ __launch_bounds__(kThreads) void mx_quantise_kernel(QuantParams p) {
     constexpr int WORDS = TYPE == mx::F32 ? 8 : 4;
-    const uint32_t base = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
-    uint32_t words[kPieces][WORDS], to[kPieces];
+    const uint32_t base = blockIdx.x * (kThreads * PIECES) + threadIdx.x;
+    uint32_t words[PIECES][WORDS], to[PIECES];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
         const uint32_t at = base + i * kThreads;
         const bool live = at < p.rows.total;
         int count = live ? 8 : 0;
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void mx_quantise_kernel(QuantParams p) {
         read_eight<TYPE>(words[i], p.x, offset, count);
     }
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
         // (a row is whole blocks, so the lanes of a quad are pieces of one block, or all behind the end)
         const uint32_t byte = mx::power_byte<TYPE>(mx::quad_max(largest_of<TYPE>(words[i])), p.ceil != 0);
         if (base + i * kThreads >= p.rows.total) continue;
@@ -101,27 +105,28 @@ __global__ __launch_bounds__(kThreads) void mx_quantise_kernel(QuantParams p) {
     }
 }
 
-// The same by tiles of 16 rows x 256 (the layout of the products): a wave takes 16 rows x 128, four rows of 256 bytes to a load, and its stores are runs of 64 bytes.  Rows
+// The same by tiles of 16 rows x 256 (the layout of the products): a wave takes 4 LOADS rows x 128, four rows of 256 bytes to a load, and its stores are runs of 64 bytes.  Rows
 // of the last tile that are not there become 0.
-template <int TYPE>
+template <int TYPE, int LOADS>
 __global__ __launch_bounds__(kThreads) void mx_quantise_tiles_kernel(QuantParams p, int rows, int steps, int groups) {
+    constexpr int PARTS = 4 / LOADS;  // of a tile
     constexpr int WORDS = TYPE == mx::F32 ? 8 : 4;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int tile = blockIdx.x / groups, window = (int)(blockIdx.x % groups) * (kThreads / 64) + wave;  // of 128 columns
+    const int at_tile = blockIdx.x / groups, tile = at_tile / PARTS, first = at_tile % PARTS * (4 * LOADS), window = (int)(blockIdx.x % groups) * (kThreads / 64) + wave;  // of 128 columns
     if (window >= 2 * steps) return;
     const int column = window * 128 + (lane & 15) * 8;
-    uint32_t words[4][WORDS];
+    uint32_t words[LOADS][WORDS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = (int64_t)tile * 16 + 4 * i + (lane >> 4);
+    for (int i = 0; i < LOADS; ++i) {
+        const int64_t row = (int64_t)tile * 16 + first + 4 * i + (lane >> 4);
         read_eight<TYPE>(words[i], p.x, row * p.rows.k + column, row < rows ? p.rows.k - column : 0);
     }
     const int64_t at = (int64_t)tile * steps + (window >> 1);
     const int block = (window & 1) * 4 + ((lane & 15) >> 2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 4 * i + (lane >> 4);
+    for (int i = 0; i < LOADS; ++i) {
+        const int r = first + 4 * i + (lane >> 4);
         const uint32_t byte = mx::power_byte<TYPE>(mx::quad_max(largest_of<TYPE>(words[i])), p.ceil != 0);
         *reinterpret_cast<uint32_t*>(p.q + at * mx::kTileBytes + block * 256 + r * 16 + (lane & 3) * 4) = mx::eight_codes<TYPE>(words[i], byte);
         if ((lane & 3) == 0) p.s[at * mx::kTilePowers + r * 8 + (block & 1) * 4 + (block >> 1)] = (uint8_t)byte;
@@ -135,11 +140,11 @@ struct DequantParams {
     int type;
 };
 
-template <bool WHOLE>
+template <bool WHOLE, int PIECES>
 __global__ __launch_bounds__(kThreads) void mx_dequantise_kernel(DequantParams p) {
-    const uint32_t base = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
+    const uint32_t base = blockIdx.x * (kThreads * PIECES) + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
         const uint32_t at = base + i * kThreads;
         if (at >= p.rows.total) return;
         uint32_t from = at;
@@ -174,17 +179,30 @@ __global__ __launch_bounds__(kThreads) void mx_dequantise_kernel(DequantParams p
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
 // slots used: K, group (K in whole blocks, or in steps of 256 for the products), stride (from one stored row to the next), algorithm (type), flags (ceil), flags2 (tiles)
+bool few_pieces(const orx_function& f, int rows) { return (int64_t)rows * (f.group / 8) <= kFewPieces; }
 int geometry(const orx_function& f, int rows, Geometry* g) {
-    g->grid[0] = f.flags2 ? ceil_div(rows, 16) * ceil_div(f.group / 128, kThreads / 64) : (uint32_t)(((int64_t)rows * (f.group / 8) + kThreads * kPieces - 1) / (kThreads * kPieces));
+    const bool few = few_pieces(f, rows);
+    const int64_t pieces = (int64_t)rows * (f.group / 8), to_a_block = kThreads * (few ? 1 : kPieces);
+    g->grid[0] = f.flags2 ? ceil_div(rows, 16) * (few ? 4 : 1) * ceil_div(f.group / 128, kThreads / 64) : (uint32_t)((pieces + to_a_block - 1) / to_a_block);
     g->block[0] = kThreads;
     return ORX_OK;
 }
-template <int TYPE>
+template <int TYPE, int PIECES>
 void quantise(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const QuantParams& p) {
     const dim3 grid(g.grid[0]), block(kThreads);
-    if (f.flags2) ORX_LAUNCH(mx_quantise_tiles_kernel<TYPE>, grid, block, 0, s, p, rows, f.group / mx::kStepK, (int)ceil_div(f.group / 128, kThreads / 64));
-    else if (f.K == f.stride) ORX_LAUNCH((mx_quantise_kernel<TYPE, true>), grid, block, 0, s, p);
-    else ORX_LAUNCH((mx_quantise_kernel<TYPE, false>), grid, block, 0, s, p);
+    if (f.flags2) ORX_LAUNCH((mx_quantise_tiles_kernel<TYPE, PIECES>), grid, block, 0, s, p, rows, f.group / mx::kStepK, (int)ceil_div(f.group / 128, kThreads / 64));
+    else if (f.K == f.stride) ORX_LAUNCH((mx_quantise_kernel<TYPE, true, PIECES>), grid, block, 0, s, p);
+    else ORX_LAUNCH((mx_quantise_kernel<TYPE, false, PIECES>), grid, block, 0, s, p);
+}
+template <int TYPE>
+void quantise(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const QuantParams& p) {
+    if (few_pieces(f, rows)) quantise<TYPE, 1>(f, rows, g, s, p);
+    else quantise<TYPE, kPieces>(f, rows, g, s, p);
+}
+template <int PIECES>
+void dequantise(const orx_function& f, const Geometry& g, hipStream_t s, const DequantParams& p) {
+    if (f.K == f.stride) ORX_LAUNCH((mx_dequantise_kernel<true, PIECES>), dim3(g.grid[0]), dim3(kThreads), 0, s, p);
+    else ORX_LAUNCH((mx_dequantise_kernel<false, PIECES>), dim3(g.grid[0]), dim3(kThreads), 0, s, p);
 }
 // Q, S, X, rows
 int quantise_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
@@ -201,8 +219,8 @@ int dequantise_launch(const orx_function& f, int rows, const Geometry& g, hipStr
     DequantParams p;
     p.q = pointer_arg<const uint8_t>(args, 0), p.s = pointer_arg<const uint8_t>(args, 1), p.y = pointer_arg<void>(args, 2);
     p.rows = rows_of(rows, f.group / 8, f.stride / 8, f.K), p.type = f.algorithm;
-    if (f.K == f.stride) ORX_LAUNCH(mx_dequantise_kernel<true>, dim3(g.grid[0]), dim3(kThreads), 0, s, p);
-    else ORX_LAUNCH(mx_dequantise_kernel<false>, dim3(g.grid[0]), dim3(kThreads), 0, s, p);
+    if (few_pieces(f, rows)) dequantise<1>(f, g, s, p);
+    else dequantise<kPieces>(f, g, s, p);
     return hip_check(hipGetLastError(), "launch mxfp4_dequantization");
 }
 
@@ -253,9 +271,9 @@ int make_quantise(const Variant& v, orx_function* f) {
     f->launch = quantise_launch;
     const bool whole = f->K == f->stride;
 #define ORX_QUANTISE(TYPE)                                                                            \
-    (f->flags2 ? reinterpret_cast<const void*>(&mx_quantise_tiles_kernel<TYPE>)                       \
-     : whole   ? reinterpret_cast<const void*>(&mx_quantise_kernel<TYPE, true>)                       \
-               : reinterpret_cast<const void*>(&mx_quantise_kernel<TYPE, false>))
+    (f->flags2 ? reinterpret_cast<const void*>(&mx_quantise_tiles_kernel<TYPE, kPieces>)                       \
+     : whole   ? reinterpret_cast<const void*>(&mx_quantise_kernel<TYPE, true, kPieces>)                       \
+               : reinterpret_cast<const void*>(&mx_quantise_kernel<TYPE, false, kPieces>))
     f->device_function = f->algorithm == mx::F16 ? ORX_QUANTISE(mx::F16) : f->algorithm == mx::BF16 ? ORX_QUANTISE(mx::BF16) : ORX_QUANTISE(mx::F32);
 #undef ORX_QUANTISE
     return ORX_OK;
@@ -265,7 +283,7 @@ int make_dequantise(const Variant& v, orx_function* f) {
     if (code != ORX_OK) return code;
     f->args = {{"Q", ArgPointer, 4}, {"S", ArgPointer, 1}, {"Y", ArgPointer, f->algorithm == mx::F32 ? 4u : 2u}, {"rows", ArgI32, 4}};
     f->launch = dequantise_launch;
-    f->device_function = f->K == f->stride ? reinterpret_cast<const void*>(&mx_dequantise_kernel<true>) : reinterpret_cast<const void*>(&mx_dequantise_kernel<false>);
+    f->device_function = f->K == f->stride ? reinterpret_cast<const void*>(&mx_dequantise_kernel<true, kPieces>) : reinterpret_cast<const void*>(&mx_dequantise_kernel<false, kPieces>);
     return ORX_OK;
 }
 
