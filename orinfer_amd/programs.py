@@ -750,9 +750,9 @@ class Mxfp4Linear(_OnDevice):
             self.projection = Kernel("mxfp4_projection", M=capacity, **shape)
             self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, layout="tiles")
             # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (weights out of cache, us of the two launches / of the one:
-            # 17408 x 5120, 1 row 16.3 / 12.4, 4 rows 16.0 / 14.9, 6 rows 16.5 / 16.7, 8 rows 16.4 / 18.5; 9728 x 2560, 1 row 9.4 / 5.9, 8 rows 9.4 / 8.5; 4096 x 4096 7.4 / 4.4, 7.6 / 6.9).
+            # 17408 x 5120, 1 row 15.1 / 12.3, 4 rows 15.0 / 15.0, 6 rows 15.2 / 16.7; 9728 x 2560, 1 row 8.3 / 5.8, 6 rows 8.2 / 7.8, 8 rows 8.2 / 8.5; 4096 x 4096 6.3 / 4.4, 6.4 / 6.2, 6.3 / 6.9).
             # Not where their codes do not fit LDS.
-            self.few_rows = min(capacity, 8 if channels <= 10240 else 6)
+            self.few_rows = min(capacity, 6 if channels <= 10240 else 4)
             self.few = _where_it_fits("mxfp4_projection", M=self.few_rows, input_dtype=name, **shape)
         self.n = channels // 2 if epilogue == "swiglu" else channels
         # the quantised rows, by tiles of 16
@@ -817,10 +817,10 @@ class Mxfp4MoeLayer(_OnDevice):
             self.k_quantise_act = Kernel("mxfp4_quantization", K=intermediate, pad=mxfp4.STEP)
             down = dict(N=hidden, K=intermediate, **grouped)
             self.k_down = Kernel("mxfp4_grouped", **down)
-            # A route to an expert or less, two for gate and up: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of
-            # 2048 x 512, 3 tokens, up 9.3 / 6.0 and down 5.9 / 4.3, 16 tokens 12.6 / 10.9 and 10.9 / 10.3, 32 tokens 14.5 / 13.3 and 11.5 / 12.5, 64 tokens 17.3 / 17.9 and 13.6 / 16.4).
-            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if block_m == 16 and routes <= 2 * experts else None
-            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if block_m == 16 and routes <= experts else None
+            # A route to an expert or less: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
+            # 7.6 / 6.0 and down 5.1 / 4.4, 8 tokens 9.7 / 8.5 and 7.4 / 7.3, 16 tokens 10.7 / 10.7 and 8.9 / 10.3; 16 x 2 of 4096 x 1536, 8 tokens, 10.7 / 9.9 and 7.9 / 6.6).
+            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if block_m == 16 and routes <= experts else None
+            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if block_m == 16 and 4 * routes <= 3 * experts else None
             self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, **common)
             self.segments = self.k_metadata.workspace()
         i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)
