@@ -15,7 +15,8 @@
 // Tried: four waves of 128 x 128 results (a third less from LDS, 1.63 us a step, but sums come out of accumulation registers by moves, 4.4-6.2 us a tile against 2.1: the same in
 // all); results by lines of 128 bytes through LDS (more instructions, and not faster: what a tile's end took was its instructions); three to six stages, a CU then holding one workgroup
 // (305 units of 128 expert rows, 1024 x 2048: 64 us with two stages and two workgroups, 80 with four and one); requests masked instead of branched around (level); barriers that do not
-// wait for the last tile's stores (no faster, and 256 x 256 spills).  Without its requests that product takes 46 us, without results 55.
+// wait for the last tile's stores (no faster, and 256 x 256 spills); results past the caches (8192 x 4096 x 4096 75 -> 103 us: an instruction stores 32 bytes of a row, the L2 joins
+// them).  Without its requests that product of experts takes 46 us, without results 55.
 #include "lds_asm.h"
 #include "mx_device.h"
 #include "mx_tiles.h"
