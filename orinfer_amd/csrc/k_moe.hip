@@ -759,8 +759,12 @@ __global__ __launch_bounds__(256) void quantize_dispatch_kernel(const __half* __
     }
 }
 
-// grid (M, ceil(H/256)): fp32 accumulate in rank order, one fp16 cast.
-__global__ __launch_bounds__(256) void moe_combine_kernel(const __half* __restrict__ expert, __half* __restrict__ output,
+__device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
+__device__ __forceinline__ float value_of(float v) { return v; }
+
+// grid (M, ceil(H/256)): fp32 accumulate in rank order, one fp16 cast.  EXPERT: the experts' rows, __half or float.
+template <typename EXPERT>
+__global__ __launch_bounds__(256) void moe_combine_kernel(const EXPERT* __restrict__ expert, __half* __restrict__ output,
                                                           const float* __restrict__ prob, const __half* __restrict__ shared,
                                                           const __half* __restrict__ shared_gate,
                                                           const int* __restrict__ slot_map, int h, int slots, int top_k) {
@@ -771,7 +775,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const __half* __restri
     for (int rank = 0; rank < top_k; ++rank) {
         const int slot = slot_map[(int64_t)row * top_k + rank];
         if (slot >= 0 && slot < slots)
-            acc += __half2float(expert[(int64_t)slot * h + col]) * prob[(int64_t)row * top_k + rank];
+            acc += value_of(expert[(int64_t)slot * h + col]) * prob[(int64_t)row * top_k + rank];
     }
     if (shared != nullptr) {
         const float gate = __fdiv_rn(1.0f, 1.0f + expf(-__half2float(shared_gate[row])));
@@ -780,9 +784,10 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const __half* __restri
     output[(int64_t)row * h + col] = __float2half_rn(acc);
 }
 
-// H a multiple of 8: a thread owns 8 consecutive columns (one 16-byte piece per rank), a workgroup
+// H a multiple of 8: a thread owns 8 consecutive columns (one or two 16-byte pieces per rank), a workgroup
 // 2048 columns of one row.  Same operations per column as above, in the same order.
-__global__ __launch_bounds__(256) void moe_combine_wide_kernel(const __half* __restrict__ expert, __half* __restrict__ output,
+template <typename EXPERT>
+__global__ __launch_bounds__(256) void moe_combine_wide_kernel(const EXPERT* __restrict__ expert, __half* __restrict__ output,
                                                                const float* __restrict__ prob,
                                                                const __half* __restrict__ shared,
                                                                const __half* __restrict__ shared_gate,
@@ -793,9 +798,10 @@ __global__ __launch_bounds__(256) void moe_combine_wide_kernel(const __half* __r
     if (col >= h) return;
     const bool aligned = ((reinterpret_cast<uintptr_t>(expert) | reinterpret_cast<uintptr_t>(output) |
                            reinterpret_cast<uintptr_t>(shared)) & 15) == 0;
-    auto load8 = [&](const __half* src, __half (&dst)[8]) {
+    auto load8 = [&](const auto* src, auto (&dst)[8]) {
         if (aligned) {
-            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(dst) / 16; ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(src)[j];
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) dst[j] = src[j];
@@ -815,7 +821,7 @@ __global__ __launch_bounds__(256) void moe_combine_wide_kernel(const __half* __r
             slot[i] = slot_map[(int64_t)row * top_k + rank];
             weight[i] = prob[(int64_t)row * top_k + rank];
         }
-        __align__(16) __half values[8][8];
+        __align__(16) EXPERT values[8][8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const bool valid = first + i < top_k && slot[i] >= 0 && slot[i] < slots;
@@ -826,7 +832,7 @@ __global__ __launch_bounds__(256) void moe_combine_wide_kernel(const __half* __r
             const bool valid = first + i < top_k && slot[i] >= 0 && slot[i] < slots;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float sum = acc[j] + __half2float(values[i][j]) * weight[i];
+                const float sum = acc[j] + value_of(values[i][j]) * weight[i];
                 acc[j] = valid ? sum : acc[j];
             }
         }
@@ -1433,20 +1439,18 @@ int combine_geometry(const orx_function& f, int rows, Geometry* g) {
     g->block[0] = 256;
     return ORX_OK;
 }
-int combine_launch(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
+template <typename EXPERT>
+int combine_rows(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
     // dynamic decode has exactly top_k assignments per live row (moe.py:514-517)
     const int slots = f.dynamic_rows ? rows * f.top_k : f.slots;
-    if (f.H % 8 == 0) {
-        ORX_LAUNCH(moe_combine_wide_kernel, dim3(g.grid[0], g.grid[1]), dim3(256), 0, s,
-                           pointer_arg<const __half>(args, 0), pointer_arg<__half>(args, 1), pointer_arg<const float>(args, 2),
-                           pointer_arg<const __half>(args, 3), pointer_arg<const __half>(args, 4),
-                           pointer_arg<const int>(args, 5), f.H, slots, f.top_k);
-        return hip_check(hipGetLastError(), "launch moe_combine");
-    }
-    ORX_LAUNCH(moe_combine_kernel, dim3(g.grid[0], g.grid[1]), dim3(256), 0, s,
-                       pointer_arg<const __half>(args, 0), pointer_arg<__half>(args, 1), pointer_arg<const float>(args, 2),
-                       pointer_arg<const __half>(args, 3), pointer_arg<const __half>(args, 4),
-                       pointer_arg<const int>(args, 5), f.H, slots, f.top_k);
+    const dim3 grid(g.grid[0], g.grid[1]), block(256);
+    const EXPERT* const expert = pointer_arg<const EXPERT>(args, 0);
+    __half* const output = pointer_arg<__half>(args, 1);
+    const float* const prob = pointer_arg<const float>(args, 2);
+    const __half *const shared = pointer_arg<const __half>(args, 3), *const shared_gate = pointer_arg<const __half>(args, 4);
+    const int* const slot_map = pointer_arg<const int>(args, 5);
+    if (f.H % 8 == 0) ORX_LAUNCH((moe_combine_wide_kernel<EXPERT>), grid, block, 0, s, expert, output, prob, shared, shared_gate, slot_map, f.H, slots, f.top_k);
+    else ORX_LAUNCH((moe_combine_kernel<EXPERT>), grid, block, 0, s, expert, output, prob, shared, shared_gate, slot_map, f.H, slots, f.top_k);
     return hip_check(hipGetLastError(), "launch moe_combine");
 }
 int make_combine(const Variant& v, orx_function* f) {
@@ -1454,18 +1458,24 @@ int make_combine(const Variant& v, orx_function* f) {
     bool bad = false;
     f->H = (int)v.integer("H", 0, &bad);
     f->slots = (int)v.integer("slots", f->M * f->top_k, &bad);
+    const std::string expert = v.string("expert_dtype", "float16", &bad);
     if (bad) return ORX_ERR_BAD_VARIANT;
     if (f->M <= 0 || f->H <= 0 || f->slots <= 0 || f->top_k <= 0) {
         set_error("moe_combine: invalid MoE mixture dimensions");
         return ORX_ERR_BAD_VARIANT;
     }
+    if (expert != "float16" && expert != "float32") {
+        set_error("moe_combine: expert_dtype must be float16 or float32");
+        return ORX_ERR_BAD_VARIANT;
+    }
+    const bool wide = expert == "float32";
     // Shared / SharedGate may be null device pointers: then no shared expert is added
-    f->args = {{"Expert", ArgPointer, 2},     {"Output", ArgPointer, 2},           {"Prob", ArgPointer, 4},
-               {"Shared", ArgPointer, 0x80000002u}, {"SharedGate", ArgPointer, 0x80000002u}, {"SlotMap", ArgPointer, 4}};
+    f->args = {{"Expert", ArgPointer, wide ? 4u : 2u}, {"Output", ArgPointer, 2},           {"Prob", ArgPointer, 4},
+               {"Shared", ArgPointer, 0x80000002u},    {"SharedGate", ArgPointer, 0x80000002u}, {"SlotMap", ArgPointer, 4}};
     if (f->dynamic_rows) f->args.push_back({"m", ArgI32, 4});
     f->geometry = combine_geometry;
-    f->launch = combine_launch;
-    f->device_function = reinterpret_cast<const void*>(&moe_combine_kernel);
+    f->launch = wide ? combine_rows<float> : combine_rows<__half>;
+    f->device_function = wide ? reinterpret_cast<const void*>(&moe_combine_kernel<float>) : reinterpret_cast<const void*>(&moe_combine_kernel<__half>);
     return ORX_OK;
 }
 
@@ -1498,7 +1508,7 @@ const Registration* moe_registrations(int* count) {
      "ColdExpert,ColdOffsets,ColdRow,Counts,TileExpert,TileOffsets,TileRow[,m]"},
     {"expert_dispatch", make_dispatch, "M, H, E=512, top_k=10, scale_group=64, dynamic_rows=false, input_dtype=int8|float16 (one scale per row)",
      "A,D,DS,IDs,RelativeSlot,RowOffsets,Scale,SlotMap[,m]"},
-    {"moe_combine", make_combine, "M, H, slots=M*top_k, top_k=10, dynamic_rows=false",
+    {"moe_combine", make_combine, "M, H, slots=M*top_k, top_k=10, dynamic_rows=false, expert_dtype=float16|float32",
      "Expert,Output,Prob,Shared,SharedGate,SlotMap[,m]"},
     };
     *count = (int)(sizeof(rows) / sizeof(rows[0]));

@@ -815,13 +815,15 @@ class Mxfp4MoeLayer(_OnDevice):
             up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", **grouped)
             self.k_up = Kernel("mxfp4_grouped", **up)
             self.k_quantise_act = Kernel("mxfp4_quantization", K=intermediate, pad=mxfp4.STEP)
-            down = dict(N=hidden, K=intermediate, **grouped)
+            # (The second products stay fp32 until they are weighted and summed: as fp16, one beyond 65504 made its token's sum infinite or NaN however small its weight, and each was
+            # a rounding more.  Its price, 128 experts x 8 of 2048 x 512, us of place and down with fp16 / fp32: 256 tokens 25.7 / 29.2, 4096 tokens 105.6 / 158.8.)
+            down = dict(N=hidden, K=intermediate, output_dtype="float32", **grouped)
             self.k_down = Kernel("mxfp4_grouped", **down)
             # A route to an expert or less: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
             # 7.6 / 6.0 and down 5.1 / 4.4, 8 tokens 9.7 / 8.5 and 7.4 / 7.3, 16 tokens 10.7 / 10.7 and 8.9 / 10.3; 16 x 2 of 4096 x 1536, 8 tokens, 10.7 / 9.9 and 7.9 / 6.6).
             self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if block_m == 16 and routes <= experts else None
             self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if block_m == 16 and 4 * routes <= 3 * experts else None
-            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, **common)
+            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, expert_dtype="float32", **common)
             self.segments = self.k_metadata.workspace()
         i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)
         f16 = dict(dtype=torch.float16, device=self.device)
@@ -836,7 +838,7 @@ class Mxfp4MoeLayer(_OnDevice):
         self.a_q, self.a_s = torch.empty((tokens, wide // 2), **u8), torch.empty((tokens, wide // 32), **u8)
         self.h_q, self.h_s = torch.empty((routes, inner // 2), **u8), torch.empty((routes, inner // 32), **u8)
         self.act = torch.empty((routes, intermediate), **f16)
-        self.down_out = torch.empty((routes, hidden), **f16)
+        self.down_out = torch.empty((routes, hidden), dtype=torch.float32, device=self.device)
         self.out = torch.empty((tokens, hidden), **f16)
 
     def route(self, logits, stream=None):
@@ -874,8 +876,8 @@ class Mxfp4MoeLayer(_OnDevice):
         self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
 
     def down(self, act, prob, shared=None, shared_gate=None, stream=None):
-        """fp16 rows in the order of the slots and fp32 weights (tokens, top_k) -> fp16 (tokens, hidden): the weighted sum of the routes' second products (rounded to fp16
-        each, as moe_combine takes them) and, where they are given, of sigmoid(shared_gate) (tokens) times shared (tokens, hidden), fp16 both."""
+        """fp16 rows in the order of the slots and fp32 weights (tokens, top_k) -> fp16 (tokens, hidden): the weighted sum, in fp32, of the routes' second products and, where they
+        are given, of sigmoid(shared_gate) (tokens) times shared (tokens, hidden), fp16 both."""
         _check_rows(act, self.assignments, self.inter, torch.float16, self.device, "act")
         _check_rows(prob, self.tokens, self.top_k, torch.float32, self.device, "prob")
         if (shared is None) != (shared_gate is None):

@@ -1,0 +1,91 @@
+"""Expert layers of MXFP4 weights as they are used, against the 64-bit oracle.
+
+Tolerances, derived: a second product is off by at most `product`'s bound (its sum of K terms in fp32).  The weighted sum then rounds once for each product and once for each addition, both in
+fp32: with the routes' and the shared expert's terms of magnitudes T, at most 2 (top_k + 1) * 2^-24 * T, for the shared expert's gate 4 * 2^-24 more of its term (exponential, sum and quotient).
+The result is rounded once to its type, half a step of it."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mxfp4 as orc
+from orinfer_amd import programs
+from tests.gpu_util import dev, host, kernel
+from tests.test_gpu_mxfp4 import check, product, rows_of, slots_of, weights
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def second_products(rows, chosen, down):
+    """rows (slots, I) as the device has them, the slots' experts -> products and their bounds, 64 bits"""
+    b = orc.values(*orc.quantise(rows.double().cpu().numpy()))
+    y, dy = (np.empty((len(b), down[0].shape[1])) for _ in range(2))
+    for e in np.unique(chosen):
+        at = chosen == e
+        y[at], dy[at] = product(b[at], orc.values(down[0][e], down[1][e]))
+    return y, dy
+
+
+def weighted(y, dy, slot, prob, shared=None, gate=None):
+    """sum of the routes' products times their weights, and its bound before the result's own rounding"""
+    p = prob.astype(np.float64)[:, :, None]
+    want, bound, size = (y[slot] * p).sum(1), (dy[slot] * p).sum(1), (np.abs(y[slot]) * p).sum(1)
+    if shared is not None:
+        term = 1 / (1 + np.exp(-gate.double().cpu().numpy()))[:, None] * shared.double().cpu().numpy()
+        want, size, bound = want + term, size + np.abs(term), bound + 4 * 2.0**-24 * np.abs(term)
+    return want, bound + 2 * (prob.shape[1] + 1) * 2.0**-24 * size
+
+
+@pytest.mark.parametrize("h", [8, 100, 2056, 4096])
+@pytest.mark.parametrize("m,top_k,offset", [(1, 1, 0), (5, 8, 0), (33, 10, 1), (7, 3, 2)])
+def test_sums_of_fp32_rows(h, m, top_k, offset):
+    """Slots that are not there count nothing; rows and results at addresses of their types' own alignment; nothing behind the result."""
+    rng = np.random.default_rng(h + m)
+    slots = m * top_k + 2
+    expert = (rng.standard_normal((slots, h)) * 1e6).astype(np.float32)
+    slot = rng.integers(0, slots, (m, top_k)).astype(np.int32)
+    slot[0, 0], slot[-1, -1] = -1, slots
+    prob = (rng.random((m, top_k)) * 1e-3).astype(np.float32)
+    there = (slot >= 0) & (slot < slots)
+    shared, gate = torch.from_numpy(rng.standard_normal((m, h))).half().to(DEV), torch.from_numpy(rng.standard_normal(m)).half().to(DEV)
+    moved = torch.empty(expert.size + offset, device=DEV)[offset:].view(slots, h).copy_(torch.from_numpy(expert))
+    for more in ((None, None), (shared, gate)):
+        out = torch.full((m * h + offset + 8,), -7.0, dtype=torch.float16, device=DEV)
+        got = out[offset:offset + m * h].view(m, h)
+        kernel("moe_combine", M=m, H=h, slots=slots, top_k=top_k, expert_dtype="float32")(Expert=moved, Output=got, Prob=dev(prob), Shared=more[0], SharedGate=more[1], SlotMap=dev(slot))
+        y = expert.astype(np.float64)
+        check(got, *weighted(y, np.zeros_like(y), np.where(there, slot, 0), prob * there, *more), torch.float16)
+        assert (out[:offset] == -7).all() and (out[offset + m * h:] == -7).all()
+
+
+@pytest.mark.parametrize("tokens,experts,top_k,hidden,inner,block_m", [(2, 64, 8, 288, 96, None), (40, 8, 2, 320, 160, 16), (64, 16, 6, 288, 128, 64), (300, 4, 2, 256, 544, 128), (300, 8, 4, 512, 256, 256)])
+def test_second_products_outside_fp16_and_a_sum_within(tokens, experts, top_k, hidden, inner, block_m):
+    """Products of both signs far beyond 65504 with small weights: their weighted sum is what fp16 holds."""
+    rng = np.random.default_rng(tokens * 7 + inner)
+    gate_up, down = weights(rng, experts, 2 * inner, hidden), weights(rng, experts, hidden, inner, low=136, high=140)
+    layer = programs.Mxfp4MoeLayer(tokens, experts, top_k, hidden, inner, *map(dev, gate_up), *map(dev, down), block_m=block_m)
+    ids = np.argsort(rng.random((tokens, experts)), 1)[:, :top_k].astype(np.int32)
+    layer.place(dev(ids))
+    order, slot = slots_of(ids)
+    rows = torch.from_numpy(rng.standard_normal((tokens * top_k, inner))).half()
+    prob = (rng.random((tokens, top_k)) * 2.0**-10).astype(np.float32)
+    y, dy = second_products(rows, ids.reshape(-1)[order], down)
+    want, bound = weighted(y, dy, slot, prob)
+    assert (np.abs(y) > 65520).mean() > 0.05 and np.abs(want).max() < 60000
+    check(layer.down(rows.to(DEV), dev(prob)), want, bound, torch.float16)
+
+
+@pytest.mark.parametrize("tokens,experts,top_k,hidden,inner", [(1, 8, 2, 64, 32), (3, 128, 8, 512, 64), (64, 60, 6, 288, 128), (700, 8, 3, 512, 256)])
+def test_a_weighted_sum_is_rounded_once(tokens, experts, top_k, hidden, inner):
+    rng = np.random.default_rng(tokens)
+    gate_up, down = weights(rng, experts, 2 * inner, hidden), weights(rng, experts, hidden, inner)
+    layer = programs.Mxfp4MoeLayer(tokens, experts, top_k, hidden, inner, *map(dev, gate_up), *map(dev, down))
+    ids = np.argsort(rng.random((tokens, experts)), 1)[:, :top_k].astype(np.int32)
+    layer.place(dev(ids))
+    order, slot = slots_of(ids)
+    rows = rows_of(rng, tokens * top_k, inner, torch.float16)
+    prob = rng.dirichlet(np.ones(top_k), tokens).astype(np.float32)
+    y, dy = second_products(rows, ids.reshape(-1)[order], down)
+    shared, gate = rows_of(rng, tokens, hidden, torch.float16).to(DEV), torch.from_numpy(rng.standard_normal(tokens)).half().to(DEV)
+    for more in ((None, None), (shared, gate)):
+        check(layer.down(rows.to(DEV), dev(prob), *more), *weighted(y, dy, slot, prob, *more), torch.float16)
