@@ -709,7 +709,15 @@ def _check_rows(x, rows, columns, dtype, device, what):
 
 
 class _OnDevice:
-    """Launches on the device of the weights, whichever is current; its current stream unless the caller names one."""
+    """Launches on the GPU of the weights, whichever is current (weights on the host go to the current one); its current stream unless the caller names one."""
+
+    @staticmethod
+    def _device_of(*tensors):
+        """The GPU that the weights are on, or the current one.  (`.cuda()` would copy a tensor of another GPU to the current one.)"""
+        devices = {t.device for t in tensors if t.is_cuda}
+        if len(devices) > 1:
+            raise ValueError(f"the weights are on several GPUs: {sorted(map(str, devices))}")
+        return devices.pop() if devices else torch.device("cuda", torch.cuda.current_device())
 
     def _call(self, body, *args, stream=None):
         if torch._C._cuda_getDevice() == self.device.index:
@@ -742,8 +750,9 @@ class Mxfp4Linear(_OnDevice):
             raise ValueError("capacity must be 1 to 2^24 rows")
         self.capacity, self.dtype = capacity, dtype
         channels, self.k = codes.shape[0], 2 * codes.shape[1]
-        self.weight, self.powers = (t.cuda() for t in mxfp4.tiles(codes, exponents, paired=epilogue == "swiglu"))
-        self.device = self.weight.device
+        codes, exponents = torch.as_tensor(codes), torch.as_tensor(exponents)
+        self.device = self._device_of(codes, exponents)
+        self.weight, self.powers = (t.to(self.device) for t in mxfp4.tiles(codes, exponents, paired=epilogue == "swiglu"))
         name = mxfp4.dtype_name(dtype)
         shape = dict(N=channels, K=self.k, dynamic_rows=True, epilogue=epilogue, output_dtype=name)
         with torch.cuda.device(self.device):
@@ -791,9 +800,10 @@ class Mxfp4MoeLayer(_OnDevice):
         if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden // 2) or tuple(down.shape) != (experts, hidden, intermediate // 2):
             raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden // 2}) and down ({experts}, {hidden}, {intermediate // 2}), "
                              f"not {tuple(gate_up.shape)} and {tuple(down.shape)}")
-        self.w1, self.p1 = (t.cuda() for t in mxfp4.tiles(gate_up, gate_up_exponents, paired=True))
-        self.w2, self.p2 = (t.cuda() for t in mxfp4.tiles(down, down_exponents))
-        self.device = self.w1.device
+        weights = tuple(map(torch.as_tensor, (gate_up, gate_up_exponents, down, down_exponents)))
+        self.device = self._device_of(*weights)
+        self.w1, self.p1 = (t.to(self.device) for t in mxfp4.tiles(*weights[:2], paired=True))
+        self.w2, self.p2 = (t.to(self.device) for t in mxfp4.tiles(*weights[2:]))
         self.bias = None
         if bias is not None:
             self.bias = torch.as_tensor(bias, dtype=torch.float32).to(self.device).contiguous()

@@ -1,7 +1,11 @@
 """What the MXFP4 layers ask for, without a GPU."""
-import pytest
+import contextlib
 
-from orinfer_amd import lib
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from orinfer_amd import lib, programs
 
 COMBINE = dict(M=4, H=256, top_k=2)
 
@@ -18,3 +22,36 @@ def test_weighted_sums_take_fp16_or_fp32_rows():
         with pytest.raises(lib.OrxError) as error:
             kernel(stream=0, **dict(named, Expert=address))
         assert error.value.code == lib.ORX_ERR_BAD_ARGUMENT
+
+
+@pytest.fixture
+def gpus(monkeypatch):
+    """Tensors of shapes alone on GPUs that are not there; GPU 0 is current."""
+    monkeypatch.setattr(torch.cuda, "device", lambda _: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(lib.Kernel, "workspace", lambda self: None)
+    with FakeTensorMode():
+        yield
+
+
+def weights(device, *shape):
+    n, k = shape[-2:]
+    return [torch.empty((*shape[:-1], k // piece), dtype=torch.uint8, device=device) for piece in (2, 32)]
+
+
+@pytest.mark.parametrize("device,stays", [("cuda:1", "cuda:1"), ("cuda:0", "cuda:0"), ("cpu", "cuda:0")])
+def test_weights_stay_on_their_gpu(gpus, device, stays):
+    linear = programs.Mxfp4Linear(*weights(device, 64, 96), 5)
+    layer = programs.Mxfp4MoeLayer(3, 4, 2, 96, 64, *weights(device, 4, 128, 96), *weights(device, 4, 96, 64), bias=[0.0] * 4)
+    for held in (linear, layer):
+        assert str(held.device) == stays
+        assert {str(t.device) for t in vars(held).values() if isinstance(t, torch.Tensor)} == {stays}
+
+
+def test_weights_of_several_gpus_are_refused(gpus):
+    here, there = weights("cuda:0", 64, 96), weights("cuda:1", 64, 96)
+    with pytest.raises(ValueError, match="several GPUs"):
+        programs.Mxfp4Linear(here[0], there[1], 5)
+    with pytest.raises(ValueError, match="several GPUs"):
+        programs.Mxfp4MoeLayer(3, 4, 2, 96, 64, *weights("cuda:0", 4, 128, 96), *weights("cuda:1", 4, 96, 64))
+    assert str(programs.Mxfp4Linear(there[0], weights("cpu", 64, 96)[1], 5).device) == "cuda:1"  # what is on the host joins the other
