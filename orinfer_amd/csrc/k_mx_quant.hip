@@ -226,21 +226,23 @@ int dequantise_launch(const orx_function& f, int rows, const Geometry& g, hipStr
 
 constexpr int kMaxK = 1 << 24;
 
-int shape(const Variant& v, orx_function* f, const char* type_key) {
+int shape(const Variant& v, orx_function* f, const char* type_key, bool tiles) {
     bool bad = false;
     f->K = (int)v.integer("K", 0, &bad);
-    const int pad = (int)v.integer("pad", mx::kBlock, &bad);
+    const int pad = tiles ? mx::kStepK : (int)v.integer("pad", mx::kBlock, &bad);
     f->algorithm = mx_type(v, type_key, "float16", &bad);
     if (bad) return ORX_ERR_BAD_VARIANT;
     if (f->K <= 0 || f->K > kMaxK || (pad != mx::kBlock && pad != mx::kStepK)) {
         set_error("%s: need 0 < K <= %d and pad 32 or 256", f->symbol.c_str(), kMaxK);
         return ORX_ERR_BAD_VARIANT;
     }
+    f->flags2 = tiles;
     f->group = pad == mx::kBlock ? (f->K + 31) / 32 * 32 : (f->K + 255) / 256 * 256;
-    f->stride = pad == mx::kBlock ? f->group : (f->group / 256 | 1) * 256;  // (for the products an odd multiple; what is behind `group` is not written)
+    f->stride = pad == mx::kBlock || tiles ? f->group : (f->group / 256 | 1) * 256;  // (for the products an odd multiple; what is behind `group` is not written)
     f->dynamic_rows = true;
-    // (pieces are counted in 32 bits, and so are a launch's threads: a quarter of them)
-    const int most = (int)std::min<int64_t>(1 << 24, ((1ll << 32) - 65536) / (f->stride / 8));
+    // Rows: pieces are counted in 32 bits (a launch's threads are a quarter of them).  Tiles: addresses are 64 bits wide, a launch's threads are fewer than 2^32.
+    const int64_t counted = tiles ? 16 * (0xFFFFFFFFll / kThreads / ceil_div(f->group / 128, kThreads / 64)) : ((1ll << 32) - 65536) / (f->stride / 8);
+    const int most = (int)std::min<int64_t>(1 << 24, counted);
     f->capacity = (int)v.integer("M", most, &bad);
     if (bad || f->capacity < 1 || f->capacity > most) {
         if (!bad) set_error("%s: M must be 1 to %d for this K", f->symbol.c_str(), most);
@@ -250,8 +252,6 @@ int shape(const Variant& v, orx_function* f, const char* type_key) {
     return ORX_OK;
 }
 int make_quantise(const Variant& v, orx_function* f) {
-    const int code = shape(v, f, "input_dtype");
-    if (code != ORX_OK) return code;
     bool bad = false;
     const std::string scale = v.string("scale", "floor", &bad);
     if (bad) return ORX_ERR_BAD_VARIANT;
@@ -261,11 +261,12 @@ int make_quantise(const Variant& v, orx_function* f) {
         set_error("mxfp4_quantization: layout must be rows or tiles, and pad goes with rows");
         return ORX_ERR_BAD_VARIANT;
     }
-    if (layout == "tiles") f->flags2 = 1, f->group = (f->K + mx::kStepK - 1) / mx::kStepK * mx::kStepK;
     if (scale != "floor" && scale != "ceil") {
         set_error("mxfp4_quantization: scale must be floor or ceil");
         return ORX_ERR_BAD_VARIANT;
     }
+    const int code = shape(v, f, "input_dtype", layout == "tiles");
+    if (code != ORX_OK) return code;
     f->flags = scale == "ceil";
     f->args = {{"Q", ArgPointer, 4}, {"S", ArgPointer, 1}, {"X", ArgPointer, f->algorithm == mx::F32 ? 4u : 2u}, {"rows", ArgI32, 4}};
     f->launch = quantise_launch;
@@ -279,7 +280,7 @@ int make_quantise(const Variant& v, orx_function* f) {
     return ORX_OK;
 }
 int make_dequantise(const Variant& v, orx_function* f) {
-    const int code = shape(v, f, "output_dtype");
+    const int code = shape(v, f, "output_dtype", false);
     if (code != ORX_OK) return code;
     f->args = {{"Q", ArgPointer, 4}, {"S", ArgPointer, 1}, {"Y", ArgPointer, f->algorithm == mx::F32 ? 4u : 2u}, {"rows", ArgI32, 4}};
     f->launch = dequantise_launch;

@@ -757,7 +757,7 @@ class Mxfp4Linear(_OnDevice):
         shape = dict(N=channels, K=self.k, dynamic_rows=True, epilogue=epilogue, output_dtype=name)
         with torch.cuda.device(self.device):
             self.projection = Kernel("mxfp4_projection", M=capacity, **shape)
-            self.quantizer = Kernel("mxfp4_quantization", K=self.k, input_dtype=name, layout="tiles")
+            self.quantizer = Kernel("mxfp4_quantization", M=capacity, K=self.k, input_dtype=name, layout="tiles")
             # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (weights out of cache, us of the two launches / of the one:
             # 17408 x 5120, 1 row 15.1 / 12.3, 4 rows 15.0 / 15.0, 6 rows 15.2 / 16.7; 9728 x 2560, 1 row 8.3 / 5.8, 6 rows 8.2 / 7.8, 8 rows 8.2 / 8.5; 4096 x 4096 6.3 / 4.4, 6.4 / 6.2, 6.3 / 6.9).
             # Not where their codes do not fit LDS.
@@ -821,10 +821,10 @@ class Mxfp4MoeLayer(_OnDevice):
             self.k_router = Kernel("router_topk", renormalize=renormalize, **common, **({} if plain else scores))
             self.k_metadata = Kernel("route_metadata", block_m=block_m, slot_maps=True, workspace=True, tile_units=True, **common)
             grouped = dict(rows=routes, E=experts, tiles=capacity, block_m=block_m)
-            self.k_quantise_tokens = Kernel("mxfp4_quantization", K=hidden, pad=mxfp4.STEP)
+            self.k_quantise_tokens = Kernel("mxfp4_quantization", M=tokens, K=hidden, pad=mxfp4.STEP)
             up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", **grouped)
             self.k_up = Kernel("mxfp4_grouped", **up)
-            self.k_quantise_act = Kernel("mxfp4_quantization", K=intermediate, pad=mxfp4.STEP)
+            self.k_quantise_act = Kernel("mxfp4_quantization", M=routes, K=intermediate, pad=mxfp4.STEP)
             # (The second products stay fp32 until they are weighted and summed: as fp16, one beyond 65504 made its token's sum infinite or NaN however small its weight, and each was
             # a rounding more.  Its price, 128 experts x 8 of 2048 x 512, us of place and down with fp16 / fp32: 256 tokens 25.7 / 29.2, 4096 tokens 105.6 / 158.8.)
             down = dict(N=hidden, K=intermediate, output_dtype="float32", **grouped)

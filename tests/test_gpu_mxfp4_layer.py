@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import mxfp4 as orc
-from orinfer_amd import programs
+from orinfer_amd import mxfp4, programs
 from tests.gpu_util import dev, host, kernel
 from tests.test_gpu_mxfp4 import check, product, rows_of, slots_of, weights
 
@@ -89,3 +89,23 @@ def test_a_weighted_sum_is_rounded_once(tokens, experts, top_k, hidden, inner):
     shared, gate = rows_of(rng, tokens, hidden, torch.float16).to(DEV), torch.from_numpy(rng.standard_normal(tokens)).half().to(DEV)
     for more in ((None, None), (shared, gate)):
         check(layer.down(rows.to(DEV), dev(prob), *more), *weighted(y, dy, slot, prob, *more), torch.float16)
+
+
+def test_tiles_of_more_rows_than_32_bits_count_pieces():
+    """2^32 pieces of eight values, 64 GiB, and some rows more: the first rows, some in the middle and the last ones, of which only three of a tile's sixteen are there."""
+    rows, k = 2**32 // 640 // 16 * 16 + 19, 5120
+    some = torch.randn((4096, k), device=DEV).half()
+    x = torch.empty((rows, k), dtype=torch.float16, device=DEV)
+    for first in range(0, rows, 4096):
+        x[first:first + 4096] = some[:rows - first]
+    x[-3:] *= 3
+    tiles = -(-rows // 16)
+    q, s = torch.empty((tiles, 20, 2048), dtype=torch.uint8, device=DEV), torch.empty((tiles, 20, 128), dtype=torch.uint8, device=DEV)
+    kernel("mxfp4_quantization", K=k, layout="tiles", M=rows)(Q=q, S=s, X=x, rows=rows)
+    for tile in (0, tiles // 2, tiles - 2, tiles - 1):
+        part = x[16 * tile:16 * tile + 16].double().cpu().numpy()
+        part = np.pad(part, ((0, 16 - len(part)), (0, 0)))
+        want = mxfp4.tiles(*map(torch.from_numpy, orc.quantise(part)))
+        assert torch.equal(q[tile].cpu().flatten(), want[0].flatten()) and torch.equal(s[tile].cpu().flatten(), want[1].flatten())
+    del x, q, s
+    torch.cuda.empty_cache()

@@ -55,3 +55,21 @@ def test_weights_of_several_gpus_are_refused(gpus):
     with pytest.raises(ValueError, match="several GPUs"):
         programs.Mxfp4MoeLayer(3, 4, 2, 96, 64, *weights("cuda:0", 4, 128, 96), *weights("cuda:1", 4, 96, 64))
     assert str(programs.Mxfp4Linear(there[0], weights("cpu", 64, 96)[1], 5).device) == "cuda:1"  # what is on the host joins the other
+
+
+@pytest.mark.parametrize("capacity,k", [(7_000_000, 5120), (1 << 24, 2080), (1 << 24, 32), (131_056, 1 << 20)])
+def test_a_linear_serves_its_capacity(gpus, capacity, k):
+    """Every launch of as many rows as the object was made for is one that can be made."""
+    linear = programs.Mxfp4Linear(*weights("cuda:0", 16, k), capacity)
+    for kernel in (linear.quantizer, linear.projection):
+        (groups, *_), (threads, *_), _ = kernel.geometry(capacity)
+        assert 0 < groups * threads < 1 << 32
+    assert linear.quantizer.geometry(capacity)[0][0] * 512 >= -(-capacity // 16) * k  # a workgroup takes 16 rows x 512 of K at most
+
+
+def test_rows_that_no_launch_takes_are_refused_where_the_object_is_made(gpus):
+    for make in (lambda: programs.Mxfp4Linear(*weights("cuda:0", 16, 1 << 20), 131_057),
+                 lambda: programs.Mxfp4MoeLayer(5_000_000, 2, 1, 8192, 32, *weights("cuda:0", 2, 64, 8192), *weights("cuda:0", 2, 8192, 32))):
+        with pytest.raises(lib.OrxError) as error:
+            make()
+        assert error.value.code == lib.ORX_ERR_BAD_VARIANT and "M must be" in str(error.value)
