@@ -708,6 +708,11 @@ def _check_rows(x, rows, columns, dtype, device, what):
         raise ValueError(f"{what} has {x.shape[0]} rows, not {rows}")
 
 
+def _apart(a, b):
+    """Two contiguous tensors share no memory."""
+    return a.data_ptr() + a.nbytes <= b.data_ptr() or b.data_ptr() + b.nbytes <= a.data_ptr()
+
+
 class _OnDevice:
     """Launches on the GPU of the weights, whichever is current (weights on the host go to the current one); its current stream unless the caller names one."""
 
@@ -780,7 +785,8 @@ class Mxfp4Linear(_OnDevice):
         return self.out if rows == self.capacity else self.out.as_strided((rows, self.n), (self.n, 1))
 
     def _run(self, x, rows, stream):
-        if rows <= self.few_rows and self.few is not None:
+        # (not rows in the object's own output, a call's result given to the next one: workgroups that have ended write over what others have yet to read)
+        if rows <= self.few_rows and self.few is not None and _apart(x, self.out):
             self.few(stream=stream, A=x, Out=self.out, W=self.weight, WS=self.powers, m=rows)
             return
         self.quantizer(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=rows)
@@ -879,7 +885,7 @@ class Mxfp4MoeLayer(_OnDevice):
         return self.act
 
     def _up(self, x, stream):
-        if self.few_up is not None:
+        if self.few_up is not None and _apart(x, self.act):  # (as Mxfp4Linear's)
             self.few_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
             return
         self.k_quantise_tokens(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=self.tokens)

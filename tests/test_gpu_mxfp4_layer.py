@@ -109,3 +109,16 @@ def test_tiles_of_more_rows_than_32_bits_count_pieces():
         assert torch.equal(q[tile].cpu().flatten(), want[0].flatten()) and torch.equal(s[tile].cpu().flatten(), want[1].flatten())
     del x, q, s
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [1, 4, 6, 40])
+def test_a_linear_of_its_own_result(rows):
+    rng = np.random.default_rng(rows)
+    codes, exponents = weights(rng, 512, 512, low=114, high=120)
+    linear = programs.Mxfp4Linear(dev(codes), dev(exponents), rows)
+    x = rows_of(rng, rows, 512, torch.float16).to(DEV)
+    w = orc.values(codes, exponents)
+    for _ in range(3):
+        once = linear.run(x).clone()
+        want, bound = product(orc.values(*orc.quantise(once.double().cpu().numpy())), w)
+        check(linear.run(linear.run(x)), want, bound, torch.float16)

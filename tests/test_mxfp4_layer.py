@@ -73,3 +73,32 @@ def test_rows_that_no_launch_takes_are_refused_where_the_object_is_made(gpus):
         with pytest.raises(lib.OrxError) as error:
             make()
         assert error.value.code == lib.ORX_ERR_BAD_VARIANT and "M must be" in str(error.value)
+
+
+def launches(made, method, *args):
+    """Which of an object's kernels a call launches, in order."""
+    seen = []
+    for name in [name for name, value in vars(made).items() if value == "kernel"]:
+        setattr(made, name, lambda name=name, **_: seen.append(name))
+    getattr(made, method)(*args, 0)
+    return seen
+
+
+def test_rows_in_the_buffer_that_a_launch_writes_are_quantised_before_it():
+    """Where every workgroup reads all rows, none may write over them."""
+    def linear(x, rows):
+        made = object.__new__(programs.Mxfp4Linear)
+        vars(made).update(few_rows=4, few="kernel", quantizer="kernel", projection="kernel", out=out, weight=None, powers=None, a_q=None, a_s=None)
+        return launches(made, "_run", x, rows)
+
+    buffer = torch.zeros(10 * 64, dtype=torch.float16)
+    out = buffer[2 * 64:8 * 64].view(6, 64)
+    for first, rows, apart in ((0, 2, True), (8, 2, True), (2, 1, False), (2, 4, False), (7, 1, False), (1, 2, False), (7, 3, False), (0, 4, False)):
+        x = buffer[first * 64:(first + rows) * 64].view(rows, 64)
+        assert linear(x, rows) == (["few"] if apart else ["quantizer", "projection"]), (first, rows)
+    assert linear(torch.zeros(5, 64).half(), 5) == ["quantizer", "projection"]
+
+    for x, want in ((out, ["k_quantise_tokens", "k_up"]), (buffer[:128].view(2, 64), ["few_up"])):
+        layer = object.__new__(programs.Mxfp4MoeLayer)
+        vars(layer).update(tokens=len(x), few_up="kernel", k_quantise_tokens="kernel", k_up="kernel", act=out, a_q=None, a_s=None, slot_token=None, tile_count=None, tile_units=None, w1=None, p1=None)
+        assert launches(layer, "_up", x) == want
