@@ -760,13 +760,16 @@ __global__ __launch_bounds__(256) void quantize_dispatch_kernel(const __half* __
 }
 
 __device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
+__device__ __forceinline__ float value_of(__bf16 v) { return (float)v; }
 __device__ __forceinline__ float value_of(float v) { return v; }
+__device__ __forceinline__ void round_to(__half& to, float v) { to = __float2half_rn(v); }
+__device__ __forceinline__ void round_to(__bf16& to, float v) { to = (__bf16)v; }
 
-// grid (M, ceil(H/256)): fp32 accumulate in rank order, one fp16 cast.  EXPERT: the experts' rows, __half or float.
-template <typename EXPERT>
-__global__ __launch_bounds__(256) void moe_combine_kernel(const EXPERT* __restrict__ expert, __half* __restrict__ output,
-                                                          const float* __restrict__ prob, const __half* __restrict__ shared,
-                                                          const __half* __restrict__ shared_gate,
+// grid (M, ceil(H/256)): fp32 accumulate in rank order, one cast.  EXPERT: the experts' rows, __half or float; VALUE: the result and the shared expert's, __half or __bf16.
+template <typename EXPERT, typename VALUE>
+__global__ __launch_bounds__(256) void moe_combine_kernel(const EXPERT* __restrict__ expert, VALUE* __restrict__ output,
+                                                          const float* __restrict__ prob, const VALUE* __restrict__ shared,
+                                                          const VALUE* __restrict__ shared_gate,
                                                           const int* __restrict__ slot_map, int h, int slots, int top_k) {
     const int row = blockIdx.x;
     const int col = blockIdx.y * 256 + threadIdx.x;
@@ -778,19 +781,19 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const EXPERT* __restri
             acc += value_of(expert[(int64_t)slot * h + col]) * prob[(int64_t)row * top_k + rank];
     }
     if (shared != nullptr) {
-        const float gate = __fdiv_rn(1.0f, 1.0f + expf(-__half2float(shared_gate[row])));
-        acc = acc + gate * __half2float(shared[(int64_t)row * h + col]);
+        const float gate = __fdiv_rn(1.0f, 1.0f + expf(-value_of(shared_gate[row])));
+        acc = acc + gate * value_of(shared[(int64_t)row * h + col]);
     }
-    output[(int64_t)row * h + col] = __float2half_rn(acc);
+    round_to(output[(int64_t)row * h + col], acc);
 }
 
 // H a multiple of 8: a thread owns 8 consecutive columns (one or two 16-byte pieces per rank), a workgroup
 // 2048 columns of one row.  Same operations per column as above, in the same order.
-template <typename EXPERT>
-__global__ __launch_bounds__(256) void moe_combine_wide_kernel(const EXPERT* __restrict__ expert, __half* __restrict__ output,
+template <typename EXPERT, typename VALUE>
+__global__ __launch_bounds__(256) void moe_combine_wide_kernel(const EXPERT* __restrict__ expert, VALUE* __restrict__ output,
                                                                const float* __restrict__ prob,
-                                                               const __half* __restrict__ shared,
-                                                               const __half* __restrict__ shared_gate,
+                                                               const VALUE* __restrict__ shared,
+                                                               const VALUE* __restrict__ shared_gate,
                                                                const int* __restrict__ slot_map, int h, int slots,
                                                                int top_k) {
     const int row = blockIdx.x;
@@ -838,16 +841,16 @@ __global__ __launch_bounds__(256) void moe_combine_wide_kernel(const EXPERT* __r
         }
     }
     if (shared != nullptr) {
-        const float gate = __fdiv_rn(1.0f, 1.0f + expf(-__half2float(shared_gate[row])));
-        __align__(16) __half values[8];
+        const float gate = __fdiv_rn(1.0f, 1.0f + expf(-value_of(shared_gate[row])));
+        __align__(16) VALUE values[8];
         load8(shared + (int64_t)row * h + col, values);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = acc[j] + gate * __half2float(values[j]);
+        for (int j = 0; j < 8; ++j) acc[j] = acc[j] + gate * value_of(values[j]);
     }
-    __align__(16) __half result[8];
+    __align__(16) VALUE result[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) result[j] = __float2half_rn(acc[j]);
-    __half* dst = output + (int64_t)row * h + col;
+    for (int j = 0; j < 8; ++j) round_to(result[j], acc[j]);
+    VALUE* dst = output + (int64_t)row * h + col;
     if (aligned) {
         *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(result);
     } else {
@@ -1439,18 +1442,18 @@ int combine_geometry(const orx_function& f, int rows, Geometry* g) {
     g->block[0] = 256;
     return ORX_OK;
 }
-template <typename EXPERT>
+template <typename EXPERT, typename VALUE>
 int combine_rows(const orx_function& f, int rows, const Geometry& g, hipStream_t s, void** args) {
     // dynamic decode has exactly top_k assignments per live row (moe.py:514-517)
     const int slots = f.dynamic_rows ? rows * f.top_k : f.slots;
     const dim3 grid(g.grid[0], g.grid[1]), block(256);
     const EXPERT* const expert = pointer_arg<const EXPERT>(args, 0);
-    __half* const output = pointer_arg<__half>(args, 1);
+    VALUE* const output = pointer_arg<VALUE>(args, 1);
     const float* const prob = pointer_arg<const float>(args, 2);
-    const __half *const shared = pointer_arg<const __half>(args, 3), *const shared_gate = pointer_arg<const __half>(args, 4);
+    const VALUE *const shared = pointer_arg<const VALUE>(args, 3), *const shared_gate = pointer_arg<const VALUE>(args, 4);
     const int* const slot_map = pointer_arg<const int>(args, 5);
-    if (f.H % 8 == 0) ORX_LAUNCH((moe_combine_wide_kernel<EXPERT>), grid, block, 0, s, expert, output, prob, shared, shared_gate, slot_map, f.H, slots, f.top_k);
-    else ORX_LAUNCH((moe_combine_kernel<EXPERT>), grid, block, 0, s, expert, output, prob, shared, shared_gate, slot_map, f.H, slots, f.top_k);
+    if (f.H % 8 == 0) ORX_LAUNCH((moe_combine_wide_kernel<EXPERT, VALUE>), grid, block, 0, s, expert, output, prob, shared, shared_gate, slot_map, f.H, slots, f.top_k);
+    else ORX_LAUNCH((moe_combine_kernel<EXPERT, VALUE>), grid, block, 0, s, expert, output, prob, shared, shared_gate, slot_map, f.H, slots, f.top_k);
     return hip_check(hipGetLastError(), "launch moe_combine");
 }
 int make_combine(const Variant& v, orx_function* f) {
@@ -1458,7 +1461,7 @@ int make_combine(const Variant& v, orx_function* f) {
     bool bad = false;
     f->H = (int)v.integer("H", 0, &bad);
     f->slots = (int)v.integer("slots", f->M * f->top_k, &bad);
-    const std::string expert = v.string("expert_dtype", "float16", &bad);
+    const std::string expert = v.string("expert_dtype", "float16", &bad), output = v.string("output_dtype", "float16", &bad);
     if (bad) return ORX_ERR_BAD_VARIANT;
     if (f->M <= 0 || f->H <= 0 || f->slots <= 0 || f->top_k <= 0) {
         set_error("moe_combine: invalid MoE mixture dimensions");
@@ -1468,14 +1471,20 @@ int make_combine(const Variant& v, orx_function* f) {
         set_error("moe_combine: expert_dtype must be float16 or float32");
         return ORX_ERR_BAD_VARIANT;
     }
-    const bool wide = expert == "float32";
+    const bool wide = expert == "float32", brain = output == "bfloat16";
+    if (output != "float16" && !(brain && wide)) {
+        set_error("moe_combine: output_dtype must be float16, or bfloat16 with expert_dtype=float32");
+        return ORX_ERR_BAD_VARIANT;
+    }
     // Shared / SharedGate may be null device pointers: then no shared expert is added
     f->args = {{"Expert", ArgPointer, wide ? 4u : 2u}, {"Output", ArgPointer, 2},           {"Prob", ArgPointer, 4},
                {"Shared", ArgPointer, 0x80000002u},    {"SharedGate", ArgPointer, 0x80000002u}, {"SlotMap", ArgPointer, 4}};
     if (f->dynamic_rows) f->args.push_back({"m", ArgI32, 4});
     f->geometry = combine_geometry;
-    f->launch = wide ? combine_rows<float> : combine_rows<__half>;
-    f->device_function = wide ? reinterpret_cast<const void*>(&moe_combine_kernel<float>) : reinterpret_cast<const void*>(&moe_combine_kernel<__half>);
+    f->launch = brain ? combine_rows<float, __bf16> : wide ? combine_rows<float, __half> : combine_rows<__half, __half>;
+    f->device_function = brain  ? reinterpret_cast<const void*>(&moe_combine_kernel<float, __bf16>)
+                         : wide ? reinterpret_cast<const void*>(&moe_combine_kernel<float, __half>)
+                                : reinterpret_cast<const void*>(&moe_combine_kernel<__half, __half>);
     return ORX_OK;
 }
 
@@ -1508,7 +1517,7 @@ const Registration* moe_registrations(int* count) {
      "ColdExpert,ColdOffsets,ColdRow,Counts,TileExpert,TileOffsets,TileRow[,m]"},
     {"expert_dispatch", make_dispatch, "M, H, E=512, top_k=10, scale_group=64, dynamic_rows=false, input_dtype=int8|float16 (one scale per row)",
      "A,D,DS,IDs,RelativeSlot,RowOffsets,Scale,SlotMap[,m]"},
-    {"moe_combine", make_combine, "M, H, slots=M*top_k, top_k=10, dynamic_rows=false, expert_dtype=float16|float32",
+    {"moe_combine", make_combine, "M, H, slots=M*top_k, top_k=10, dynamic_rows=false, expert_dtype=float16|float32, output_dtype=float16|bfloat16 (expert_dtype=float32)",
      "Expert,Output,Prob,Shared,SharedGate,SlotMap[,m]"},
     };
     *count = (int)(sizeof(rows) / sizeof(rows[0]));

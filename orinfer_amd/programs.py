@@ -794,14 +794,19 @@ class Mxfp4Linear(_OnDevice):
 
 
 class Mxfp4MoeLayer(_OnDevice):
-    """Routed experts with MXFP4 weights for `tokens` fp16 rows: router, places of the routes, gate | up with SwiGLU, down, weighted sum.
+    """Routed experts with MXFP4 weights for `tokens` rows: router, places of the routes, gate | up with SwiGLU, down, weighted sum.
 
     gate_up (E, 2 I, H / 2) and gate_up_exponents (E, 2 I, H / 32): gate channels, then up channels; down (E, H, I / 2), down_exponents (E, H, I / 32); uint8.
     scoring, bias (E fp32 values added for the choice only), groups, top_groups, group_best, renormalize and scale: the router's (k_router_scores.hip); as they stand here, the softmax router.
+    dtype: of the rows, the shared expert's values, the activations between the two products and the result, torch.float16 or torch.bfloat16.  An activation beyond fp16's 65504 becomes
+    infinite there, its block of 32 NaN and so its token's result: bfloat16 is for layers whose activations leave fp16's range.
     `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own.  They work on the object's buffers: one stream at a time."""
 
     def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, gate_up_exponents, down, down_exponents, *, scoring="softmax", bias=None, groups=1,
-                 top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None):
+                 top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None, dtype=torch.float16):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+        self.dtype = dtype
         self.tokens, self.experts, self.top_k, self.hidden, self.inter = tokens, experts, top_k, hidden, intermediate
         if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden // 2) or tuple(down.shape) != (experts, hidden, intermediate // 2):
             raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden // 2}) and down ({experts}, {hidden}, {intermediate // 2}), "
@@ -820,6 +825,7 @@ class Mxfp4MoeLayer(_OnDevice):
             block_m = 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
         self.block_m = block_m
         capacity = -(-routes // block_m) + min(experts, routes)
+        name = mxfp4.dtype_name(dtype)
         common = dict(M=tokens, E=experts, top_k=top_k)
         scores = dict(scoring=scoring, bias=bias is not None, groups=groups, top_groups=groups if top_groups is None else top_groups, group_best=group_best, scale=scale)
         plain = scoring == "softmax" and bias is None and groups == 1 and top_groups in (None, 1) and scale == 1.0
@@ -827,22 +833,23 @@ class Mxfp4MoeLayer(_OnDevice):
             self.k_router = Kernel("router_topk", renormalize=renormalize, **common, **({} if plain else scores))
             self.k_metadata = Kernel("route_metadata", block_m=block_m, slot_maps=True, workspace=True, tile_units=True, **common)
             grouped = dict(rows=routes, E=experts, tiles=capacity, block_m=block_m)
-            self.k_quantise_tokens = Kernel("mxfp4_quantization", M=tokens, K=hidden, pad=mxfp4.STEP)
-            up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", **grouped)
+            self.k_quantise_tokens = Kernel("mxfp4_quantization", M=tokens, K=hidden, input_dtype=name, pad=mxfp4.STEP)
+            up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", output_dtype=name, **grouped)
             self.k_up = Kernel("mxfp4_grouped", **up)
-            self.k_quantise_act = Kernel("mxfp4_quantization", M=routes, K=intermediate, pad=mxfp4.STEP)
+            self.k_quantise_act = Kernel("mxfp4_quantization", M=routes, K=intermediate, input_dtype=name, pad=mxfp4.STEP)
             # (The second products stay fp32 until they are weighted and summed: as fp16, one beyond 65504 made its token's sum infinite or NaN however small its weight, and each was
             # a rounding more.  Its price, 128 experts x 8 of 2048 x 512, us of place and down with fp16 / fp32: 256 tokens 25.7 / 29.2, 4096 tokens 105.6 / 158.8.)
             down = dict(N=hidden, K=intermediate, output_dtype="float32", **grouped)
             self.k_down = Kernel("mxfp4_grouped", **down)
-            # A route to an expert or less: the products quantise their rows themselves, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
+            # A route to an expert or less: the products quantise their rows themselves where these are fp16, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
             # 7.6 / 6.0 and down 5.1 / 4.4, 8 tokens 9.7 / 8.5 and 7.4 / 7.3, 16 tokens 10.7 / 10.7 and 8.9 / 10.3; 16 x 2 of 4096 x 1536, 8 tokens, 10.7 / 9.9 and 7.9 / 6.6).
-            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if block_m == 16 and routes <= experts else None
-            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if block_m == 16 and 4 * routes <= 3 * experts else None
-            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, expert_dtype="float32", **common)
+            few = block_m == 16 and dtype == torch.float16
+            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if few and routes <= experts else None
+            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if few and 4 * routes <= 3 * experts else None
+            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, expert_dtype="float32", output_dtype=name, **common)
             self.segments = self.k_metadata.workspace()
         i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)
-        f16 = dict(dtype=torch.float16, device=self.device)
+        values = dict(dtype=dtype, device=self.device)
         self.ids = torch.empty((tokens, top_k), **i32)
         self.prob = torch.empty((tokens, top_k), dtype=torch.float32, device=self.device)
         self.counts, self.row_offsets, self.tile_offsets = (torch.empty(experts, **i32) for _ in range(3))
@@ -853,9 +860,9 @@ class Mxfp4MoeLayer(_OnDevice):
         wide, inner = mxfp4.padded(hidden), mxfp4.padded(intermediate)
         self.a_q, self.a_s = torch.empty((tokens, wide // 2), **u8), torch.empty((tokens, wide // 32), **u8)
         self.h_q, self.h_s = torch.empty((routes, inner // 2), **u8), torch.empty((routes, inner // 32), **u8)
-        self.act = torch.empty((routes, intermediate), **f16)
+        self.act = torch.empty((routes, intermediate), **values)
         self.down_out = torch.empty((routes, hidden), dtype=torch.float32, device=self.device)
-        self.out = torch.empty((tokens, hidden), **f16)
+        self.out = torch.empty((tokens, hidden), **values)
 
     def route(self, logits, stream=None):
         """fp32 logits (tokens, experts) -> the routes' experts (tokens, top_k) int32 and weights fp32."""
@@ -879,8 +886,8 @@ class Mxfp4MoeLayer(_OnDevice):
                         TileUnits=self.tile_units, Workspace=self.segments)
 
     def up(self, x, stream=None):
-        """fp16 rows (tokens, hidden) -> silu(gate) * up of every route, fp16 (tokens * top_k, intermediate) in the order of the slots."""
-        _check_rows(x, self.tokens, self.hidden, torch.float16, self.device, "x")
+        """Rows (tokens, hidden) -> silu(gate) * up of every route, (tokens * top_k, intermediate) in the order of the slots, of the layer's dtype both."""
+        _check_rows(x, self.tokens, self.hidden, self.dtype, self.device, "x")
         self._call(self._up, x, stream=stream)
         return self.act
 
@@ -892,15 +899,15 @@ class Mxfp4MoeLayer(_OnDevice):
         self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
 
     def down(self, act, prob, shared=None, shared_gate=None, stream=None):
-        """fp16 rows in the order of the slots and fp32 weights (tokens, top_k) -> fp16 (tokens, hidden): the weighted sum, in fp32, of the routes' second products and, where they
-        are given, of sigmoid(shared_gate) (tokens) times shared (tokens, hidden), fp16 both."""
-        _check_rows(act, self.assignments, self.inter, torch.float16, self.device, "act")
+        """Rows in the order of the slots and fp32 weights (tokens, top_k) -> (tokens, hidden): the weighted sum, in fp32, of the routes' second products and, where they are given,
+        of sigmoid(shared_gate) (tokens) times shared (tokens, hidden); rows, result and these two of the layer's dtype."""
+        _check_rows(act, self.assignments, self.inter, self.dtype, self.device, "act")
         _check_rows(prob, self.tokens, self.top_k, torch.float32, self.device, "prob")
         if (shared is None) != (shared_gate is None):
             raise ValueError("shared and shared_gate go together")
         if shared is not None:
-            _check_rows(shared, self.tokens, self.hidden, torch.float16, self.device, "shared")
-            _check_rows(shared_gate.view(-1, 1), self.tokens, 1, torch.float16, self.device, "shared_gate")
+            _check_rows(shared, self.tokens, self.hidden, self.dtype, self.device, "shared")
+            _check_rows(shared_gate.view(-1, 1), self.tokens, 1, self.dtype, self.device, "shared_gate")
         self._call(self._down, act, prob, shared, shared_gate, stream=stream)
         return self.out
 

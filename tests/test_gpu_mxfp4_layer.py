@@ -122,3 +122,118 @@ def test_a_linear_of_its_own_result(rows):
         once = linear.run(x).clone()
         want, bound = product(orc.values(*orc.quantise(once.double().cpu().numpy())), w)
         check(linear.run(linear.run(x)), want, bound, torch.float16)
+
+
+def layer_case(tokens, experts, top_k, hidden, inner, dtype, powers=(113, 118), **options):
+    rng = np.random.default_rng(tokens * 31 + experts)
+    gate_up, down = weights(rng, experts, 2 * inner, hidden, low=powers[0], high=powers[1]), weights(rng, experts, hidden, inner)
+    options["block_m"] = options.get("block_m")
+    layer = programs.Mxfp4MoeLayer(tokens, experts, top_k, hidden, inner, *map(dev, gate_up), *map(dev, down), dtype=dtype, **options)
+    x, shared = rows_of(rng, tokens, hidden, dtype).to(DEV), rows_of(rng, tokens, hidden, dtype).to(DEV)
+    gate = torch.from_numpy(rng.standard_normal(tokens) * 2).to(dtype).to(DEV)
+    logits = (rng.standard_normal((tokens, experts)) * 2).astype(np.float32)
+    return layer, gate_up, down, x, logits, shared, gate
+
+
+def check_run(layer, gate_up, down, x, logits, shared, gate, routing):
+    """`run` step by step: routes and weights, activations from the rows, the result from the activations as the device left them."""
+    got = layer.run(x, dev(logits), shared, gate)
+    scale = {"scale": float(np.float32(routing["scale"]))} if "scale" in routing else {}
+    ids, prob = orc.routes(logits, layer.top_k, **dict(routing, **scale))
+    np.testing.assert_array_equal(host(layer.ids), ids)
+    np.testing.assert_allclose(host(layer.prob), prob, rtol=2e-6 if not routing else 2.0**-23, atol=2.0**-149)
+    order, slot = slots_of(ids)
+    np.testing.assert_array_equal(host(layer.slot_map), slot)
+    chosen, inner = ids.reshape(-1)[order], layer.inter
+    a = orc.values(*orc.quantise(x.double().cpu().numpy()))[order // layer.top_k]
+    want, bound = np.empty((order.size, inner)), np.empty((order.size, inner))
+    for e in np.unique(chosen):
+        at = chosen == e
+        w = orc.values(gate_up[0][e], gate_up[1][e])
+        (g, dg), (up, du) = product(a[at], w[:inner]), product(a[at], w[inner:])
+        with np.errstate(over="ignore"):
+            want[at] = orc.silu(g) * up
+        bound[at] = 1.1 * dg * (np.abs(up) + du) + np.abs(g) * du + 8 * 2.0**-24 * np.abs(want[at])
+    check(layer.act, want, bound, layer.dtype)
+    assert torch.isfinite(layer.act).all()
+    y, dy = second_products(layer.act, chosen, down)
+    check(got, *weighted(y, dy, slot, host(layer.prob), shared, gate), layer.dtype)
+    return want
+
+
+ROUTINGS = [{}, dict(scoring="sigmoid", scale=2.5), dict(scoring="sigmoid", groups=8, top_groups=3, group_best=1), dict(scoring="softmax", groups=4, top_groups=2, renormalize=False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("routing", range(4))
+@pytest.mark.parametrize("tokens,experts,top_k,hidden,inner", [(1, 8, 2, 64, 32), (3, 128, 8, 512, 96), (48, 64, 6, 512, 160), (300, 16, 4, 288, 544), (1100, 8, 3, 256, 128)])
+def test_a_whole_layer_with_and_without_a_shared_expert(tokens, experts, top_k, hidden, inner, routing, dtype):
+    routing = dict(ROUTINGS[routing])
+    if routing:
+        routing["bias"] = np.linspace(-0.1, 0.1, experts).astype(np.float32)[::-1].copy()
+    case = layer_case(tokens, experts, top_k, hidden, inner, dtype, **routing)
+    check_run(*case, routing)
+    check_run(*case[:5], None, None, routing)
+
+
+@pytest.mark.parametrize("block_m", [16, 64, 128, 256])
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_bf16_experts_in_units_of_every_size(tokens, block_m):
+    case = layer_case(tokens, 8, 3, 320, 224, torch.bfloat16, block_m=block_m)
+    check_run(*case, {})
+
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(2, 64, 8), (40, 16, 4), (300, 4, 2), (700, 2, 1)])
+def test_activations_outside_fp16(tokens, experts, top_k):
+    """Activations beyond 65504, which fp16 cannot hold, and results of the same layer."""
+    case = layer_case(tokens, experts, top_k, 256, 96, torch.bfloat16, powers=(131, 136))
+    act = check_run(*case, {})
+    assert (np.abs(act) > 65520).mean() > 0.05
+    # the layer's own parts and a graph of it give the same
+    layer, _, _, x, logits, shared, gate = case
+    logits = dev(logits)
+    eager = layer.run(x, logits, shared, gate).clone()
+    ids, prob = layer.route(logits)
+    layer.place(ids)
+    assert torch.equal(layer.down(layer.up(x), prob, shared, gate), eager)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        out = layer.run(x, logits, shared, gate)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        x.neg_()
+        logits.copy_(logits.roll(1, 1))
+        torch.cuda.synchronize()
+        eager = layer.run(x, logits, shared, gate).clone()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("h", [8, 100, 2056])
+def test_sums_in_bf16(h):
+    rng = np.random.default_rng(h)
+    m, top_k, slots = 9, 6, 40
+    expert = (rng.standard_normal((slots, h)) * 1e6).astype(np.float32)
+    slot, prob = rng.integers(0, slots, (m, top_k)).astype(np.int32), rng.random((m, top_k)).astype(np.float32)
+    shared, gate = torch.from_numpy(rng.standard_normal((m, h)) * 1e5).bfloat16().to(DEV), torch.from_numpy(rng.standard_normal(m)).bfloat16().to(DEV)
+    for more in ((None, None), (shared, gate)):
+        for offset in (0, 1):
+            out = torch.full((m * h + 9,), -7.0, dtype=torch.bfloat16, device=DEV)
+            got = out[offset:offset + m * h].view(m, h)
+            kernel("moe_combine", M=m, H=h, slots=slots, top_k=top_k, expert_dtype="float32", output_dtype="bfloat16")(
+                Expert=dev(expert), Output=got, Prob=dev(prob), Shared=more[0], SharedGate=more[1], SlotMap=dev(slot))
+            y = expert.astype(np.float64)
+            check(got, *weighted(y, np.zeros_like(y), slot, prob, *more), torch.bfloat16)
+            assert (out[:offset] == -7).all() and (out[offset + m * h:] == -7).all()
+
+
+def test_a_layer_refuses_values_of_another_type():
+    layer, _, _, x, logits, shared, gate = layer_case(4, 8, 2, 64, 32, torch.bfloat16)
+    logits = dev(logits)
+    _, prob = layer.route(logits)
+    for call in (lambda: layer.up(x.half()), lambda: layer.down(layer.act.half(), prob), lambda: layer.down(layer.act, prob, shared.half(), gate),
+                 lambda: layer.down(layer.act, prob, shared, gate.half()), lambda: layer.run(x.float(), logits)):
+        with pytest.raises(ValueError):
+            call()

@@ -102,3 +102,21 @@ def test_rows_in_the_buffer_that_a_launch_writes_are_quantised_before_it():
         layer = object.__new__(programs.Mxfp4MoeLayer)
         vars(layer).update(tokens=len(x), few_up="kernel", k_quantise_tokens="kernel", k_up="kernel", act=out, a_q=None, a_s=None, slot_token=None, tile_count=None, tile_units=None, w1=None, p1=None)
         assert launches(layer, "_up", x) == want
+
+
+def test_layers_are_of_fp16_or_bf16(gpus):
+    arguments = [3, 4, 2, 96, 64, *weights("cuda:0", 4, 128, 96), *weights("cuda:0", 4, 96, 64)]
+    for dtype in (torch.float16, torch.bfloat16):
+        layer = programs.Mxfp4MoeLayer(*arguments, dtype=dtype)
+        assert layer.act.dtype == layer.out.dtype == dtype and layer.down_out.dtype == torch.float32
+    with pytest.raises(ValueError):
+        programs.Mxfp4MoeLayer(*arguments, dtype=torch.float32)
+
+
+def test_weighted_sums_are_fp16_or_bf16():
+    plain, brain = (lib.Kernel("moe_combine", **COMBINE, expert_dtype="float32", output_dtype=name) for name in ("float16", "bfloat16"))
+    assert brain.arg_names == plain.arg_names and brain.geometry() == plain.geometry()
+    for bad in (dict(output_dtype="bfloat16"), dict(output_dtype="float32"), dict(expert_dtype="float32", output_dtype="float32")):
+        with pytest.raises(lib.OrxError) as error:
+            lib.Kernel("moe_combine", **COMBINE, **bad)
+        assert error.value.code == lib.ORX_ERR_BAD_VARIANT and "output_dtype" in str(error.value)
