@@ -828,7 +828,7 @@ class Mxfp4MoeLayer(_OnDevice):
         name = mxfp4.dtype_name(dtype)
         common = dict(M=tokens, E=experts, top_k=top_k)
         scores = dict(scoring=scoring, bias=bias is not None, groups=groups, top_groups=groups if top_groups is None else top_groups, group_best=group_best, scale=scale)
-        plain = scoring == "softmax" and bias is None and groups == 1 and top_groups in (None, 1) and scale == 1.0
+        plain = scoring == "softmax" and bias is None and groups == 1 and top_groups in (None, 1) and group_best in (1, 2) and scale == 1.0
         with torch.cuda.device(self.device):
             self.k_router = Kernel("router_topk", renormalize=renormalize, **common, **({} if plain else scores))
             self.k_metadata = Kernel("route_metadata", block_m=block_m, slot_maps=True, workspace=True, tile_units=True, **common)

@@ -120,3 +120,10 @@ def test_weighted_sums_are_fp16_or_bf16():
         with pytest.raises(lib.OrxError) as error:
             lib.Kernel("moe_combine", **COMBINE, **bad)
         assert error.value.code == lib.ORX_ERR_BAD_VARIANT and "output_dtype" in str(error.value)
+
+
+@pytest.mark.parametrize("options", [dict(group_best=3), dict(group_best=0), dict(groups=2, group_best=3), dict(top_groups=2), dict(scoring="relu"), dict(scale=0.0), dict(block_m=32)])
+def test_layers_refuse_routing_that_is_not_served(gpus, options):
+    with pytest.raises(lib.OrxError) as error:
+        programs.Mxfp4MoeLayer(3, 4, 2, 96, 64, *weights("cuda:0", 4, 128, 96), *weights("cuda:0", 4, 96, 64), **options)
+    assert error.value.code == lib.ORX_ERR_BAD_VARIANT
