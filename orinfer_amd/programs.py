@@ -800,7 +800,7 @@ class Mxfp4MoeLayer(_OnDevice):
     scoring, bias (E fp32 values added for the choice only), groups, top_groups, group_best, renormalize and scale: the router's (k_router_scores.hip); as they stand here, the softmax router.
     dtype: of the rows, the shared expert's values, the activations between the two products and the result, torch.float16 or torch.bfloat16.  An activation beyond fp16's 65504 becomes
     infinite there, its block of 32 NaN and so its token's result: bfloat16 is for layers whose activations leave fp16's range.
-    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own.  They work on the object's buffers: one stream at a time."""
+    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own (`place` before `up` and `down`).  They work on the object's buffers: one stream at a time."""
 
     def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, gate_up_exponents, down, down_exponents, *, scoring="softmax", bias=None, groups=1,
                  top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None, dtype=torch.float16):
@@ -855,7 +855,10 @@ class Mxfp4MoeLayer(_OnDevice):
         self.counts, self.row_offsets, self.tile_offsets = (torch.empty(experts, **i32) for _ in range(3))
         self.relative, self.slot_map = torch.empty((tokens, top_k), **i32), torch.empty((tokens, top_k), **i32)
         self.slot_token = torch.empty(routes, **i32)
-        self.tile_count = torch.empty(1, **i32)
+        # (no units until a launch has listed them, not even for work that has passed `place` by and not waited for it)
+        self.tile_count = torch.zeros(1, **i32)
+        self.slot_map.fill_(-1)
+        self.placed = False
         self.tile_expert, self.tile_row, self.tile_units = torch.empty(capacity, **i32), torch.empty(capacity, **i32), torch.empty((capacity, 4), **i32)
         wide, inner = mxfp4.padded(hidden), mxfp4.padded(intermediate)
         self.a_q, self.a_s = torch.empty((tokens, wide // 2), **u8), torch.empty((tokens, wide // 32), **u8)
@@ -878,7 +881,12 @@ class Mxfp4MoeLayer(_OnDevice):
         """Experts of every token's routes, int32 in [0, experts) -> the order of the slots: by expert, then by token (`slot_map`, `slot_token`)."""
         _check_rows(ids, self.tokens, self.top_k, torch.int32, self.device, "ids")
         self._call(self._place, ids, stream=stream)
+        self.placed = True
         return self.slot_map
+
+    def _check_placed(self):
+        if not self.placed:
+            raise RuntimeError("the routes have no places yet: `place` comes before `up` and `down`")
 
     def _place(self, ids, stream):
         self.k_metadata(stream=stream, Counts=self.counts, IDs=ids, RelativeSlot=self.relative, RowMax=None, RowOffsets=self.row_offsets, SlotMap=self.slot_map,
@@ -888,6 +896,7 @@ class Mxfp4MoeLayer(_OnDevice):
     def up(self, x, stream=None):
         """Rows (tokens, hidden) -> silu(gate) * up of every route, (tokens * top_k, intermediate) in the order of the slots, of the layer's dtype both."""
         _check_rows(x, self.tokens, self.hidden, self.dtype, self.device, "x")
+        self._check_placed()
         self._call(self._up, x, stream=stream)
         return self.act
 
@@ -908,6 +917,7 @@ class Mxfp4MoeLayer(_OnDevice):
         if shared is not None:
             _check_rows(shared, self.tokens, self.hidden, self.dtype, self.device, "shared")
             _check_rows(shared_gate.view(-1, 1), self.tokens, 1, self.dtype, self.device, "shared_gate")
+        self._check_placed()
         self._call(self._down, act, prob, shared, shared_gate, stream=stream)
         return self.out
 

@@ -237,3 +237,8 @@ def test_a_layer_refuses_values_of_another_type():
                  lambda: layer.down(layer.act, prob, shared, gate.half()), lambda: layer.run(x.float(), logits)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_a_new_layer_lists_nothing():
+    layer, *_ = layer_case(4, 8, 2, 64, 32, torch.float16)
+    assert layer.tile_count.tolist() == [0] and (layer.slot_map == -1).all()

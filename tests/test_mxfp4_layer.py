@@ -127,3 +127,12 @@ def test_layers_refuse_routing_that_is_not_served(gpus, options):
     with pytest.raises(lib.OrxError) as error:
         programs.Mxfp4MoeLayer(3, 4, 2, 96, 64, *weights("cuda:0", 4, 128, 96), *weights("cuda:0", 4, 96, 64), **options)
     assert error.value.code == lib.ORX_ERR_BAD_VARIANT
+
+
+def test_experts_have_no_rows_before_they_have_places(gpus):
+    """Lists that no launch has written would send the products anywhere."""
+    layer = programs.Mxfp4MoeLayer(3, 4, 2, 96, 64, *weights("cuda:0", 4, 128, 96), *weights("cuda:0", 4, 96, 64))
+    x = torch.empty((3, 96), dtype=torch.float16, device="cuda:0")
+    for call in (lambda: layer.up(x), lambda: layer.down(layer.act, layer.prob)):
+        with pytest.raises(RuntimeError, match="place"):
+            call()
