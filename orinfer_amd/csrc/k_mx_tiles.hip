@@ -9,8 +9,10 @@
 // LOOK: quarters of a step that operands are read ahead, two where the registers hold them (128 x 128: 333 rows 17.6 / 17.9, experts of 2048 x 512 70.2 / 74.0).
 //
 // v_mfma_scale_f32_32x32x64 takes 32 cycles, 16 x 16 x 128 18, so the former: 6.2 PFLOP/s on random codes straight from registers, 5.4 the latter.  The multipliers do not run out of
-// work there, the chip runs into its power: 1.5 GHz with random codes, 2.35 with zeros (9.6 PFLOP/s).  With operands from LDS and requests the step of a 256 x 256 tile takes
-// 1.6-1.75 us on all CUs, 4.9-5.2 PFLOP/s; what is left is the start of a launch and the results.  8192 x 4096 x 4096 75 us (3.65 PFLOP/s), 8192 x 17408 x 5120 410 us (3.55).
+// work there, the chip runs into its power: 1.5 GHz with random codes, 2.35 with zeros (9.6 PFLOP/s).  The account of 8192 x 17408 x 5120, 2176 tiles of 256 x 256, eight or nine to a CU,
+// by the time at each tile's steps and results in a launch of 377 us: 1.9 before the first step, 33.0 for the first tile's 20 steps (1.65 each), 39.3 for those of each later tile (1.95; with
+// all CUs at it, 4.4 PFLOP/s, and taken for power, which was not measured apart), 2.7 for the results of each; the CUs with eight tiles end 41 before the others.  Launches behind one another take
+// 360-395 (3.7-4.05 PFLOP/s).  8192 x 4096 x 4096, two tiles to a CU: 1.4, then 16 steps of 1.6-1.8 and 2-3 of results each, all ended at 62-71, the launch 66-76 (3.6-4.15).
 // A 128 x 128 step alone on a CU takes 0.5-0.65 us, 0.3 without its requests, 0.15 without its multiplies either.
 // Tried: four waves of 128 x 128 results (a third less from LDS, 1.63 us a step, but sums come out of accumulation registers by moves, 4.4-6.2 us a tile against 2.1: the same in
 // all); results by lines of 128 bytes through LDS (more instructions, and not faster: what a tile's end took was its instructions); three to six stages, a CU then holding one workgroup

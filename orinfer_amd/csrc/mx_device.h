@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 }
 
 // Eight codes of one block, rounded to nearest, ties to the even code, saturating: the conversion instruction divides by the power of the scale's exponent
-// field, also by 2^-127 where that is zero (it agrees with the rule for every fp16 and bf16 value and powers of 2^-127 to 2^127).
+// field, also by 2^-127 where that is zero (it agrees with the rule for every fp16 and bf16 value, fp32 values of every exponent, and every power that power_byte gives).
 template <int TYPE>
 __device__ __forceinline__ uint32_t eight_codes(const uint32_t* words, uint32_t byte) {
     typedef _Float16 half2v __attribute__((ext_vector_type(2)));

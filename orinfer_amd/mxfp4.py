@@ -55,7 +55,7 @@ def quantize(x, scale="floor", pad=BLOCK):
 
 
 def dequantize(codes, exponents, k, dtype=torch.float16, pad=BLOCK):
-    """What codes and exponents stand for, (..., k) of `dtype` (exact in bf16 and fp32; fp16 rounds what it cannot hold)."""
+    """What codes and exponents stand for, (..., k) of `dtype` (exact in bf16 and fp32, infinite above their range, which bytes 253 and 254 reach; fp16 rounds what it cannot hold)."""
     if not codes.is_cuda or codes.device != exponents.device:
         raise ValueError("dequantize takes two tensors on one GPU")
     if (codes.dtype != torch.uint8 or exponents.dtype != torch.uint8 or codes.shape[-1] != padded(k, pad) // 2 or exponents.shape[-1] != padded(k, pad) // BLOCK
