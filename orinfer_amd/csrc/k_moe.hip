@@ -765,6 +765,10 @@ __device__ __forceinline__ float value_of(float v) { return v; }
 __device__ __forceinline__ void round_to(__half& to, float v) { to = __float2half_rn(v); }
 __device__ __forceinline__ void round_to(__bf16& to, float v) { to = (__bf16)v; }
 
+// A route of weight 0 (an expert that a bias closed, chosen for want of others) counts nothing, whatever its row holds; with fp16 rows its product is added as the reference does.
+template <typename EXPERT>
+__device__ __forceinline__ bool counts(float weight) { return std::is_same_v<EXPERT, __half> || weight != 0.f; }
+
 // grid (M, ceil(H/256)): fp32 accumulate in rank order, one cast.  EXPERT: the experts' rows, __half or float; VALUE: the result and the shared expert's, __half or __bf16.
 template <typename EXPERT, typename VALUE>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const EXPERT* __restrict__ expert, VALUE* __restrict__ output,
@@ -777,8 +781,9 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const EXPERT* __restri
     float acc = 0.f;
     for (int rank = 0; rank < top_k; ++rank) {
         const int slot = slot_map[(int64_t)row * top_k + rank];
-        if (slot >= 0 && slot < slots)
-            acc += value_of(expert[(int64_t)slot * h + col]) * prob[(int64_t)row * top_k + rank];
+        const float weight = prob[(int64_t)row * top_k + rank];
+        if (slot >= 0 && slot < slots && counts<EXPERT>(weight))
+            acc += value_of(expert[(int64_t)slot * h + col]) * weight;
     }
     if (shared != nullptr) {
         const float gate = __fdiv_rn(1.0f, 1.0f + expf(-value_of(shared_gate[row])));
@@ -832,7 +837,7 @@ __global__ __launch_bounds__(256) void moe_combine_wide_kernel(const EXPERT* __r
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool valid = first + i < top_k && slot[i] >= 0 && slot[i] < slots;
+            const bool valid = first + i < top_k && slot[i] >= 0 && slot[i] < slots && counts<EXPERT>(weight[i]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float sum = acc[j] + value_of(values[i][j]) * weight[i];

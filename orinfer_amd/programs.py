@@ -908,7 +908,7 @@ class Mxfp4MoeLayer(_OnDevice):
         self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
 
     def down(self, act, prob, shared=None, shared_gate=None, stream=None):
-        """Rows in the order of the slots and fp32 weights (tokens, top_k) -> (tokens, hidden): the weighted sum, in fp32, of the routes' second products and, where they are given,
+        """Rows in the order of the slots and fp32 weights (tokens, top_k) -> (tokens, hidden): the weighted sum, in fp32, of the routes' second products (those of weight 0 count nothing) and, where they are given,
         of sigmoid(shared_gate) (tokens) times shared (tokens, hidden); rows, result and these two of the layer's dtype."""
         _check_rows(act, self.assignments, self.inter, self.dtype, self.device, "act")
         _check_rows(prob, self.tokens, self.top_k, torch.float32, self.device, "prob")

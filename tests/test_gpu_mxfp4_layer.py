@@ -242,3 +242,38 @@ def test_a_layer_refuses_values_of_another_type():
 def test_a_new_layer_lists_nothing():
     layer, *_ = layer_case(4, 8, 2, 64, 32, torch.float16)
     assert layer.tile_count.tolist() == [0] and (layer.slot_map == -1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens,experts,top_k", [(2, 16, 6), (50, 16, 6), (300, 16, 10)])
+def test_closed_experts_of_nan_weights_count_nothing(tokens, experts, top_k, dtype):
+    """A bias closes all experts but four, whose weights are numbers; the others' are not, and they fill up the routes."""
+    bias = np.zeros(experts, np.float32)
+    bias[4:] = -np.inf
+    rng = np.random.default_rng(tokens)
+    gate_up, down = weights(rng, experts, 512, 256, low=113, high=118), weights(rng, experts, 256, 256)
+    gate_up[1][4:10], down[1][10:] = 255, 255
+    layer = programs.Mxfp4MoeLayer(tokens, experts, top_k, 256, 256, *map(dev, gate_up), *map(dev, down), scoring="sigmoid", bias=bias, dtype=dtype)
+    x, logits = rows_of(rng, tokens, 256, dtype).to(DEV), rng.standard_normal((tokens, experts)).astype(np.float32)
+    got = layer.run(x, dev(logits))
+    ids, _ = orc.routes(logits, top_k, scoring="sigmoid", bias=bias)
+    np.testing.assert_array_equal(host(layer.ids), ids)
+    prob = host(layer.prob)
+    assert (prob[:, 4:] == 0).all() and (prob[:, :4] > 0).all()
+    order, slot = slots_of(ids)
+    chosen = ids.reshape(-1)[order]
+    act = layer.act.clone()
+    act[torch.from_numpy(chosen >= 4).to(DEV)] = 0
+    numbers = down[0], np.where(np.arange(experts)[:, None, None] < 4, down[1], 0).astype(np.uint8)
+    check(got, *weighted(*second_products(act, chosen, numbers), slot, prob), dtype)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("h", [64, 100])
+def test_sums_without_the_rows_of_weight_0(h):
+    expert = torch.full((6, h), float("nan"), device=DEV)
+    expert[1], expert[4] = float("inf"), 3.0
+    out = torch.empty((2, h), dtype=torch.float16, device=DEV)
+    slot, prob = dev(np.array([[0, 1, 4], [2, 3, 5]], np.int32)), dev(np.array([[0, 0, 0.5], [0, 0, -0.0]], np.float32))
+    kernel("moe_combine", M=2, H=h, slots=6, top_k=3, expert_dtype="float32")(Expert=expert, Output=out, Prob=prob, Shared=None, SharedGate=None, SlotMap=slot)
+    assert (out[0] == 1.5).all() and (out[1] == 0).all()
