@@ -284,7 +284,7 @@ struct Table {
     const Registration* rows;
     int count;
 };
-constexpr int kTables = 6;
+constexpr int kTables = 7;
 void tables(Table out[kTables]) {
     out[0].rows = quant_registrations(&out[0].count);
     out[1].rows = gemv_registrations(&out[1].count);
@@ -292,6 +292,7 @@ void tables(Table out[kTables]) {
     out[3].rows = moe_registrations(&out[3].count);
     out[4].rows = plane_registrations(&out[4].count);
     out[5].rows = mx_registrations(&out[5].count);
+    out[6].rows = byte_registrations(&out[6].count);
 }
 const Registration* find(const char* symbol) {
     Table t[kTables];

@@ -140,6 +140,7 @@ const Registration* gemm_registrations(int* count);
 const Registration* moe_registrations(int* count);
 const Registration* plane_registrations(int* count);
 const Registration* mx_registrations(int* count);
+const Registration* byte_registrations(int* count);
 int make_router_scores(const Variant& v, bool renormalize, orx_function* f);
 
 template <typename T>

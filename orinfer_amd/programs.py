@@ -12,7 +12,7 @@ import math
 import numpy as np
 import torch
 
-from . import codebook, mxfp4
+from . import byte_tiles, codebook, int8, mxfp4
 from .lib import ORX_ERR_BAD_VARIANT, Kernel, OrxError, current_stream
 
 
@@ -793,63 +793,30 @@ class Mxfp4Linear(_OnDevice):
         self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, WS=self.powers, m=rows)
 
 
-class Mxfp4MoeLayer(_OnDevice):
-    """Routed experts with MXFP4 weights for `tokens` rows: router, places of the routes, gate | up with SwiGLU, down, weighted sum.
+class _ExpertLayer(_OnDevice):
+    """What layers of routed experts have in common: the router, the places of the routes, the weighted sum, and the buffers of all of these."""
 
-    gate_up (E, 2 I, H / 2) and gate_up_exponents (E, 2 I, H / 32): gate channels, then up channels; down (E, H, I / 2), down_exponents (E, H, I / 32); uint8.
-    scoring, bias (E fp32 values added for the choice only), groups, top_groups, group_best, renormalize and scale: the router's (k_router_scores.hip); as they stand here, the softmax router.
-    dtype: of the rows, the shared expert's values, the activations between the two products and the result, torch.float16 or torch.bfloat16.  An activation beyond fp16's 65504 becomes
-    infinite there, its block of 32 NaN and so its token's result: bfloat16 is for layers whose activations leave fp16's range.
-    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own (`place` before `up` and `down`).  They work on the object's buffers: one stream at a time."""
-
-    def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, gate_up_exponents, down, down_exponents, *, scoring="softmax", bias=None, groups=1,
-                 top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None, dtype=torch.float16):
-        if dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+    def _set_up(self, tokens, experts, top_k, hidden, intermediate, dtype, block_m, *, scoring, bias, groups, top_groups, group_best, renormalize, scale):
+        """Kernels and buffers, with the layer's GPU in `device`."""
         self.dtype = dtype
         self.tokens, self.experts, self.top_k, self.hidden, self.inter = tokens, experts, top_k, hidden, intermediate
-        if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden // 2) or tuple(down.shape) != (experts, hidden, intermediate // 2):
-            raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden // 2}) and down ({experts}, {hidden}, {intermediate // 2}), "
-                             f"not {tuple(gate_up.shape)} and {tuple(down.shape)}")
-        weights = tuple(map(torch.as_tensor, (gate_up, gate_up_exponents, down, down_exponents)))
-        self.device = self._device_of(*weights)
-        self.w1, self.p1 = (t.to(self.device) for t in mxfp4.tiles(*weights[:2], paired=True))
-        self.w2, self.p2 = (t.to(self.device) for t in mxfp4.tiles(*weights[2:]))
         self.bias = None
         if bias is not None:
             self.bias = torch.as_tensor(bias, dtype=torch.float32).to(self.device).contiguous()
             if self.bias.shape != (experts,):
                 raise ValueError(f"bias must have {experts} values")
         routes = self.assignments = tokens * top_k
-        if block_m is None:
-            block_m = 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
         self.block_m = block_m
         capacity = -(-routes // block_m) + min(experts, routes)
-        name = mxfp4.dtype_name(dtype)
         common = dict(M=tokens, E=experts, top_k=top_k)
         scores = dict(scoring=scoring, bias=bias is not None, groups=groups, top_groups=groups if top_groups is None else top_groups, group_best=group_best, scale=scale)
         plain = scoring == "softmax" and bias is None and groups == 1 and top_groups in (None, 1) and group_best in (1, 2) and scale == 1.0
         with torch.cuda.device(self.device):
             self.k_router = Kernel("router_topk", renormalize=renormalize, **common, **({} if plain else scores))
             self.k_metadata = Kernel("route_metadata", block_m=block_m, slot_maps=True, workspace=True, tile_units=True, **common)
-            grouped = dict(rows=routes, E=experts, tiles=capacity, block_m=block_m)
-            self.k_quantise_tokens = Kernel("mxfp4_quantization", M=tokens, K=hidden, input_dtype=name, pad=mxfp4.STEP)
-            up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", output_dtype=name, **grouped)
-            self.k_up = Kernel("mxfp4_grouped", **up)
-            self.k_quantise_act = Kernel("mxfp4_quantization", M=routes, K=intermediate, input_dtype=name, pad=mxfp4.STEP)
-            # (The second products stay fp32 until they are weighted and summed: as fp16, one beyond 65504 made its token's sum infinite or NaN however small its weight, and each was
-            # a rounding more.  Its price, 128 experts x 8 of 2048 x 512, us of place and down with fp16 / fp32: 256 tokens 25.7 / 29.2, 4096 tokens 105.6 / 158.8.)
-            down = dict(N=hidden, K=intermediate, output_dtype="float32", **grouped)
-            self.k_down = Kernel("mxfp4_grouped", **down)
-            # A route to an expert or less: the products quantise their rows themselves where these are fp16, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
-            # 7.6 / 6.0 and down 5.1 / 4.4, 8 tokens 9.7 / 8.5 and 7.4 / 7.3, 16 tokens 10.7 / 10.7 and 8.9 / 10.3; 16 x 2 of 4096 x 1536, 8 tokens, 10.7 / 9.9 and 7.9 / 6.6).
-            few = block_m == 16 and dtype == torch.float16
-            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if few and routes <= experts else None
-            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if few and 4 * routes <= 3 * experts else None
-            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, expert_dtype="float32", output_dtype=name, **common)
+            self.k_combine = Kernel("moe_combine", H=hidden, slots=routes, expert_dtype="float32", output_dtype=mxfp4.dtype_name(dtype), **common)
             self.segments = self.k_metadata.workspace()
-        i32, u8 = dict(dtype=torch.int32, device=self.device), dict(dtype=torch.uint8, device=self.device)
-        values = dict(dtype=dtype, device=self.device)
+        i32, values = dict(dtype=torch.int32, device=self.device), dict(dtype=dtype, device=self.device)
         self.ids = torch.empty((tokens, top_k), **i32)
         self.prob = torch.empty((tokens, top_k), dtype=torch.float32, device=self.device)
         self.counts, self.row_offsets, self.tile_offsets = (torch.empty(experts, **i32) for _ in range(3))
@@ -860,12 +827,13 @@ class Mxfp4MoeLayer(_OnDevice):
         self.slot_map.fill_(-1)
         self.placed = False
         self.tile_expert, self.tile_row, self.tile_units = torch.empty(capacity, **i32), torch.empty(capacity, **i32), torch.empty((capacity, 4), **i32)
-        wide, inner = mxfp4.padded(hidden), mxfp4.padded(intermediate)
-        self.a_q, self.a_s = torch.empty((tokens, wide // 2), **u8), torch.empty((tokens, wide // 32), **u8)
-        self.h_q, self.h_s = torch.empty((routes, inner // 2), **u8), torch.empty((routes, inner // 32), **u8)
         self.act = torch.empty((routes, intermediate), **values)
+        # (The second products stay fp32 until they are weighted and summed: as fp16, one beyond 65504 made its token's sum infinite or NaN however small its weight, and each was
+        # a rounding more.  Its price with MXFP4, 128 experts x 8 of 2048 x 512, us of place and down with fp16 / fp32: 256 tokens 25.7 / 29.2, 4096 tokens 105.6 / 158.8.)
         self.down_out = torch.empty((routes, hidden), dtype=torch.float32, device=self.device)
         self.out = torch.empty((tokens, hidden), **values)
+        # what the grouped kernels are made for
+        self.grouped = dict(rows=routes, E=experts, tiles=capacity, block_m=block_m)
 
     def route(self, logits, stream=None):
         """fp32 logits (tokens, experts) -> the routes' experts (tokens, top_k) int32 and weights fp32."""
@@ -900,13 +868,6 @@ class Mxfp4MoeLayer(_OnDevice):
         self._call(self._up, x, stream=stream)
         return self.act
 
-    def _up(self, x, stream):
-        if self.few_up is not None and _apart(x, self.act):  # (as Mxfp4Linear's)
-            self.few_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
-            return
-        self.k_quantise_tokens(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=self.tokens)
-        self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w1, WS=self.p1)
-
     def down(self, act, prob, shared=None, shared_gate=None, stream=None):
         """Rows in the order of the slots and fp32 weights (tokens, top_k) -> (tokens, hidden): the weighted sum, in fp32, of the routes' second products (those of weight 0 count nothing) and, where they are given,
         of sigmoid(shared_gate) (tokens) times shared (tokens, hidden); rows, result and these two of the layer's dtype."""
@@ -922,14 +883,222 @@ class Mxfp4MoeLayer(_OnDevice):
         return self.out
 
     def _down(self, act, prob, shared, shared_gate, stream):
-        if self.few_down is not None:
-            self.few_down(stream=stream, A=act, Out=self.down_out, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w2, WS=self.p2)
-        else:
-            self.k_quantise_act(stream=stream, Q=self.h_q, S=self.h_s, X=act, rows=self.assignments)
-            self.k_down(stream=stream, A=self.h_q, AS=self.h_s, Out=self.down_out, TileCount=self.tile_count, TileUnits=self.tile_units, W=self.w2, WS=self.p2)
+        self._second_products(act, stream)
         self.k_combine(stream=stream, Expert=self.down_out, Output=self.out, Prob=prob, Shared=shared, SharedGate=shared_gate, SlotMap=self.slot_map)
 
     def run(self, x, logits, shared=None, shared_gate=None, stream=None):
         self.route(logits, stream=stream)
         self.place(self.ids, stream=stream)
         return self.down(self.up(x, stream=stream), self.prob, shared, shared_gate, stream=stream)
+
+
+class Mxfp4MoeLayer(_ExpertLayer):
+    """Routed experts with MXFP4 weights for `tokens` rows: router, places of the routes, gate | up with SwiGLU, down, weighted sum.
+
+    gate_up (E, 2 I, H / 2) and gate_up_exponents (E, 2 I, H / 32): gate channels, then up channels; down (E, H, I / 2), down_exponents (E, H, I / 32); uint8.
+    scoring, bias (E fp32 values added for the choice only), groups, top_groups, group_best, renormalize and scale: the router's (k_router_scores.hip); as they stand here, the softmax router.
+    dtype: of the rows, the shared expert's values, the activations between the two products and the result, torch.float16 or torch.bfloat16.  An activation beyond fp16's 65504 becomes
+    infinite there, its block of 32 NaN and so its token's result: bfloat16 is for layers whose activations leave fp16's range.
+    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own (`place` before `up` and `down`).  They work on the object's buffers: one stream at a time."""
+
+    def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, gate_up_exponents, down, down_exponents, *, scoring="softmax", bias=None, groups=1,
+                 top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None, dtype=torch.float16):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+        if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden // 2) or tuple(down.shape) != (experts, hidden, intermediate // 2):
+            raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden // 2}) and down ({experts}, {hidden}, {intermediate // 2}), "
+                             f"not {tuple(gate_up.shape)} and {tuple(down.shape)}")
+        weights = tuple(map(torch.as_tensor, (gate_up, gate_up_exponents, down, down_exponents)))
+        self.device = self._device_of(*weights)
+        self.w1, self.p1 = (t.to(self.device) for t in mxfp4.tiles(*weights[:2], paired=True))
+        self.w2, self.p2 = (t.to(self.device) for t in mxfp4.tiles(*weights[2:]))
+        routes = tokens * top_k
+        if block_m is None:
+            block_m = 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
+        self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
+                     renormalize=renormalize, scale=scale)
+        name = mxfp4.dtype_name(dtype)
+        with torch.cuda.device(self.device):
+            self.k_quantise_tokens = Kernel("mxfp4_quantization", M=tokens, K=hidden, input_dtype=name, pad=mxfp4.STEP)
+            up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", output_dtype=name, **self.grouped)
+            self.k_up = Kernel("mxfp4_grouped", **up)
+            self.k_quantise_act = Kernel("mxfp4_quantization", M=routes, K=intermediate, input_dtype=name, pad=mxfp4.STEP)
+            down = dict(N=hidden, K=intermediate, output_dtype="float32", **self.grouped)
+            self.k_down = Kernel("mxfp4_grouped", **down)
+            # A route to an expert or less: the products quantise their rows themselves where these are fp16, one launch instead of two (us without / with it: 128 experts x 8 of 2048 x 512, 3 tokens, up
+            # 7.6 / 6.0 and down 5.1 / 4.4, 8 tokens 9.7 / 8.5 and 7.4 / 7.3, 16 tokens 10.7 / 10.7 and 8.9 / 10.3; 16 x 2 of 4096 x 1536, 8 tokens, 10.7 / 9.9 and 7.9 / 6.6).
+            few = block_m == 16 and dtype == torch.float16
+            self.few_up = _where_it_fits("mxfp4_grouped", input_dtype="float16", **up) if few and routes <= experts else None
+            self.few_down = _where_it_fits("mxfp4_grouped", input_dtype="float16", **down) if few and 4 * routes <= 3 * experts else None
+        u8 = dict(dtype=torch.uint8, device=self.device)
+        wide, inner = mxfp4.padded(hidden), mxfp4.padded(intermediate)
+        self.a_q, self.a_s = torch.empty((tokens, wide // 2), **u8), torch.empty((tokens, wide // 32), **u8)
+        self.h_q, self.h_s = torch.empty((routes, inner // 2), **u8), torch.empty((routes, inner // 32), **u8)
+
+    def _up(self, x, stream):
+        if self.few_up is not None and _apart(x, self.act):  # (as Mxfp4Linear's)
+            self.few_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, W=self.w1, WS=self.p1, TileCount=self.tile_count, TileUnits=self.tile_units)
+            return
+        self.k_quantise_tokens(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=self.tokens)
+        self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, W=self.w1, WS=self.p1, TileCount=self.tile_count, TileUnits=self.tile_units)
+
+    def _second_products(self, act, stream):
+        if self.few_down is not None:
+            self.few_down(stream=stream, A=act, Out=self.down_out, W=self.w2, WS=self.p2, TileCount=self.tile_count, TileUnits=self.tile_units)
+            return
+        self.k_quantise_act(stream=stream, Q=self.h_q, S=self.h_s, X=act, rows=self.assignments)
+        self.k_down(stream=stream, A=self.h_q, AS=self.h_s, Out=self.down_out, W=self.w2, WS=self.p2, TileCount=self.tile_count, TileUnits=self.tile_units)
+
+
+class Int8Linear(_OnDevice):
+    """Rows of 16-bit values, quantised to 8-bit integers with a scale (zero_points: and a zero point) for each, times weights (N, K) of int8 with fp32 scales (N), plus a bias (N) if one is given,
+    up to `capacity` rows at a time (the rules: int8.py).  K is up to 65536.  epilogue="swiglu": the upper half of the channels are the up channels of the gate channels in the lower half, and
+    silu(gate) * up comes out.  `run` returns the object's own output buffer, or a view of its first rows, which the next call overwrites; one object serves one stream at a time."""
+
+    def __init__(self, weight, scale, capacity, *, bias=None, zero_points=False, dtype=torch.float16, epilogue="none"):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+        weight, scale = torch.as_tensor(weight), torch.as_tensor(scale)
+        if weight.ndim != 2 or weight.dtype != torch.int8:
+            raise ValueError("weight must be int8 (N, K)")
+        if not 0 < capacity <= 1 << 24:
+            raise ValueError("capacity must be 1 to 2^24 rows")
+        self.capacity, self.dtype, self.zero_points = capacity, dtype, bool(zero_points)
+        channels, self.k = weight.shape
+        bias = None if bias is None else torch.as_tensor(bias)
+        if scale.shape != (channels,) or (bias is not None and bias.shape != (channels,)):
+            raise ValueError(f"scale and bias must have {channels} values")
+        self.device = self._device_of(weight, scale, *([] if bias is None else [bias]))
+        paired = epilogue == "swiglu"
+        self.weight = byte_tiles.tiles(weight, paired).to(self.device)
+        self.channel = dict(WS=byte_tiles.channels(scale.float(), paired).to(self.device))
+        if bias is not None:
+            self.channel["Bias"] = byte_tiles.channels(bias.float(), paired).to(self.device)
+        if self.zero_points:
+            self.channel["WSum"] = byte_tiles.channels(weight.sum(1, dtype=torch.int32), paired).to(self.device)
+        name = int8.dtype_name(dtype)
+        shape = dict(N=channels, K=self.k, dynamic_rows=True, zero_points=self.zero_points, bias=bias is not None, epilogue=epilogue, output_dtype=name)
+        with torch.cuda.device(self.device):
+            self.projection = Kernel("int8_token_projection", M=capacity, **shape)
+            self.quantizer = Kernel("int8_token_quantization", M=capacity, K=self.k, input_dtype=name, zero_points=self.zero_points)
+            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two.  Not where their codes do not fit LDS, or a row its threads.
+            self.few, self.few_rows = None, 0
+            for rows in (4, 2, 1):
+                if self.few is None and rows <= capacity:
+                    self.few, self.few_rows = _where_it_fits("int8_token_projection", M=rows, input_dtype=name, **shape), rows
+        self.n = channels // 2 if paired else channels
+        self.a_q = torch.empty((capacity, int8.padded(self.k)), dtype=torch.int8, device=self.device)
+        self.a_s = torch.empty(capacity, dtype=torch.float32, device=self.device)
+        self.a_z = torch.empty(capacity, dtype=torch.int32, device=self.device) if self.zero_points else None
+        self.out = torch.empty((capacity, self.n), dtype=dtype, device=self.device)
+
+    def run(self, x, stream=None):
+        _check_rows(x, None, self.k, self.dtype, self.device, "x")
+        rows = x.shape[0]
+        if rows > self.capacity:
+            raise ValueError(f"{rows} rows are more than the capacity of {self.capacity}")
+        if rows:
+            self._call(self._run, x, rows, stream=stream)
+        return self.out if rows == self.capacity else self.out.as_strided((rows, self.n), (self.n, 1))
+
+    def _run(self, x, rows, stream):
+        if rows <= self.few_rows and self.few is not None and _apart(x, self.out):  # (as Mxfp4Linear's)
+            self.few(stream=stream, A=x, Out=self.out, W=self.weight, m=rows, **self.channel)
+            return
+        zero = ({"Z": self.a_z}, {"AZ": self.a_z}) if self.zero_points else ({}, {})
+        self.quantizer(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=rows, **zero[0])
+        self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, m=rows, **zero[1], **self.channel)
+
+
+def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):
+    if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden) or tuple(down.shape) != (experts, hidden, intermediate):
+        raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden}) and down ({experts}, {hidden}, {intermediate}), not {tuple(gate_up.shape)} and {tuple(down.shape)}")
+    if gate_up.dtype not in dtypes or down.dtype != gate_up.dtype:
+        raise ValueError(f"gate_up and down must both be {' or '.join(map(str, dtypes))}, not {gate_up.dtype} and {down.dtype}")
+
+
+class Int8MoeLayer(_ExpertLayer):
+    """Routed experts with weights of 8-bit integers and fp32 scales for each channel, for `tokens` rows that are quantised with a scale for each (int8.py): router, places of the routes,
+    gate | up with SwiGLU, down, weighted sum.
+
+    gate_up (E, 2 I, H) int8 with gate_up_scale (E, 2 I): gate channels, then up channels; down (E, H, I) int8 with down_scale (E, H).
+    scoring, bias (E fp32 values added for the choice only), groups, top_groups, group_best, renormalize and scale: the router's (k_router_scores.hip); as they stand here, the softmax router.
+    dtype: of the rows, the shared expert's values, the activations between the two products and the result, torch.float16 or torch.bfloat16.  An activation beyond fp16's 65504 becomes
+    infinite there and its token's result NaN: bfloat16 is for layers whose activations leave fp16's range.
+    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own (`place` before `up` and `down`).  They work on the object's buffers: one stream at a time."""
+
+    def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, gate_up_scale, down, down_scale, *, scoring="softmax", bias=None, groups=1,
+                 top_groups=None, group_best=2, renormalize=True, scale=1.0, block_m=None, dtype=torch.float16):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+        gate_up, gate_up_scale, down, down_scale = map(torch.as_tensor, (gate_up, gate_up_scale, down, down_scale))
+        _check_experts(gate_up, down, experts, hidden, intermediate, (torch.int8,))
+        if tuple(gate_up_scale.shape) != (experts, 2 * intermediate) or tuple(down_scale.shape) != (experts, hidden):
+            raise ValueError(f"gate_up_scale must be ({experts}, {2 * intermediate}) and down_scale ({experts}, {hidden}), not {tuple(gate_up_scale.shape)} and {tuple(down_scale.shape)}")
+        self.device = self._device_of(gate_up, gate_up_scale, down, down_scale)
+        self.w1, self.s1 = byte_tiles.tiles(gate_up, paired=True).to(self.device), byte_tiles.channels(gate_up_scale.float(), paired=True).to(self.device)
+        self.w2, self.s2 = byte_tiles.tiles(down).to(self.device), byte_tiles.channels(down_scale.float()).to(self.device)
+        routes = tokens * top_k
+        if block_m is None:
+            block_m = 16
+        self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
+                     renormalize=renormalize, scale=scale)
+        name = int8.dtype_name(dtype)
+        with torch.cuda.device(self.device):
+            self.k_quantise_tokens = Kernel("int8_token_quantization", M=tokens, K=hidden, input_dtype=name)
+            self.k_quantise_act = Kernel("int8_token_quantization", M=routes, K=intermediate, input_dtype=name)
+            up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", output_dtype=name, **self.grouped)
+            down = dict(N=hidden, K=intermediate, output_dtype="float32", **self.grouped)
+            self.k_up, self.k_down = Kernel("int8_token_grouped", **up), Kernel("int8_token_grouped", **down)
+            # A route to an expert or less: the products quantise their rows themselves, one launch instead of two.
+            few = block_m == 16 and routes <= experts
+            self.few_up = _where_it_fits("int8_token_grouped", input_dtype=name, **up) if few else None
+            self.few_down = _where_it_fits("int8_token_grouped", input_dtype=name, **down) if few else None
+        i8, f32 = dict(dtype=torch.int8, device=self.device), dict(dtype=torch.float32, device=self.device)
+        self.a_q, self.a_s = torch.empty((tokens, int8.padded(hidden)), **i8), torch.empty(tokens, **f32)
+        self.h_q, self.h_s = torch.empty((routes, int8.padded(intermediate)), **i8), torch.empty(routes, **f32)
+
+    def _up(self, x, stream):
+        if self.few_up is not None and _apart(x, self.act):  # (as Mxfp4Linear's)
+            self.few_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, W=self.w1, WS=self.s1, TileCount=self.tile_count, TileUnits=self.tile_units)
+            return
+        self.k_quantise_tokens(stream=stream, Q=self.a_q, S=self.a_s, X=x, rows=self.tokens)
+        self.k_up(stream=stream, A=self.a_q, AS=self.a_s, Out=self.act, SlotToken=self.slot_token, W=self.w1, WS=self.s1, TileCount=self.tile_count, TileUnits=self.tile_units)
+
+    def _second_products(self, act, stream):
+        if self.few_down is not None:
+            self.few_down(stream=stream, A=act, Out=self.down_out, W=self.w2, WS=self.s2, TileCount=self.tile_count, TileUnits=self.tile_units)
+            return
+        self.k_quantise_act(stream=stream, Q=self.h_q, S=self.h_s, X=act, rows=self.assignments)
+        self.k_down(stream=stream, A=self.h_q, AS=self.h_s, Out=self.down_out, W=self.w2, WS=self.s2, TileCount=self.tile_count, TileUnits=self.tile_units)
+
+
+class HalfMoeLayer(_ExpertLayer):
+    """Routed experts with weights of fp16 or bf16 for `tokens` rows of that type: router, places of the routes, gate | up with SwiGLU, down, weighted sum; products and sums in fp32.
+
+    gate_up (E, 2 I, H): gate channels, then up channels; down (E, H, I); H and I are multiples of 8, and the rows given to `up` and `down` start at addresses that are multiples of 16.
+    The router's arguments: as Int8MoeLayer's.  An activation beyond fp16's 65504 becomes infinite there: bf16 is for layers whose activations leave fp16's range.
+    `run` does all of it; `route`, `place`, `up` and `down` are its parts, for a caller with routes of its own (`place` before `up` and `down`).  They work on the object's buffers: one stream at a time."""
+
+    def __init__(self, tokens, experts, top_k, hidden, intermediate, gate_up, down, *, scoring="softmax", bias=None, groups=1, top_groups=None, group_best=2, renormalize=True, scale=1.0,
+                 block_m=None):
+        gate_up, down = torch.as_tensor(gate_up), torch.as_tensor(down)
+        _check_experts(gate_up, down, experts, hidden, intermediate, (torch.float16, torch.bfloat16))
+        self.device = self._device_of(gate_up, down)
+        self.w1, self.w2 = byte_tiles.tiles(gate_up, paired=True).to(self.device), byte_tiles.tiles(down).to(self.device)
+        if block_m is None:
+            block_m = 16
+        self._set_up(tokens, experts, top_k, hidden, intermediate, gate_up.dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
+                     renormalize=renormalize, scale=scale)
+        name = int8.dtype_name(gate_up.dtype)
+        with torch.cuda.device(self.device):
+            self.k_up = Kernel("half_grouped", N=2 * intermediate, K=hidden, gather=True, dtype=name, epilogue="swiglu", output_dtype=name, **self.grouped)
+            self.k_down = Kernel("half_grouped", N=hidden, K=intermediate, dtype=name, output_dtype="float32", **self.grouped)
+
+    def _up(self, x, stream):
+        if not _apart(x, self.act):  # (workgroups that have ended would write over what others have yet to read)
+            x = x.clone()
+        self.k_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, W=self.w1, TileCount=self.tile_count, TileUnits=self.tile_units)
+
+    def _second_products(self, act, stream):
+        self.k_down(stream=stream, A=act, Out=self.down_out, W=self.w2, TileCount=self.tile_count, TileUnits=self.tile_units)
