@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "byte_device.h"
+#include "byte_tiles.h"
 #include "orx_internal.h"
 
 namespace orx {
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
         w += tile * p.steps * kTileBytes, channels = tile * 16;
     }
     auto row_at = [&](int local) {
-        int64_t row = first_row + min(local, rows - 1);  // (rows that are not there repeat the last: their sums go nowhere)
+        int64_t row = max(first_row + min(local, rows - 1), 0);  // (rows that are not there repeat the last: their sums go nowhere)
         if (GROUPED && p.slot_token != nullptr) row = p.slot_token[row];
         return row;
     };
@@ -208,13 +209,16 @@ constexpr int kMostLds = 80 * 1024;
 
 int steps_of(const orx_function& f) { return (f.K * (f.flags2 == I8 ? 1 : 2) + kStep - 1) / kStep; }
 
-// Rows to a unit, and waves.
+// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS (0: the kernel above, 32 channels), or its waves
 struct Plan {
-    int rows, waves;
+    int rows, channels, waves;
 };
+Plan few_rows(int unit_rows) { return {unit_rows, 0, unit_rows == 64 ? 4 : 8}; }
+Plan tiles_of(int rows) { return {rows, rows == 256 ? 256 : 128, 0}; }
 Plan plan(const orx_function& f, int rows) {
-    if (f.E > 0) return {16, 8};
-    return rows <= 16 ? Plan{16, 8} : rows <= 32 ? Plan{32, 8} : Plan{64, 4};
+    if (f.E > 0) return f.block_m == 16 ? few_rows(16) : tiles_of(f.block_m);
+    if (rows <= 64) return few_rows(rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
+    return tiles_of(rows >= 1024 ? 256 : 128);
 }
 uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
     const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * 2 * 1024;
@@ -225,13 +229,19 @@ uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
 int geometry(const orx_function& f, int rows, Geometry* g) {
     const Plan plan = orx::plan(f, rows);
     const int64_t units = f.E > 0 ? (int64_t)f.tiles : ceil_div(rows, plan.rows);
-    const int64_t blocks = units * ceil_div(f.slots, 2);
+    int64_t blocks = units * ceil_div(f.slots, plan.channels ? plan.channels / 16 : 2);
     if (blocks >= (1ll << 32) / 512) {
         set_error("%s: %d rows of %d channels are more than one launch takes", f.symbol.c_str(), rows, f.N);
         return ORX_ERR_ROWS;
     }
-    g->block[0] = 64 * plan.waves;
-    g->shared = few_rows_lds(f, rows, plan);
+    if (plan.channels) {
+        blocks = std::min<int64_t>(blocks, (int64_t)device_compute_units() * byte_tiles_to_a_cu(plan.rows));
+        g->block[0] = byte_tiles_threads(plan.rows);
+        g->shared = byte_tiles_lds(plan.rows, plan.channels);
+    } else {
+        g->block[0] = 64 * plan.waves;
+        g->shared = few_rows_lds(f, rows, plan);
+    }
     g->grid[0] = (uint32_t)blocks;
     return ORX_OK;
 }
@@ -255,6 +265,7 @@ int launch_dense(const orx_function& f, const Product& p, const Geometry& g, hip
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
+    if (plan.channels) return launch_byte_tiles(p, f.flags2, plan.rows, plan.channels, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
     if (f.E > 0) {
         if (f.flags2 == F16) return launch_of<F16, 1, 8, 2, -1, false, true>(f, p, g, s);
         if (f.flags2 == BF16) return launch_of<BF16, 1, 8, 2, -1, false, true>(f, p, g, s);
@@ -303,7 +314,7 @@ int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream
 // Rows that a product quantises itself: their codes fit LDS, and a thread holds its part of a row.
 bool quantises(const orx_function& f, int rows) {
     const int row_waves = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1;
-    return rows <= 16 && few_rows_lds(f, rows, {16, 8}) <= (uint32_t)kMostLds && steps_of(f) * 16 <= row_waves * 64 * kPieces;
+    return rows <= 16 && few_rows_lds(f, rows, few_rows(16)) <= (uint32_t)kMostLds && steps_of(f) * 16 <= row_waves * 64 * kPieces;
 }
 
 // What all three have: N, K, epilogue, types.
@@ -346,8 +357,8 @@ int make_grouped(const Variant& v, orx_function* f) {
     if (bad) return ORX_ERR_BAD_VARIANT;
     const int code = shape(v, f);
     if (code != ORX_OK) return code;
-    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || f->block_m != 16) {
-        set_error("%s: need rows, E and tiles above 0 and block_m 16", f->symbol.c_str());
+    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 64 && f->block_m != 128 && f->block_m != 256)) {
+        set_error("%s: need rows, E and tiles above 0 and block_m 16, 64, 128 or 256", f->symbol.c_str());
         return ORX_ERR_BAD_VARIANT;
     }
     f->capacity = f->M;

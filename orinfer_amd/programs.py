@@ -914,7 +914,7 @@ class Mxfp4MoeLayer(_ExpertLayer):
         self.w2, self.p2 = (t.to(self.device) for t in mxfp4.tiles(*weights[2:]))
         routes = tokens * top_k
         if block_m is None:
-            block_m = 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
+            block_m = _unit_rows(routes, experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = mxfp4.dtype_name(dtype)
@@ -1010,6 +1010,11 @@ class Int8Linear(_OnDevice):
         self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, m=rows, **zero[1], **self.channel)
 
 
+def _unit_rows(routes, experts):
+    """Rows to a unit of the experts' products, by the routes that an expert has in the mean."""
+    return 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
+
+
 def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):
     if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden) or tuple(down.shape) != (experts, hidden, intermediate):
         raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden}) and down ({experts}, {hidden}, {intermediate}), not {tuple(gate_up.shape)} and {tuple(down.shape)}")
@@ -1040,7 +1045,7 @@ class Int8MoeLayer(_ExpertLayer):
         self.w2, self.s2 = byte_tiles.tiles(down).to(self.device), byte_tiles.channels(down_scale.float()).to(self.device)
         routes = tokens * top_k
         if block_m is None:
-            block_m = 16
+            block_m = _unit_rows(tokens * top_k, experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(dtype)
@@ -1087,7 +1092,7 @@ class HalfMoeLayer(_ExpertLayer):
         self.device = self._device_of(gate_up, down)
         self.w1, self.w2 = byte_tiles.tiles(gate_up, paired=True).to(self.device), byte_tiles.tiles(down).to(self.device)
         if block_m is None:
-            block_m = 16
+            block_m = _unit_rows(tokens * top_k, experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, gate_up.dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(gate_up.dtype)

@@ -118,6 +118,13 @@ def test_16_bit_layers_whose_rows_end_within_a_step(tokens, experts, top_k, hidd
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("block_m", [16, 64, 128, 256])
+@pytest.mark.parametrize("tokens,hidden,inner", [(40, 328, 224), (300, 64, 64), (900, 136, 520)])
+def test_units_of_every_size(tokens, hidden, inner, block_m, kind, dtype):
+    check_run(*make(kind, dtype, tokens, 8, 3, hidden, inner, block_m=block_m), {})
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 def test_experts_without_rows_and_all_rows_to_one(kind, dtype):
     layer, gate_up, down, x, _, shared, gate = make(kind, dtype, 70, 16, 2, 264, 136)
     prob = torch.rand((70, 2), device=DEV)
@@ -193,7 +200,7 @@ def test_rows_in_the_layers_own_buffer(kind, dtype):
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
 @pytest.mark.parametrize("output", ["float16", "bfloat16", "float32"])
-@pytest.mark.parametrize("block_m", [16])
+@pytest.mark.parametrize("block_m", [16, 64, 128, 256])
 def test_grouped_writes_its_rows_and_columns_only(kind, dtype, output, block_m):
     """Units of odd lengths, one of them empty, rows and channels behind the ends untouched."""
     rng = np.random.default_rng(3)

@@ -144,7 +144,8 @@ def test_shapes_of_quantize():
 
 # ---- linears -----------------------------------------------------------------------------------------------------------------------------------
 LINEARS = [(1, 16, 128), (1, 9, 7), (1, 300, 2560), (2, 33, 5000), (3, 48, 640), (4, 31, 4097), (5, 96, 1000), (16, 128, 1024), (17, 40, 129), (31, 260, 2560), (33, 513, 512), (64, 100, 1111),
-           (65, 300, 300), (130, 520, 1280), (200, 1030, 384), (300, 264, 2048), (513, 700, 257)]
+           (65, 300, 300), (130, 520, 1280), (200, 1030, 384), (300, 264, 2048), (513, 700, 257),
+           (1024, 256, 64), (1030, 520, 300), (2500, 1100, 640)]
 
 
 @pytest.mark.parametrize("zero_points,biased", [(False, False), (True, True), (True, False), (False, True)])
@@ -163,7 +164,7 @@ def test_linear(rows, n, k, dtype, zero_points, biased):
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
-@pytest.mark.parametrize("rows,n,k", [(1, 32, 128), (1, 34, 2000), (3, 300, 1111), (20, 66, 512), (64, 1000, 256), (150, 258, 640), (400, 514, 300)])
+@pytest.mark.parametrize("rows,n,k", [(1, 32, 128), (1, 34, 2000), (3, 300, 1111), (20, 66, 512), (64, 1000, 256), (150, 258, 640), (400, 514, 300), (1500, 1058, 520)])
 def test_linear_with_swiglu(rows, n, k, zero_points):
     rng = np.random.default_rng(rows * n + k)
     x = rows_of(rng, rows, k, torch.bfloat16)
@@ -208,7 +209,7 @@ def test_rows_that_are_not_finite_stay_to_themselves(rows):
 
 
 @pytest.mark.parametrize("name", list(TYPES))
-@pytest.mark.parametrize("rows,n,k", [(1, 33, 256), (6, 130, 384), (70, 50, 129), (260, 530, 128)])
+@pytest.mark.parametrize("rows,n,k", [(1, 33, 256), (6, 130, 384), (70, 50, 129), (260, 530, 128), (1100, 300, 300)])
 def test_projection_writes_its_rows_and_columns_only(rows, n, k, name):
     rng = np.random.default_rng(n)
     x = rows_of(rng, rows, k, torch.float32)
