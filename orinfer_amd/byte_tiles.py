@@ -20,8 +20,8 @@ def _check_paired(n, paired):
 
 
 def tiles(weight, paired=False):
-    """Weights (..., N, K) of int8, fp16 or bf16 laid out for the products, uint8: 16 channels x 128 bytes of K are 2048 bytes, [piece of 16 bytes][channel][16]; tiles of the same channels lie
-    along K behind one another.  N is padded to 16 and K to 128 bytes with zeros.
+    """Weights (..., N, K) of int8, fp16 or bf16 laid out for the products, uint8: 16 channels x 128 bytes of K are 2048 bytes, [piece of 16 bytes][channel][16]; the tiles of the same K
+    lie behind one another.  N is padded to 16 and K to 128 bytes with zeros.
     paired: the upper half of the N rows are the up channels of the gate channels in the lower half (SwiGLU); tiles of the two halves take turns."""
     weight = torch.as_tensor(weight)
     if weight.ndim < 2 or weight.dtype not in (torch.int8, torch.float16, torch.bfloat16):
@@ -34,7 +34,7 @@ def tiles(weight, paired=False):
     rows = _by_16(weight.contiguous().view(torch.uint8), -2, paired)  # (..., tiles, 16, bytes)
     steps = -(-width // STEP)
     rows = torch.nn.functional.pad(rows, (0, STEP * steps - width)).unflatten(-1, (steps, 8, 16))  # (..., tiles, 16, steps, 8, 16)
-    return rows.movedim(-4, -2).contiguous()                                                      # (..., tiles, steps, 8, 16, 16)
+    return rows.movedim((-3, -5, -2, -4), (-5, -4, -3, -2)).contiguous()                          # (..., steps, tiles, 8, 16, 16)
 
 
 def channels(values, paired=False):

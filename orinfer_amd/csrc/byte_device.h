@@ -3,7 +3,7 @@
 // One instruction takes 64 bytes of K of either kind (v_mfma_i32_16x16x64_i8, v_mfma_f32_16x16x32_f16 and _bf16): a lane holds 16 bytes of one row, lane l those of row l % 16
 // at byte 16 (l / 16), and of a result four neighbouring rows of the first operand and one of the second.  So one kernel moves the bytes of all three, in steps of 128.
 //
-// Weights are laid out once: a tile is 16 channels x 128 bytes of K, 2048 bytes as [piece 0..7][channel][16 bytes]; the tiles of the same channels lie along K behind one another.
+// Weights are laid out once: a tile is 16 channels x 128 bytes of K, 2048 bytes as [piece 0..7][channel][16 bytes]; the tiles of the same K lie behind one another.
 // A wave's load of an operand is whole kilobytes, with nothing to unpack.  Channels are padded to 16 and K to 128 bytes with zeros.  What a channel has (scale, sum, bias) lies by tiles too.
 // SwiGLU: tiles of gate channels and of their up channels take turns, so a lane has both of a pair.
 //
@@ -79,23 +79,22 @@ struct RowScale {
     int zero;
 };
 
-// Four channels of one row: channel c of the tile `at` / 16 of the expert's (by tiles).
-template <int KIND, bool GROUPED>
-__device__ __forceinline__ v4f scaled(const Product& p, typename Operands<KIND>::Sum sum, int64_t at, const RowScale& row) {
+// What four channels have: their scales, and with zero points and biases those sums and biases (zeros where there are none).
+struct Channels {
+    v4f scale;
+    v4i sum;
+    v4f bias;
+};
+// Four channels of one row.  EXTRAS: zero points and biases there may be.
+template <int KIND, bool EXTRAS>
+__device__ __forceinline__ v4f scaled(typename Operands<KIND>::Sum sum, const Channels& channel, const RowScale& row) {
     v4f y;
     if constexpr (KIND == I8) {
-        const v4f scale = *reinterpret_cast<const v4f*>(p.w_scale + at);
-        if (!GROUPED && p.w_sum != nullptr) {
-            const v4i channel = *reinterpret_cast<const v4i*>(p.w_sum + at);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] -= row.zero * channel[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = ((float)sum[j] * scale[j]) * row.scale;
-        if (!GROUPED && p.bias != nullptr) {
-            const v4f bias = *reinterpret_cast<const v4f*>(p.bias + at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] += bias[j];
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (EXTRAS) sum[j] -= row.zero * channel.sum[j];
+            y[j] = ((float)sum[j] * channel.scale[j]) * row.scale;
+            if constexpr (EXTRAS) y[j] += channel.bias[j];
         }
     } else {
         y = sum;

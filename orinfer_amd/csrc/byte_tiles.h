@@ -1,4 +1,4 @@
-// Host side of the products by byte tiles from LDS (k_byte_tiles.hip).
+// Host side of the products by byte tiles from LDS (byte_tiles_kernel.h, k_byte_tiles_*.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -8,11 +8,18 @@
 
 namespace orx {
 
-// Tiles of 256 x 256, 128 x 128 or 64 x 128 rows x channels; `blocks` workgroups, each of which takes every blocks-th tile.
-int launch_byte_tiles(const bytes::Product& p, int kind, int rows, int channels, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s);
-inline uint32_t byte_tiles_lds(int rows, int channels) { return 2u * (rows + channels) * bytes::kStep; }
-inline uint32_t byte_tiles_threads(int rows) { return rows == 256 ? 512 : 256; }
-// workgroups that a CU holds (its LDS)
-inline uint32_t byte_tiles_to_a_cu(int rows) { return rows == 256 ? 1 : rows == 128 ? 2 : 3; }
+enum { kTiles256, kTiles128x256, kTiles128, kTiles64 };  // rows x channels 256 x 256, 128 x 256, 128 x 128, 64 x 128
+
+struct TilesShape {
+    int rows, channels, threads, lds, to_a_cu;  // to_a_cu: workgroups that a CU holds, by its LDS and registers
+};
+TilesShape byte_tiles_shape(int kind, int form, bool grouped);
+// `blocks` workgroups, each of which takes every blocks-th tile
+int launch_byte_tiles_i8(const bytes::Product& p, int form, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s);
+int launch_byte_tiles_f16(const bytes::Product& p, int form, bool swiglu, uint32_t blocks, hipStream_t s);  // (experts)
+int launch_byte_tiles_bf16(const bytes::Product& p, int form, bool swiglu, uint32_t blocks, hipStream_t s);
+inline int launch_byte_tiles(const bytes::Product& p, int kind, int form, bool grouped, bool swiglu, uint32_t blocks, hipStream_t s) {
+    return kind == bytes::I8 ? launch_byte_tiles_i8(p, form, grouped, swiglu, blocks, s) : kind == bytes::F16 ? launch_byte_tiles_f16(p, form, swiglu, blocks, s) : launch_byte_tiles_bf16(p, form, swiglu, blocks, s);
+}
 
 }  // namespace orx

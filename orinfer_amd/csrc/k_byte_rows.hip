@@ -89,10 +89,10 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
     auto load = [&](Step& s, int step) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const int64_t tile = min(group * TILES + t, p.tiles - 1);
-            const Buffer codes(w + tile * p.steps * kTileBytes, p.steps * kTileBytes);
-            s.w[t][0] = codes.load_16(lane * 16 + step * kTileBytes);
-            s.w[t][1] = codes.load_16(lane * 16 + step * kTileBytes + 1024);
+            const int64_t tile = (int64_t)step * p.tiles + min(group * TILES + t, p.tiles - 1);
+            const Buffer codes(w + tile * kTileBytes, step < p.steps ? kTileBytes : 0);
+            s.w[t][0] = codes.load_16(lane * 16);
+            s.w[t][1] = codes.load_16(lane * 16 + 1024);
         }
         if constexpr (!QUANTISE) {
             // (16-bit rows end where they end: pieces behind that are 0, and read the row's first one)
@@ -190,8 +190,14 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
             Sum all = sums[0][i * TILES + t * KINDS + kind][l];
 #pragma unroll
             for (int other = 1; other < WAVES; ++other) all += sums[other][i * TILES + t * KINDS + kind][l];
-            const int tile = min(group * TILES + t * KINDS + kind, p.tiles - 1);
-            total[kind] = scaled<KIND, GROUPED>(p, all, channels + tile * 16 + 4 * (l >> 4), KIND == I8 ? row_scales[min(row, rows - 1)] : RowScale{});
+            const int64_t at = channels + min(group * TILES + t * KINDS + kind, p.tiles - 1) * 16 + 4 * (l >> 4);
+            Channels channel = {};
+            if constexpr (KIND == I8) {
+                channel.scale = *reinterpret_cast<const v4f*>(p.w_scale + at);
+                if (ZERO) channel.sum = *reinterpret_cast<const v4i*>(p.w_sum + at);
+                if (!GROUPED && p.bias != nullptr) channel.bias = *reinterpret_cast<const v4f*>(p.bias + at);
+            }
+            total[kind] = scaled<KIND, !GROUPED>(all, channel, KIND == I8 ? row_scales[min(row, rows - 1)] : RowScale{});
         }
         if constexpr (SWIGLU) {
 #pragma unroll
@@ -209,16 +215,15 @@ constexpr int kMostLds = 80 * 1024;
 
 int steps_of(const orx_function& f) { return (f.K * (f.flags2 == I8 ? 1 : 2) + kStep - 1) / kStep; }
 
-// What a launch of `rows` rows runs: a unit's rows, and channels to a workgroup of the tiles from LDS (0: the kernel above, 32 channels), or its waves
+// What a launch of `rows` rows runs: a unit's rows, and the form of the tiles from LDS (-1: the kernel above, 32 channels to a workgroup), or its waves
 struct Plan {
-    int rows, channels, waves;
+    int rows, form, waves;
 };
-Plan few_rows(int unit_rows) { return {unit_rows, 0, unit_rows == 64 ? 4 : 8}; }
-Plan tiles_of(int rows) { return {rows, rows == 256 ? 256 : 128, 0}; }
+Plan few_rows(int unit_rows) { return {unit_rows, -1, unit_rows == 64 ? 4 : 8}; }
 Plan plan(const orx_function& f, int rows) {
-    if (f.E > 0) return f.block_m == 16 ? few_rows(16) : tiles_of(f.block_m);
+    if (f.E > 0) return f.block_m == 16 ? few_rows(16) : Plan{f.block_m, f.block_m == 64 ? kTiles64 : f.block_m == 256 ? kTiles256 : kTiles128x256, 0};
     if (rows <= 64) return few_rows(rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
-    return tiles_of(rows >= 1024 ? 256 : 128);
+    return rows >= 1024 ? Plan{256, kTiles256, 0} : Plan{128, kTiles128, 0};
 }
 uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
     const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * 2 * 1024;
@@ -228,16 +233,17 @@ uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
 
 int geometry(const orx_function& f, int rows, Geometry* g) {
     const Plan plan = orx::plan(f, rows);
+    const TilesShape shape = plan.form < 0 ? TilesShape{plan.rows, 32} : byte_tiles_shape(f.flags2, plan.form, f.E > 0);
     const int64_t units = f.E > 0 ? (int64_t)f.tiles : ceil_div(rows, plan.rows);
-    int64_t blocks = units * ceil_div(f.slots, plan.channels ? plan.channels / 16 : 2);
+    int64_t blocks = units * ceil_div(f.slots, shape.channels / 16);
     if (blocks >= (1ll << 32) / 512) {
         set_error("%s: %d rows of %d channels are more than one launch takes", f.symbol.c_str(), rows, f.N);
         return ORX_ERR_ROWS;
     }
-    if (plan.channels) {
-        blocks = std::min<int64_t>(blocks, (int64_t)device_compute_units() * byte_tiles_to_a_cu(plan.rows));
-        g->block[0] = byte_tiles_threads(plan.rows);
-        g->shared = byte_tiles_lds(plan.rows, plan.channels);
+    if (plan.form >= 0) {
+        blocks = std::min<int64_t>(blocks, (int64_t)device_compute_units() * shape.to_a_cu);
+        g->block[0] = shape.threads;
+        g->shared = shape.lds;
     } else {
         g->block[0] = 64 * plan.waves;
         g->shared = few_rows_lds(f, rows, plan);
@@ -265,7 +271,7 @@ int launch_dense(const orx_function& f, const Product& p, const Geometry& g, hip
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
-    if (plan.channels) return launch_byte_tiles(p, f.flags2, plan.rows, plan.channels, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
+    if (plan.form >= 0) return launch_byte_tiles(p, f.flags2, plan.form, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
     if (f.E > 0) {
         if (f.flags2 == F16) return launch_of<F16, 1, 8, 2, -1, false, true>(f, p, g, s);
         if (f.flags2 == BF16) return launch_of<BF16, 1, 8, 2, -1, false, true>(f, p, g, s);

@@ -37,5 +37,16 @@ __device__ __forceinline__ void everybody_arrived() {
     asm volatile("" ::: "memory");
 }
 
+// The same, but the newest PENDING of this wave's requests may be on their way where `all` is above 0.
+template <int PENDING>
+__device__ __forceinline__ void everybody_arrived_but(int all) {
+    static_assert(PENDING > 0 && PENDING < 64, "vmcnt has six bits");
+    asm volatile("s_cmp_gt_i32 %0, 0\n\ts_cbranch_scc0 .Lnone%=\n\ts_waitcnt vmcnt(%1)\n\ts_branch .Ldone%=\n.Lnone%=:\n\ts_waitcnt vmcnt(0)\n.Ldone%=:" ::"s"(all), "n"(PENDING) : "memory", "scc");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 }  // namespace tile_requests
 }  // namespace orx

@@ -30,7 +30,7 @@ def test_tiles_hold_every_byte_where_a_lane_reads_it(n, k, paired, dtype):
     w = byte_tiles.tiles(raw.view(dtype), paired=paired)
     half = n // 2 if paired else n
     tiles, steps = -(-half // 16) * (2 if paired else 1), -(-k * size // 128)
-    assert w.shape == (2, tiles, steps, 8, 16, 16) and w.is_contiguous() and w.dtype == torch.uint8
+    assert w.shape == (2, steps, tiles, 8, 16, 16) and w.is_contiguous() and w.dtype == torch.uint8
     wide = torch.nn.functional.pad(raw, (0, steps * 128 - k * size)).view(2, n, steps, 8, 16)
     values = torch.arange(1.0, n + 1)
     channels = byte_tiles.channels(values, paired=paired)
@@ -40,7 +40,7 @@ def test_tiles_hold_every_byte_where_a_lane_reads_it(n, k, paired, dtype):
             row = (tile // 2 * 16 + r) if paired else tile * 16 + r
             live = row < half
             row += half if paired and tile % 2 else 0
-            assert torch.equal(w[:, tile, :, :, r], wide[:, row] if live else torch.zeros_like(wide[:, 0]))
+            assert torch.equal(w[:, :, tile, :, r], wide[:, row] if live else torch.zeros_like(wide[:, 0]))
             assert channels[tile, r] == (values[row] if live else 0)
 
 
