@@ -7,8 +7,9 @@
 // A wave's load of an operand is whole kilobytes, with nothing to unpack.  Channels are padded to 16 and K to 128 bytes with zeros.  What a channel has (scale, sum, bias) lies by tiles too.
 // SwiGLU: tiles of gate channels and of their up channels take turns, so a lane has both of a pair.
 //
-// Rows of 8-bit integers: x = (q - z) s with an fp32 scale s, and a zero point z or none, for each row; a row's codes take an odd multiple of 128 bytes (rows that lie a multiple of 4 KiB
-// apart meet in few channels of the L2), zeros behind K up to a multiple of 128.  Channel c has an fp32 scale t and S = sum of its weights w:
+// Rows of 8-bit integers: x = (q - z) s with an fp32 scale s, and a zero point z or none, for each row, zeros behind K up to a multiple of 128.  Dense rows lie by tiles of 16 rows x 128,
+// [piece][row][16], the tiles of the same rows along K behind one another; rows of experts, which a product takes from anywhere, an odd multiple of 128 bytes apart (at a multiple of 4 KiB they
+// meet in few channels of the L2).  Channel c has an fp32 scale t and S = sum of its weights w:
 //   y = (sum_k q w - z S) t s + bias, the bracket exact in 32 bits up to K = 65536 (255 * 128 * 65536 < 2^31), then one rounding for each operation and one for the output.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -53,7 +54,7 @@ __device__ __forceinline__ typename Operands<KIND>::Sum multiply(v4i weight, v4i
 
 // What a product reads and writes.
 struct Product {
-    const uint8_t* a;      // rows, `pitch` bytes apart
+    const uint8_t* a;      // dense rows of 8-bit integers by tiles, others `pitch` bytes apart
     const float* scale;    // of the rows (8-bit integers)
     const int* zero;       // zero points of the rows, or null
     const uint8_t* w;      // tiles

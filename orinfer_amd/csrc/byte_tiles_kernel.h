@@ -1,7 +1,7 @@
 // Products of many rows with weights by byte tiles, dense and routed experts: tiles of the output from LDS.
 //
 // DOWN x ACROSS waves share a tile, each ROWS x CHANNELS blocks of 16 x 16 of it; K goes in steps of 128 bytes.  Rows and weights come from memory to LDS without passing a register, two
-// stages.  Weights arrive as they are laid out, a kilobyte to a request; of a row, which lies anywhere, the 128 bytes of a step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the
+// or three stages.  Weights and dense rows arrive as they are laid out, a kilobyte to a request; of an expert's row, which lies anywhere, the 128 bytes of a step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the
 // sixteen rows of a read meet different banks.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied, and
 // results drain under the next multiplies.
 #pragma once
@@ -33,8 +33,9 @@ template <int KIND, typename FORM, bool WIDE, bool GROUPED, bool SWIGLU>
 __global__ __launch_bounds__(64 * FORM::waves, 2) void byte_tiles_kernel(Product p) {
     using Sum = typename Operands<KIND>::Sum;
     constexpr int ROWS = FORM::rows, CHANNELS = FORM::channels, DOWN = FORM::down, WAVES = FORM::waves, STAGES = FORM::stages, BM = FORM::bm, BN = FORM::bn;
-    constexpr int A_REQUESTS = BM / 8 / WAVES, W_REQUESTS = BN / 16 / WAVES;  // of a wave and step: eight rows, a tile
-    constexpr int kAll = A_REQUESTS + W_REQUESTS, kLoads = A_REQUESTS + 2 * W_REQUESTS;
+    constexpr bool TILED = !GROUPED;  // the rows' layout
+    constexpr int A_REQUESTS = BM / (TILED ? 16 : 8) / WAVES, W_REQUESTS = BN / 16 / WAVES;  // of a wave and step: a tile of rows or eight rows, a tile
+    constexpr int kAll = A_REQUESTS + W_REQUESTS, kLoads = (TILED ? 2 : 1) * A_REQUESTS + 2 * W_REQUESTS;
     constexpr int kW = BM * kStep, kStage = FORM::stage;
     constexpr int kScales = STAGES * kStage, kScaleBytes = FORM::template scales<GROUPED>(), kTokens = kScales + (KIND == I8 ? (STAGES + 1) * kScaleBytes : 0);
     constexpr int kZeros = 4 * BM, kChannels = GROUPED ? 4 * BM : 8 * BM;  // of a tile's scales
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(64 * FORM::waves, 2) void byte_tiles_kernel(Product
     };
 
     // ---- requests ----
-    const uint8_t* a_from[A_REQUESTS];  // this lane's piece of eight rows
+    const uint8_t* a_from[A_REQUESTS];  // a tile, or this lane's piece of eight rows
     const uint8_t* w_from[W_REQUESTS];  // a tile
     auto piece_of = [&](int b) __attribute__((always_inline)) { return (lane & 7) ^ ((((wave * A_REQUESTS + b) * 8 + (lane >> 3)) >> 1) & 7); };
     // 16-bit rows may end within a step: the pieces behind come from the weights' padding, which is 0
@@ -103,7 +104,10 @@ __global__ __launch_bounds__(64 * FORM::waves, 2) void byte_tiles_kernel(Product
         load_at = tile_of(load_tile);
         const Tile& t = load_at;
 #pragma unroll
-        for (int b = 0; b < A_REQUESTS; ++b) a_from[b] = p.a + row_of(t, (wave * A_REQUESTS + b) * 8 + (lane >> 3), load_tile) * p.pitch + piece_of(b) * 16;
+        for (int b = 0; b < A_REQUESTS; ++b) {
+            if constexpr (TILED) a_from[b] = uniform_pointer(p.a + (int64_t)min(t.first_row / 16 + wave * A_REQUESTS + b, (p.m - 1) / 16) * p.steps * kTileBytes);
+            else a_from[b] = p.a + row_of(t, (wave * A_REQUESTS + b) * 8 + (lane >> 3), load_tile) * p.pitch + piece_of(b) * 16;
+        }
         const int64_t expert = (int64_t)t.expert * p.steps * p.tiles;
 #pragma unroll
         for (int b = 0; b < W_REQUESTS; ++b) w_from[b] = uniform_pointer(p.w + (expert + min(t.group * (BN / 16) + wave * W_REQUESTS + b, p.tiles - 1)) * kTileBytes);
@@ -137,7 +141,10 @@ __global__ __launch_bounds__(64 * FORM::waves, 2) void byte_tiles_kernel(Product
         // (uniform, which the compiler does not see in every form)
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds_base + stage);
         const int take = __builtin_amdgcn_readfirstlane(wanted);
-        if constexpr (ID < A_REQUESTS) {
+        if constexpr (ID < A_REQUESTS && TILED) {
+            request_tile(lane * 16, a_from[ID], to + (wave * A_REQUESTS + ID) * kTileBytes, take);
+            a_from[ID] += kTileBytes;
+        } else if constexpr (ID < A_REQUESTS) {
             const uint8_t* from = a_from[ID];
             if constexpr (KIND != I8) from = load_step == partial_step && piece_of(ID) >= last_pieces ? zeros : from;
             request_16_from(from, to + (wave * A_REQUESTS + ID) * 1024, take);
@@ -151,14 +158,14 @@ __global__ __launch_bounds__(64 * FORM::waves, 2) void byte_tiles_kernel(Product
 
     // ---- operands: halves of a step, 64 bytes of K ----
     const int r = lane & 15, piece = lane >> 4;  // row or channel of a block; pieces `piece` and 4 behind of a step
-    const uint32_t a_at = (wave_m * 16 * ROWS + r) * kStep + (piece ^ ((r >> 1) & 7)) * 16;
+    const uint32_t a_at = TILED ? wave_m * ROWS * kTileBytes + lane * 16 : (wave_m * 16 * ROWS + r) * kStep + (piece ^ ((r >> 1) & 7)) * 16;
     const uint32_t w_at = kW + wave_n * CHANNELS * kTileBytes + lane * 16;
     // A half's operands are read while the half before is multiplied.  Rows, where there are many, into the registers whose last multiply has just been issued.
     constexpr int kHeldRows = ROWS > 4 ? 1 : 2;
     v4i fa[kHeldRows][ROWS], fw[2][CHANNELS];
     auto read_row = [&](auto half, auto i, uint32_t stage) __attribute__((always_inline)) {
         constexpr int H = decltype(half)::value, I = decltype(i)::value;
-        fa[H % kHeldRows][I] = *reinterpret_cast<const v4i*>(lds + ((a_at ^ (H * 64)) + stage) + I * (16 * kStep));
+        fa[H % kHeldRows][I] = *reinterpret_cast<const v4i*>(lds + ((TILED ? a_at : a_at ^ (H * 64)) + stage) + I * (16 * kStep) + (TILED ? H * 1024 : 0));
     };
     auto read_weight = [&](auto half, auto j, uint32_t stage) __attribute__((always_inline)) {
         constexpr int H = decltype(half)::value, J = decltype(j)::value;

@@ -14,6 +14,9 @@ namespace {
 
 using namespace bytes;
 
+// Waves that share a row which is quantised here, of all that a workgroup has.
+__host__ __device__ constexpr int rows_waves(int rows, int waves) { return rows == 1 ? waves : rows == 2 ? waves / 2 : rows <= waves / 2 ? waves / (rows <= 4 ? 4 : 8) : 1; }
+
 // 16 bytes of a lane from a buffer of `bytes`; what lies behind its end reads as 0 and is not fetched.
 struct Buffer {
     __amdgpu_buffer_rsrc_t from;
@@ -21,34 +24,44 @@ struct Buffer {
     __device__ __forceinline__ v4i load_16(int offset) const { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0)); }
 };
 
-constexpr int kPieces = 8;  // of eight values, of a thread, that a row of a workgroup of eight waves may take (QUANTISE)
+// ROWS blocks of 16 rows to a workgroup of WAVES waves, and two tiles of 16 channels (SwiGLU: gate and up), one where the rows are quantised here and a tile has its results for itself.
+// SOURCE: mx::F16 or mx::BF16 rows to quantise, up to PIECES pieces of eight values to a thread; -1 rows as the product takes them.
+constexpr int tiles_of(int source, bool swiglu) { return source >= 0 && !swiglu ? 1 : 2; }
 
-// ROWS blocks of 16 rows, two tiles of 16 channels (SwiGLU: gate and up) to a workgroup of WAVES waves.  SOURCE: mx::F16 or mx::BF16 rows to quantise, -1 rows as the product takes them.
-template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, bool ZERO, bool GROUPED, bool SWIGLU>
-__global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
+template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool ZERO, bool GROUPED, bool SWIGLU>
+__global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void byte_rows_kernel(Product p) {
     using Sum = typename Operands<KIND>::Sum;
-    constexpr int TILES = 2;
+    constexpr int TILES = tiles_of(SOURCE, SWIGLU);
     constexpr bool QUANTISE = SOURCE >= 0;
-    extern __shared__ __align__(16) uint8_t lds[];  // sums, or the rows' codes before them
-    Sum(*const sums)[ROWS * TILES][64] = reinterpret_cast<Sum(*)[ROWS * TILES][64]>(lds);
+    constexpr bool TILED = KIND == I8 && !GROUPED && !QUANTISE;  // the rows' layout
+    extern __shared__ __align__(16) uint8_t lds[];  // the rows' codes, and behind them the waves' sums (dense: two items' in turn)
     __shared__ RowRange ranges[WAVES];
-    __shared__ RowScale row_scales[16 * ROWS];
+    __shared__ RowScale row_scales[GROUPED ? 1 : 2][16 * ROWS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int groups = (p.tiles + TILES - 1) / TILES;
-    const int unit = blockIdx.x / groups, group = blockIdx.x % groups;
-    int first_row = unit * (16 * ROWS), rows = min(p.m - first_row, 16 * ROWS);
-    const uint8_t* w = p.w;
-    int64_t channels = 0;  // of the experts in front of this one
-    if (GROUPED) {
-        if (unit >= *p.unit_count) return;
-        const int4 u = p.units[unit];
-        first_row = __builtin_amdgcn_readfirstlane(u.y), rows = __builtin_amdgcn_readfirstlane(u.z);
-        const int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane(u.x) * p.tiles;
-        w += tile * p.steps * kTileBytes, channels = tile * 16;
-    }
-    auto row_at = [&](int local) {
-        int64_t row = max(first_row + min(local, rows - 1), 0);  // (rows that are not there repeat the last: their sums go nowhere)
+
+    // ---- items: the rows of a unit by TILES tiles of channels; dense launches deal several to a workgroup, whose weights follow one another without a pause ----
+    struct Item {
+        int first_row, rows, group;
+        int64_t tile;  // of its expert, the first
+    };
+    const int items = GROUPED ? 0 : groups * ((p.m + 16 * ROWS - 1) / (16 * ROWS));
+    auto item_of = [&](int id) __attribute__((always_inline)) {
+        Item item;
+        const int unit = id / groups;
+        item.group = id % groups, item.first_row = unit * (16 * ROWS), item.rows = min(p.m - item.first_row, 16 * ROWS), item.tile = 0;
+        if (GROUPED) {
+            const int4 u = p.units[unit];
+            item.first_row = __builtin_amdgcn_readfirstlane(u.y), item.rows = __builtin_amdgcn_readfirstlane(u.z);
+            item.tile = (int64_t)__builtin_amdgcn_readfirstlane(u.x) * p.steps * p.tiles;
+        }
+        return item;
+    };
+    Item item = item_of(blockIdx.x);  // (a list holds as many units as there are workgroups for: read beside their number)
+    if (GROUPED && (int)(blockIdx.x / groups) >= __builtin_amdgcn_readfirstlane(*p.unit_count)) return;
+    auto row_at = [&](const Item& item, int local) __attribute__((always_inline)) {
+        int64_t row = max(item.first_row + min(local, item.rows - 1), 0);  // (rows that are not there repeat the last: their sums go nowhere)
         if (GROUPED && p.slot_token != nullptr) row = p.slot_token[row];
         return row;
     };
@@ -56,13 +69,13 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
 
     // ---- rows to quantise: what a thread holds of its row ----
     constexpr int TYPE = QUANTISE ? SOURCE : mx::F16;
-    const int row_waves = rows == 1 ? WAVES : rows == 2 ? WAVES / 2 : rows <= 4 ? WAVES / 4 : 1;  // to a row
+    const int rows = item.rows, row_waves = rows_waves(rows, WAVES);  // to a row
     const int row_pieces = p.steps * 16, my_row = wave / row_waves, in_row = wave % row_waves * 64 + lane;
-    uint32_t words[QUANTISE ? kPieces : 1][4];
-    auto read_row = [&](int row) {
-        const uint16_t* const x = reinterpret_cast<const uint16_t*>(p.a) + row_at(row) * (p.row_bytes);  // (row_bytes of codes, as many values)
+    uint32_t words[QUANTISE ? PIECES : 1][4];
+    auto read_row = [&](int row) __attribute__((always_inline)) {
+        const uint16_t* const x = reinterpret_cast<const uint16_t*>(p.a) + row_at(item, row) * p.row_bytes;  // (row_bytes of codes, as many values)
 #pragma unroll
-        for (int i = 0; i < (QUANTISE ? kPieces : 0); ++i) {
+        for (int i = 0; i < (QUANTISE ? PIECES : 0); ++i) {
             const int first = (in_row + i * row_waves * 64) * 8, count = p.row_bytes - first;
             v4u four = {0, 0, 0, 0};
             if (i * row_waves * 64 < row_pieces) {
@@ -82,19 +95,33 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
         v4i w[TILES][2], a[ROWS][2];
     };
     const uint8_t* a[ROWS];
-    if constexpr (!QUANTISE) {
+    auto aim = [&](const Item& item) __attribute__((always_inline)) {
+        if constexpr (!QUANTISE) {
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) a[i] = p.a + row_at(16 * i + r) * p.pitch;
-    }
-    auto load = [&](Step& s, int step) {
+            for (int i = 0; i < ROWS; ++i)
+                a[i] = TILED ? p.a + (int64_t)min(item.first_row / 16 + i, (p.m - 1) / 16) * p.steps * kTileBytes : p.a + row_at(item, 16 * i + r) * p.pitch;
+        }
+    };
+    auto load = [&](Step& s, const Item& item, int step) __attribute__((always_inline)) {  // (what lies behind the last step reads as 0)
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const int64_t tile = (int64_t)step * p.tiles + min(group * TILES + t, p.tiles - 1);
-            const Buffer codes(w + tile * kTileBytes, step < p.steps ? kTileBytes : 0);
+            const int64_t tile = item.tile + (int64_t)step * p.tiles + min(item.group * TILES + t, p.tiles - 1);
+            const Buffer codes(p.w + tile * kTileBytes, step < p.steps ? kTileBytes : 0);
             s.w[t][0] = codes.load_16(lane * 16);
             s.w[t][1] = codes.load_16(lane * 16 + 1024);
         }
-        if constexpr (!QUANTISE) {
+        if constexpr (TILED) {
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                if constexpr (ROWS <= 2) {  // (beside the weights' loads; with 64 rows plain loads are faster)
+                    const Buffer codes(a[i] + (int64_t)step * kTileBytes, step < p.steps ? kTileBytes : 0);
+                    s.a[i][0] = codes.load_16(lane * 16), s.a[i][1] = codes.load_16(lane * 16 + 1024);
+                } else {
+                    const uint8_t* const from = a[i] + (int64_t)min(step, p.steps - 1) * kTileBytes + lane * 16;
+                    s.a[i][0] = *reinterpret_cast<const v4i*>(from), s.a[i][1] = *reinterpret_cast<const v4i*>(from + 1024);
+                }
+            }
+        } else if constexpr (!QUANTISE) {
             // (16-bit rows end where they end: pieces behind that are 0, and read the row's first one)
             const int at = min(step, p.steps - 1) * kStep + piece * 16;
             const bool there[2] = {KIND == I8 || at < p.row_bytes, KIND == I8 || at + 64 < p.row_bytes};
@@ -108,18 +135,20 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
         }
     };
     Step held[AHEAD];
+    aim(item);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load(held[i], wave + i * WAVES);
+    for (int i = 0; i < AHEAD; ++i) load(held[i], item, wave + i * WAVES);
 
     // ---- the rows' codes ----
     const int live = min(rows, 16);
+    const uint32_t codes_bytes = QUANTISE ? (uint32_t)p.steps * kStep * live : 0;
     if constexpr (QUANTISE) {
         for (int first = 0; first < rows; first += WAVES / row_waves) {
             const int row = first + my_row;
             if (first > 0) read_row(min(row, rows - 1));
             RowRange range = {0, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) widen<TYPE, ZERO>(range, words[i]);
+            for (int i = 0; i < PIECES; ++i) widen<TYPE, ZERO>(range, words[i]);
             range = over_wave<TYPE, ZERO>(range);
             if (row_waves > 1) {  // (then one round takes all rows)
                 if (lane == 0) ranges[wave] = range;
@@ -132,108 +161,129 @@ __global__ __launch_bounds__(WAVES * 64) void byte_rows_kernel(Product p) {
             const RowCode code = code_of<TYPE, ZERO>(range);
             if (row < rows) {
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
+                for (int i = 0; i < PIECES; ++i) {
                     const int at = in_row + i * row_waves * 64;
                     if (at < row_pieces) *reinterpret_cast<uint2*>(lds + ((int64_t)(at >> 1) * live + row) * 16 + (at & 1) * 8) = eight_codes<TYPE, ZERO>(words[i], code);
                 }
-                if (wave % row_waves == 0 && lane == 0) row_scales[row] = {stored_scale(code), code.zero};
+                if (wave % row_waves == 0 && lane == 0) row_scales[0][row] = {stored_scale(code), code.zero};
             }
         }
         __syncthreads();
-    } else if constexpr (KIND == I8) {
-        for (int i = threadIdx.x; i < 16 * ROWS; i += WAVES * 64) {
-            const int64_t row = row_at(i);
-            row_scales[i] = {p.scale[row], ZERO ? p.zero[row] : 0};
-        }
     }
 
-    Sum sum[ROWS][TILES];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) sum[i][t] = Sum{};
-    auto multiply_step = [&](Step& s, int step) {
-        if constexpr (QUANTISE) {
-            const int there = min(step, p.steps - 1), row = min(r, live - 1);
-            const uint8_t* const from = lds + ((there * 8 + piece) * live + row) * 16;
-            s.a[0][0] = *reinterpret_cast<const v4i*>(from);
-            s.a[0][1] = *reinterpret_cast<const v4i*>(from + 4 * live * 16);
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) sum[i][t] = multiply<KIND>(s.w[t][half], s.a[i][half], sum[i][t]);
-    };
-#pragma unroll 1
-    for (int step = wave; step < p.steps; step += AHEAD * WAVES) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (step + i * WAVES < p.steps) multiply_step(held[i], step + i * WAVES);
-            if (step + (i + AHEAD) * WAVES < p.steps) load(held[i], step + (i + AHEAD) * WAVES);
-        }
-    }
-    if constexpr (QUANTISE) __syncthreads();  // (the sums take the codes' place)
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) sums[wave][i * TILES + t][lane] = sum[i][t];
-    __syncthreads();
+    const int chunks = (p.steps + AHEAD * WAVES - 1) / (AHEAD * WAVES);  // of AHEAD steps to a wave
     constexpr int KINDS = SWIGLU ? 2 : 1;
-    for (int q = threadIdx.x; q < ROWS * TILES / KINDS * 64; q += WAVES * 64) {
-        const int l = q & 63, i = (q >> 6) / (TILES / KINDS), t = (q >> 6) % (TILES / KINDS);
-        const int row = 16 * i + (l & 15);
-        v4f total[KINDS];
-#pragma unroll
-        for (int kind = 0; kind < KINDS; ++kind) {
-            Sum all = sums[0][i * TILES + t * KINDS + kind][l];
-#pragma unroll
-            for (int other = 1; other < WAVES; ++other) all += sums[other][i * TILES + t * KINDS + kind][l];
-            const int64_t at = channels + min(group * TILES + t * KINDS + kind, p.tiles - 1) * 16 + 4 * (l >> 4);
-            Channels channel = {};
-            if constexpr (KIND == I8) {
-                channel.scale = *reinterpret_cast<const v4f*>(p.w_scale + at);
-                if (ZERO) channel.sum = *reinterpret_cast<const v4i*>(p.w_sum + at);
-                if (!GROUPED && p.bias != nullptr) channel.bias = *reinterpret_cast<const v4f*>(p.bias + at);
+    int turn = 0;
+#pragma unroll 1
+    for (int id = blockIdx.x;;) {
+        const int next_id = id + (int)gridDim.x;
+        const bool more = !GROUPED && next_id < items;
+        const Item next = more ? item_of(next_id) : item;
+        if constexpr (KIND == I8 && !QUANTISE) {
+            for (int i = threadIdx.x; i < 16 * ROWS; i += WAVES * 64) {
+                const int64_t row = row_at(item, i);
+                row_scales[turn][i] = {p.scale[row], ZERO ? p.zero[row] : 0};
             }
-            total[kind] = scaled<KIND, !GROUPED>(all, channel, KIND == I8 ? row_scales[min(row, rows - 1)] : RowScale{});
         }
-        if constexpr (SWIGLU) {
+        Sum sum[ROWS][TILES];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) total[0][j] = mx::swiglu(total[0][j], total[KINDS - 1][j]);
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) sum[i][t] = Sum{};
+        auto multiply_step = [&](Step& s, int step) __attribute__((always_inline)) {
+            if constexpr (QUANTISE) {
+                const int there = min(step, p.steps - 1), row = min(r, live - 1);
+                const uint8_t* const from = lds + ((there * 8 + piece) * live + row) * 16;
+                s.a[0][0] = *reinterpret_cast<const v4i*>(from);
+                s.a[0][1] = *reinterpret_cast<const v4i*>(from + 4 * live * 16);
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) sum[i][t] = multiply<KIND>(s.w[t][half], s.a[i][half], sum[i][t]);
+        };
+        int step = wave;
+#pragma unroll 1
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            // (the next chunk's weights, or the next item's first ones, or none)
+            const bool last = chunk == chunks - 1;
+            if (last && more) aim(next);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                // (an infinity of a 16-bit row times the zeros behind the last step would be NaN)
+                if (KIND == I8 || step + i * WAVES < p.steps) multiply_step(held[i], step + i * WAVES);
+                const int then = last ? (more ? wave + i * WAVES : p.steps) : step + (i + AHEAD) * WAVES;
+                if (!GROUPED || then < p.steps) load(held[i], last ? next : item, then);
+            }
+            step += AHEAD * WAVES;
         }
-        if (row < rows)
-            mx::store_four(p.out, p.type, (int64_t)(first_row + row) * p.cols, ((group * TILES) / KINDS + t) * 16 + 4 * (l >> 4), p.cols, total[0]);
+        Sum(*const sums)[ROWS * TILES][64] = reinterpret_cast<Sum(*)[ROWS * TILES][64]>(lds + codes_bytes) + turn * WAVES;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) sums[wave][i * TILES + t][lane] = sum[i][t];
+        __syncthreads();
+        for (int q = threadIdx.x; q < ROWS * TILES / KINDS * 64; q += WAVES * 64) {
+            const int l = q & 63, i = (q >> 6) / (TILES / KINDS), t = (q >> 6) % (TILES / KINDS);
+            const int row = 16 * i + (l & 15);
+            v4f total[KINDS];
+#pragma unroll
+            for (int kind = 0; kind < KINDS; ++kind) {
+                Sum all = sums[0][i * TILES + t * KINDS + kind][l];
+#pragma unroll
+                for (int other = 1; other < WAVES; ++other) all += sums[other][i * TILES + t * KINDS + kind][l];
+                const int64_t at = item.tile / p.steps * 16 + min(item.group * TILES + t * KINDS + kind, p.tiles - 1) * 16 + 4 * (l >> 4);
+                Channels channel = {};
+                if constexpr (KIND == I8) {
+                    channel.scale = *reinterpret_cast<const v4f*>(p.w_scale + at);
+                    if (ZERO) channel.sum = *reinterpret_cast<const v4i*>(p.w_sum + at);
+                    if (!GROUPED && p.bias != nullptr) channel.bias = *reinterpret_cast<const v4f*>(p.bias + at);
+                }
+                total[kind] = scaled<KIND, !GROUPED>(all, channel, KIND == I8 ? row_scales[QUANTISE ? 0 : turn][min(row, item.rows - 1)] : RowScale{});
+            }
+            if constexpr (SWIGLU) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) total[0][j] = mx::swiglu(total[0][j], total[KINDS - 1][j]);
+            }
+            if (row < item.rows)
+                mx::store_four(p.out, p.type, (int64_t)(item.first_row + row) * p.cols, ((item.group * TILES) / KINDS + t) * 16 + 4 * (l >> 4), p.cols, total[0]);
+        }
+        if (!more) return;
+        item = next, id = next_id;
+        turn ^= GROUPED ? 0 : 1;
     }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
 // slots used: M (rows; experts: slots), N, K, E, tiles (units), block_m, flags, flags2 (kind), algorithm (output type), H (output columns), slots (16-channel tiles), packed_k (source of the rows, plus 1)
 enum { kSwiglu = 1, kGather = 2, kZero = 4, kBias = 8 };
-constexpr int kMostLds = 80 * 1024;
+constexpr int kMostLds = 128 * 1024;
 
 int steps_of(const orx_function& f) { return (f.K * (f.flags2 == I8 ? 1 : 2) + kStep - 1) / kStep; }
 
-// What a launch of `rows` rows runs: a unit's rows, and the form of the tiles from LDS (-1: the kernel above, 32 channels to a workgroup), or its waves
+// What a launch of `rows` rows runs: a unit's rows, and the form of the tiles from LDS (-1: the kernel above), or its waves
 struct Plan {
     int rows, form, waves;
 };
-Plan few_rows(int unit_rows) { return {unit_rows, -1, unit_rows == 64 ? 4 : 8}; }
+// Of few steps fewer waves have one.
+Plan few_rows(const orx_function& f, int unit_rows) { return {unit_rows, -1, unit_rows == 64 || (unit_rows == 16 && steps_of(f) <= 8) ? 4 : 8}; }
 Plan plan(const orx_function& f, int rows) {
-    if (f.E > 0) return f.block_m == 16 ? few_rows(16) : Plan{f.block_m, f.block_m == 64 ? kTiles64 : f.block_m == 256 ? kTiles256 : kTiles128x256, 0};
-    if (rows <= 64) return few_rows(rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
+    if (f.E > 0) return f.block_m == 16 ? few_rows(f, 16) : Plan{f.block_m, f.block_m == 64 ? kTiles64 : f.block_m == 256 ? kTiles256 : kTiles128x256, 0};
+    if (rows <= 64) return few_rows(f, rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
     return rows >= 1024 ? Plan{256, kTiles256, 0} : Plan{128, kTiles128, 0};
 }
+int tiles_of(const orx_function& f) { return tiles_of(f.packed_k - 1, f.flags & kSwiglu); }
 uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
-    const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * 2 * 1024;
+    const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * tiles_of(f) * 1024;
     const uint32_t codes = f.packed_k == 0 ? 0 : (uint32_t)steps_of(f) * kStep * std::min(f.E > 0 ? 16 : rows, 16);
-    return std::max(sums, codes);
+    return codes + (f.E > 0 ? 1 : 2) * sums;
 }
 
 int geometry(const orx_function& f, int rows, Geometry* g) {
     const Plan plan = orx::plan(f, rows);
-    const TilesShape shape = plan.form < 0 ? TilesShape{plan.rows, 32} : byte_tiles_shape(f.flags2, plan.form, f.E > 0);
+    const TilesShape shape = plan.form < 0 ? TilesShape{plan.rows, 16 * tiles_of(f)} : byte_tiles_shape(f.flags2, plan.form, f.E > 0);
     const int64_t units = f.E > 0 ? (int64_t)f.tiles : ceil_div(rows, plan.rows);
     int64_t blocks = units * ceil_div(f.slots, shape.channels / 16);
     if (blocks >= (1ll << 32) / 512) {
@@ -247,40 +297,64 @@ int geometry(const orx_function& f, int rows, Geometry* g) {
     } else {
         g->block[0] = 64 * plan.waves;
         g->shared = few_rows_lds(f, rows, plan);
+        // As many workgroups as the CUs hold at once, all with as many items.  (Sixteen waves to a CU; with a second round of few workgroups 32 rows of 17408 x 5120 took 19.4 us.)
+        if (f.E == 0) {
+            const int64_t most = (int64_t)device_compute_units() * std::min(16 / plan.waves, (int)(160 * 1024 / (g->shared + 1024)));
+            blocks = ceil_div(blocks, ceil_div(blocks, most));
+        }
     }
     g->grid[0] = (uint32_t)blocks;
     return ORX_OK;
 }
 
-template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, bool ZERO, bool GROUPED, bool SWIGLU>
+// Pieces to a thread where the rows are quantised by the product: a row of the most that there may be at once (of an expert 16).
+int pieces_of(const orx_function& f, int rows, int waves) { return (steps_of(f) * 16 + 64 * rows_waves(f.E > 0 ? 16 : rows, waves) - 1) / (64 * rows_waves(f.E > 0 ? 16 : rows, waves)); }
+
+template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool ZERO, bool GROUPED, bool SWIGLU>
 int launch_one(const Product& p, const Geometry& g, hipStream_t s) {
-    constexpr auto kernel = &byte_rows_kernel<KIND, ROWS, WAVES, AHEAD, SOURCE, ZERO, GROUPED, SWIGLU>;
+    constexpr auto kernel = &byte_rows_kernel<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, ZERO, GROUPED, SWIGLU>;
     static DeviceOnce ready;
     const int code = ready.run([] { return hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds), "hipFuncSetAttribute"); });
     if (code != ORX_OK) return code;
     ORX_LAUNCH(kernel, dim3(g.grid[0]), dim3(64 * WAVES), g.shared, s, p);
     return hip_check(hipGetLastError(), "launch byte product");
 }
-template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, bool ZERO, bool GROUPED>
+template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool GROUPED>
 int launch_of(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
-    return f.flags & kSwiglu ? launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, ZERO, GROUPED, true>(p, g, s) : launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, ZERO, GROUPED, false>(p, g, s);
+    const bool swiglu = f.flags & kSwiglu;
+    if constexpr (KIND == I8 && !GROUPED)
+        if (f.flags & kZero)
+            return swiglu ? launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, true, GROUPED, true>(p, g, s) : launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, true, GROUPED, false>(p, g, s);
+    return swiglu ? launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, false, GROUPED, true>(p, g, s) : launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, false, GROUPED, false>(p, g, s);
 }
-template <int ROWS, int WAVES, int AHEAD, int SOURCE>
-int launch_dense(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
-    return f.flags & kZero ? launch_of<I8, ROWS, WAVES, AHEAD, SOURCE, true, false>(f, p, g, s) : launch_of<I8, ROWS, WAVES, AHEAD, SOURCE, false, false>(f, p, g, s);
+// 16 rows as the product takes them: two steps on their way, of an expert's that has many four (dense, which follow one another, they do not fit the registers).
+template <int KIND, bool GROUPED>
+int launch_16(const orx_function& f, int waves, const Product& p, const Geometry& g, hipStream_t s) {
+    if (waves == 4) return launch_of<KIND, 1, 4, 2, -1, 1, GROUPED>(f, p, g, s);
+    if constexpr (GROUPED)
+        if (steps_of(f) > 16) return launch_of<KIND, 1, 8, 4, -1, 1, GROUPED>(f, p, g, s);
+    return launch_of<KIND, 1, 8, 2, -1, 1, GROUPED>(f, p, g, s);
+}
+template <int SOURCE, bool GROUPED>
+int launch_quantising(const orx_function& f, int rows, int waves, const Product& p, const Geometry& g, hipStream_t s) {
+    if (waves == 4) return launch_of<I8, 1, 4, 2, SOURCE, 4, GROUPED>(f, p, g, s);
+    if (pieces_of(f, rows, waves) > 4) return launch_of<I8, 1, 8, 2, SOURCE, 8, GROUPED>(f, p, g, s);
+    return f.flags & kSwiglu && !GROUPED ? launch_of<I8, 1, 8, 2, SOURCE, 4, GROUPED>(f, p, g, s) : launch_of<I8, 1, 8, 4, SOURCE, 4, GROUPED>(f, p, g, s);
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
     if (plan.form >= 0) return launch_byte_tiles(p, f.flags2, plan.form, f.E > 0, f.flags & kSwiglu, g.grid[0], s);
-    if (f.E > 0) {
-        if (f.flags2 == F16) return launch_of<F16, 1, 8, 2, -1, false, true>(f, p, g, s);
-        if (f.flags2 == BF16) return launch_of<BF16, 1, 8, 2, -1, false, true>(f, p, g, s);
-        if (f.packed_k == 0) return launch_of<I8, 1, 8, 2, -1, false, true>(f, p, g, s);
-        return f.packed_k - 1 == mx::F16 ? launch_of<I8, 1, 8, 2, mx::F16, false, true>(f, p, g, s) : launch_of<I8, 1, 8, 2, mx::BF16, false, true>(f, p, g, s);
+    if (f.packed_k != 0) {
+        const bool brains = f.packed_k - 1 == mx::BF16;
+        if (f.E > 0) return brains ? launch_quantising<mx::BF16, true>(f, rows, plan.waves, p, g, s) : launch_quantising<mx::F16, true>(f, rows, plan.waves, p, g, s);
+        return brains ? launch_quantising<mx::BF16, false>(f, rows, plan.waves, p, g, s) : launch_quantising<mx::F16, false>(f, rows, plan.waves, p, g, s);
     }
-    if (f.packed_k != 0) return f.packed_k - 1 == mx::F16 ? launch_dense<1, 8, 2, mx::F16>(f, p, g, s) : launch_dense<1, 8, 2, mx::BF16>(f, p, g, s);
-    if (plan.rows == 16) return launch_dense<1, 8, 2, -1>(f, p, g, s);
-    return plan.rows == 32 ? launch_dense<2, 8, 2, -1>(f, p, g, s) : launch_dense<4, 4, 1, -1>(f, p, g, s);
+    if (f.E > 0) {
+        if (f.flags2 == F16) return launch_16<F16, true>(f, plan.waves, p, g, s);
+        return f.flags2 == BF16 ? launch_16<BF16, true>(f, plan.waves, p, g, s) : launch_16<I8, true>(f, plan.waves, p, g, s);
+    }
+    if (plan.rows == 16) return launch_16<I8, false>(f, plan.waves, p, g, s);
+    return plan.rows == 32 ? launch_of<I8, 2, 8, 2, -1, 1, false>(f, p, g, s) : launch_of<I8, 4, 4, 1, -1, 1, false>(f, p, g, s);
 }
 
 Product product_of(const orx_function& f, int rows) {
@@ -318,9 +392,10 @@ int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream
 }
 
 // Rows that a product quantises itself: their codes fit LDS, and a thread holds its part of a row.
+constexpr int kMostPieces = 8;
 bool quantises(const orx_function& f, int rows) {
-    const int row_waves = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1;
-    return rows <= 16 && few_rows_lds(f, rows, few_rows(16)) <= (uint32_t)kMostLds && steps_of(f) * 16 <= row_waves * 64 * kPieces;
+    const Plan plan = few_rows(f, 16);
+    return rows <= 16 && few_rows_lds(f, rows, plan) <= (uint32_t)kMostLds && pieces_of(f, rows, plan.waves) <= (plan.waves == 4 ? 4 : kMostPieces);
 }
 
 // What all three have: N, K, epilogue, types.
@@ -369,7 +444,7 @@ int make_grouped(const Variant& v, orx_function* f) {
     }
     f->capacity = f->M;
     if (f->packed_k != 0 && (f->block_m != 16 || !quantises(*f, 16))) {
-        set_error("%s: 16-bit rows go with block_m 16 and K up to %d", f->symbol.c_str(), 64 * 8 * kPieces);
+        set_error("%s: 16-bit rows go with block_m 16 and K up to %d", f->symbol.c_str(), 64 * 8 * kMostPieces);
         return ORX_ERR_BAD_VARIANT;
     }
     f->args = {{"A", ArgPointer, f->packed_k != 0 ? 2u : 16u}};
@@ -399,7 +474,7 @@ int make_int8_projection(const Variant& v, orx_function* f) {
     }
     f->capacity = f->M;
     if (f->packed_k != 0 && !quantises(*f, f->M)) {
-        set_error("int8_token_projection: 16-bit rows go with M up to 16 and short K: codes of all rows up to %d bytes, rows of %d values (M 1: 8 times that, 2: 4, 4: 2)", kMostLds, 64 * 8 * kPieces);
+        set_error("int8_token_projection: 16-bit rows go with M up to 16 and short K: codes of all rows up to %d bytes, rows of %d values (M 1: 8 times that, 2: 4, 4: 2)", kMostLds, 64 * 8 * kMostPieces);
         return ORX_ERR_BAD_VARIANT;
     }
     f->args = {{"A", ArgPointer, f->packed_k != 0 ? 2u : 16u}};

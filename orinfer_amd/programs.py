@@ -980,14 +980,15 @@ class Int8Linear(_OnDevice):
         shape = dict(N=channels, K=self.k, dynamic_rows=True, zero_points=self.zero_points, bias=bias is not None, epilogue=epilogue, output_dtype=name)
         with torch.cuda.device(self.device):
             self.projection = Kernel("int8_token_projection", M=capacity, **shape)
-            self.quantizer = Kernel("int8_token_quantization", M=capacity, K=self.k, input_dtype=name, zero_points=self.zero_points)
+            self.quantizer = Kernel("int8_token_quantization", M=capacity, K=self.k, input_dtype=name, zero_points=self.zero_points, layout="tiles")
             # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two.  Not where their codes do not fit LDS, or a row its threads.
             self.few, self.few_rows = None, 0
             for rows in (4, 2, 1):
                 if self.few is None and rows <= capacity:
                     self.few, self.few_rows = _where_it_fits("int8_token_projection", M=rows, input_dtype=name, **shape), rows
         self.n = channels // 2 if paired else channels
-        self.a_q = torch.empty((capacity, int8.padded(self.k)), dtype=torch.int8, device=self.device)
+        # the quantised rows, by tiles of 16
+        self.a_q = torch.empty((-(-capacity // 16), -(-self.k // int8.STEP), 2048), dtype=torch.int8, device=self.device)
         self.a_s = torch.empty(capacity, dtype=torch.float32, device=self.device)
         self.a_z = torch.empty(capacity, dtype=torch.int32, device=self.device) if self.zero_points else None
         self.out = torch.empty((capacity, self.n), dtype=dtype, device=self.device)

@@ -60,7 +60,8 @@ def swiglu(want, bound):
 # ---- quantisation ------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("zero_points", [False, True])
 @pytest.mark.parametrize("name", list(TYPES))
-@pytest.mark.parametrize("rows,k", [(1, 1), (1, 8), (3, 33), (5, 100), (7, 2560), (64, 264), (130, 1000), (33, 4096), (9, 2049), (6, 8200), (5, 17408), (2, 40001)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 8), (3, 33), (5, 100), (7, 2560), (64, 264), (130, 1000), (33, 4096), (9, 2049), (6, 8200), (5, 17408), (2, 40001), (4100, 500), (4097, 7),
+                                    (1025, 1100), (1024, 4096), (1026, 5120), (1030, 9000)])
 def test_quantisation_is_the_oracles(rows, k, name, zero_points):
     x = rows_of(np.random.default_rng(rows * k), rows, k, TYPES[name], side=1.0 * zero_points)
     codes, scales, zeros = orc.quantise(x.double().numpy(), zero_points)
@@ -78,6 +79,22 @@ def test_quantisation_is_the_oracles(rows, k, name, zero_points):
     assert (q[:rows, written:] == 91).all() and (q[rows] == 91).all() and s[rows] == 7.5 and z[rows] == 91
     again = int8.quantize(x.to(DEV), zero_points)
     assert torch.equal(again[0], q[:rows, :k]) and torch.equal(again[1], s[:rows]) and (not zero_points or torch.equal(again[2], z[:rows]))
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("rows,k", [(1, 128), (1, 7), (5, 300), (16, 256), (17, 2560), (100, 1000), (33, 4096), (4099, 200), (1030, 1500), (1025, 5000), (19, 9000)])
+def test_quantisation_by_tiles(rows, k, name, zero_points):
+    x = rows_of(np.random.default_rng(rows * k), rows, k, TYPES[name], side=1.0 * zero_points).to(DEV)
+    want = int8.quantize(x, zero_points)
+    tiles, steps = -(-rows // 16), -(-k // 128)
+    q = torch.full((tiles * steps * 2048 + 16,), 91, dtype=torch.int8, device=DEV)
+    s, z = torch.full((rows + 1,), 7.5, device=DEV), torch.full((rows + 1,), 91, dtype=torch.int32, device=DEV)
+    kernel("int8_token_quantization", K=k, input_dtype=name, zero_points=zero_points, layout="tiles")(Q=q, S=s, X=x, rows=rows, **({"Z": z} if zero_points else {}))
+    got = q[:-16].view(tiles, steps, 8, 16, 16).permute(0, 3, 1, 2, 4).reshape(tiles * 16, steps * 128)
+    assert torch.equal(got[:rows, :k], want[0]) and torch.equal(s[:rows], want[1]) and s[rows] == 7.5 and z[rows] == 91 and (q[-16:] == 91).all()
+    assert (got[rows:] == 91).all()  # rows that are not there stay as they were
+    assert torch.equal(z[:rows], want[2]) if zero_points else (got[:rows, k:] == 0).all()
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
@@ -214,7 +231,9 @@ def test_projection_writes_its_rows_and_columns_only(rows, n, k, name):
     rng = np.random.default_rng(n)
     x = rows_of(rng, rows, k, torch.float32)
     w, scale = weights_of(rng, n, k)
-    q, s = int8.quantize(x.to(DEV))
+    q = torch.empty((-(-rows // 16), -(-k // 128), 2048), dtype=torch.int8, device=DEV)
+    s = torch.empty(rows, device=DEV)
+    kernel("int8_token_quantization", K=k, input_dtype="float32", layout="tiles")(Q=q, S=s, X=x.to(DEV), rows=rows)
     project = kernel("int8_token_projection", M=rows + 3, N=n, K=k, dynamic_rows=True, output_dtype=name)
     out = torch.full((rows + 3, n), 91.0, dtype=TYPES[name], device=DEV)
     tiles, channels = byte_tiles.tiles(torch.from_numpy(w)).to(DEV), byte_tiles.channels(torch.from_numpy(scale)).to(DEV)

@@ -73,7 +73,7 @@ GROUPED = dict(rows=12, E=4, N=96, K=320, tiles=8)
 
 @pytest.mark.parametrize("symbol,variant", [
     ("int8_token_quantization", dict(K=0)), ("int8_token_quantization", dict(K=64, input_dtype="int8")), ("int8_token_quantization", dict(K=64, M=0)), ("int8_token_quantization", dict(K=1 << 25)),
-    ("int8_token_quantization", dict(K=64, zero_points=1)), ("int8_token_quantization", dict(K=64, pad=128)),
+    ("int8_token_quantization", dict(K=64, zero_points=1)), ("int8_token_quantization", dict(K=64, pad=128)), ("int8_token_quantization", dict(K=64, layout="columns")),
     ("int8_token_projection", dict(M=17, N=96, K=320, input_dtype="float16")), ("int8_token_projection", dict(M=1, N=96, K=1 << 16, input_dtype="float16")),
     ("int8_token_projection", dict(M=16, N=96, K=8192, input_dtype="bfloat16")), ("int8_token_projection", dict(M=1, N=96, K=320, input_dtype="float32")),
     ("int8_token_projection", dict(M=0, N=96, K=320)), ("int8_token_projection", dict(M=1, N=0, K=320)), ("int8_token_projection", dict(M=1, N=96, K=65537)),
