@@ -4,10 +4,10 @@
 // at byte 16 (l / 16), and of a result four neighbouring rows of the first operand and one of the second.  So one kernel moves the bytes of all three, in steps of 128.
 //
 // Weights are laid out once: a tile is 16 channels x 128 bytes of K, 2048 bytes as [piece 0..7][channel][16 bytes]; the tiles of the same K lie behind one another.
-// A wave's load of an operand is whole kilobytes, with nothing to unpack.  Channels are padded to 16 and K to 128 bytes with zeros.  What a channel has (scale, sum, bias) lies by tiles too.
+// A wave's load of an operand is whole kilobytes, with nothing to unpack.  Channels are padded to 64, four tiles, and K to 256 bytes, two steps, with zeros.  What a channel has (scale, sum, bias) lies by tiles too.
 // SwiGLU: tiles of gate channels and of their up channels take turns, so a lane has both of a pair.
 //
-// Rows of 8-bit integers: x = (q - z) s with an fp32 scale s, and a zero point z or none, for each row, zeros behind K up to a multiple of 128.  Dense rows lie by tiles of 16 rows x 128,
+// Rows of 8-bit integers: x = (q - z) s with an fp32 scale s, and a zero point z or none, for each row, zeros behind K up to a multiple of 256.  Dense rows lie by tiles of 16 rows x 128,
 // [piece][row][16], the tiles of the same rows along K behind one another; rows of experts, which a product takes from anywhere, an odd multiple of 128 bytes apart (at a multiple of 4 KiB they
 // meet in few channels of the L2).  Channel c has an fp32 scale t and S = sum of its weights w:
 //   y = (sum_k q w - z S) t s + bias, the bracket exact in 32 bits up to K = 65536 (255 * 128 * 65536 < 2^31), then one rounding for each operation and one for the output.
@@ -26,9 +26,10 @@ using mx::v4f;
 using mx::v4i;
 using mx::v4u;
 
-constexpr int kStep = 128;        // bytes of K to a step
+constexpr int kStep = 128;        // bytes of K to a step, of which there are pairs
 constexpr int kTileBytes = 2048;  // 16 channels of a step
 constexpr int kMostIntegerK = 65536;
+constexpr int steps_of_bytes(int64_t bytes) { return (int)((bytes + 2 * kStep - 1) / (2 * kStep) * 2); }
 
 enum Kind { I8 = 0, F16 = 1, BF16 = 2 };  // of the operands
 
@@ -51,6 +52,16 @@ __device__ __forceinline__ typename Operands<KIND>::Sum multiply(v4i weight, v4i
     else if constexpr (KIND == F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, weight), __builtin_bit_cast(half8, row), sum, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(brain8, weight), __builtin_bit_cast(brain8, row), sum, 0, 0, 0);
 }
+
+// The same in one register, in and out: left to itself the compiler moves the sums about between unrolled steps, which takes the registers of half a set more.  What it would have inserted is on
+// the caller: two instructions between the last write of an operand by an instruction (not a load) and the multiply, and a pause (settle) in front of the first reading of a sum.
+template <int KIND>
+__device__ __forceinline__ void multiply_in_place(typename Operands<KIND>::Sum& sum, const v4i& weight, const v4i& row) {
+    if constexpr (KIND == I8) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+v"(sum) : "v"(weight), "v"(row));
+    else if constexpr (KIND == F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(sum) : "v"(weight), "v"(row));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(sum) : "v"(weight), "v"(row));
+}
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15"); }
 
 // What a product reads and writes.
 struct Product {

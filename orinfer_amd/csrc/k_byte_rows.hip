@@ -32,21 +32,21 @@ template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool
 __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void byte_rows_kernel(Product p) {
     using Sum = typename Operands<KIND>::Sum;
     constexpr int TILES = tiles_of(SOURCE, SWIGLU);
-    constexpr bool QUANTISE = SOURCE >= 0;
+    constexpr bool QUANTISE = SOURCE >= 0, DEALT = QUANTISE && !GROUPED;
     constexpr bool TILED = KIND == I8 && !GROUPED && !QUANTISE;  // the rows' layout
-    extern __shared__ __align__(16) uint8_t lds[];  // the rows' codes, and behind them the waves' sums (dense: two items' in turn)
+    extern __shared__ __align__(16) uint8_t lds[];  // the rows' codes, and behind them the waves' sums (where several items are dealt, two items' in turn)
     __shared__ RowRange ranges[WAVES];
-    __shared__ RowScale row_scales[GROUPED ? 1 : 2][16 * ROWS];
+    __shared__ RowScale row_scales[16 * ROWS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int groups = (p.tiles + TILES - 1) / TILES;
 
-    // ---- items: the rows of a unit by TILES tiles of channels; dense launches deal several to a workgroup, whose weights follow one another without a pause ----
+    // ---- items: the rows of a unit by TILES tiles of channels; where dense rows are quantised here several to a workgroup (once then for all), whose weights follow one another without a pause ----
     struct Item {
         int first_row, rows, group;
         int64_t tile;  // of its expert, the first
     };
-    const int items = GROUPED ? 0 : groups * ((p.m + 16 * ROWS - 1) / (16 * ROWS));
+    const int items = !DEALT ? 0 : groups * ((p.m + 16 * ROWS - 1) / (16 * ROWS));
     auto item_of = [&](int id) __attribute__((always_inline)) {
         Item item;
         const int unit = id / groups;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
         if constexpr (TILED) {
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-                if constexpr (ROWS <= 2) {  // (beside the weights' loads; with 64 rows plain loads are faster)
+                if constexpr (ROWS == 1) {  // (beside the weights' loads; with 64 rows plain loads are faster)
                     const Buffer codes(a[i] + (int64_t)step * kTileBytes, step < p.steps ? kTileBytes : 0);
                     s.a[i][0] = codes.load_16(lane * 16), s.a[i][1] = codes.load_16(lane * 16 + 1024);
                 } else {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
                     const int at = in_row + i * row_waves * 64;
                     if (at < row_pieces) *reinterpret_cast<uint2*>(lds + ((int64_t)(at >> 1) * live + row) * 16 + (at & 1) * 8) = eight_codes<TYPE, ZERO>(words[i], code);
                 }
-                if (wave % row_waves == 0 && lane == 0) row_scales[0][row] = {stored_scale(code), code.zero};
+                if (wave % row_waves == 0 && lane == 0) row_scales[row] = {stored_scale(code), code.zero};
             }
         }
         __syncthreads();
@@ -177,12 +177,12 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
 #pragma unroll 1
     for (int id = blockIdx.x;;) {
         const int next_id = id + (int)gridDim.x;
-        const bool more = !GROUPED && next_id < items;
+        const bool more = DEALT && next_id < items;
         const Item next = more ? item_of(next_id) : item;
         if constexpr (KIND == I8 && !QUANTISE) {
             for (int i = threadIdx.x; i < 16 * ROWS; i += WAVES * 64) {
                 const int64_t row = row_at(item, i);
-                row_scales[turn][i] = {p.scale[row], ZERO ? p.zero[row] : 0};
+                row_scales[i] = {p.scale[row], ZERO ? p.zero[row] : 0};
             }
         }
         Sum sum[ROWS][TILES];
@@ -212,10 +212,10 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
             if (last && more) aim(next);
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                // (an infinity of a 16-bit row times the zeros behind the last step would be NaN)
-                if (KIND == I8 || step + i * WAVES < p.steps) multiply_step(held[i], step + i * WAVES);
+                // (dealt items load zeros behind the last step, others nothing)
+                if (DEALT || step + i * WAVES < p.steps) multiply_step(held[i], step + i * WAVES);
                 const int then = last ? (more ? wave + i * WAVES : p.steps) : step + (i + AHEAD) * WAVES;
-                if (!GROUPED || then < p.steps) load(held[i], last ? next : item, then);
+                if (DEALT || then < p.steps) load(held[i], last ? next : item, then);
             }
             step += AHEAD * WAVES;
         }
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
                     if (ZERO) channel.sum = *reinterpret_cast<const v4i*>(p.w_sum + at);
                     if (!GROUPED && p.bias != nullptr) channel.bias = *reinterpret_cast<const v4f*>(p.bias + at);
                 }
-                total[kind] = scaled<KIND, !GROUPED>(all, channel, KIND == I8 ? row_scales[QUANTISE ? 0 : turn][min(row, item.rows - 1)] : RowScale{});
+                total[kind] = scaled<KIND, !GROUPED>(all, channel, KIND == I8 ? row_scales[min(row, item.rows - 1)] : RowScale{});
             }
             if constexpr (SWIGLU) {
 #pragma unroll
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
         }
         if (!more) return;
         item = next, id = next_id;
-        turn ^= GROUPED ? 0 : 1;
+        turn ^= 1;
     }
 }
 
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
 enum { kSwiglu = 1, kGather = 2, kZero = 4, kBias = 8 };
 constexpr int kMostLds = 128 * 1024;
 
-int steps_of(const orx_function& f) { return (f.K * (f.flags2 == I8 ? 1 : 2) + kStep - 1) / kStep; }
+int steps_of(const orx_function& f) { return steps_of_bytes((int64_t)f.K * (f.flags2 == I8 ? 1 : 2)); }
 
 // What a launch of `rows` rows runs: a unit's rows, and the form of the tiles from LDS (-1: the kernel above), or its waves
 struct Plan {
@@ -269,16 +269,34 @@ struct Plan {
 };
 // Of few steps fewer waves have one.
 Plan few_rows(const orx_function& f, int unit_rows) { return {unit_rows, -1, unit_rows == 64 || (unit_rows == 16 && steps_of(f) <= 8) ? 4 : 8}; }
+// Of dense launches the form whose estimate is least: fixed + step * steps * rounds over the CUs, in units of 10 ns.  Fitted to times of 1 to 8192 rows by seven sizes of weights (2048 x 1024
+// to 17408 x 5120 and 5120 x 17408); the estimates are within a fifth, except below the time that the weights take from memory, and the form that is picked within a tenth of the fastest.  us at
+// 7168 x 5120 of the kernel above with 16 and with 64 rows, and of tiles of 64 x 64, 64 x 128, 128 x 128, 128 x 256 and 256 x 256:
+//     16 rows: 9.1, 11.3, 14.7, 18.7, 23, 33, -;  64: -, 12.5, 15.3, 22, 24, 35, -;  128: -, 18, 15.5, 21, 28, 39, -;  256: -, 28, 25, 21, 28, 39, 61;  512: -, 47, 43, 38, 28, 39, 59;
+//     1024: -, -, -, 86, 58, 40, 59;  4096: 256 x 256 128 and 128 x 256 132;  8192: 247 and 242
+struct Form {
+    int form, rows, channels, fixed, step;
+};
+constexpr Form kForms[] = {{-1, 16, 32, 500, 10}, {-1, 64, 32, 600, 15}, {kTiles64x64, 64, 64, 300, 27}, {kTiles64, 64, 128, 300, 47}, {kTiles128, 128, 128, 400, 54}, {kWide128, 128, 256, 600, 72}, {kTiles256, 256, 256, 800, 125}};
 Plan plan(const orx_function& f, int rows) {
-    if (f.E > 0) return f.block_m == 16 ? few_rows(f, 16) : Plan{f.block_m, f.block_m == 64 ? kTiles64 : f.block_m == 256 ? kTiles256 : kTiles128x256, 0};
-    if (rows <= 64) return few_rows(f, rows <= 16 ? 16 : rows <= 32 ? 32 : 64);
-    return rows >= 1024 ? Plan{256, kTiles256, 0} : Plan{128, kTiles128, 0};
+    if (f.E > 0) return f.block_m == 16 ? few_rows(f, 16) : Plan{f.block_m, f.block_m == 64 ? kWide64 : kWide128, 0};
+    if (f.packed_k != 0) return few_rows(f, 16);
+    const int64_t units = device_compute_units();
+    const Form* best = nullptr;
+    int64_t least = 0;
+    for (const Form& form : kForms) {
+        if (form.form == kWide128 && (int64_t)f.slots * steps_of(f) * kTileBytes >= 1ll << 32) continue;  // (its loads of weights count 32 bits)
+        const int64_t tiles = (int64_t)ceil_div(rows, form.rows) * ceil_div(f.slots, form.channels / 16);
+        const int64_t estimate = form.fixed + (tiles + units - 1) / units * form.step * steps_of(f);
+        if (best == nullptr || estimate < least) least = estimate, best = &form;
+    }
+    return best->form < 0 ? few_rows(f, best->rows) : Plan{best->rows, best->form, 0};
 }
 int tiles_of(const orx_function& f) { return tiles_of(f.packed_k - 1, f.flags & kSwiglu); }
 uint32_t few_rows_lds(const orx_function& f, int rows, const Plan& plan) {
     const uint32_t sums = (uint32_t)plan.waves * (plan.rows / 16) * tiles_of(f) * 1024;
     const uint32_t codes = f.packed_k == 0 ? 0 : (uint32_t)steps_of(f) * kStep * std::min(f.E > 0 ? 16 : rows, 16);
-    return codes + (f.E > 0 ? 1 : 2) * sums;
+    return codes + (f.E == 0 && f.packed_k != 0 ? 2 : 1) * sums;
 }
 
 int geometry(const orx_function& f, int rows, Geometry* g) {
@@ -297,8 +315,9 @@ int geometry(const orx_function& f, int rows, Geometry* g) {
     } else {
         g->block[0] = 64 * plan.waves;
         g->shared = few_rows_lds(f, rows, plan);
-        // As many workgroups as the CUs hold at once, all with as many items.  (Sixteen waves to a CU; with a second round of few workgroups 32 rows of 17408 x 5120 took 19.4 us.)
-        if (f.E == 0) {
+        // Of rows that are quantised here as many workgroups as the CUs hold at once, sixteen waves to a CU, all with as many items.  (Others take one item: 9.1 us either way at 7168 x 5120, and 20.6
+        // instead of 24.8 at 17408 x 5120, where workgroups that end early make room for the next.)
+        if (f.E == 0 && f.packed_k != 0) {
             const int64_t most = (int64_t)device_compute_units() * std::min(16 / plan.waves, (int)(160 * 1024 / (g->shared + 1024)));
             blocks = ceil_div(blocks, ceil_div(blocks, most));
         }
@@ -354,7 +373,7 @@ int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream
         return f.flags2 == BF16 ? launch_16<BF16, true>(f, plan.waves, p, g, s) : launch_16<I8, true>(f, plan.waves, p, g, s);
     }
     if (plan.rows == 16) return launch_16<I8, false>(f, plan.waves, p, g, s);
-    return plan.rows == 32 ? launch_of<I8, 2, 8, 2, -1, 1, false>(f, p, g, s) : launch_of<I8, 4, 4, 1, -1, 1, false>(f, p, g, s);
+    return launch_of<I8, 4, 4, 1, -1, 1, false>(f, p, g, s);
 }
 
 Product product_of(const orx_function& f, int rows) {
@@ -425,7 +444,7 @@ int shape(const Variant& v, orx_function* f) {
         return ORX_ERR_BAD_VARIANT;
     }
     f->H = swiglu ? f->N / 2 : f->N;
-    f->slots = (f->H + 15) / 16 * (swiglu ? 2 : 1);
+    f->slots = swiglu ? (f->H + 31) / 32 * 4 : (f->H + 63) / 64 * 4;
     f->geometry = geometry;
     return ORX_OK;
 }
@@ -438,11 +457,15 @@ int make_grouped(const Variant& v, orx_function* f) {
     if (bad) return ORX_ERR_BAD_VARIANT;
     const int code = shape(v, f);
     if (code != ORX_OK) return code;
-    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 64 && f->block_m != 128 && f->block_m != 256)) {
-        set_error("%s: need rows, E and tiles above 0 and block_m 16, 64, 128 or 256", f->symbol.c_str());
+    if (f->M <= 0 || f->M > 1 << 24 || f->E <= 0 || f->tiles <= 0 || f->tiles > 1 << 24 || (f->block_m != 16 && f->block_m != 64 && f->block_m != 128)) {
+        set_error("%s: need rows, E and tiles above 0 and block_m 16, 64 or 128", f->symbol.c_str());
         return ORX_ERR_BAD_VARIANT;
     }
     f->capacity = f->M;
+    if (f->block_m > 16 && (int64_t)f->slots * steps_of(*f) * kTileBytes >= 1ll << 32) {  // (weights' loads count 32 bits from an expert's first one)
+        set_error("%s: an expert's weights of 4 GiB and more go with block_m 16", f->symbol.c_str());
+        return ORX_ERR_BAD_VARIANT;
+    }
     if (f->packed_k != 0 && (f->block_m != 16 || !quantises(*f, 16))) {
         set_error("%s: 16-bit rows go with block_m 16 and K up to %d", f->symbol.c_str(), 64 * 8 * kMostPieces);
         return ORX_ERR_BAD_VARIANT;

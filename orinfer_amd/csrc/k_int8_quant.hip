@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * DEAL::ROWS * DEAL::WAVES, 4) void int8_quantis
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
-// slots used: K, group (K in whole steps of 128), stride (from one stored row to the next), algorithm (type), flags (zero points), flags2 (by tiles)
+// slots used: K, group (K in whole pairs of steps), stride (from one stored row to the next), algorithm (type), flags (zero points), flags2 (by tiles)
 constexpr int kMaxK = 1 << 24;
 constexpr uint32_t kMostGroups = 1 << 21;  // (a launch's threads are fewer than 2^32)
 
@@ -219,7 +219,7 @@ int make_quantise(const Variant& v, orx_function* f) {
         set_error("int8_token_quantization: need 0 < K <= %d and M from 1 to %d", kMaxK, 1 << 24);
         return ORX_ERR_BAD_VARIANT;
     }
-    f->group = (f->K + kStep - 1) / kStep * kStep;
+    f->group = steps_of_bytes(f->K) * kStep;
     f->stride = (f->group / kStep | 1) * kStep;
     f->dynamic_rows = true;
     f->geometry = geometry;
@@ -243,10 +243,10 @@ const Registration* byte_registrations(int* count) {
          "M, N, K, dynamic_rows=false, input_dtype=int8|float16|bfloat16 (few rows), zero_points=false, bias=false, epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
          "A[,AS][,AZ][,Bias],Out,W,WS[,WSum][,m]"},
         {"int8_token_grouped", make_int8_grouped,
-         "rows, E, N, K, tiles, block_m=16|64|128|256, gather=false, input_dtype=int8|float16|bfloat16 (block_m=16), epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
+         "rows, E, N, K, tiles, block_m=16|64|128, gather=false, input_dtype=int8|float16|bfloat16 (block_m=16), epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
          "A[,AS],Out[,SlotToken],TileCount,TileUnits,W,WS"},
         {"half_grouped", make_half_grouped,
-         "rows, E, N, K, tiles, block_m=16|64|128|256, gather=false, dtype=float16|bfloat16, epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
+         "rows, E, N, K, tiles, block_m=16|64|128, gather=false, dtype=float16|bfloat16, epilogue=none|swiglu, output_dtype=float16|bfloat16|float32",
          "A,Out[,SlotToken],TileCount,TileUnits,W"},
     };
     *count = (int)(sizeof(rows) / sizeof(rows[0]));

@@ -10,7 +10,7 @@ import torch
 
 from .lib import Kernel
 
-STEP = 128   # K of a step of the products
+STEP = 128   # K of a step of the products, which take K padded to pairs of steps
 MOST_K = 65536  # that a product adds exactly
 DTYPES = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}
 
@@ -23,7 +23,12 @@ def dtype_name(dtype):
 
 def padded(k):
     """Bytes from one stored row to the next: an odd multiple of 128 (at even distances rows meet in few channels of the L2)."""
-    return (-(-k // STEP) | 1) * STEP
+    return (steps(k) | 1) * STEP
+
+
+def steps(k):
+    """Steps that the products take of K."""
+    return -(-k // (2 * STEP)) * 2
 
 
 @functools.lru_cache(maxsize=256)

@@ -914,7 +914,7 @@ class Mxfp4MoeLayer(_ExpertLayer):
         self.w2, self.p2 = (t.to(self.device) for t in mxfp4.tiles(*weights[2:]))
         routes = tokens * top_k
         if block_m is None:
-            block_m = _unit_rows(routes, experts)
+            block_m = 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
         self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = mxfp4.dtype_name(dtype)
@@ -988,7 +988,7 @@ class Int8Linear(_OnDevice):
                     self.few, self.few_rows = _where_it_fits("int8_token_projection", M=rows, input_dtype=name, **shape), rows
         self.n = channels // 2 if paired else channels
         # the quantised rows, by tiles of 16
-        self.a_q = torch.empty((-(-capacity // 16), -(-self.k // int8.STEP), 2048), dtype=torch.int8, device=self.device)
+        self.a_q = torch.empty((-(-capacity // 16), int8.steps(self.k), 2048), dtype=torch.int8, device=self.device)
         self.a_s = torch.empty(capacity, dtype=torch.float32, device=self.device)
         self.a_z = torch.empty(capacity, dtype=torch.int32, device=self.device) if self.zero_points else None
         self.out = torch.empty((capacity, self.n), dtype=dtype, device=self.device)
@@ -1013,7 +1013,7 @@ class Int8Linear(_OnDevice):
 
 def _unit_rows(routes, experts):
     """Rows to a unit of the experts' products, by the routes that an expert has in the mean."""
-    return 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128 if routes < 512 * experts else 256
+    return 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128
 
 
 def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):

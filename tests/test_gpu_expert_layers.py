@@ -90,7 +90,7 @@ def check_parts(layer, gate_up, down, x, ids, shared, gate, got):
 
 
 ROUTINGS = [{}, dict(scoring="sigmoid", groups=4, top_groups=2, scale=2.5)]
-SHAPES = [(1, 8, 2, 64, 32), (1, 60, 6, 256, 136), (3, 128, 8, 512, 96), (48, 64, 6, 512, 160), (300, 16, 4, 296, 264), (1100, 8, 3, 256, 128)]
+SHAPES = [(1, 8, 2, 64, 32), (1, 60, 6, 256, 136), (3, 128, 8, 512, 96), (48, 64, 6, 512, 160), (300, 16, 4, 296, 264), (1100, 8, 3, 256, 128), (2, 16, 2, 5192, 72), (2, 16, 2, 72, 5192)]
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
@@ -118,8 +118,8 @@ def test_16_bit_layers_whose_rows_end_within_a_step(tokens, experts, top_k, hidd
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
-@pytest.mark.parametrize("block_m", [16, 64, 128, 256])
-@pytest.mark.parametrize("tokens,hidden,inner", [(40, 328, 224), (300, 64, 64), (900, 136, 520)])
+@pytest.mark.parametrize("block_m", [16, 64, 128])
+@pytest.mark.parametrize("tokens,hidden,inner", [(40, 328, 224), (300, 64, 64), (900, 136, 520), (40, 5192, 72), (40, 72, 5192)])
 def test_units_of_every_size(tokens, hidden, inner, block_m, kind, dtype):
     check_run(*make(kind, dtype, tokens, 8, 3, hidden, inner, block_m=block_m), {})
 
@@ -200,7 +200,7 @@ def test_rows_in_the_layers_own_buffer(kind, dtype):
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
 @pytest.mark.parametrize("output", ["float16", "bfloat16", "float32"])
-@pytest.mark.parametrize("block_m", [16, 64, 128, 256])
+@pytest.mark.parametrize("block_m", [16, 64, 128])
 def test_grouped_writes_its_rows_and_columns_only(kind, dtype, output, block_m):
     """Units of odd lengths, one of them empty, rows and channels behind the ends untouched."""
     rng = np.random.default_rng(3)

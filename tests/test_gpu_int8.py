@@ -69,7 +69,7 @@ def test_quantisation_is_the_oracles(rows, k, name, zero_points):
     q = torch.full((rows + 1, int8.padded(k)), 91, dtype=torch.int8, device=DEV)
     s, z = torch.full((rows + 1,), 7.5, device=DEV), torch.full((rows + 1,), 91, dtype=torch.int32, device=DEV)
     kernel("int8_token_quantization", K=k, input_dtype=name, zero_points=zero_points)(Q=q, S=s, X=x.to(DEV), rows=rows, **({"Z": z} if zero_points else {}))
-    written = -(-k // 128) * 128
+    written = -(-k // 256) * 256
     np.testing.assert_array_equal(q[:rows, :k].cpu().numpy(), codes)
     np.testing.assert_array_equal(s[:rows].cpu().double().numpy(), scales)
     if zero_points:
@@ -87,7 +87,7 @@ def test_quantisation_is_the_oracles(rows, k, name, zero_points):
 def test_quantisation_by_tiles(rows, k, name, zero_points):
     x = rows_of(np.random.default_rng(rows * k), rows, k, TYPES[name], side=1.0 * zero_points).to(DEV)
     want = int8.quantize(x, zero_points)
-    tiles, steps = -(-rows // 16), -(-k // 128)
+    tiles, steps = -(-rows // 16), int8.steps(k)
     q = torch.full((tiles * steps * 2048 + 16,), 91, dtype=torch.int8, device=DEV)
     s, z = torch.full((rows + 1,), 7.5, device=DEV), torch.full((rows + 1,), 91, dtype=torch.int32, device=DEV)
     kernel("int8_token_quantization", K=k, input_dtype=name, zero_points=zero_points, layout="tiles")(Q=q, S=s, X=x, rows=rows, **({"Z": z} if zero_points else {}))
@@ -162,7 +162,7 @@ def test_shapes_of_quantize():
 # ---- linears -----------------------------------------------------------------------------------------------------------------------------------
 LINEARS = [(1, 16, 128), (1, 9, 7), (1, 300, 2560), (2, 33, 5000), (3, 48, 640), (4, 31, 4097), (5, 96, 1000), (16, 128, 1024), (17, 40, 129), (31, 260, 2560), (33, 513, 512), (64, 100, 1111),
            (65, 300, 300), (130, 520, 1280), (200, 1030, 384), (300, 264, 2048), (513, 700, 257),
-           (1024, 256, 64), (1030, 520, 300), (2500, 1100, 640)]
+           (1024, 256, 64), (1030, 520, 300), (2500, 1100, 640), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2048, 4098, 2560)]
 
 
 @pytest.mark.parametrize("zero_points,biased", [(False, False), (True, True), (True, False), (False, True)])
@@ -181,7 +181,7 @@ def test_linear(rows, n, k, dtype, zero_points, biased):
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
-@pytest.mark.parametrize("rows,n,k", [(1, 32, 128), (1, 34, 2000), (3, 300, 1111), (20, 66, 512), (64, 1000, 256), (150, 258, 640), (400, 514, 300), (1500, 1058, 520)])
+@pytest.mark.parametrize("rows,n,k", [(1, 32, 128), (1, 34, 2000), (3, 300, 1111), (20, 66, 512), (64, 1000, 256), (150, 258, 640), (400, 514, 300), (1500, 1058, 520), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2040, 4106, 2560)])
 def test_linear_with_swiglu(rows, n, k, zero_points):
     rng = np.random.default_rng(rows * n + k)
     x = rows_of(rng, rows, k, torch.bfloat16)
@@ -231,7 +231,7 @@ def test_projection_writes_its_rows_and_columns_only(rows, n, k, name):
     rng = np.random.default_rng(n)
     x = rows_of(rng, rows, k, torch.float32)
     w, scale = weights_of(rng, n, k)
-    q = torch.empty((-(-rows // 16), -(-k // 128), 2048), dtype=torch.int8, device=DEV)
+    q = torch.empty((-(-rows // 16), int8.steps(k), 2048), dtype=torch.int8, device=DEV)
     s = torch.empty(rows, device=DEV)
     kernel("int8_token_quantization", K=k, input_dtype="float32", layout="tiles")(Q=q, S=s, X=x.to(DEV), rows=rows)
     project = kernel("int8_token_projection", M=rows + 3, N=n, K=k, dynamic_rows=True, output_dtype=name)

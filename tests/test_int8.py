@@ -29,7 +29,7 @@ def test_tiles_hold_every_byte_where_a_lane_reads_it(n, k, paired, dtype):
     raw = torch.from_numpy(rng.integers(0, 256, (2, n, k * size), dtype=np.uint8))
     w = byte_tiles.tiles(raw.view(dtype), paired=paired)
     half = n // 2 if paired else n
-    tiles, steps = -(-half // 16) * (2 if paired else 1), -(-k * size // 128)
+    tiles, steps = -(-n // 64) * 4, -(-k * size // 256) * 2
     assert w.shape == (2, steps, tiles, 8, 16, 16) and w.is_contiguous() and w.dtype == torch.uint8
     wide = torch.nn.functional.pad(raw, (0, steps * 128 - k * size)).view(2, n, steps, 8, 16)
     values = torch.arange(1.0, n + 1)
