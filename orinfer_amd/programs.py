@@ -981,9 +981,11 @@ class Int8Linear(_OnDevice):
         with torch.cuda.device(self.device):
             self.projection = Kernel("int8_token_projection", M=capacity, **shape)
             self.quantizer = Kernel("int8_token_quantization", M=capacity, K=self.k, input_dtype=name, zero_points=self.zero_points, layout="tiles")
-            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two.  Not where their codes do not fit LDS, or a row its threads.
+            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (us, two and one, of 4096 x 4096: 1 row 10.8 and 7.8, 8 11.1 and 9.6, 12 11.1
+            # and 11.9; of 17408 x 5120: 1 row 23.4 and 21.0, 4 23.7 and 22.2; of 24576 x 1536, the least that it gives: 12.8 and 12.2, 8 rows 12.9 and 12.9, 12 12.6 and 14.2).  Not where
+            # their codes do not fit LDS, or a row its threads.
             self.few, self.few_rows = None, 0
-            for rows in (4, 2, 1):
+            for rows in (8, 4, 2, 1):
                 if self.few is None and rows <= capacity:
                     self.few, self.few_rows = _where_it_fits("int8_token_projection", M=rows, input_dtype=name, **shape), rows
         self.n = channels // 2 if paired else channels
@@ -1011,9 +1013,12 @@ class Int8Linear(_OnDevice):
         self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, m=rows, **zero[1], **self.channel)
 
 
-def _unit_rows(routes, experts):
-    """Rows to a unit of the experts' products, by the routes that an expert has in the mean."""
-    return 16 if routes <= 10 * experts else 64 if routes < 192 * experts else 128
+def _unit_rows(routes, experts, expert_bytes):
+    """Rows to a unit of the experts' products, by the routes that an expert has in the mean.  (us of both products with units of 16, 64 and 128 rows, popularity like 1 / rank^1.1: fp16, 128
+    experts of 2048 and 512, 4 routes to an expert 65, 66, 67, 8 90, 90, 86, 16 140, 110, 124, 25 182, 123, 132, 32 -, 151, 140; 16 experts of 4096 and 1536, 4 67, 73, 82, 8 94, 85, 92,
+    25 169, 119, 115, 50 252, 167, 136; int8, the same: 4 36, 39, 40, 16 81, 64, 72, 25 109, 72, 80, 32 -, 90, 84; 35, 36, 42, 25 83, 65, 66, 50 128, 90, 79.)  Kernels of 64 and 128 rows
+    count the bytes of an expert's matrix in 32 bits."""
+    return 16 if routes <= 10 * experts or expert_bytes >= 1 << 32 else 64 if routes < 30 * experts else 128
 
 
 def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):
@@ -1046,7 +1051,7 @@ class Int8MoeLayer(_ExpertLayer):
         self.w2, self.s2 = byte_tiles.tiles(down).to(self.device), byte_tiles.channels(down_scale.float()).to(self.device)
         routes = tokens * top_k
         if block_m is None:
-            block_m = _unit_rows(tokens * top_k, experts)
+            block_m = _unit_rows(tokens * top_k, experts, max(self.w1.nbytes, self.w2.nbytes) // experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(dtype)
@@ -1056,10 +1061,12 @@ class Int8MoeLayer(_ExpertLayer):
             up = dict(N=2 * intermediate, K=hidden, gather=True, epilogue="swiglu", output_dtype=name, **self.grouped)
             down = dict(N=hidden, K=intermediate, output_dtype="float32", **self.grouped)
             self.k_up, self.k_down = Kernel("int8_token_grouped", **up), Kernel("int8_token_grouped", **down)
-            # A route to an expert or less: the products quantise their rows themselves, one launch instead of two.
-            few = block_m == 16 and routes <= experts
-            self.few_up = _where_it_fits("int8_token_grouped", input_dtype=name, **up) if few else None
-            self.few_down = _where_it_fits("int8_token_grouped", input_dtype=name, **down) if few else None
+            # Few routes: the products quantise their rows themselves, one launch instead of two, but every workgroup again (32 gate | up channels or 16 down channels to one): values that
+            # are quantised up to 2^21.  (us, two launches and one: 128 experts of 2048 and 512, up 16 routes, 2^20: 11.2 and 9.5, 64, 2^22: 25.0 and 25.6; down 16, 2^20: 9.3 and 7.4, 64,
+            # 2^22: 14.4 and 17.6; 16 experts of 4096 and 1536, up 2, 0.8 10^6: 10.6 and 8.4, 8, 3.1 10^6: 23.3 and 26.7; down 2: 8.6 and 6.3, 8: 13.6 and 17.6.)
+            few_up, few_down = block_m == 16 and routes * -(-intermediate // 16) * hidden < 1 << 21, block_m == 16 and routes * -(-hidden // 16) * intermediate < 1 << 21
+            self.few_up = _where_it_fits("int8_token_grouped", input_dtype=name, **up) if few_up else None
+            self.few_down = _where_it_fits("int8_token_grouped", input_dtype=name, **down) if few_down else None
         i8, f32 = dict(dtype=torch.int8, device=self.device), dict(dtype=torch.float32, device=self.device)
         self.a_q, self.a_s = torch.empty((tokens, int8.padded(hidden)), **i8), torch.empty(tokens, **f32)
         self.h_q, self.h_s = torch.empty((routes, int8.padded(intermediate)), **i8), torch.empty(routes, **f32)
@@ -1093,7 +1100,7 @@ class HalfMoeLayer(_ExpertLayer):
         self.device = self._device_of(gate_up, down)
         self.w1, self.w2 = byte_tiles.tiles(gate_up, paired=True).to(self.device), byte_tiles.tiles(down).to(self.device)
         if block_m is None:
-            block_m = _unit_rows(tokens * top_k, experts)
+            block_m = _unit_rows(tokens * top_k, experts, max(self.w1.nbytes, self.w2.nbytes) // experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, gate_up.dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(gate_up.dtype)
@@ -1103,7 +1110,8 @@ class HalfMoeLayer(_ExpertLayer):
 
     def _up(self, x, stream):
         if not _apart(x, self.act):  # (workgroups that have ended would write over what others have yet to read)
-            x = x.clone()
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+                x = x.clone()
         self.k_up(stream=stream, A=x, Out=self.act, SlotToken=self.slot_token, W=self.w1, TileCount=self.tile_count, TileUnits=self.tile_units)
 
     def _second_products(self, act, stream):
