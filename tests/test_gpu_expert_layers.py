@@ -199,6 +199,53 @@ def test_rows_in_the_layers_own_buffer(kind, dtype):
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+def test_a_stream_that_the_caller_names(kind, dtype):
+    """All of a call, the copy of rows that lie in the layer's own buffer as well, is behind what that stream has to do."""
+    tokens, hidden, inner, top_k = 4, 64, 64, 2
+    layer, gate_up, _, x, logits, _, _ = make(kind, dtype, tokens, 8, top_k, hidden, inner)
+    ids, _ = layer.route(dev(logits))
+    layer.place(ids)
+    side = torch.cuda.Stream()
+    rows = layer.act[:tokens]
+    rows.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        rows.copy_(x)
+    got = layer.up(rows, stream=side.cuda_stream)
+    side.synchronize()
+    order, _ = slots_of(host(ids))
+    check(got, *gate_up.products(x, host(ids).reshape(-1)[order], order // top_k, swiglu), dtype)
+
+
+@pytest.mark.parametrize("block_m", [16, 64, 128])
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_banks_beyond_4_gib(kind, dtype, block_m):
+    """Ten experts of half a GiB each and one of 300 rows; the last expert's results."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    experts, n, k, slots = 10, 8192, 65536 if kind == "int8" else 32768, 300
+    values = torch.randint(-15, 16, (experts, 512, n // 16, 8, 16, 16 if kind == "int8" else 8), dtype=torch.int8, device=DEV, generator=g)
+    tiles = values if kind == "int8" else values.to(dtype)
+    x = torch.randint(-15, 16, (slots, k), dtype=torch.int8, device=DEV, generator=g)
+    x[:, 0] = 127  # (scale 1, codes the values themselves)
+    units = torch.zeros((-(-slots // block_m), 4), dtype=torch.int32, device=DEV)
+    for i in range(len(units)):
+        units[i, :3] = torch.tensor([9, i * block_m, min(block_m, slots - i * block_m)])
+    out = torch.empty((slots, n), device=DEV)
+    shape = dict(rows=slots, E=experts, N=n, K=k, tiles=len(units), block_m=block_m, output_dtype="float32")
+    common = dict(Out=out, TileCount=torch.tensor([len(units)], dtype=torch.int32, device=DEV), TileUnits=units, W=tiles)
+    if kind == "int8":
+        q, s = int8.quantize(x.half())
+        assert (s == 1).all()
+        kernel("int8_token_grouped", **shape)(A=q, AS=s, WS=torch.ones((experts, n), device=DEV), **common)
+    else:
+        kernel("half_grouped", dtype=int8.dtype_name(dtype), **shape)(A=x.to(dtype), **common)
+    for tile in (0, n // 16 - 1):
+        w = values[9, :, tile].movedim(2, 0).reshape(16, k).double()
+        assert torch.equal(out[:, tile * 16:tile * 16 + 16].double(), x.double() @ w.T)  # (whole numbers below 2^24, and so are all sums on the way)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 @pytest.mark.parametrize("output", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("block_m", [16, 64, 128])
 def test_grouped_writes_its_rows_and_columns_only(kind, dtype, output, block_m):

@@ -226,7 +226,7 @@ def test_rows_that_are_not_finite_stay_to_themselves(rows):
 
 
 @pytest.mark.parametrize("name", list(TYPES))
-@pytest.mark.parametrize("rows,n,k", [(1, 33, 256), (6, 130, 384), (70, 50, 129), (260, 530, 128), (1100, 300, 300)])
+@pytest.mark.parametrize("rows,n,k", [(1, 33, 256), (6, 130, 384), (70, 50, 129), (260, 530, 128), (1100, 300, 300), (30, 130, 2560), (490, 250, 4096), (1020, 1050, 129), (1020, 2042, 520), (2045, 2042, 520), (2045, 4106, 2560)])
 def test_projection_writes_its_rows_and_columns_only(rows, n, k, name):
     rng = np.random.default_rng(n)
     x = rows_of(rng, rows, k, torch.float32)
@@ -291,6 +291,43 @@ def test_two_streams_with_objects_of_their_own():
     torch.cuda.synchronize()
     for linear, x in zip(linears, xs):
         check(linear.out, *product(*orc.quantise(x.cpu().double().numpy()), w, scale), torch.float16)
+
+
+def test_matrices_and_rows_beyond_4_gib():
+    """Bytes of weights, of rows and of results that 32 bits do not count.  (Codes are random, the weights' laid out already: each tile has its own multiple, told by its channels' results.)"""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    n, k = 66000, 65536  # 4.3 GB of weights
+    tiles = torch.randint(-127, 128, (k // 128, -(-n // 64) * 4, 8, 16, 16), dtype=torch.int8, device=DEV, generator=g)
+    scale = torch.rand(-(-n // 64) * 64, device=DEV, generator=g) / 2**20
+    last = list(range(65984, 66000))
+    for rows in (1, 30, 60, 200, 500):  # (a launch of every kind that the sizes allow)
+        x = torch.randint(-127, 128, (rows, k), device=DEV, generator=g)
+        x[:, 0] = 127  # (scale 1, codes the values themselves)
+        q, s = torch.empty((-(-rows // 16), k // 128, 2048), dtype=torch.int8, device=DEV), torch.empty(rows, device=DEV)
+        kernel("int8_token_quantization", K=k, input_dtype="float32", layout="tiles")(Q=q, S=s, X=x.float(), rows=rows)
+        out = torch.empty((rows, n), device=DEV)
+        kernel("int8_token_projection", M=rows, N=n, K=k, output_dtype="float32")(A=q, AS=s, Out=out, W=tiles, WS=scale)
+        for tile in (0, last[0] // 16):
+            w = tiles[:, tile].movedim(2, 0).reshape(16, k).double()  # (16 channels, K in order: steps, pieces, bytes)
+            want = (x.double() @ w.T) * scale[tile * 16:tile * 16 + 16].double()
+            assert ((out[:, tile * 16:tile * 16 + 16].double() - want).abs() <= 3 * 2.0**-24 * 1.0001 * want.abs()).all(), (rows, tile)
+    del tiles, out
+    rows, n, k = 140000, 40, 65000  # 9 GB of codes
+    x = torch.randint(-127, 128, (rows, k), dtype=torch.int8, device=DEV, generator=g).half()
+    x[:, 0] = 127
+    w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device=DEV, generator=g)
+    linear = programs.Int8Linear(w, torch.full((n,), 2.0**-14), rows, dtype=torch.float16)
+    out = linear.run(x)
+    want = x[-300:].double() @ w.double().T / 2.0**14
+    assert ((out[-300:].double() - want).abs() <= (2.0**-11 + 2.0**-20) * want.abs() + 2.0**-25).all()
+    del x, linear, out
+    rows, n, k = 1 << 20, 4200, 64  # 8.8 GB of results
+    x = torch.randint(-127, 128, (rows, k), dtype=torch.int8, device=DEV, generator=g).half()
+    x[:, 0] = 127
+    w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device=DEV, generator=g)
+    out = programs.Int8Linear(w, torch.full((n,), 2.0**-10), rows, dtype=torch.float16).run(x)
+    want = x[-300:].double() @ w.double().T / 2.0**10
+    assert ((out[-300:].double() - want).abs() <= (2.0**-11 + 2.0**-20) * want.abs() + 2.0**-25).all()
 
 
 def test_refusals_of_tensors():
