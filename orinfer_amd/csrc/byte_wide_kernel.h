@@ -183,6 +183,7 @@ __global__ __launch_bounds__(256, 2) void byte_wide_kernel(Product p) {
     using N2 = std::integral_constant<int, 2>;
     uint32_t stage = 0;
     int left = my_tiles * p.steps;  // steps, with this one
+    bool is_short = false;          // the tile's rows are at most 64
     Weights next_w, after_w;        // of the next step and of the one behind it
     // Half H of a step of parity PARITY; behind every multiply stands at most a read, a load or a request.  In the second half, once the first row's multiplies are on
     // their way, the next step's rows are there, and nobody reads the last step's any more.  (Of the requests and loads of a wave at least sixteen are newer than those rows' requests, which
@@ -192,7 +193,10 @@ __global__ __launch_bounds__(256, 2) void byte_wide_kernel(Product p) {
         using Other = std::integral_constant<int, 1 - H>;
         using Refilled = std::integral_constant<int, (SLOT + 3) % 4>;
         const uint32_t next = (stage + kStage) & (kStages - 1);
-        Each<ROWS>::run([&](auto i) {
+        // Rows behind a short tile's 64 are not multiplied: the first four blocks' registers then get the next half's rows.
+        constexpr int FULL = ROWS == 8 && GROUPED ? 4 : ROWS;
+        const uint32_t behind = FULL == ROWS ? 0 : (a_at ^ ((is_short ? 1 - H : H) * 64)) + (is_short ? (H == 0 ? stage : next) : stage + FULL * 16 * kStep);
+        auto one_row = [&](auto i) __attribute__((always_inline)) {
             constexpr int I = decltype(i)::value;
             Each<CHANNELS>::run([&](auto jj) {
                 constexpr int JJ = decltype(jj)::value, J = I & 1 ? CHANNELS - 1 - JJ : JJ;  // one operand changes between neighbours
@@ -205,7 +209,7 @@ __global__ __launch_bounds__(256, 2) void byte_wide_kernel(Product p) {
                 }
                 // Loads of weights behind the first row's second multiply and later ones; requests behind the barrier, and in front of the loads: the compiler does not count them where it waits for
                 // weights, so a wait is for as many loads more (the other way round, of older loads: half of their time on the way).
-                constexpr int AT = I * CHANNELS + JJ, FIRST = H == 1 ? CHANNELS : 1, EVERY = (ROWS * CHANNELS - FIRST) / (H == 1 ? CHANNELS + A_REQUESTS : CHANNELS);
+                constexpr int AT = I * CHANNELS + JJ, FIRST = H == 1 ? CHANNELS : 1, EVERY = (FULL * CHANNELS - FIRST) / (H == 1 ? CHANNELS + A_REQUESTS : CHANNELS);
                 if constexpr (AT >= FIRST && (AT - FIRST) % EVERY == 0) {
                     constexpr int Q = (AT - FIRST) / EVERY;
                     constexpr int W = H == 1 ? Q - A_REQUESTS : Q;
@@ -213,12 +217,16 @@ __global__ __launch_bounds__(256, 2) void byte_wide_kernel(Product p) {
                     else if constexpr (W < CHANNELS) load_weight(Refilled{}, Other{}, std::integral_constant<int, W>{}, H == 0 ? next_w : after_w);
                 }
                 if constexpr (JJ == CHANNELS - 1) {
-                    if constexpr (I + 4 < ROWS) read_row(half, std::integral_constant<int, I + 4>{}, stage);
+                    if constexpr (FULL < ROWS && I < FULL) fa[I] = *reinterpret_cast<const v4i*>(lds + behind + I * (16 * kStep));
+                    else if constexpr (I + 4 < ROWS) read_row(half, std::integral_constant<int, I + 4>{}, stage);
                     else read_row(Other{}, std::integral_constant<int, I + 4 - ROWS>{}, H == 0 ? stage : next);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             });
-        });
+        };
+        Each<FULL>::run([&](auto i) { one_row(i); });
+        if constexpr (FULL < ROWS)
+            if (!is_short) Each<ROWS - FULL>::run([&](auto i) { one_row(std::integral_constant<int, FULL + decltype(i)::value>{}); });
     };
 
     // ---- results: block (i, j) has channels 4 piece .. of row r; pairs of blocks change rows of lanes, and a lane has eight neighbours ----
@@ -318,6 +326,7 @@ __global__ __launch_bounds__(256, 2) void byte_wide_kernel(Product p) {
     };
 #pragma unroll 1
     for (int tile = 0; tile < my_tiles; ++tile) {
+        is_short = ROWS == 8 && GROUPED && tile_of(tile).rows <= 64;
         // (the first step as one of its own, whose sums start at 0, takes the registers of a second set of sums)
         Each<ROWS * CHANNELS>::run([&](auto at) {
             Sum& one = sum[decltype(at)::value / CHANNELS][decltype(at)::value % CHANNELS];
