@@ -21,16 +21,16 @@ using lds_asm::Each;
 
 template <int KIND, int ROWS, bool GROUPED>
 struct Wide {
-    static constexpr int waves = 4, stages = 4, channels = 4, bm = 16 * ROWS, bn = 16 * channels * waves, stage = bm * kStep;
+    static constexpr int waves = ROWS <= 4 ? 2 : 4, to_a_cu = ROWS <= 4 ? 4 : 2, stages = 4, channels = 4, bm = 16 * ROWS, bn = 16 * channels * waves, stage = bm * kStep;
     // what a tile's rows and channels have, for the results: scales, and of dense rows zero points, sums and biases; of the tile that is multiplied and of two more
     static constexpr int scale_bytes = 4 * (GROUPED ? bm + bn : 2 * bm + 3 * bn), ring = KIND == I8 ? 3 * scale_bytes : 0;
     static constexpr int tokens = GROUPED ? 2 * 4 * bm : 0;
     static constexpr int lds = stages * stage + ring + tokens;
-    static_assert(lds <= 80 * 1024, "two workgroups to a CU");
+    static_assert(to_a_cu * lds <= 160 * 1024 && to_a_cu * waves == 8, "a CU's LDS, two waves to a SIMD");
 };
 
 template <int KIND, int ROWS, bool WIDE, bool GROUPED, bool SWIGLU>
-__global__ __launch_bounds__(256, 2) void byte_wide_kernel(Product p) {
+__global__ __launch_bounds__(ROWS <= 4 ? 128 : 256, 2) void byte_wide_kernel(Product p) {
     using Sum = typename Operands<KIND>::Sum;
     using FORM = Wide<KIND, ROWS, GROUPED>;
     constexpr int WAVES = FORM::waves, CHANNELS = FORM::channels, BM = FORM::bm, BN = FORM::bn, kStage = FORM::stage, kStages = FORM::stages * kStage;
@@ -354,7 +354,7 @@ int launch_wide(const Product& p, uint32_t blocks, hipStream_t s) {
     static DeviceOnce ready;
     const int code = ready.run([] { return hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds), "hipFuncSetAttribute"); });
     if (code != ORX_OK) return code;
-    ORX_LAUNCH(kernel, dim3(blocks), dim3(256), kLds, s, p);
+    ORX_LAUNCH(kernel, dim3(blocks), dim3(64 * Wide<KIND, ROWS, GROUPED>::waves), kLds, s, p);
     return hip_check(hipGetLastError(), "launch byte product");
 }
 template <int KIND, int ROWS, bool GROUPED>

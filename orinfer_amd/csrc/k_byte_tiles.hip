@@ -287,7 +287,7 @@ TilesShape byte_tiles_shape(int kind, int form, bool grouped) {
     if (form == kWide128 || form == kWide64) {
         auto shape = [](auto wide) {
             using WIDE = decltype(wide);
-            return TilesShape{WIDE::bm, WIDE::bn, 256, WIDE::lds, 2};
+            return TilesShape{WIDE::bm, WIDE::bn, 64 * WIDE::waves, WIDE::lds, WIDE::to_a_cu};
         };
         if (kind != I8) return form == kWide128 ? shape(Wide<F16, 8, true>{}) : shape(Wide<F16, 4, true>{});
         if (!grouped) return shape(Wide<I8, 8, false>{});
