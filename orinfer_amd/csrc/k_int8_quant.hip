@@ -145,21 +145,30 @@ __global__ __launch_bounds__(64 * DEAL::ROWS * DEAL::WAVES, 4) void int8_quantis
 constexpr int kMaxK = 1 << 24;
 constexpr uint32_t kMostGroups = 1 << 21;  // (a launch's threads are fewer than 2^32)
 
-// The deal for `rows` rows of K values; and whether they are whole pieces of eight, which the others only have few of.
+// The deal for `rows` rows of K values; and whether they are whole pieces of eight, which the others only have few of.  us of bf16 rows, the deal taken first (rows x K):
+//   four rows to a wave or one: 32768 x 512 15.1 and 16.7, 4096 x 512 7.1 and 5.6;
+//   by rows: eight rows to a workgroup or one: 8192 x 2048 12.9 and 14.8, 2048 x 2048 7.6 and 6.2, 8192 x 4096 24.1 and 20.4, 8192 x 8192 47.8 and 34.0; four waves to a row or sixteen:
+//     8192 x 5120 23.3 and 46.0, 2048 x 17408 29.5 and 24.0, 64 x 17408 11.2 and 5.7;
+//   by tiles: eight rows or one: 8192 x 2048 14.3 and 22.0, 2048 x 4096 10.2 and 13.8, 1024 x 4096 8.9 and 7.6; of eight rows two waves to a row or one: 8192 x 4096 23.4 and 26.0, 8192 x 8192
+//     52.5 and 65.2, 8192 x 1024 10.0 and 8.4; with zero points, which take more registers, two pieces to a thread or four: 8192 x 5120 36.2 and 41.7, but 8192 x 4096 29.4, 32.2 and with
+//     one wave that holds the row 27.7.
 template <typename BODY>
-void with_deal(int rows, int k, BODY body) {
+void with_deal(const orx_function& f, int rows, BODY body) {
+    const int k = f.K;
+    const bool zero = f.flags, tiles = f.flags2;
     if (k % 8) {
-        if (k <= 8192 && (rows >= 1024 || k <= 1024)) body(Deal<1, 8, 1, 4>{}, std::false_type{});
+        if (k <= 1024 || (tiles && k <= 8192 && rows >= 2048)) body(Deal<1, 8, 1, 4>{}, std::false_type{});
         else body(Deal<1, 1, 4, 4>{}, std::false_type{});
-    } else if (k <= 512 && rows >= 4096) body(Deal<4, 8, 1, 1>{}, std::true_type{});
-    else if (k <= 2048 && (rows >= 1024 || k <= 1024)) body(Deal<1, 8, 1, 4>{}, std::true_type{});
-    else if (k <= 4096 && rows >= 1024) body(Deal<1, 8, 1, 8>{}, std::true_type{});
-    else if (k <= 8192 && rows >= 1024) body(Deal<1, 8, 2, 8>{}, std::true_type{});
-    else if (k <= 8192) body(Deal<1, 1, 4, 4>{}, std::true_type{});
-    else body(Deal<1, 1, 16, 4>{}, std::true_type{});
+    } else if (k <= 512 && rows >= 16384) body(Deal<4, 8, 1, 1>{}, std::true_type{});
+    else if (k <= 1024 || (!tiles && k <= 2048 && rows >= 4096)) body(Deal<1, 8, 1, 4>{}, std::true_type{});
+    else if (k > 8192) body(Deal<1, 1, 16, 4>{}, std::true_type{});
+    else if (!tiles || rows < (k <= 2048 ? 1024 : 1536)) body(Deal<1, 1, 4, 4>{}, std::true_type{});
+    else if (zero && k > 2048 && k <= 4096 && rows >= 4096) body(Deal<1, 8, 1, 8>{}, std::true_type{});
+    else if (zero || k <= 2048) body(Deal<1, 8, 2, 2>{}, std::true_type{});
+    else body(Deal<1, 8, 2, 4>{}, std::true_type{});
 }
 int geometry(const orx_function& f, int rows, Geometry* g) {
-    with_deal(rows, f.K, [&](auto deal, auto) {
+    with_deal(f, rows, [&](auto deal, auto) {
         using DEAL = decltype(deal);
         g->grid[0] = std::min<uint32_t>(ceil_div(rows, DEAL::ROWS * DEAL::EACH), kMostGroups);
         g->block[0] = 64 * DEAL::ROWS * DEAL::WAVES;
@@ -182,7 +191,7 @@ int launch_one(const Geometry& g, hipStream_t s, const QuantParams& p) {
 template <int TYPE, bool ZERO>
 int quantise(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const QuantParams& p) {
     int code = ORX_OK;
-    with_deal(rows, f.K, [&](auto deal, auto whole) {
+    with_deal(f, rows, [&](auto deal, auto whole) {
         using DEAL = decltype(deal);
         constexpr bool WHOLE = decltype(whole)::value;
         code = f.flags2 ? launch_one<TYPE, DEAL, WHOLE, ZERO, true>(g, s, p) : launch_one<TYPE, DEAL, WHOLE, ZERO, false>(g, s, p);
