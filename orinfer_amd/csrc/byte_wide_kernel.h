@@ -1,11 +1,14 @@
 // Products of many rows with weights by byte tiles, dense and routed experts: rows through LDS, weights straight into registers.
 //
-// A workgroup of four waves takes 16 ROWS rows x 256 channels, each wave all of these rows and 64 of the channels; K goes in steps of 128 bytes.  Waves that share rows and channels both read
+// A workgroup of four waves takes 128 rows x 256 channels (units of 64 rows: two waves, 128 channels, four workgroups to a CU, which even out better: 16 experts of 4096 x 1536 in fp16, 400 routes, 49
+// -> 44 us), each wave all of these rows and 64 of the channels; K goes in steps of 128 bytes.  Waves that share rows and channels both read
 // more from LDS than it gives: with 64 x 64 results to a wave a step's reads and writes take 1.4 times its multiplies (128 x 256 results to eight waves, all operands through LDS, three
 // stages: 0.84 us a step where the multiplies are 0.43).  Here a wave's weights are its own, so they pass no LDS: four half-steps of them are held or on their way in registers, whole kilobytes a
 // load.  Rows come from memory to LDS without passing a register, four stages; a step's LDS traffic is 0.6 of the multiplies' time, the L1's 0.75.  Two workgroups share a CU: one multiplies
 // while the other waits or stores.  Of a row of experts, which lies anywhere, the 128 bytes of a step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the sixteen rows of a read
 // meet different banks; dense rows arrive by tiles.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied.
+// us of 128 experts, 32768 routes: gate | up 1024 x 2048 100-107 int8 (268 MB of weights and 1.4 PFLOP/s at once), 180-200 in bf16 (537 MB and 0.73 PFLOP/s), down 2048 x 512 106-110 and 152-157, of which
+// 268 MB of fp32 results.  Bound by the weights' and rows' way from memory, which two workgroups to a CU overlap with the multiplies as they come.
 #pragma once
 #include "byte_tiles.h"
 #include "lds_asm.h"

@@ -3,6 +3,8 @@
 // Bound by the weights' bytes: a wave streams whole tiles (2 KiB a step and 16 channels) into registers, AHEAD steps on their way; the steps are dealt to the waves of a workgroup, whose sums
 // meet in LDS.  The weights are the first operand, so a lane ends with four neighbouring channels of one row.
 // 16-bit rows of a product in 8-bit integers (QUANTISE): a workgroup makes their codes itself, into LDS, while its first weights are on their way.
+// us: a bf16 row by 9728 x 2560 int8 7.6 (25 MB, 3.3 TB/s: half of it start, row and first weights), 16 rows of codes by 17408 x 5120 20.6 (4.3 TB/s), by 4096 x 4096 7.2; three tokens' routes to
+// 128 experts of 1024 x 2048 9.6 int8 (50 MB, 5.2 TB/s), one token's in bf16 8.1 (34 MB, 4.1 TB/s).
 #include <algorithm>
 
 #include "byte_device.h"
