@@ -82,6 +82,7 @@ struct Product {
     const int4* units;
     const int* unit_count;
     int most_units;  // that the list holds
+    int runs;  // of neighbouring tiles that an XCD has, where weights go straight to registers
     const int* slot_token;
 };
 

@@ -45,11 +45,14 @@ __global__ __launch_bounds__(ROWS <= 4 ? 128 : 256, 2) void byte_wide_kernel(Pro
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 
-    // ---- which results: tiles blockIdx.x, blockIdx.x + gridDim.x, .. of an order in which every XCD has one run ----
+    // ---- which results: of an order in which every XCD has p.runs runs, every so many tiles of those of the XCD ----
     const int groups = (p.tiles + BN / 16 - 1) / (BN / 16);
     const int row_tiles = GROUPED ? min(__builtin_amdgcn_readfirstlane(*p.unit_count), p.most_units) : (p.m + BM - 1) / BM;
     const int total = row_tiles * groups;
-    const int my_tiles = __builtin_amdgcn_readfirstlane((total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int xcd = blockIdx.x & 7, of_xcd = blockIdx.x >> 3, workgroups = ((int)gridDim.x + 7 - xcd) >> 3;
+    const int run = (total + 8 * p.runs - 1) / (8 * p.runs), runs = run == 0 ? 0 : (total + run - 1) / run;
+    const int tiles_of_xcd = (runs + 7 - xcd) / 8 * run - (runs > 0 && (runs - 1) % 8 == xcd ? runs * run - total : 0);
+    const int my_tiles = __builtin_amdgcn_readfirstlane((tiles_of_xcd - of_xcd + workgroups - 1) / workgroups);
     if (my_tiles <= 0) return;
     struct Tile {
         int first_row, rows, group, expert;
@@ -58,8 +61,7 @@ __global__ __launch_bounds__(ROWS <= 4 ? 128 : 256, 2) void byte_wide_kernel(Pro
     typedef int int4v __attribute__((ext_vector_type(4)));
     const auto units = reinterpret_cast<const __attribute__((address_space(4))) int4v*>(reinterpret_cast<uint64_t>(p.units));
     auto tile_of = [&](int number) __attribute__((always_inline)) {
-        const int at = (int)blockIdx.x + number * (int)gridDim.x, xcd = at & 7;
-        const int id = xcd * (total >> 3) + min(xcd, total & 7) + (at >> 3);
+        const int at = of_xcd + number * workgroups, id = (at / run * 8 + xcd) * run + at % run;
         Tile t;
         if (GROUPED) {
             const int4v u = units[__builtin_amdgcn_readfirstlane(id / groups)];

@@ -381,6 +381,7 @@ int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream
 Product product_of(const orx_function& f, int rows) {
     Product p = {};
     p.m = rows, p.cols = f.H, p.steps = steps_of(f), p.tiles = f.slots, p.type = f.algorithm;
+    p.runs = 1;
     p.row_bytes = f.K * (f.flags2 == I8 ? 1 : 2);
     p.pitch = f.flags2 == I8 ? (int64_t)(p.steps | 1) * kStep : p.row_bytes;
     return p;
@@ -407,6 +408,10 @@ int grouped_launch(const orx_function& f, int rows, const Geometry& g, hipStream
     p.out = pointer_arg<void>(args, at++);
     if (f.flags & kGather) p.slot_token = pointer_arg<const int>(args, at++);
     p.unit_count = pointer_arg<const int>(args, at++), p.units = pointer_arg<const int4>(args, at++), p.most_units = f.tiles;
+    // Units come largest first, those that multiply half last: with one run to an XCD the last XCDs have little to do, with short runs XCDs share units and experts.  (us of both products with 1, 2, 4
+    // and 8 runs; fp16, 128 experts of 2048 and 512: 256 tokens, units of 64 110, 107, 104, 105, 1024, of 128 187, 170, 172, 169, 4096 345, 348, 336, 341; 16 experts of 4096 and 1536: 2048 tokens,
+    // 48 units 226, 225, 241, 249, 4096, 80 units 379, 380, 387, 408.)
+    p.runs = f.tiles >= 128 ? 4 : f.tiles >= 32 ? 2 : 1;
     p.w = pointer_arg<const uint8_t>(args, at++);
     if (f.flags2 == I8) p.w_scale = pointer_arg<const float>(args, at++);
     return launch_product(f, rows, g, s, p);
