@@ -199,6 +199,27 @@ def test_rows_in_the_layers_own_buffer(kind, dtype):
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+def test_rows_in_the_layers_own_buffer_within_a_graph(kind, dtype):
+    tokens, hidden, inner, top_k = 4, 64, 64, 2
+    layer, gate_up, _, x, logits, _, _ = make(kind, dtype, tokens, 8, top_k, hidden, inner)
+    ids, _ = layer.route(dev(logits))
+    layer.place(ids)
+    rows = layer.act[:tokens]
+    layer.up(rows.copy_(x))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer.up(rows)
+    order, _ = slots_of(host(ids))
+    for seed in range(3):
+        fresh = rows_of(np.random.default_rng(seed), tokens, hidden, dtype)
+        rows.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(got, *gate_up.products(fresh, host(ids).reshape(-1)[order], order // top_k, swiglu), dtype)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 def test_a_stream_that_the_caller_names(kind, dtype):
     """All of a call, the copy of rows that lie in the layer's own buffer as well, is behind what that stream has to do."""
     tokens, hidden, inner, top_k = 4, 64, 64, 2

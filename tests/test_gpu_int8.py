@@ -160,7 +160,7 @@ def test_shapes_of_quantize():
 
 
 # ---- linears -----------------------------------------------------------------------------------------------------------------------------------
-LINEARS = [(1, 16, 128), (1, 9, 7), (1, 300, 2560), (2, 33, 5000), (3, 48, 640), (4, 31, 4097), (5, 96, 1000), (16, 128, 1024), (17, 40, 129), (31, 260, 2560), (33, 513, 512), (64, 100, 1111),
+LINEARS = [(1, 16, 128), (1, 9, 7), (1, 1, 1), (6, 1, 300), (7, 300, 2560), (8, 130, 2048), (8, 70, 4100), (1, 300, 2560), (2, 33, 5000), (3, 48, 640), (4, 31, 4097), (5, 96, 1000), (16, 128, 1024), (17, 40, 129), (31, 260, 2560), (33, 513, 512), (64, 100, 1111),
            (65, 300, 300), (130, 520, 1280), (200, 1030, 384), (300, 264, 2048), (513, 700, 257),
            (1024, 256, 64), (1030, 520, 300), (2500, 1100, 640), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2048, 4098, 2560)]
 
