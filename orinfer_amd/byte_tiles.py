@@ -40,6 +40,6 @@ def tiles(weight, paired=False):
 
 def channels(values, paired=False):
     """What the channels have, (..., N), in the order of the tiles, (..., tiles, 16), padded with zeros."""
-    values = torch.as_tensor(values)
+    values = torch.as_tensor(values).detach()
     _check_paired(values.shape[-1], paired)
     return _by_16(values, -1, paired).contiguous()
