@@ -5,7 +5,7 @@
 // under the next multiplies.
 // 256 x 256 results, two stages: bound by the multiplier where tiles fill the CUs (1.25 us a step, 1.7 times the multiplies' own time).
 // 128 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: a step's time is that of its way from memory, so four and six stages of it are under way (128: 0.54 us a step, with two
-// stages 0.8, with two stages and half of K to either half of a workgroup 0.65; 64 x 128: 0.47, 0.75 and 0.55).  Of 64 x 64 four stages leave room for two workgroups to a CU (0.27 each).
+// stages 0.8, with two stages and half of K to either half of a workgroup 0.65; by eight waves 29.0 us at 128 rows of 17408 x 5120, by four 30.9; 64 x 128: 0.47, 0.75 and 0.55).  Of 64 x 64 four stages leave room for two workgroups to a CU (0.27 each).
 #include "byte_wide_kernel.h"
 #include "lds_asm.h"
 #include "orx_internal.h"
@@ -268,7 +268,7 @@ template <typename BODY>
 auto with_form(int form, BODY body) {
     switch (form) {
         case kTiles256: return body(Form<8, 4, 2, 4, 2>{});
-        case kTiles128: return body(Form<4, 4, 2, 2, 4>{});
+        case kTiles128: return body(Form<2, 4, 4, 2, 4>{});
         case kTiles64: return body(Form<2, 4, 2, 2, 6>{});
         default: return body(Form<1, 4, 4, 1, 4>{});
     }
