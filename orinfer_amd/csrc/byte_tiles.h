@@ -8,8 +8,8 @@
 
 namespace orx {
 
-// rows x channels: 256 x 256, 128 x 128, 64 x 128, 64 x 64 (dense); 128 x 256 with weights straight to registers; 64 x 256 of those (experts)
-enum { kTiles256, kTiles128, kTiles64, kTiles64x64, kWide128, kWide64 };
+// rows x channels: 256 x 256, 128 x 128, 96 x 128, 64 x 128, 64 x 64 (dense); 128 x 256 with weights straight to registers; 64 x 256 of those (experts)
+enum { kTiles256, kTiles128, kTiles96, kTiles64, kTiles64x64, kWide128, kWide64 };
 
 struct TilesShape {
     int rows, channels, threads, lds, to_a_cu;  // to_a_cu: workgroups that a CU holds, by its LDS and registers

@@ -45,14 +45,12 @@ __global__ __launch_bounds__(ROWS <= 4 ? 128 : 256, 2) void byte_wide_kernel(Pro
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 
-    // ---- which results: of an order in which every XCD has p.runs runs, every so many tiles of those of the XCD ----
+    // ---- which results: tiles blockIdx.x, blockIdx.x + gridDim.x, .. of an order in which every XCD has p.runs runs (and one of the last few tiles) ----
     const int groups = (p.tiles + BN / 16 - 1) / (BN / 16);
     const int row_tiles = GROUPED ? min(__builtin_amdgcn_readfirstlane(*p.unit_count), p.most_units) : (p.m + BM - 1) / BM;
     const int total = row_tiles * groups;
-    const int xcd = blockIdx.x & 7, of_xcd = blockIdx.x >> 3, workgroups = ((int)gridDim.x + 7 - xcd) >> 3;
-    const int run = (total + 8 * p.runs - 1) / (8 * p.runs), runs = run == 0 ? 0 : (total + run - 1) / run;
-    const int tiles_of_xcd = (runs + 7 - xcd) / 8 * run - (runs > 0 && (runs - 1) % 8 == xcd ? runs * run - total : 0);
-    const int my_tiles = __builtin_amdgcn_readfirstlane((tiles_of_xcd - of_xcd + workgroups - 1) / workgroups);
+    const int of_xcd = total >> 3, run = (of_xcd + p.runs - 1) / p.runs;
+    const int my_tiles = __builtin_amdgcn_readfirstlane((total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x);
     if (my_tiles <= 0) return;
     struct Tile {
         int first_row, rows, group, expert;
@@ -61,7 +59,9 @@ __global__ __launch_bounds__(ROWS <= 4 ? 128 : 256, 2) void byte_wide_kernel(Pro
     typedef int int4v __attribute__((ext_vector_type(4)));
     const auto units = reinterpret_cast<const __attribute__((address_space(4))) int4v*>(reinterpret_cast<uint64_t>(p.units));
     auto tile_of = [&](int number) __attribute__((always_inline)) {
-        const int at = of_xcd + number * workgroups, id = (at / run * 8 + xcd) * run + at % run;
+        const int at = (int)blockIdx.x + number * (int)gridDim.x, xcd = at & 7, nth = at >> 3;
+        const int before = run == 0 ? 0 : nth / run * run;  // tiles of this XCD in earlier runs
+        const int id = nth < of_xcd ? before * 8 + xcd * min(run, of_xcd - before) + nth - before : at;
         Tile t;
         if (GROUPED) {
             const int4v u = units[__builtin_amdgcn_readfirstlane(id / groups)];

@@ -272,14 +272,16 @@ struct Plan {
 // Of few steps fewer waves have one.
 Plan few_rows(const orx_function& f, int unit_rows) { return {unit_rows, -1, unit_rows == 64 || (unit_rows == 16 && steps_of(f) <= 8) ? 4 : 8}; }
 // Of dense launches the form whose estimate is least: fixed + step * steps * rounds over the CUs, in units of 10 ns.  Fitted to times of 1 to 8192 rows by seven sizes of weights (2048 x 1024
-// to 17408 x 5120 and 5120 x 17408); the estimates are within a fifth, except below the time that the weights take from memory, and the form that is picked within a tenth of the fastest.  us at
-// 7168 x 5120 of the kernel above with 16 and with 64 rows, and of tiles of 64 x 64, 64 x 128, 128 x 128, 128 x 256 and 256 x 256:
-//     16 rows: 9.1, 11.3, 14.7, 18.7, 23, 33, -;  64: -, 12.5, 15.3, 22, 24, 35, -;  128: -, 18, 15.5, 21, 28, 39, -;  256: -, 28, 25, 21, 28, 39, 61;  512: -, 47, 43, 38, 28, 39, 59;
-//     1024: -, -, -, 86, 58, 40, 59;  4096: 256 x 256 128 and 128 x 256 132;  8192: 247 and 242
+// to 17408 x 5120 and 5120 x 17408); the estimates are within a fifth, except below the time that the weights take from memory, and the form that is picked within a tenth of the fastest, within a fifth
+// at 96 and 128 rows of 5120 x 17408 (40 by tiles of 64 x 64, 32 to 35 by the kernel above with 64 rows).  us at
+// 7168 x 5120 of the kernel above with 16 and with 64 rows, and of tiles of 64 x 64, 64 x 128, 96 x 128, 128 x 128, 128 x 256 and 256 x 256:
+//     16 rows: 9.1, 11.3, 14.7, 18.7, -, 23, 33, -;  64: -, 12.5, 15.3, 22, 23, 24, 35, -;  128: -, 18, 15.5, 21, 22, 27, 39, -;  256: -, 27, 25, 21, 24, 27, 39, 61;
+//     333: -, 35, 33, 35, 23, 26, 37, 57;  512: -, 45, 43, 38, 41, 27, 39, 59;  1024: -, -, 71, 67, -, 51, 40, 59;  4096: 256 x 256 128 and 128 x 256 132;  8192: 247 and 242
 struct Form {
     int form, rows, channels, fixed, step;
 };
-constexpr Form kForms[] = {{-1, 16, 32, 500, 10}, {-1, 64, 32, 600, 15}, {kTiles64x64, 64, 64, 300, 27}, {kTiles64, 64, 128, 300, 47}, {kTiles128, 128, 128, 400, 54}, {kWide128, 128, 256, 600, 72}, {kTiles256, 256, 256, 800, 125}};
+constexpr Form kForms[] = {{-1, 16, 32, 500, 10}, {-1, 64, 32, 600, 15}, {kTiles64x64, 64, 64, 300, 27}, {kTiles64, 64, 128, 300, 46}, {kTiles96, 96, 128, 400, 47}, {kTiles128, 128, 128, 400, 53},
+                           {kWide128, 128, 256, 600, 72}, {kTiles256, 256, 256, 800, 125}};
 Plan plan(const orx_function& f, int rows) {
     if (f.E > 0) return f.block_m == 16 ? few_rows(f, 16) : Plan{f.block_m, f.block_m == 64 ? kWide64 : kWide128, 0};
     if (f.packed_k != 0) return few_rows(f, 16);

@@ -4,8 +4,9 @@
 // request as they are laid out.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied, and results drain
 // under the next multiplies.
 // 256 x 256 results, two stages: bound by the multiplier where tiles fill the CUs (1.25 us a step, 1.7 times the multiplies' own time).
-// 128 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: a step's time is that of its way from memory, so four and six stages of it are under way (128: 0.54 us a step, with two
-// stages 0.8, with two stages and half of K to either half of a workgroup 0.65; by eight waves 29.0 us at 128 rows of 17408 x 5120, by four 30.9; 64 x 128: 0.47, 0.75 and 0.55).  Of 64 x 64 four stages leave room for two workgroups to a CU (0.27 each).
+// 128 x 128, 96 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: a step's time is that of its way from memory, so four, five and six stages of it are under way (128 x 128: 0.54 us a
+// step, with two stages 0.8, with two stages and half of K to either half of a workgroup 0.65; by eight waves 29.0 us at 128 rows of 17408 x 5120, by four 30.9; 96 x 128: 0.47; 64 x 128: 0.46, with
+// two stages 0.75, with halves of K 0.55).  Of 64 x 64 four stages leave room for two workgroups to a CU (0.27 each).
 #include "byte_wide_kernel.h"
 #include "lds_asm.h"
 #include "orx_internal.h"
@@ -21,9 +22,9 @@ using lds_asm::Each;
 template <int ROWS, int CHANNELS, int DOWN, int ACROSS, int STAGES>
 struct Form {
     static constexpr int rows = ROWS, channels = CHANNELS, across = ACROSS, stages = STAGES;
-    static constexpr int bm = 16 * ROWS * DOWN, bn = 16 * CHANNELS * ACROSS, waves = DOWN * ACROSS, stage = (bm + bn) * kStep;
+    static constexpr int bm = 16 * ROWS * DOWN, row_places = (bm + 63) / 64 * 64, bn = 16 * CHANNELS * ACROSS, waves = DOWN * ACROSS, stage = (bm + bn) * kStep;
     // what a tile's rows and channels have, for the results: scales, zero points, sums and biases; of the tile that is multiplied and of as many as there are stages
-    static constexpr int scale_bytes = 4 * (2 * bm + 3 * bn), lds = STAGES * stage + (STAGES + 1) * scale_bytes;
+    static constexpr int scale_bytes = 4 * (2 * row_places + 3 * bn), lds = STAGES * stage + (STAGES + 1) * scale_bytes;
     static_assert(lds <= 160 * 1024, "a CU's LDS");
 };
 
@@ -31,10 +32,12 @@ template <typename FORM, bool WIDE, bool SWIGLU>
 __global__ __launch_bounds__(64 * FORM::waves, FORM::waves / 4 * (160 * 1024 / FORM::lds)) void byte_tiles_kernel(Product p) {
     using Sum = Operands<I8>::Sum;
     constexpr int ROWS = FORM::rows, CHANNELS = FORM::channels, ACROSS = FORM::across, WAVES = FORM::waves, STAGES = FORM::stages, BM = FORM::bm, BN = FORM::bn;
-    constexpr int A_REQUESTS = BM / 16 / WAVES, W_REQUESTS = BN / 16 / WAVES;  // of a wave and step, whole tiles
-    constexpr int kAll = A_REQUESTS + W_REQUESTS, kLoads = 2 * kAll;
+    constexpr bool HALF = BM / 16 % WAVES != 0;  // rows are requested by halves of tiles
+    constexpr int A_REQUESTS = BM / (HALF ? 8 : 16) / WAVES, W_REQUESTS = BN / 16 / WAVES;  // of a wave and step
+    constexpr int kAll = A_REQUESTS + W_REQUESTS, kLoads = (HALF ? 1 : 2) * A_REQUESTS + 2 * W_REQUESTS;
+    static_assert(A_REQUESTS * WAVES == BM / (HALF ? 8 : 16) && W_REQUESTS * WAVES == BN / 16, "all of a stage");
     constexpr int kW = BM * kStep, kStage = FORM::stage, kScales = STAGES * kStage, kScaleBytes = FORM::scale_bytes;
-    constexpr int kZeros = 4 * BM, kChannels = 8 * BM;  // of a tile's scales
+    constexpr int kZeros = 4 * FORM::row_places, kChannels = 8 * FORM::row_places;  // of a tile's scales
     extern __shared__ __align__(128) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -69,12 +72,15 @@ __global__ __launch_bounds__(64 * FORM::waves, FORM::waves / 4 * (160 * 1024 / F
     auto aim = [&]() __attribute__((always_inline)) {
         load_at = tile_of(load_tile);
 #pragma unroll
-        for (int b = 0; b < A_REQUESTS; ++b) a_from[b] = uniform_pointer(p.a + (int64_t)min(load_at.first_row / 16 + wave * A_REQUESTS + b, (p.m - 1) / 16) * p.steps * kTileBytes);
+        for (int b = 0; b < A_REQUESTS; ++b) {
+            const int at = wave * A_REQUESTS + b;
+            a_from[b] = uniform_pointer(p.a + (int64_t)min(load_at.first_row / 16 + (HALF ? at / 2 : at), (p.m - 1) / 16) * p.steps * kTileBytes + (HALF ? at % 2 * 1024 : 0));
+        }
 #pragma unroll
         for (int b = 0; b < W_REQUESTS; ++b) w_from[b] = uniform_pointer(p.w + (int64_t)min(load_at.group * (BN / 16) + wave * W_REQUESTS + b, p.tiles - 1) * kTileBytes);
     };
     auto request_scales = [&]() __attribute__((always_inline)) {  // in front of a tile's first step
-        constexpr int R = BM / 64, C = BN / 64, CHUNKS = 2 * R + 3 * C;
+        constexpr int R = FORM::row_places / 64, C = BN / 64, CHUNKS = 2 * R + 3 * C;
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds_base + kScales + load_scales);
 #pragma unroll
         for (int c = 0; c < (CHUNKS + WAVES - 1) / WAVES; ++c) {
@@ -100,7 +106,8 @@ __global__ __launch_bounds__(64 * FORM::waves, FORM::waves / 4 * (160 * 1024 / F
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds_base + stage);
         const int take = __builtin_amdgcn_readfirstlane(wanted);
         if constexpr (ID < A_REQUESTS) {
-            request_tile(lane * 16, a_from[ID], to + (wave * A_REQUESTS + ID) * kTileBytes, take);
+            if constexpr (HALF) request_half_tile(lane * 16, a_from[ID], to + (wave * A_REQUESTS + ID) * (kTileBytes / 2), take);
+            else request_tile(lane * 16, a_from[ID], to + (wave * A_REQUESTS + ID) * kTileBytes, take);
             a_from[ID] += kTileBytes;
         } else {
             constexpr int B = ID - A_REQUESTS;
@@ -269,6 +276,7 @@ auto with_form(int form, BODY body) {
     switch (form) {
         case kTiles256: return body(Form<8, 4, 2, 4, 2>{});
         case kTiles128: return body(Form<2, 4, 4, 2, 4>{});
+        case kTiles96: return body(Form<3, 4, 2, 2, 5>{});
         case kTiles64: return body(Form<2, 4, 2, 2, 6>{});
         default: return body(Form<1, 4, 4, 1, 4>{});
     }

@@ -22,6 +22,10 @@ __device__ __forceinline__ const uint8_t* uniform_pointer(const uint8_t* pointer
 __device__ __forceinline__ void request_4_from(const uint8_t* lane_address, uint32_t lds_wave_base, int wanted) {
     asm volatile(ORX_WANTED("global_load_lds_dword %0, off") ::"v"(lane_address), "s"(lds_wave_base), "s"(wanted) : "memory", "m0", "scc");
 }
+// one kilobyte
+__device__ __forceinline__ void request_half_tile(uint32_t lane_offset, const uint8_t* uniform_base, uint32_t lds_wave_base, int wanted) {
+    asm volatile(ORX_WANTED("global_load_lds_dwordx4 %0, %3") ::"v"(lane_offset), "s"(lds_wave_base), "s"(wanted), "s"(uniform_base) : "memory", "m0", "scc");
+}
 // two kilobytes that lie together on both sides
 __device__ __forceinline__ void request_tile(uint32_t lane_offset, const uint8_t* uniform_base, uint32_t lds_wave_base, int wanted) {
     asm volatile(ORX_WANTED("global_load_lds_dwordx4 %0, %3\n\tglobal_load_lds_dwordx4 %0, %3 offset:1024") ::"v"(lane_offset), "s"(lds_wave_base), "s"(wanted), "s"(uniform_base)

@@ -162,7 +162,7 @@ def test_shapes_of_quantize():
 # ---- linears -----------------------------------------------------------------------------------------------------------------------------------
 LINEARS = [(1, 16, 128), (1, 9, 7), (1, 1, 1), (6, 1, 300), (7, 300, 2560), (8, 130, 2048), (8, 70, 4100), (1, 300, 2560), (2, 33, 5000), (3, 48, 640), (4, 31, 4097), (5, 96, 1000), (16, 128, 1024), (17, 40, 129), (31, 260, 2560), (33, 513, 512), (64, 100, 1111),
            (65, 300, 300), (130, 520, 1280), (200, 1030, 384), (300, 264, 2048), (513, 700, 257),
-           (1024, 256, 64), (1030, 520, 300), (2500, 1100, 640), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2048, 4098, 2560)]
+           (1024, 256, 64), (1030, 520, 300), (2500, 1100, 640), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2048, 4098, 2560), (1500, 2050, 520), (2048, 2050, 1111), (2048, 5000, 2560)]
 
 
 @pytest.mark.parametrize("zero_points,biased", [(False, False), (True, True), (True, False), (False, True)])
@@ -181,7 +181,7 @@ def test_linear(rows, n, k, dtype, zero_points, biased):
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
-@pytest.mark.parametrize("rows,n,k", [(1, 32, 128), (1, 34, 2000), (3, 300, 1111), (20, 66, 512), (64, 1000, 256), (150, 258, 640), (400, 514, 300), (1500, 1058, 520), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2040, 4106, 2560)])
+@pytest.mark.parametrize("rows,n,k", [(1, 32, 128), (1, 34, 2000), (3, 300, 1111), (20, 66, 512), (64, 1000, 256), (150, 258, 640), (400, 514, 300), (1500, 1058, 520), (500, 258, 4096), (1024, 1058, 129), (1024, 2050, 520), (2048, 2050, 520), (2040, 4106, 2560), (1500, 2050, 520), (2048, 2050, 1111), (2040, 5004, 2560)])
 def test_linear_with_swiglu(rows, n, k, zero_points):
     rng = np.random.default_rng(rows * n + k)
     x = rows_of(rng, rows, k, torch.bfloat16)
@@ -226,7 +226,7 @@ def test_rows_that_are_not_finite_stay_to_themselves(rows):
 
 
 @pytest.mark.parametrize("name", list(TYPES))
-@pytest.mark.parametrize("rows,n,k", [(1, 33, 256), (6, 130, 384), (70, 50, 129), (260, 530, 128), (1100, 300, 300), (30, 130, 2560), (490, 250, 4096), (1020, 1050, 129), (1020, 2042, 520), (2045, 2042, 520), (2045, 4106, 2560)])
+@pytest.mark.parametrize("rows,n,k", [(1, 33, 256), (6, 130, 384), (70, 50, 129), (260, 530, 128), (1100, 300, 300), (30, 130, 2560), (490, 250, 4096), (1020, 1050, 129), (1020, 2042, 520), (2045, 2042, 520), (2045, 4106, 2560), (500, 258, 4096), (2045, 2050, 1111), (2045, 5002, 2560)])
 def test_projection_writes_its_rows_and_columns_only(rows, n, k, name):
     rng = np.random.default_rng(n)
     x = rows_of(rng, rows, k, torch.float32)
@@ -300,7 +300,7 @@ def test_matrices_and_rows_beyond_4_gib():
     tiles = torch.randint(-127, 128, (k // 128, -(-n // 64) * 4, 8, 16, 16), dtype=torch.int8, device=DEV, generator=g)
     scale = torch.rand(-(-n // 64) * 64, device=DEV, generator=g) / 2**20
     last = list(range(65984, 66000))
-    for rows in (1, 30, 60, 200, 500):  # (a launch of every kind that the sizes allow)
+    for rows in (1, 30, 60, 200, 300, 500):  # (a launch of every kind that the sizes allow)
         x = torch.randint(-127, 128, (rows, k), device=DEV, generator=g)
         x[:, 0] = 127  # (scale 1, codes the values themselves)
         q, s = torch.empty((-(-rows // 16), k // 128, 2048), dtype=torch.int8, device=DEV), torch.empty(rows, device=DEV)

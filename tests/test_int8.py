@@ -121,11 +121,12 @@ def test_records_name_the_kernel_that_runs():
 
 @pytest.mark.parametrize("rows,n,k,kind", [
     (1, 130, 2560, "16 rows"), (16, 7168, 5120, "16 rows"), (500, 258, 4096, "64 rows"), (64, 5120, 17408, "64 rows"), (1, 66, 129, "64 x 64"), (128, 7168, 5120, "64 x 64"),
-    (1024, 1058, 129, "64 x 128"), (32, 17408, 5120, "64 x 128"), (1024, 2050, 520, "128 x 128"), (333, 7168, 5120, "128 x 128"), (2048, 2050, 520, "128 x 256"),
-    (1024, 7168, 5120, "128 x 256"), (2048, 4098, 2560, "256 x 256"), (8192, 4096, 4096, "256 x 256"), (300, 65472, 65536, "128 x 256"), (300, 66000, 65536, "256 x 256")])
+    (1024, 1058, 129, "64 x 128"), (32, 17408, 5120, "64 x 128"), (1024, 2050, 520, "96 x 128"), (333, 7168, 5120, "96 x 128"), (1500, 2050, 520, "128 x 128"), (500, 7168, 5120, "128 x 128"),
+    (2048, 2050, 1111, "128 x 256"), (1024, 7168, 5120, "128 x 256"), (2048, 5000, 2560, "256 x 256"), (8192, 4096, 4096, "256 x 256"), (300, 65472, 65536, "128 x 256"),
+    (500, 66000, 65536, "256 x 256")])
 def test_which_kernel_the_rows_of_a_linear_start(rows, n, k, kind):
     """(as many rows as a test on the GPU has for each; a matrix of 4 GiB is not for the kernel that counts its bytes in 32 bits)"""
-    lds = {(512, 16384): "16 rows", (256, 32768): "64 rows", (256, 71936): "64 x 64", (256, 161792): "64 x 128", (512, 143872): "128 x 128", (256, 77824): "128 x 256", (512, 146432): "256 x 256"}
+    lds = {(512, 16384): "16 rows", (256, 32768): "64 rows", (256, 71936): "64 x 64", (256, 161792): "64 x 128", (256, 158720): "96 x 128", (512, 143872): "128 x 128", (256, 77824): "128 x 256", (512, 146432): "256 x 256"}
     (_, threads, shared), = started(lib.Kernel("int8_token_projection", M=rows, N=n, K=k))
     assert lds.get((threads, shared), (threads, shared)) == kind
 
