@@ -7,7 +7,7 @@
 // load.  Rows come from memory to LDS without passing a register, four stages; a step's LDS traffic is 0.6 of the multiplies' time, the L1's 0.75.  Two workgroups share a CU: one multiplies
 // while the other waits or stores.  Of a row of experts, which lies anywhere, the 128 bytes of a step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the sixteen rows of a read
 // meet different banks; dense rows arrive by tiles.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied.
-// us of 128 experts, 32768 routes: gate | up 1024 x 2048 100-107 int8 (268 MB of weights and 1.4 PFLOP/s at once), 180-200 in bf16 (537 MB and 0.73 PFLOP/s), down 2048 x 512 106-110 and 152-157, of which
+// us of 128 experts, 32768 routes: gate | up 1024 x 2048 99-103 int8 (268 MB of weights and 1.4 PFLOP/s at once), 180-190 in bf16 (537 MB and 0.74 PFLOP/s), down 2048 x 512 97-106 and 140-145, of which
 // 268 MB of fp32 results.  Bound by the weights' and rows' way from memory, which two workgroups to a CU overlap with the multiplies as they come.
 #pragma once
 #include "byte_tiles.h"
