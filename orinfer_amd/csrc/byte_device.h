@@ -121,41 +121,50 @@ __device__ __forceinline__ v4f scaled(typename Operands<KIND>::Sum sum, const Ch
 // fp32, has the scale NaN and codes 0, so its products are NaN.
 constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100
 
-// What a row's values leave: the bits of the largest magnitude, and with zero points the largest value and the largest of the negatives' magnitudes.
+// What a row's values leave, bits as the type orders its magnitudes: `high` of the largest magnitude; with zero points of the largest value that is not negative, and `low` of the lowest value,
+// with its sign (without it where none is negative).  As whole numbers the values from 0 on order as they are and lie above the negative ones, and without a sign the negative ones lie
+// above the others, the lowest on top: one maximum each.
 struct RowRange {
-    uint32_t bits;  // as the type orders its magnitudes
-    float high, low;
+    uint32_t high, low;
 };
 template <int TYPE, bool ZERO, int WORDS>
 __device__ __forceinline__ void widen(RowRange& range, const uint32_t (&words)[WORDS]) {
+    typedef short signed_pair __attribute__((ext_vector_type(2)));
+    typedef unsigned short pair __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int j = 0; j < WORDS; ++j) range.bits = TYPE == mx::F32 ? max(range.bits, words[j] & 0x7FFFFFFFu) : mx::pair_max(range.bits, words[j]);  // (16 bits: both halves apart)
-    if constexpr (ZERO) {
-        auto one = [&](float v) { range.high = fmaxf(range.high, v), range.low = fmaxf(range.low, -v); };
-#pragma unroll
-        for (int j = 0; j < WORDS; ++j) {
-            if constexpr (TYPE == mx::F32) one(__uint_as_float(words[j]));
-            else one(mx::Bits<TYPE>::value(words[j] & 0xFFFFu)), one(mx::Bits<TYPE>::value(words[j] >> 16));
+    for (int j = 0; j < WORDS; ++j) {
+        if constexpr (!ZERO) range.high = TYPE == mx::F32 ? max(range.high, words[j] & 0x7FFFFFFFu) : mx::pair_max(range.high, words[j]);  // (16 bits: both halves apart)
+        else if constexpr (TYPE == mx::F32) range.high = (uint32_t)max((int)range.high, (int)words[j]), range.low = max(range.low, words[j]);
+        else {
+            range.high = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(signed_pair, range.high), __builtin_bit_cast(signed_pair, words[j])));
+            range.low = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, range.low), __builtin_bit_cast(pair, words[j])));
         }
     }
 }
 // over the wave, known to all of it
 template <int TYPE, bool ZERO>
 __device__ __forceinline__ RowRange over_wave(RowRange range) {
-    range.bits = wave_max_u32(TYPE == mx::F32 ? range.bits : max(range.bits & 0xFFFFu, range.bits >> 16));
-    if constexpr (ZERO) range.high = wave_max_magnitude(range.high), range.low = wave_max_magnitude(range.low);
-    return range;
+    auto both = [](uint32_t bits) { return wave_max_u32(TYPE == mx::F32 ? bits : max(bits & 0xFFFFu, bits >> 16)); };
+    return {both(range.high), ZERO ? both(range.low) : 0u};
 }
+__device__ __forceinline__ RowRange wider(const RowRange& a, const RowRange& b) { return {max(a.high, b.high), max(a.low, b.low)}; }
 struct RowCode {
     float scale, inverse;
     int zero;
     bool bad;
 };
+// the largest of the negatives' magnitudes
+template <int TYPE>
+__device__ __forceinline__ uint32_t low_bits(const RowRange& range) {
+    constexpr uint32_t sign = TYPE == mx::F32 ? 0x80000000u : 0x8000u;
+    return range.low & sign ? range.low & (sign - 1) : 0u;
+}
 template <int TYPE, bool ZERO>
 __device__ __forceinline__ RowCode row_code(const RowRange& range) {
     RowCode code;
-    const float span = ZERO ? range.high + range.low : mx::Bits<TYPE>::value(range.bits);
-    code.bad = range.bits >= mx::Bits<TYPE>::infinity || span == __builtin_inff();
+    const uint32_t low = ZERO ? low_bits<TYPE>(range) : 0u;
+    const float span = mx::Bits<TYPE>::value(range.high) + (ZERO ? mx::Bits<TYPE>::value(low) : 0.f);
+    code.bad = max(range.high, low) >= mx::Bits<TYPE>::infinity || span == __builtin_inff();
     code.scale = fmaxf(__fdiv_rn(code.bad ? 0.f : span, ZERO ? 255.f : 127.f), kSmallestScale);
     code.inverse = __fdiv_rn(1.f, code.scale);
     code.zero = 0;
@@ -219,7 +228,7 @@ __device__ __forceinline__ uint2 eight_codes(const uint32_t (&words)[WORDS], con
 template <int TYPE, bool ZERO>
 __device__ __forceinline__ RowCode code_of(const RowRange& range) {
     RowCode code = row_code<TYPE, ZERO>(range);
-    if constexpr (ZERO) code.zero = code.bad ? 0 : zero_point(range.low, code);
+    if constexpr (ZERO) code.zero = code.bad ? 0 : zero_point(mx::Bits<TYPE>::value(low_bits<TYPE>(range)), code);
     return code;
 }
 __device__ __forceinline__ float stored_scale(const RowCode& code) { return code.bad ? __uint_as_float(0x7FC00000u) : code.scale; }

@@ -148,17 +148,14 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void 
         for (int first = 0; first < rows; first += WAVES / row_waves) {
             const int row = first + my_row;
             if (first > 0) read_row(min(row, rows - 1));
-            RowRange range = {0, 0.f, 0.f};
+            RowRange range = {0, 0};
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) widen<TYPE, ZERO>(range, words[i]);
             range = over_wave<TYPE, ZERO>(range);
             if (row_waves > 1) {  // (then one round takes all rows)
                 if (lane == 0) ranges[wave] = range;
                 __syncthreads();
-                for (int i = 0; i < row_waves; ++i) {
-                    const RowRange other = ranges[my_row * row_waves + i];
-                    range.bits = max(range.bits, other.bits), range.high = fmaxf(range.high, other.high), range.low = fmaxf(range.low, other.low);
-                }
+                for (int i = 0; i < row_waves; ++i) range = wider(range, ranges[my_row * row_waves + i]);
             }
             const RowCode code = code_of<TYPE, ZERO>(range);
             if (row < rows) {

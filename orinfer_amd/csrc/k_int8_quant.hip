@@ -85,7 +85,7 @@ __global__ __launch_bounds__(64 * DEAL::ROWS * DEAL::WAVES, 4) void int8_quantis
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
             const bool live = row[e] < p.rows;
-            RowRange range = {0, 0.f, 0.f};
+            RowRange range = {0, 0};
 #pragma unroll
             for (int i = 0; i < HELD; ++i) widen<TYPE, ZERO>(range, words[e][i]);
             for (int piece = at + HELD * THREADS; live && piece < p.pieces; piece += THREADS) {
@@ -99,10 +99,7 @@ __global__ __launch_bounds__(64 * DEAL::ROWS * DEAL::WAVES, 4) void int8_quantis
                 if ((threadIdx.x & 63) == 0) mine[wave] = range;
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < WAVES; ++i) {
-                    const RowRange other = mine[wave / WAVES * WAVES + i];
-                    range.bits = max(range.bits, other.bits), range.high = fmaxf(range.high, other.high), range.low = fmaxf(range.low, other.low);
-                }
+                for (int i = 0; i < WAVES; ++i) range = wider(range, mine[wave / WAVES * WAVES + i]);
             }
             const RowCode code = code_of<TYPE, ZERO>(range);
             auto place = [&](int piece) -> uint8_t* {
@@ -145,26 +142,24 @@ __global__ __launch_bounds__(64 * DEAL::ROWS * DEAL::WAVES, 4) void int8_quantis
 constexpr int kMaxK = 1 << 24;
 constexpr uint32_t kMostGroups = 1 << 21;  // (a launch's threads are fewer than 2^32)
 
-// The deal for `rows` rows of K values; and whether they are whole pieces of eight, which the others only have few of.  us of bf16 rows, the deal taken first (rows x K):
-//   four rows to a wave or one: 32768 x 512 15.1 and 16.7, 4096 x 512 7.1 and 5.6;
-//   by rows: eight rows to a workgroup or one: 8192 x 2048 12.9 and 14.8, 2048 x 2048 7.6 and 6.2, 8192 x 4096 24.1 and 20.4, 8192 x 8192 47.8 and 34.0; four waves to a row or sixteen:
+// The deal for `rows` rows of K values; and whether they are whole pieces of eight, which the others only have few of.  us of bf16 rows, with zero points up to a tenth more, the deal taken first
+// (rows x K):
+//   four rows to a wave or one: 32768 x 512 15.0 and 16.6, 8192 x 512 7.3 and 6.6;
+//   by rows: eight rows to a workgroup or one: 8192 x 2048 12.3 and 14.6, 2048 x 2048 7.6 and 6.5, 8192 x 4096 22.7 and 19.6, 8192 x 8192 48.8 and 34.6; four waves to a row or sixteen:
 //     8192 x 5120 23.3 and 46.0, 2048 x 17408 29.5 and 24.0, 64 x 17408 11.2 and 5.7;
-//   by tiles: eight rows or one: 8192 x 2048 14.3 and 22.0, 2048 x 4096 10.2 and 13.8, 1024 x 4096 8.9 and 7.6; of eight rows two waves to a row or one: 8192 x 4096 23.4 and 26.0, 8192 x 8192
-//     52.5 and 65.2, 8192 x 1024 10.0 and 8.4; with zero points, which take more registers, two pieces to a thread or four: 8192 x 5120 36.2 and 41.7, but 8192 x 4096 29.4, 32.2 and with
-//     one wave that holds the row 27.7.
+//   by tiles: eight rows or one: 2048 x 2048 6.6 and 9.4, 2048 x 4096 10.2 and 13.9, 1024 x 4096 8.6 and 7.4; of eight rows two waves to a row or one: 8192 x 4096 23.7 and 25.8, 8192 x 8192
+//     52.1 and 64.6, 4096 x 2048 8.9 and 10.0, 8192 x 2048 14.7 and 13.3.
 template <typename BODY>
 void with_deal(const orx_function& f, int rows, BODY body) {
     const int k = f.K;
-    const bool zero = f.flags, tiles = f.flags2;
+    const bool tiles = f.flags2;
     if (k % 8) {
         if (k <= 1024 || (tiles && k <= 8192 && rows >= 2048)) body(Deal<1, 8, 1, 4>{}, std::false_type{});
         else body(Deal<1, 1, 4, 4>{}, std::false_type{});
     } else if (k <= 512 && rows >= 16384) body(Deal<4, 8, 1, 1>{}, std::true_type{});
-    else if (k <= 1024 || (!tiles && k <= 2048 && rows >= 4096)) body(Deal<1, 8, 1, 4>{}, std::true_type{});
+    else if (k <= 1024 || (k <= 2048 && rows >= 8192)) body(Deal<1, 8, 1, 4>{}, std::true_type{});
     else if (k > 8192) body(Deal<1, 1, 16, 4>{}, std::true_type{});
     else if (!tiles || rows < (k <= 2048 ? 1024 : 1536)) body(Deal<1, 1, 4, 4>{}, std::true_type{});
-    else if (zero && k > 2048 && k <= 4096 && rows >= 4096) body(Deal<1, 8, 1, 8>{}, std::true_type{});
-    else if (zero || k <= 2048) body(Deal<1, 8, 2, 2>{}, std::true_type{});
     else body(Deal<1, 8, 2, 4>{}, std::true_type{});
 }
 int geometry(const orx_function& f, int rows, Geometry* g) {
