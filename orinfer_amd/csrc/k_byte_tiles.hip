@@ -4,9 +4,10 @@
 // request as they are laid out.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied, and results drain
 // under the next multiplies.
 // 256 x 256 results, two stages: bound by the multiplier where tiles fill the CUs (1.25 us a step, 1.7 times the multiplies' own time).
-// 128 x 128, 96 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: a step's time is that of its way from memory, so four, five and six stages of it are under way (128 x 128: 0.54 us a
-// step, with two stages 0.8, with two stages and half of K to either half of a workgroup 0.65; by eight waves 29.0 us at 128 rows of 17408 x 5120, by four 30.9; 96 x 128: 0.47; 64 x 128: 0.46, with
+// 128 x 128, 96 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: bound by what a CU takes in, 50-60 GB/s of operands in any form, with four, five and six stages under way (128 x 128:
+// 0.54 us a step of 32 KB, with two stages 0.8, with two stages and half of K to either half of a workgroup 0.65; by eight waves 29.0 us at 128 rows of 17408 x 5120, by four 30.9; 96 x 128: 0.47; 64 x 128: 0.46, with
 // two stages 0.75, with halves of K 0.55).  Of 64 x 64 four stages leave room for two workgroups to a CU (0.27 each).
+// (A wave more that brought later steps' lines to the L2 made all of them 30-50 % slower: the lines that are asked for are what counts.)
 #include "byte_wide_kernel.h"
 #include "lds_asm.h"
 #include "orx_internal.h"
