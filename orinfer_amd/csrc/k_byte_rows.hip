@@ -30,8 +30,9 @@ struct Buffer {
 // SOURCE: mx::F16 or mx::BF16 rows to quantise, up to PIECES pieces of eight values to a thread; -1 rows as the product takes them.
 constexpr int tiles_of(int source, bool swiglu) { return source >= 0 && !swiglu ? 1 : 2; }
 
+// (Two workgroups to a CU, of long rows too where gate and up are: 8 rows of 9728 x 2560 15.7 -> 12.1 us, of 14336 x 4096 20.6 -> 15.6; without gate and up those took 16.2 -> 19.6.)
 template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool ZERO, bool GROUPED, bool SWIGLU>
-__global__ __launch_bounds__(WAVES * 64, ROWS == 1 && PIECES <= 4 ? 4 : 2) void byte_rows_kernel(Product p) {
+__global__ __launch_bounds__(WAVES * 64, ROWS == 1 && (PIECES <= 4 || SWIGLU) ? 4 : 2) void byte_rows_kernel(Product p) {
     using Sum = typename Operands<KIND>::Sum;
     constexpr int TILES = tiles_of(SOURCE, SWIGLU);
     constexpr bool QUANTISE = SOURCE >= 0, DEALT = QUANTISE && !GROUPED;
@@ -339,13 +340,15 @@ int launch_one(const Product& p, const Geometry& g, hipStream_t s) {
     ORX_LAUNCH(kernel, dim3(g.grid[0]), dim3(64 * WAVES), g.shared, s, p);
     return hip_check(hipGetLastError(), "launch byte product");
 }
+template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool GROUPED, bool SWIGLU>
+int launch_with(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
+    if constexpr (KIND == I8 && !GROUPED)
+        if (f.flags & kZero) return launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, true, GROUPED, SWIGLU>(p, g, s);
+    return launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, false, GROUPED, SWIGLU>(p, g, s);
+}
 template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool GROUPED>
 int launch_of(const orx_function& f, const Product& p, const Geometry& g, hipStream_t s) {
-    const bool swiglu = f.flags & kSwiglu;
-    if constexpr (KIND == I8 && !GROUPED)
-        if (f.flags & kZero)
-            return swiglu ? launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, true, GROUPED, true>(p, g, s) : launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, true, GROUPED, false>(p, g, s);
-    return swiglu ? launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, false, GROUPED, true>(p, g, s) : launch_one<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, false, GROUPED, false>(p, g, s);
+    return f.flags & kSwiglu ? launch_with<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, GROUPED, true>(f, p, g, s) : launch_with<KIND, ROWS, WAVES, AHEAD, SOURCE, PIECES, GROUPED, false>(f, p, g, s);
 }
 // 16 rows as the product takes them: two steps on their way, of an expert's that has many four (dense, which follow one another, they do not fit the registers).
 template <int KIND, bool GROUPED>
@@ -359,7 +362,9 @@ template <int SOURCE, bool GROUPED>
 int launch_quantising(const orx_function& f, int rows, int waves, const Product& p, const Geometry& g, hipStream_t s) {
     if (waves == 4) return launch_of<I8, 1, 4, 2, SOURCE, 4, GROUPED>(f, p, g, s);
     if (pieces_of(f, rows, waves) > 4) return launch_of<I8, 1, 8, 2, SOURCE, 8, GROUPED>(f, p, g, s);
-    return f.flags & kSwiglu && !GROUPED ? launch_of<I8, 1, 8, 2, SOURCE, 4, GROUPED>(f, p, g, s) : launch_of<I8, 1, 8, 4, SOURCE, 4, GROUPED>(f, p, g, s);
+    if constexpr (GROUPED) return launch_of<I8, 1, 8, 4, SOURCE, 4, true>(f, p, g, s);
+    // (gate and up, dealt: four steps of both do not fit the registers)
+    return f.flags & kSwiglu ? launch_with<I8, 1, 8, 2, SOURCE, 4, GROUPED, true>(f, p, g, s) : launch_with<I8, 1, 8, 4, SOURCE, 4, GROUPED, false>(f, p, g, s);
 }
 int launch_product(const orx_function& f, int rows, const Geometry& g, hipStream_t s, const Product& p) {
     const Plan plan = orx::plan(f, rows);
