@@ -1015,10 +1015,10 @@ class Int8Linear(_OnDevice):
 
 def _unit_rows(routes, experts, expert_bytes):
     """Rows to a unit of the experts' products, by the routes that an expert has in the mean.  (us of both products with units of 16, 64 and 128 rows, popularity like 1 / rank^1.1: fp16, 128
-    experts of 2048 and 512, 4 routes to an expert 65, 66, 67, 8 90, 90, 86, 16 140, 110, 124, 25 182, 123, 132, 32 -, 151, 140; 16 experts of 4096 and 1536, 4 67, 73, 82, 8 94, 85, 92,
-    25 169, 119, 115, 50 252, 167, 136; int8, the same: 4 36, 39, 40, 16 81, 64, 72, 25 109, 72, 80, 32 -, 90, 84; 35, 36, 42, 25 83, 65, 66, 50 128, 90, 79.)  Kernels of 64 and 128 rows
-    count the bytes of an expert's matrix in 32 bits."""
-    return 16 if routes <= 10 * experts or expert_bytes >= 1 << 32 else 64 if routes < 30 * experts else 128
+    experts of 2048 and 512, 4 routes to an expert 65, 65, 66, 8 90, 82, 82, 16 141, 103, 112, 25 182, 119, 120, 32 217, 130, 127; 16 experts of 4096 and 1536, 8 93, 94, 88, 16 133, 109, 110,
+    32 183, 120, 116, 50 252, 154, 135; int8, the same: 4 36, 37, 39, 8 51, 46, 49, 16 81, 59, 63, 25 112, 68, 68, 32 131, 74, 75; 8 46, 49, 50, 16 68, 60, 64, 32 93, 66, 69, 50 128, 84,
+    79.)  Kernels of 64 and 128 rows count the bytes of an expert's matrix in 32 bits."""
+    return 16 if routes < 8 * experts or expert_bytes >= 1 << 32 else 64 if routes < 30 * experts else 128
 
 
 def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):
