@@ -30,7 +30,8 @@ struct Buffer {
 // SOURCE: mx::F16 or mx::BF16 rows to quantise, up to PIECES pieces of eight values to a thread; -1 rows as the product takes them.
 constexpr int tiles_of(int source, bool swiglu) { return source >= 0 && !swiglu ? 1 : 2; }
 
-// (Two workgroups to a CU, of long rows too where gate and up are: 8 rows of 9728 x 2560 15.7 -> 12.1 us, of 14336 x 4096 20.6 -> 15.6; without gate and up those took 16.2 -> 19.6.)
+// (Two workgroups to a CU, of long rows too where gate and up are, us of one and two: 8 rows of 9728 x 2560 13.7 and 10.9, with zero points 16.6 and 12.9, of 14336 x 4096 28.0 and 19.6, 25.9 and
+// 18.6, 4 rows of 17408 x 5120 29.6 and 26.0, 32.9 and 28.2; without gate and up 8 rows took 16.2 and 19.6.  Long rows of bf16 leave 12 to 20 bytes to scratch in front of the first multiply, nothing behind.)
 template <int KIND, int ROWS, int WAVES, int AHEAD, int SOURCE, int PIECES, bool ZERO, bool GROUPED, bool SWIGLU>
 __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && (PIECES <= 4 || SWIGLU) ? 4 : 2) void byte_rows_kernel(Product p) {
     using Sum = typename Operands<KIND>::Sum;
@@ -242,6 +243,9 @@ __global__ __launch_bounds__(WAVES * 64, ROWS == 1 && (PIECES <= 4 || SWIGLU) ? 
                     if (!GROUPED && p.bias != nullptr) channel.bias = *reinterpret_cast<const v4f*>(p.bias + at);
                 }
                 total[kind] = scaled<KIND, !GROUPED>(all, channel, KIND == I8 ? row_scales[min(row, item.rows - 1)] : RowScale{});
+                // (One kind's sums after the other's: both at once, beside the next item's weights on their way, left 44 bytes to scratch with zero points, and every reload waited for those weights:
+                // 8 rows of 9728 x 2560 14.2 -> 12.9 us, one of 17408 x 5120 28.7 -> 23.5.)
+                if constexpr (QUANTISE && SWIGLU) asm volatile("" : "+v"(total[kind])::"memory");
             }
             if constexpr (SWIGLU) {
 #pragma unroll

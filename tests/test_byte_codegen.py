@@ -24,3 +24,13 @@ def test_sums_stay_where_they_are_between_multiplies(built):  # noqa: F811
             if ins.multiply:
                 operands = ins.text.partition(" ")[2].split(", ")
                 assert operands[0] == operands[3], (name, ins.text)
+
+
+def test_nothing_is_reloaded_while_the_next_weights_are_on_their_way(built):  # noqa: F811
+    """A reload from scratch waits for every load in front of it: from the first multiply on the kernel of few rows has the next weights under way."""
+    for name, (code, _) in built.items():
+        if "byte_rows_kernel" not in name:
+            continue
+        first = next(i for i, (_, ins) in enumerate(code) if ins.multiply)
+        late = [ins.text for _, ins in code[first:] if ins.name.startswith("scratch_")]
+        assert not late, (name, late[:5])
