@@ -981,12 +981,16 @@ class Int8Linear(_OnDevice):
         with torch.cuda.device(self.device):
             self.projection = Kernel("int8_token_projection", M=capacity, **shape)
             self.quantizer = Kernel("int8_token_quantization", M=capacity, K=self.k, input_dtype=name, zero_points=self.zero_points, layout="tiles")
-            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two (us, two and one, of 4096 x 4096: 1 row 10.8 and 7.8, 8 11.1 and 9.6, 12 11.1
-            # and 11.9; of 17408 x 5120: 1 row 23.4 and 21.0, 4 23.7 and 22.2; of 24576 x 1536, the least that it gives: 12.8 and 12.2, 8 rows 12.9 and 12.9, 12 12.6 and 14.2).  Not where
-            # their codes do not fit LDS, or a row its threads.
+            # Few rows: the projection quantises them itself, every workgroup all of them, one launch instead of two.  us, two and one:
+            #   no zero points, no SwiGLU: 4096 x 4096, 1 row 9.0 and 8.0, 8 9.1 and 9.2; 17408 x 5120, 1 22.9 and 20.4, 4 23.4 and 22.0; 9728 x 2560, 8 12.0 and 10.6; 24576 x 1536, 8 13.7 and 12.3;
+            #   zero points: 9728 x 2560, 4 12.6 and 10.7, 8 12.7 and 12.3; 8192 x 4096, 4 level, 8 11.8 and 13.9; 17408 x 5120, 4 23.4 and 22.4;
+            #   SwiGLU: 9728 x 2560, 8 12.1 and 11.1; 8192 x 4096, 4 11.3 and 10.5, 8 11.6 and 12.2; 17408 x 5120, 2 level, 4 23.4 and 25.9; 8192 x 8192, 2 17.4 and 15.6, 4 17.7 and 18.4;
+            #   both: 9728 x 2560, 8 level; 8192 x 4096, 4 11.0 and 10.2, 8 12.0 and 13.7; 17408 x 5120, 2 22.8 and 23.5, 4 23.6 and 26.8.
+            # Not where their codes do not fit LDS, or a row its threads.
+            most = 2 if paired and self.k > 4096 else 4 if (paired or self.zero_points) and self.k > 2560 else 8
             self.few, self.few_rows = None, 0
             for rows in (8, 4, 2, 1):
-                if self.few is None and rows <= capacity:
+                if self.few is None and rows <= min(capacity, most):
                     self.few, self.few_rows = _where_it_fits("int8_token_projection", M=rows, input_dtype=name, **shape), rows
         self.n = channels // 2 if paired else channels
         # the quantised rows, by tiles of 16
