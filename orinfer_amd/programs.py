@@ -990,8 +990,9 @@ class Int8Linear(_OnDevice):
             most = 2 if paired and self.k > 4096 else 4 if (paired or self.zero_points) and self.k > 2560 else 8
             self.few, self.few_rows = None, 0
             for rows in (8, 4, 2, 1):
-                if self.few is None and rows <= min(capacity, most):
-                    self.few, self.few_rows = _where_it_fits("int8_token_projection", M=rows, input_dtype=name, **shape), rows
+                if self.few is None and rows <= most:
+                    self.few_rows = min(rows, capacity)
+                    self.few = _where_it_fits("int8_token_projection", M=self.few_rows, input_dtype=name, **shape)
         self.n = channels // 2 if paired else channels
         # the quantised rows, by tiles of 16
         self.a_q = torch.empty((-(-capacity // 16), int8.steps(self.k), 2048), dtype=torch.int8, device=self.device)

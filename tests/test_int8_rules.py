@@ -17,3 +17,8 @@ def test_rows_that_one_launch_quantises_and_multiplies(gpus, k, plain, zeros, ga
     """(more of them are faster in two launches, or do not fit)"""
     assert few_rows(64, k) == plain and few_rows(64, k, zero_points=True) == zeros
     assert few_rows(64, k, epilogue="swiglu") == few_rows(64, k, epilogue="swiglu", zero_points=True) == gated
+
+
+@pytest.mark.parametrize("k,rows", [(512, [1, 2, 3, 4, 5, 6, 7, 8]), (4097, [1, 2, 3, 4, 4, 4, 4, 4])])
+def test_a_linear_made_for_few_rows_takes_all_of_them_in_one_launch(gpus, k, rows):  # noqa: F811
+    assert [few_rows(64, k, capacity) for capacity in range(1, 9)] == rows
