@@ -1018,12 +1018,20 @@ class Int8Linear(_OnDevice):
         self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, m=rows, **zero[1], **self.channel)
 
 
-def _unit_rows(routes, experts, expert_bytes):
-    """Rows to a unit of the experts' products, by the routes that an expert has in the mean.  (us of both products with units of 16, 64 and 128 rows, popularity like 1 / rank^1.1: fp16, 128
-    experts of 2048 and 512, 4 routes to an expert 65, 65, 66, 8 90, 82, 82, 16 141, 103, 112, 25 182, 119, 120, 32 217, 130, 127; 16 experts of 4096 and 1536, 8 93, 94, 88, 16 133, 109, 110,
-    32 183, 120, 116, 50 252, 154, 135; int8, the same: 4 36, 37, 39, 8 51, 46, 49, 16 81, 59, 63, 25 112, 68, 68, 32 131, 74, 75; 8 46, 49, 50, 16 68, 60, 64, 32 93, 66, 69, 50 128, 84,
-    79.)  Kernels of 64 and 128 rows count the bytes of an expert's matrix in 32 bits."""
-    return 16 if routes < 8 * experts or expert_bytes >= 1 << 32 else 64 if routes < 30 * experts else 128
+def _unit_rows(routes, experts, intermediate, expert_bytes):
+    """Rows to a unit of the experts' products, by the routes that an expert has in the mean and by the first products' tiles of 64 x 128 at one unit to an expert: 1024 fill the GPU, and where there
+    are fewer, short units, whose tiles are 16 x 32, spread the work.  Times of both products, int8, with units of 64 over those with 16 and of 128 over those with 64 (popularity like 1 / rank^1.1
+    and even; bf16 is within a tenth of these):
+        1024 tiles, 128 experts of 2048 and 512: 8 routes to an expert 0.97 and 1.05, 12 0.95 and 1.01, 16 0.89 and 0.84; 30 1.10 and 1.02, 36 1.01 and 1.02, 56 0.98 and 0.93;
+        720, 60 of 1024 and 768: 8 1.10 and 1.12, 12 1.02 and 1.11, 16 0.98 and 0.98; 44 1.11 and 1.06, 64 1.02 and 0.88;
+        384, 16 of 4096 and 1536: 8 1.01 and 1.06, 12 0.98 and 1.00; 44 1.07 and 1.00, 64 0.98 and 0.81;
+        256, 32 of 4096 and 512: 12 1.11 and 1.18, 20 1.00 and 0.90; 64 1.05 and 0.90, 112 0.89 and 1.00;
+        128, 8 of 1024 and 1024: 20 1.70 and 1.59, 48 1.40 and 1.41, 96 1.03 and 1.03; 128 1.24 and 1.30, 256 1.12 and 1.14;
+        16, 8 of 256 and 128: 64 1.61 and 1.65, 256 1.18 and 1.18; 512 1.42 and 1.42.
+    Kernels of 64 and 128 rows count the bytes of an expert's matrix in 32 bits."""
+    tiles = experts * -(-2 * intermediate // 128)
+    short, long = (8, 36) if tiles >= 1024 else (max(12, 5120 // tiles), max(64, 28672 // tiles))
+    return 16 if routes < short * experts or expert_bytes >= 1 << 32 else 64 if routes < long * experts else 128
 
 
 def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):
@@ -1056,7 +1064,7 @@ class Int8MoeLayer(_ExpertLayer):
         self.w2, self.s2 = byte_tiles.tiles(down).to(self.device), byte_tiles.channels(down_scale.float()).to(self.device)
         routes = tokens * top_k
         if block_m is None:
-            block_m = _unit_rows(tokens * top_k, experts, max(self.w1.nbytes, self.w2.nbytes) // experts)
+            block_m = _unit_rows(tokens * top_k, experts, intermediate, max(self.w1.nbytes, self.w2.nbytes) // experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(dtype)
@@ -1105,7 +1113,7 @@ class HalfMoeLayer(_ExpertLayer):
         self.device = self._device_of(gate_up, down)
         self.w1, self.w2 = byte_tiles.tiles(gate_up, paired=True).to(self.device), byte_tiles.tiles(down).to(self.device)
         if block_m is None:
-            block_m = _unit_rows(tokens * top_k, experts, max(self.w1.nbytes, self.w2.nbytes) // experts)
+            block_m = _unit_rows(tokens * top_k, experts, intermediate, max(self.w1.nbytes, self.w2.nbytes) // experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, gate_up.dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(gate_up.dtype)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from orinfer_amd import programs
+from tests.test_int8 import LAYERS
 from tests.test_mxfp4_layer import gpus  # noqa: F401  (fixture)
 
 
@@ -22,3 +23,21 @@ def test_rows_that_one_launch_quantises_and_multiplies(gpus, k, plain, zeros, ga
 @pytest.mark.parametrize("k,rows", [(512, [1, 2, 3, 4, 5, 6, 7, 8]), (4097, [1, 2, 3, 4, 4, 4, 4, 4])])
 def test_a_linear_made_for_few_rows_takes_all_of_them_in_one_launch(gpus, k, rows):  # noqa: F811
     assert [few_rows(64, k, capacity) for capacity in range(1, 9)] == rows
+
+
+@pytest.mark.parametrize("kind", LAYERS)
+@pytest.mark.parametrize("experts,inner,first,second", [
+    (128, 512, 8, 36), (256, 256, 8, 36),       # 1024 tiles of the first products at one unit to an expert: the GPU is full
+    (60, 768, 12, 64), (16, 1536, 13, 74), (32, 512, 20, 112), (8, 1024, 40, 224), (8, 128, 320, 1792)])
+def test_rows_to_a_unit(gpus, kind, experts, inner, first, second):  # noqa: F811
+    """The fewer tiles there are, the more routes to an expert are faster in short units."""
+    make, bank = kind
+
+    def unit(routes):
+        return make(routes, experts, 1, 8, inner, *bank("cuda:0", experts, 2 * inner, 8), *bank("cuda:0", experts, 8, inner)).block_m
+
+    assert [unit(bound * experts + more) for bound in (first, second) for more in (-1, 0)] == [16, 64, 64, 128]
+
+
+def test_matrices_of_4_gib_go_in_units_of_16():
+    assert [programs._unit_rows(100000, 16, 1536, size) for size in ((1 << 32) - 1, 1 << 32)] == [128, 16]
