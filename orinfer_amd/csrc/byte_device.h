@@ -7,9 +7,9 @@
 // A wave's load of an operand is whole kilobytes, with nothing to unpack.  Channels are padded to 64, four tiles, and K to 256 bytes, two steps, with zeros.  What a channel has (scale, sum, bias) lies by tiles too.
 // SwiGLU: tiles of gate channels and of their up channels take turns, so a lane has both of a pair.
 //
-// Rows of 8-bit integers: x = (q - z) s with an fp32 scale s, and a zero point z or none, for each row, zeros behind K up to a multiple of 256.  Dense rows lie by tiles of 16 rows x 128,
-// [piece][row][16], the tiles of the same rows along K behind one another; rows of experts, which a product takes from anywhere, an odd multiple of 128 bytes apart (at a multiple of 4 KiB they
-// meet in few channels of the L2).  Channel c has an fp32 scale t and S = sum of its weights w:
+// Rows of 8-bit integers: x = (q - z) s with an fp32 scale s, and a zero point z or none, for each row; behind K, up to a multiple of 256, the code of 0 (z, or 0 without zero points), which meets the
+// weights' zeros.  Dense rows lie by tiles of 16 rows x 128, [piece][row][16], the tiles of the same rows along K behind one another; rows of experts, which a product takes from anywhere, an odd
+// multiple of 128 bytes apart (at a multiple of 4 KiB they meet in few channels of the L2).  Channel c has an fp32 scale t and S = sum of its weights w:
 //   y = (sum_k q w - z S) t s + bias, the bracket exact in 32 bits up to K = 65536 (255 * 128 * 65536 < 2^31), then one rounding for each operation and one for the output.
 #pragma once
 #include <hip/hip_runtime.h>

@@ -18,7 +18,7 @@ struct QuantParams {
     uint8_t* q;
     float* s;
     int* z;
-    int rows, k, pieces;  // pieces of eight codes that a row has, zeros behind K among them
+    int rows, k, pieces;  // pieces of eight codes that a row has, those behind K among them
     int64_t pitch;  // by rows
     int steps;      // by tiles of 16 rows
 };

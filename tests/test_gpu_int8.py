@@ -341,3 +341,25 @@ def test_refusals_of_tensors():
         int8.quantize(torch.zeros((2, 0), device=DEV))
     with pytest.raises(ValueError):
         int8.quantize(torch.zeros((2, 4), dtype=torch.float64, device=DEV))
+
+
+@pytest.mark.parametrize("layout", ["rows", "tiles"])
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("rows,k", [(3, 33), (40, 300), (1030, 1100), (2050, 1501), (1601, 5000), (9, 9001)])
+def test_behind_k_stands_the_code_of_0(rows, k, name, zero_points, layout):
+    """... up to a multiple of 256: the row's zero point, or 0 without zero points and in rows that are not finite."""
+    x = rows_of(np.random.default_rng(rows + k), rows, k, TYPES[name], side=1.0 * zero_points)
+    x[rows // 2, k // 2] = torch.inf
+    steps = int8.steps(k)
+    q = torch.full((-(-rows // 16) * 16 * (steps | 1) * 128,), 91, dtype=torch.int8, device=DEV)
+    s, z = torch.empty(rows, device=DEV), torch.zeros(rows, dtype=torch.int32, device=DEV)
+    kernel("int8_token_quantization", K=k, input_dtype=name, zero_points=zero_points, layout=layout)(Q=q, S=s, X=x.to(DEV), rows=rows, **({"Z": z} if zero_points else {}))
+    if layout == "tiles":
+        tiles = -(-rows // 16)
+        got = q[:tiles * steps * 2048].view(tiles, steps, 8, 16, 16).permute(0, 3, 1, 2, 4).reshape(tiles * 16, steps * 128)[:rows]
+    else:
+        got = q.view(-1, (steps | 1) * 128)[:rows, :steps * 128]
+    assert torch.equal(got[:, k:].int(), z[:, None].expand(rows, steps * 128 - k)) and (got[rows // 2] == 0).all() and s[rows // 2].isnan()
+    if zero_points:
+        assert (z != 0).any()

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from orinfer_amd import programs
+from orinfer_amd import lib, programs
 from tests.test_int8 import LAYERS
 from tests.test_mxfp4_layer import gpus  # noqa: F401  (fixture)
 
@@ -41,3 +41,20 @@ def test_rows_to_a_unit(gpus, kind, experts, inner, first, second):  # noqa: F81
 
 def test_matrices_of_4_gib_go_in_units_of_16():
     assert [programs._unit_rows(100000, 16, 1536, size) for size in ((1 << 32) - 1, 1 << 32)] == [128, 16]
+
+
+@pytest.mark.parametrize("rows,most", [(1, 32768), (2, 16384), (3, 8192), (4, 8192), (5, 4096), (8, 4096), (16, 4096), (17, 0)])
+@pytest.mark.parametrize("epilogue", ["none", "swiglu"])
+def test_the_longest_rows_that_a_projection_quantises(rows, most, epilogue):
+    for k in (most, most + 1):
+        shape = dict(M=rows, N=64, K=k or 1, input_dtype="bfloat16", epilogue=epilogue, zero_points=True)
+        if k == most and most:
+            assert lib.Kernel("int8_token_projection", **shape).arg_names == ["A", "Out", "W", "WS", "WSum"]
+        else:
+            with pytest.raises(lib.OrxError) as error:
+                lib.Kernel("int8_token_projection", **shape)
+            assert error.value.code == lib.ORX_ERR_BAD_VARIANT
+    grouped = dict(rows=12, E=4, N=64, tiles=8, input_dtype="float16", epilogue=epilogue)
+    assert lib.Kernel("int8_token_grouped", K=4096, **grouped).arg_names[0] == "A"
+    with pytest.raises(lib.OrxError):
+        lib.Kernel("int8_token_grouped", K=4097, **grouped)
