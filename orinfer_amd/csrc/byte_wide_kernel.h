@@ -7,8 +7,11 @@
 // load.  Rows come from memory to LDS without passing a register, four stages; a step's LDS traffic is 0.6 of the multiplies' time, the L1's 0.75.  Two workgroups share a CU: one multiplies
 // while the other waits or stores.  Of a row of experts, which lies anywhere, the 128 bytes of a step keep their 16-byte piece p at p ^ ((row >> 1) & 7), so that the sixteen rows of a read
 // meet different banks; dense rows arrive by tiles.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied.
-// us of 128 experts, 32768 routes: gate | up 1024 x 2048 99-103 int8 (268 MB of weights and 1.4 PFLOP/s at once), 180-190 in bf16 (537 MB and 0.74 PFLOP/s), down 2048 x 512 97-106 and 140-145, of which
-// 268 MB of fp32 results.  Bound by the weights' and rows' way from memory, which two workgroups to a CU overlap with the multiplies as they come.
+// us of 128 experts, 32768 routes: gate | up 1024 x 2048 98-105 int8, 185-206 in bf16, down 2048 x 512 98-106 and 140-148.  Bound by memory at 4.6 to 5.1 TB/s, a large copy's 5.1: they read 463 and 919
+// MB and 238 and 482 beside 268 of fp32 results, of which an expert's weights come about one and a half times (the list has its short last unit far from its full ones, and at the ends of runs two
+// XCDs share an expert); the pipe is busy in 0.38 and 0.42, 0.18 and 0.26 of the cycles.
+// The int8 form of 128 rows with a gather and SwiGLU to 16 bits leaves 32 bytes to scratch (of request_tokens, read again where a tile is aimed at), to fp32 8; the dense ones with SwiGLU 44 and 108, around
+// the results (1024 and 2048 rows of 17408 x 5120: 99 and 173 us, without SwiGLU 95 and 177).
 #pragma once
 #include "byte_tiles.h"
 #include "lds_asm.h"

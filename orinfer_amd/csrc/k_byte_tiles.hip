@@ -3,8 +3,10 @@
 // DOWN x ACROSS waves share a tile, each ROWS x CHANNELS blocks of 16 x 16 of it; K goes in steps of 128 bytes.  Rows and weights come from memory to LDS without passing a register, a kilobyte to a
 // request as they are laid out.  A workgroup goes through its tiles as one sequence of steps: the next tile's first steps are on their way while the last ones are multiplied, and results drain
 // under the next multiplies.
-// 256 x 256 results, two stages: bound by the multiplier where tiles fill the CUs (1.25 us a step, 1.7 times the multiplies' own time).
-// 128 x 128, 96 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: bound by what a CU takes in, 50-60 GB/s of operands in any form, with four, five and six stages under way (128 x 128:
+// 256 x 256 results, two stages: bound by the multiplier where tiles fill the CUs (1.25 us a step, 1.7 times the multiplies' own time at 2.4 GHz: at 8192 rows of 4096 x 4096 the pipe is busy in 0.64 of
+// the cycles, and these take 1.8 GHz, where launches that multiply less run at 2.0 to 2.5).
+// 128 x 128, 96 x 128, 64 x 128 and 64 x 64, for launches of fewer tiles than CUs: a CU took in 50-60 GB/s of operands in every form.  No unit is full then (333 rows of 7168 x 5120: pipe 0.26 of the
+// cycles, LDS 0.16, 21 bytes a cycle from the L2, 2.3 TB/s from memory; waves wait in 0.38): it is what latency and one workgroup to a CU leave.  Four, five and six stages are under way (128 x 128:
 // 0.54 us a step of 32 KB, with two stages 0.8, with two stages and half of K to either half of a workgroup 0.65; by eight waves 29.0 us at 128 rows of 17408 x 5120, by four 30.9; 96 x 128: 0.47; 64 x 128: 0.46, with
 // two stages 0.75, with halves of K 0.55).  Of 64 x 64 four stages leave room for two workgroups to a CU (0.27 each).
 // (A wave more that brought later steps' lines to the L2 made all of them 30-50 % slower: the lines that are asked for are what counts.)
