@@ -319,3 +319,25 @@ def test_refusals():
     with pytest.raises(lib.OrxError) as error:
         layer.up(moved)
     assert error.value.code == lib.ORX_ERR_BAD_ARGUMENT and "aligned" in str(error.value)
+
+
+@pytest.mark.parametrize("dtype,smallest", [(F16, 2.0**-24), (BF16, 2.0**-133)])
+@pytest.mark.parametrize("block_m", [16, 64, 128])
+@pytest.mark.parametrize("of_rows", [False, True])
+def test_subnormal_values_count(of_rows, block_m, dtype, smallest):
+    """Whole multiples of the type's smallest value, below its smallest normal one, times whole numbers (bf16: of 2^110): the sums are whole multiples of fp32's, exact."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    experts, n, k, slots = 3, 72, 264, 150
+    small, large = ((slots, k), (experts, n, k)) if of_rows else ((experts, n, k), (slots, k))
+    small = (torch.randint(-7, 8, small, device=DEV, generator=g).double() * smallest).to(dtype)
+    large = (torch.randint(-7, 8, large, device=DEV, generator=g).double() * (1.0 if dtype == F16 else 2.0**110)).to(dtype)
+    assert 0 < small.abs().max() < torch.finfo(dtype).smallest_normal
+    x, w = (small, large) if of_rows else (large, small)
+    units = torch.tensor([[i % experts, first, min(block_m, slots - first), 0] for i, first in enumerate(range(0, slots, block_m))], dtype=torch.int32, device=DEV)
+    out = torch.empty((slots, n), device=DEV)
+    kernel("half_grouped", rows=slots, E=experts, N=n, K=k, tiles=len(units), block_m=block_m, dtype=int8.dtype_name(dtype), output_dtype="float32")(
+        A=x, Out=out, TileCount=torch.tensor([len(units)], dtype=torch.int32, device=DEV), TileUnits=units, W=byte_tiles.tiles(w))
+    for e, first, rows, _ in units.tolist():
+        at = slice(first, first + rows)
+        want = x[at].double() @ w[e].double().t().contiguous()
+        assert want.any() and torch.equal(out[at].double(), want)
