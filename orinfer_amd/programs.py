@@ -1021,7 +1021,7 @@ class Int8Linear(_OnDevice):
 def _unit_rows(routes, experts, intermediate, expert_bytes):
     """Rows to a unit of the experts' products, by the routes that an expert has in the mean and by the first products' tiles of 64 x 128 at one unit to an expert: 1024 fill the GPU, and where there
     are fewer, short units, whose tiles are 16 x 32, spread the work.  Times of both products, int8, with units of 64 over those with 16 and of 128 over those with 64 (popularity like 1 / rank^1.1
-    and even; bf16 is within a tenth of these):
+    and even; bf16 is within 0.2 of these):
         1024 tiles, 128 experts of 2048 and 512: 8 routes to an expert 0.97 and 1.05, 12 0.95 and 1.01, 16 0.89 and 0.84; 30 1.10 and 1.02, 36 1.01 and 1.02, 56 0.98 and 0.93;
         720, 60 of 1024 and 768: 8 1.10 and 1.12, 12 1.02 and 1.11, 16 0.98 and 0.98; 44 1.11 and 1.06, 64 1.02 and 0.88;
         384, 16 of 4096 and 1536: 8 1.01 and 1.06, 12 0.98 and 1.00; 44 1.07 and 1.00, 64 0.98 and 0.81;
