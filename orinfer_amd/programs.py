@@ -1035,6 +1035,8 @@ def _unit_rows(routes, experts, intermediate, expert_bytes):
 
 
 def _check_experts(gate_up, down, experts, hidden, intermediate, dtypes):
+    if experts < 1:
+        raise ValueError("there must be at least one expert")
     if tuple(gate_up.shape) != (experts, 2 * intermediate, hidden) or tuple(down.shape) != (experts, hidden, intermediate):
         raise ValueError(f"gate_up must be ({experts}, {2 * intermediate}, {hidden}) and down ({experts}, {hidden}, {intermediate}), not {tuple(gate_up.shape)} and {tuple(down.shape)}")
     if gate_up.dtype not in dtypes or down.dtype != gate_up.dtype:

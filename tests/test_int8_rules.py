@@ -58,3 +58,10 @@ def test_the_longest_rows_that_a_projection_quantises(rows, most, epilogue):
     assert lib.Kernel("int8_token_grouped", K=4096, **grouped).arg_names[0] == "A"
     with pytest.raises(lib.OrxError):
         lib.Kernel("int8_token_grouped", K=4097, **grouped)
+
+
+@pytest.mark.parametrize("kind", LAYERS)
+def test_a_layer_without_experts_is_refused(gpus, kind):  # noqa: F811
+    make, bank = kind
+    with pytest.raises(ValueError, match="expert"):
+        make(3, 0, 2, 96, 64, *bank("cuda:0", 0, 128, 96), *bank("cuda:0", 0, 96, 64))
