@@ -1018,19 +1018,19 @@ class Int8Linear(_OnDevice):
         self.projection(stream=stream, A=self.a_q, AS=self.a_s, Out=self.out, W=self.weight, m=rows, **zero[1], **self.channel)
 
 
-def _unit_rows(routes, experts, intermediate, expert_bytes):
-    """Rows to a unit of the experts' products, by the routes that an expert has in the mean and by the first products' tiles of 64 x 128 at one unit to an expert: 1024 fill the GPU, and where there
-    are fewer, short units, whose tiles are 16 x 32, spread the work.  Times of both products, int8, with units of 64 over those with 16 and of 128 over those with 64 (popularity like 1 / rank^1.1
-    and even; bf16 is within 0.2 of these):
-        1024 tiles, 128 experts of 2048 and 512: 8 routes to an expert 0.97 and 1.05, 12 0.95 and 1.01, 16 0.89 and 0.84; 30 1.10 and 1.02, 36 1.01 and 1.02, 56 0.98 and 0.93;
-        720, 60 of 1024 and 768: 8 1.10 and 1.12, 12 1.02 and 1.11, 16 0.98 and 0.98; 44 1.11 and 1.06, 64 1.02 and 0.88;
-        384, 16 of 4096 and 1536: 8 1.01 and 1.06, 12 0.98 and 1.00; 44 1.07 and 1.00, 64 0.98 and 0.81;
-        256, 32 of 4096 and 512: 12 1.11 and 1.18, 20 1.00 and 0.90; 64 1.05 and 0.90, 112 0.89 and 1.00;
-        128, 8 of 1024 and 1024: 20 1.70 and 1.59, 48 1.40 and 1.41, 96 1.03 and 1.03; 128 1.24 and 1.30, 256 1.12 and 1.14;
-        16, 8 of 256 and 128: 64 1.61 and 1.65, 256 1.18 and 1.18; 512 1.42 and 1.42.
+def _unit_rows(routes, experts, hidden, intermediate, expert_bytes):
+    """Rows to a unit of the experts' products, by the routes that an expert has in the mean and by the tiles of 64 x 128 that both products have at one unit to an expert: where these are few, short
+    units spread the work over the GPU.  Measured at 892 banks (4 to 256 experts of 256 to 4096 and 128 to 1536, int8 and bf16, 5 to 400 routes to an expert, popularity like 1 / rank^1.1 or even):
+    this rule's units take 1.01 times the best of the three in the geometric mean, 1.09 at the 95th and 1.19 at the 99th percentile; bounds of 8 and 30 routes whatever the bank 1.20, 1.98, 2.64.
+    Times with units of 64 over those with 16, and of 128 over 64 (int8, popularity skewed and even; bf16 is within 0.2 of these):
+        3072 tiles, 128 experts of 2048 and 512: 8 routes to an expert 0.97 and 1.05, 12 0.95 and 1.01, 16 0.89 and 0.84; 36 1.01 and 1.02, 56 0.98 and 0.93;
+        1200, 60 of 1024 and 768: 8 1.10 and 1.12, 12 1.02 and 1.11, 16 0.98 and 0.98; 44 1.11 and 1.06, 64 1.02 and 0.88;
+        896, 16 of 4096 and 1536: 8 1.01 and 1.06, 14 0.95 and 0.92; 44 1.07 and 1.00, 64 0.98 and 0.81;
+        192, 8 of 1024 and 1024: 20 1.70 and 1.59, 48 1.40 and 1.41, 96 1.03 and 1.03; 256 1.12 and 1.14, 512 1.06 and 1.07;
+        32, 8 of 256 and 128: 64 1.61 and 1.65, 256 1.18 and 1.18; 512 1.42 and 1.42.
     Kernels of 64 and 128 rows count the bytes of an expert's matrix in 32 bits."""
-    tiles = experts * -(-2 * intermediate // 128)
-    short, long = (8, 36) if tiles >= 1024 else (max(12, 5120 // tiles), max(64, 28672 // tiles))
+    tiles = experts * (-(-2 * intermediate // 128) + -(-hidden // 128))
+    short, long = max(8, 12288 // tiles), max(48, 81920 // tiles)
     return 16 if routes < short * experts or expert_bytes >= 1 << 32 else 64 if routes < long * experts else 128
 
 
@@ -1066,7 +1066,7 @@ class Int8MoeLayer(_ExpertLayer):
         self.w2, self.s2 = byte_tiles.tiles(down).to(self.device), byte_tiles.channels(down_scale.float()).to(self.device)
         routes = tokens * top_k
         if block_m is None:
-            block_m = _unit_rows(tokens * top_k, experts, intermediate, max(self.w1.nbytes, self.w2.nbytes) // experts)
+            block_m = _unit_rows(tokens * top_k, experts, hidden, intermediate, max(self.w1.nbytes, self.w2.nbytes) // experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(dtype)
@@ -1115,7 +1115,7 @@ class HalfMoeLayer(_ExpertLayer):
         self.device = self._device_of(gate_up, down)
         self.w1, self.w2 = byte_tiles.tiles(gate_up, paired=True).to(self.device), byte_tiles.tiles(down).to(self.device)
         if block_m is None:
-            block_m = _unit_rows(tokens * top_k, experts, intermediate, max(self.w1.nbytes, self.w2.nbytes) // experts)
+            block_m = _unit_rows(tokens * top_k, experts, hidden, intermediate, max(self.w1.nbytes, self.w2.nbytes) // experts)
         self._set_up(tokens, experts, top_k, hidden, intermediate, gate_up.dtype, block_m, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best,
                      renormalize=renormalize, scale=scale)
         name = int8.dtype_name(gate_up.dtype)

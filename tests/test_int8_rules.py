@@ -25,22 +25,29 @@ def test_a_linear_made_for_few_rows_takes_all_of_them_in_one_launch(gpus, k, row
     assert [few_rows(64, k, capacity) for capacity in range(1, 9)] == rows
 
 
-@pytest.mark.parametrize("kind", LAYERS)
-@pytest.mark.parametrize("experts,inner,first,second", [
-    (128, 512, 8, 36), (256, 256, 8, 36),       # 1024 tiles of the first products at one unit to an expert: the GPU is full
-    (60, 768, 12, 64), (16, 1536, 13, 74), (32, 512, 20, 112), (8, 1024, 40, 224), (8, 128, 320, 1792)])
-def test_rows_to_a_unit(gpus, kind, experts, inner, first, second):  # noqa: F811
-    """The fewer tiles there are, the more routes to an expert are faster in short units."""
-    make, bank = kind
-
+@pytest.mark.parametrize("experts,hidden,inner,first,second", [
+    (128, 2048, 512, 8, 48), (128, 3264, 224, 8, 48), (60, 1024, 768, 10, 68), (16, 4096, 1536, 13, 91), (32, 4096, 512, 9, 64), (8, 1024, 1024, 64, 426), (8, 256, 128, 384, 2560)])
+def test_rows_to_a_unit(experts, hidden, inner, first, second):
+    """The fewer tiles both products have, the more routes to an expert are faster in short units."""
     def unit(routes):
-        return make(routes, experts, 1, 8, inner, *bank("cuda:0", experts, 2 * inner, 8), *bank("cuda:0", experts, 8, inner)).block_m
+        return programs._unit_rows(routes, experts, hidden, inner, 1 << 20)
 
     assert [unit(bound * experts + more) for bound in (first, second) for more in (-1, 0)] == [16, 64, 64, 128]
 
 
+@pytest.mark.parametrize("kind", LAYERS)
+def test_a_layer_takes_the_rule_for_its_own_bank(gpus, kind):  # noqa: F811
+    make, bank = kind
+
+    def unit(routes, **options):
+        return make(routes, 8, 1, 1024, 128, *bank("cuda:0", 8, 256, 1024), *bank("cuda:0", 8, 1024, 128), **options).block_m
+
+    assert [unit(8 * bound + more) for bound in (153, 1024) for more in (-1, 0)] == [16, 64, 64, 128]  # (80 tiles)
+    assert unit(8, block_m=64) == 64
+
+
 def test_matrices_of_4_gib_go_in_units_of_16():
-    assert [programs._unit_rows(100000, 16, 1536, size) for size in ((1 << 32) - 1, 1 << 32)] == [128, 16]
+    assert [programs._unit_rows(100000, 16, 4096, 1536, size) for size in ((1 << 32) - 1, 1 << 32)] == [128, 16]
 
 
 @pytest.mark.parametrize("rows,most", [(1, 32768), (2, 16384), (3, 8192), (4, 8192), (5, 4096), (8, 4096), (16, 4096), (17, 0)])
